@@ -1,0 +1,479 @@
+// Inner products in 8-bit floating point: the row quantizer, the weights' layout, the product and the gated product.
+//
+// A block of 128 values shares a float32 scale. Its codes become halves, which hold every e4m3 value exactly, and four v_mfma_f32_16x16x32_f16 sum
+// the block's products, 16 outputs x 16 rows, still without scales; the sum goes to the running one with one multiply-add per value, by the product of
+// the two blocks' scales. Weights are the first operand, rows of the input the second: a lane's four results are then four neighbouring outputs of
+// one row, so the row's scale is one register of the lane and the weights' scale one value of the wave.
+//
+// The matrix core's own 8-bit products (v_mfma_f32_16x16x128_f8f6f4, v_mfma_f32_16x16x32_fp8_fp8) add groups of eight with 13 bits beneath the largest
+// of them; what is smaller is cut off. A product of normal rows is 3e-5 off then (measured), where float32 sums of the exact products are 3e-8 off.
+#include "common.h"
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v2i __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+
+namespace {
+
+constexpr int kBlk = EXHIP_F8_BLOCK;
+constexpr int kRsrcWord3 = 0x00020000;
+constexpr float kLargest = 448.f;                   // of e4m3
+constexpr float kLeastScale = 0x1p-100f;            // keeps 1 / scale finite and blocks of zeros at zero
+constexpr int kMostStride = 1 << 22;                // of a row of codes: offsets inside a tile's rows stay below 2^31
+
+// What the last block's codes of a row are ANDed with: `left` values of 16 are the row's own.
+__device__ __forceinline__ v4i keep_first(int left) {
+    v4i m;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        const int v = left - 4 * d;
+        m[d] = v >= 4 ? -1 : v <= 0 ? 0 : (1 << (8 * v)) - 1;
+    }
+    return m;
+}
+
+// ---- the quantizer ----
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Eight {  // eight values at any alignment of their type
+    T v[8];
+};
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(uint16_t v) { return exhip_h2f(v); }
+
+// The largest of a block, from 16 lanes of eight values each. (fmaxf leaves NaN out.)
+__device__ __forceinline__ float block_max(float a) {
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) a = fmaxf(a, __shfl_xor(a, d));
+    return a;
+}
+__device__ __forceinline__ float scale_of(float most) { return fmaxf(most / kLargest, kLeastScale); }
+__device__ __forceinline__ int four_codes(float a, float b, float c, float d) {
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+
+// 16 rows x one block a group of 256.
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int x_stride, int m, int k, uint8_t* __restrict__ y, int y_stride,
+                                                            float* __restrict__ scale) {
+    const int row = blockIdx.x * 16 + threadIdx.x / 16, b = blockIdx.y, at = b * kBlk + (threadIdx.x % 16) * 8;
+    float v[8];
+    const T* const src = x + (size_t)(row < m ? row : 0) * x_stride + at;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    if (row < m) {
+        if (at + 8 <= k) {
+            const Eight<T> t = *reinterpret_cast<const Eight<T>*>(src);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = as_float(t.v[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (at + e < k) v[e] = as_float(src[e]);
+        }
+    }
+    float a = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(v[e]));
+    const float s = scale_of(block_max(a)), r = 1.f / s;
+    if (row >= m) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= r;
+    const v2i q = {four_codes(v[0], v[1], v[2], v[3]), four_codes(v[4], v[5], v[6], v[7])};
+    uint8_t* const dst = y + (size_t)row * y_stride + at;
+    if (at + 8 <= k) {
+        *reinterpret_cast<v2i*>(dst) = q;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (at + e < k) dst[e] = (uint8_t)(q[e / 4] >> (8 * (e % 4)));
+    }
+    if (threadIdx.x % 16 == 0) scale[(size_t)b * m + row] = s;
+}
+
+// One 128 x 128 block of a weight matrix a group. Runs once for a model: two readings of the block.
+__global__ __launch_bounds__(256) void quantize_blocks_kernel(const float* __restrict__ w, int n, int k, int blocks_k, uint8_t* __restrict__ y,
+                                                              float* __restrict__ scale) {
+    const int bn = blockIdx.x / blocks_k, bk = blockIdx.x % blocks_k;
+    const int col = bk * kBlk + threadIdx.x % kBlk, row0 = bn * kBlk + threadIdx.x / kBlk;
+    __shared__ float part[256];
+    float a = 0.f;
+    if (col < k)
+        for (int r = 0; r < kBlk && row0 + r < n; r += 2) a = fmaxf(a, fabsf(w[(size_t)(row0 + r) * k + col]));
+    part[threadIdx.x] = a;
+    __syncthreads();
+    for (int d = 128; d > 0; d >>= 1) {
+        if ((int)threadIdx.x < d) part[threadIdx.x] = fmaxf(part[threadIdx.x], part[threadIdx.x + d]);
+        __syncthreads();
+    }
+    const float s = scale_of(part[0]), inv = 1.f / s;
+    if (threadIdx.x == 0) scale[blockIdx.x] = s;
+    if (col < k)
+        for (int r = 0; r < kBlk && row0 + r < n; r += 2)
+            y[(size_t)(row0 + r) * k + col] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(w[(size_t)(row0 + r) * k + col] * inv, 0.f, 0, false);
+}
+
+// ---- the weights' layout ----
+// Tiles of 16 outputs x 128 values, a tile row's blocks one after the other: [tile][block][half of 64 values][lane][16 bytes], where lane l holds output l % 16
+// and values 64 half + 16 (l / 16) and on. A wave reads a tile as two runs of 1 KB. Gated weights alternate, 16 outputs of the gate, the same 16 of the other
+// projection, so that a wave has both sides of its outputs. Outputs and values that do not exist are zeros.
+__global__ __launch_bounds__(256) void pack_f8_kernel(const uint8_t* __restrict__ w, const uint8_t* __restrict__ w_up, int n, int k, int blocks_k, size_t pieces,
+                                                      v4i* __restrict__ packed) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= pieces) return;
+    const int lane = i % 64, half = i / 64 % 2;
+    const size_t tile_block = i / 128;
+    const int block = tile_block % blocks_k, tile = tile_block / blocks_k;
+    const uint8_t* const from = w_up && tile % 2 ? w_up : w;
+    const int row = (w_up ? tile / 2 : tile) * 16 + lane % 16, col = block * kBlk + half * 64 + lane / 16 * 16;
+    union { uint8_t b[16]; v4i v; } u;
+    for (int e = 0; e < 16; ++e) u.b[e] = row < n && col + e < k ? from[(size_t)row * k + col + e] : 0;
+    packed[i] = u.v;
+}
+
+// ---- the products ----
+struct F8Params {
+    const uint8_t* x;
+    const float* x_scale;
+    const uint8_t* w;
+    const float *w_scale, *w_scale_up;  // of a gated product: the gate's, the other projection's
+    const float *bias, *bias_up;
+    float* y_f32;
+    uint16_t* y_f16;
+    uint8_t* y_f8;
+    float* y_scale;
+    int m, n, k, x_stride, y_stride;
+    int blocks_k, tiles;  // blocks along k, tiles of 16 outputs (of both projections)
+    int gate;
+    int groups_n;  // groups side by side along the outputs
+};
+
+__device__ __forceinline__ float gated(int gate, float g, float u) {
+    switch (gate) {
+    case EXHIP_GATE_SILU: return g / (1.f + expf(-g)) * u;
+    case EXHIP_GATE_GELU: return 0.5f * g * (1.f + erff(g * 0.70710678118654752f)) * u;
+    case EXHIP_GATE_SIGMOID: return u / (1.f + expf(-g));
+    default: return (g > 0.f ? g : g != g ? g : 0.f) * u;
+    }
+}
+
+// Sixteen codes as halves, which hold every e4m3 value: piece s of four has the values 4 s .. 4 s + 3 of each of the lane's two runs.
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ v8h halves_of(int a, int b) {
+    const v2h p = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, false), q = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, true);
+    const v2h r = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, false), s = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, true);
+    return v8h{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
+}
+struct Halves {
+    v8h v[4];
+};
+__device__ __forceinline__ Halves halves_of(v4i lo, v4i hi) {
+    Halves h;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) h.v[s] = halves_of(lo[s], hi[s]);
+    return h;
+}
+// One block's products of 16 outputs and 16 rows.
+__device__ __forceinline__ v4f block_product(const Halves& w, const Halves& x) {
+    v4f c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.v[s], x.v[s], c, 0, 0, 0);
+    return c;
+}
+
+// Four neighbouring outputs of a row.
+__device__ __forceinline__ void store_outputs(const F8Params& p, int row, int j, v4f v) {
+    const size_t at = (size_t)row * p.y_stride + j;
+    const bool whole = j + 4 <= p.n && p.y_stride % 4 == 0;
+    if (p.y_f32) {
+        if (whole && ((uintptr_t)p.y_f32 & 15) == 0) *reinterpret_cast<v4f*>(p.y_f32 + at) = v;
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (j + e < p.n) p.y_f32[at + e] = v[e];
+    }
+    if (p.y_f16) {
+        const v4h h = __builtin_convertvector(v, v4h);
+        if (whole && ((uintptr_t)p.y_f16 & 7) == 0) *reinterpret_cast<v4h*>(p.y_f16 + at) = h;
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (j + e < p.n) p.y_f16[at + e] = exhip_f2h(v[e]);
+    }
+}
+
+// A group of WN x WK waves takes WN * TN tiles of outputs and 16 TM rows; wave (wn, wk) its own TN tiles and every WK-th block. The waves' sums are
+// added in the order of wk.
+template <int TN, int TM, int WN, int WK, bool GATED>
+__global__ __launch_bounds__(64 * WN * WK) void f8_rows_kernel(const F8Params p) {
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, wn = wave % WN, wk = wave / WN;
+    const int group_n = blockIdx.x % p.groups_n, tile0 = (group_n * WN + wn) * TN, row0 = blockIdx.x / p.groups_n * (16 * TM);
+    const int q = lane / 16, col = lane % 16;
+    const int rows = min(16 * TM, p.m - row0), tail = p.k % kBlk;
+    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.x) + (size_t)row0 * p.x_stride, 0,
+                                                                      (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16, kRsrcWord3);
+    v4f acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int t = 0; t < TM; ++t) acc[i][t] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int b = wk; b < p.blocks_k; b += WK) {
+        Halves x[TM];
+        float xs[TM];
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            const int row = 16 * t + col, off = row < rows ? row * p.x_stride + b * kBlk + q * 16 : 0x7fffffff - 64;
+            v4i lo = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xr, off, 0, 0));
+            v4i hi = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xr, off + 64, 0, 0));
+            if (tail && b == p.blocks_k - 1) {
+                lo &= keep_first(tail - q * 16);
+                hi &= keep_first(tail - 64 - q * 16);
+            }
+            x[t] = halves_of(lo, hi);
+            xs[t] = p.x_scale[(size_t)b * p.m + row0 + min(row, rows - 1)];
+        }
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+            const int tile = min(tile0 + i, p.tiles - 1);
+            const v4i* const wp = reinterpret_cast<const v4i*>(p.w) + ((size_t)tile * p.blocks_k + b) * 128 + lane;
+            const Halves w = halves_of(wp[0], wp[64]);
+            const int block_n = (GATED ? tile / 2 : tile) / (kBlk / 16);
+            const float ws = (GATED && tile % 2 ? p.w_scale_up : p.w_scale)[(size_t)block_n * p.blocks_k + b];
+#pragma unroll
+            for (int t = 0; t < TM; ++t) {
+                const v4f part = block_product(w, x[t]);
+                const float s = ws * xs[t];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][t][e] = __builtin_fmaf(part[e], s, acc[i][t][e]);
+            }
+        }
+    }
+    if constexpr (WK > 1) {
+        __shared__ v4f joined[WK - 1][WN][TN * TM][64];
+        if (wk > 0)
+#pragma unroll
+            for (int i = 0; i < TN * TM; ++i) joined[wk - 1][wn][i][lane] = acc[i / TM][i % TM];
+        __syncthreads();
+        if (wk == 0)
+#pragma unroll
+            for (int o = 0; o < WK - 1; ++o)
+#pragma unroll
+                for (int i = 0; i < TN * TM; ++i) acc[i / TM][i % TM] += joined[o][wn][i][lane];
+    }
+    if constexpr (!GATED) {
+        if (wk > 0) return;
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+            const int j = (tile0 + i) * 16 + q * 4;
+            if (j >= p.n) continue;
+            v4f bias = {0.f, 0.f, 0.f, 0.f};
+            if (p.bias)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bias[e] = p.bias[min(j + e, p.n - 1)];
+#pragma unroll
+            for (int t = 0; t < TM; ++t) {
+                const int row = 16 * t + col;
+                if (row < rows) store_outputs(p, row0 + row, j, acc[i][t] + bias);
+            }
+        }
+    } else {
+        static_assert(TN % 2 == 0, "both sides of an output are one wave's");
+        v4f h[TN / 2][TM];
+        if (wk == 0)
+#pragma unroll
+            for (int i = 0; i < TN / 2; ++i) {
+                const int j = (tile0 / 2 + i) * 16 + q * 4;
+#pragma unroll
+                for (int t = 0; t < TM; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float g = acc[2 * i][t][e], u = acc[2 * i + 1][t][e];
+                        if (p.bias) {
+                            g += p.bias[min(j + e, p.n - 1)];
+                            u += p.bias_up[min(j + e, p.n - 1)];
+                        }
+                        h[i][t][e] = j + e < p.n ? gated(p.gate, g, u) : 0.f;
+                    }
+                if (p.y_f16 && j < p.n)
+#pragma unroll
+                    for (int t = 0; t < TM; ++t)
+                        if (16 * t + col < rows) store_outputs(p, row0 + 16 * t + col, j, h[i][t]);
+            }
+        if (!p.y_f8) return;
+        // the group's outputs are one block of the result (WN * TN == 16): its largest value per row
+        __shared__ float most[WN][16 * TM];
+        float a[TM];
+        if (wk == 0)
+#pragma unroll
+            for (int t = 0; t < TM; ++t) {
+                a[t] = 0.f;
+#pragma unroll
+                for (int i = 0; i < TN / 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) a[t] = fmaxf(a[t], fabsf(h[i][t][e]));
+                a[t] = fmaxf(a[t], __shfl_xor(a[t], 16));
+                a[t] = fmaxf(a[t], __shfl_xor(a[t], 32));
+                if (q == 0) most[wn][16 * t + col] = a[t];
+            }
+        __syncthreads();
+        if (wk > 0) return;
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            const int row = 16 * t + col;
+            if (row >= rows) continue;
+            float top = most[0][row];
+#pragma unroll
+            for (int o = 1; o < WN; ++o) top = fmaxf(top, most[o][row]);
+            const float s = scale_of(top), r = 1.f / s;
+            if (wn == 0 && q == 0) p.y_scale[(size_t)group_n * p.m + row0 + row] = s;
+#pragma unroll
+            for (int i = 0; i < TN / 2; ++i) {
+                const int j = (tile0 / 2 + i) * 16 + q * 4;
+                const int code = four_codes(h[i][t][0] * r, h[i][t][1] * r, h[i][t][2] * r, h[i][t][3] * r);
+                uint8_t* const dst = p.y_f8 + (size_t)(row0 + row) * p.y_stride + j;
+                if (j + 4 <= p.n) *reinterpret_cast<int*>(dst) = code;
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (j + e < p.n) dst[e] = (uint8_t)(code >> (8 * e));
+            }
+        }
+    }
+}
+
+int blocks_of(int v) { return v / kBlk + (v % kBlk != 0); }
+bool aligned(const void* p, uintptr_t to) { return (uintptr_t)p % to == 0; }
+bool sizes_ok(int n, int k) { return n > 0 && k > 0 && n <= (1 << 24) && k <= kMostStride; }
+
+template <typename T>
+int quantize_rows(exhip_ctx* ctx, const char* name, const T* x, int x_stride, int m, int k, uint8_t* y, int y_stride, float* scale) {
+    EXHIP_REQUIRE(ctx && x && y && scale, "%s: NULL argument", name);
+    EXHIP_REQUIRE(m > 0 && k > 0 && k <= kMostStride && x_stride >= k, "%s: %d rows of %d values, %d apart: sizes are positive, a row at most 2^22 values", name, m, k, x_stride);
+    EXHIP_REQUIRE(y_stride >= k && y_stride % 16 == 0 && y_stride <= kMostStride && aligned(y, 16), "%s: rows of codes begin on 16 bytes and hold the row (stride %d)", name, y_stride);
+    EXHIP_REQUIRE(aligned(x, sizeof(T)) && aligned(scale, 4), "%s: an operand's address is not that of its type", name);
+    const exhip_on_device on(ctx->device);
+    EXHIP_CHECK(on.error);
+    hipLaunchKernelGGL(quantize_rows_kernel<T>, dim3(m / 16 + (m % 16 != 0), blocks_of(k)), dim3(256), 0, ctx->stream, x, x_stride, m, k, y, y_stride, scale);
+    EXHIP_LAUNCH_CHECK();
+    return 0;
+}
+
+int check_product(exhip_ctx* ctx, const char* name, const exhip_f8_desc* d, const uint8_t* x, const float* x_scale, const void* w, const float* w_scale, const float* bias) {
+    EXHIP_REQUIRE(ctx && d && x && x_scale && w && w_scale, "%s: NULL argument", name);
+    EXHIP_REQUIRE(d->m > 0 && sizes_ok(d->n_out, d->k_in), "%s: %d rows, %d outputs, %d inputs: sizes are positive, at most 2^24 outputs of 2^22 inputs", name, d->m, d->n_out, d->k_in);
+    EXHIP_REQUIRE(d->x_stride >= d->k_in && d->x_stride % 16 == 0 && d->x_stride <= kMostStride && aligned(x, 16),
+                  "%s: rows of codes begin on 16 bytes and hold the row (stride %d)", name, d->x_stride);
+    EXHIP_REQUIRE(d->y_stride >= d->n_out, "%s: result rows of %d values are %d apart", name, d->n_out, d->y_stride);
+    EXHIP_REQUIRE(aligned(w, 16) && aligned(x_scale, 4) && aligned(w_scale, 4) && aligned(bias, 4), "%s: an operand's address is not that of its type", name);
+    return 0;
+}
+
+F8Params params_of(const exhip_f8_desc* d, const uint8_t* x, const float* x_scale, const void* w, bool gated_product) {
+    F8Params p = {};
+    p.x = x;
+    p.x_scale = x_scale;
+    p.w = static_cast<const uint8_t*>(w);
+    p.m = d->m;
+    p.n = d->n_out;
+    p.k = d->k_in;
+    p.x_stride = d->x_stride;
+    p.y_stride = d->y_stride;
+    p.blocks_k = blocks_of(d->k_in);
+    p.tiles = (d->n_out + 15) / 16 * (gated_product ? 2 : 1);
+    return p;
+}
+
+template <int TN, int TM, int WN, int WK, bool GATED>
+int launch_rows(exhip_ctx* ctx, F8Params p) {
+    constexpr int tiles = TN * WN, rows = 16 * TM, threads = 64 * WN * WK;
+    p.groups_n = (p.tiles + tiles - 1) / tiles;
+    const long long groups = (long long)p.groups_n * (p.m / rows + (p.m % rows != 0));
+    EXHIP_REQUIRE(groups <= 0x7fffffff / threads, "inner product: %d rows of %d outputs are more than one launch takes", p.m, p.n);
+    const exhip_on_device on(ctx->device);
+    EXHIP_CHECK(on.error);
+    hipLaunchKernelGGL((f8_rows_kernel<TN, TM, WN, WK, GATED>), dim3((unsigned)groups), dim3(threads), 0, ctx->stream, p);
+    EXHIP_LAUNCH_CHECK();
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int exhip_quantize_rows_f32_to_f8(exhip_ctx* ctx, const float* x, int x_stride, int m, int k, uint8_t* y, int y_stride, float* scale) {
+    return quantize_rows(ctx, "exhip_quantize_rows_f32_to_f8", x, x_stride, m, k, y, y_stride, scale);
+}
+extern "C" int exhip_quantize_rows_f16_to_f8(exhip_ctx* ctx, const uint16_t* x, int x_stride, int m, int k, uint8_t* y, int y_stride, float* scale) {
+    return quantize_rows(ctx, "exhip_quantize_rows_f16_to_f8", x, x_stride, m, k, y, y_stride, scale);
+}
+
+extern "C" int exhip_quantize_blocks_f32_to_f8(exhip_ctx* ctx, const float* w, int n, int k, uint8_t* y, float* scale) {
+    EXHIP_REQUIRE(ctx && w && y && scale, "exhip_quantize_blocks_f32_to_f8: NULL argument");
+    EXHIP_REQUIRE(sizes_ok(n, k), "exhip_quantize_blocks_f32_to_f8: %d x %d: sizes are positive, at most 2^24 outputs of 2^22 inputs", n, k);
+    EXHIP_REQUIRE(aligned(w, 4) && aligned(scale, 4), "exhip_quantize_blocks_f32_to_f8: an operand's address is not that of its type");
+    const long long blocks = (long long)blocks_of(n) * blocks_of(k);
+    EXHIP_REQUIRE(blocks <= 0x7fffffff / 256, "exhip_quantize_blocks_f32_to_f8: %lld blocks are more than one launch takes", blocks);
+    const exhip_on_device on(ctx->device);
+    EXHIP_CHECK(on.error);
+    hipLaunchKernelGGL(quantize_blocks_kernel, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, w, n, k, blocks_of(k), y, scale);
+    EXHIP_LAUNCH_CHECK();
+    return 0;
+}
+
+extern "C" size_t exhip_f8_packed_bytes(int n_out, int k_in, int gated_weights) {
+    if (!sizes_ok(n_out, k_in)) {
+        exhip_set_error("exhip_f8_packed_bytes: %d outputs, %d inputs: sizes are positive, at most 2^24 outputs of 2^22 inputs", n_out, k_in);
+        return 0;
+    }
+    return (size_t)((n_out + 15) / 16) * (gated_weights ? 2 : 1) * blocks_of(k_in) * 2048;
+}
+
+extern "C" int exhip_f8_pack_weights(exhip_ctx* ctx, int n_out, int k_in, const uint8_t* w, const uint8_t* w_up, void* packed) {
+    EXHIP_REQUIRE(ctx && w && packed, "exhip_f8_pack_weights: NULL argument");
+    const size_t bytes = exhip_f8_packed_bytes(n_out, k_in, w_up != nullptr);
+    if (bytes == 0) return EXHIP_ERR_ARG;
+    EXHIP_REQUIRE(aligned(packed, 16), "exhip_f8_pack_weights: packed weights begin on 16 bytes");
+    const size_t pieces = bytes / 16, groups = (pieces + 255) / 256;
+    EXHIP_REQUIRE(groups <= 0x7fffffff / 256, "exhip_f8_pack_weights: %zu bytes are more than one launch takes", bytes);
+    const exhip_on_device on(ctx->device);
+    EXHIP_CHECK(on.error);
+    hipLaunchKernelGGL(pack_f8_kernel, dim3((unsigned)groups), dim3(256), 0, ctx->stream, w, w_up, n_out, k_in, blocks_of(k_in), pieces, static_cast<v4i*>(packed));
+    EXHIP_LAUNCH_CHECK();
+    return 0;
+}
+
+extern "C" int exhip_innerproduct_f8(exhip_ctx* ctx, const exhip_f8_desc* d, const uint8_t* x, const float* x_scale, const void* w_packed, const float* w_scale,
+                                     const float* bias, float* y_f32, uint16_t* y_f16) {
+    const int rc = check_product(ctx, "exhip_innerproduct_f8", d, x, x_scale, w_packed, w_scale, bias);
+    if (rc != 0) return rc;
+    EXHIP_REQUIRE((y_f32 || y_f16) && aligned(y_f32, 4) && aligned(y_f16, 2), "exhip_innerproduct_f8: no result, or one whose address is not that of its type");
+    F8Params p = params_of(d, x, x_scale, w_packed, false);
+    p.w_scale = w_scale;
+    p.bias = bias;
+    p.y_f32 = y_f32;
+    p.y_f16 = y_f16;
+    return p.m <= 16 ? launch_rows<4, 1, 1, 4, false>(ctx, p) : launch_rows<4, 4, 1, 2, false>(ctx, p);
+}
+
+extern "C" int exhip_innerproduct_gated_f8(exhip_ctx* ctx, const exhip_f8_desc* d, int gate, const uint8_t* x, const float* x_scale, const void* w_packed,
+                                           const float* w_scale_gate, const float* w_scale_up, const float* bias_gate, const float* bias_up, uint16_t* y_f16,
+                                           uint8_t* y_f8, float* y_scale) {
+    const char* const name = "exhip_innerproduct_gated_f8";
+    const int rc = check_product(ctx, name, d, x, x_scale, w_packed, w_scale_gate, bias_gate);
+    if (rc != 0) return rc;
+    EXHIP_REQUIRE(w_scale_up && aligned(w_scale_up, 4) && aligned(bias_up, 4) && !bias_gate == !bias_up, "%s: both projections have scales, and both a bias or neither", name);
+    EXHIP_REQUIRE(gate >= EXHIP_GATE_SILU && gate <= EXHIP_GATE_RELU, "%s: unknown activation %d", name, gate);
+    EXHIP_REQUIRE(!y_f16 != !y_f8 && !y_f8 == !y_scale, "%s: one result: halves, or codes and their scales", name);
+    EXHIP_REQUIRE(aligned(y_f16, 2) && aligned(y_scale, 4), "%s: a result's address is not that of its type", name);
+    EXHIP_REQUIRE(!y_f8 || (aligned(y_f8, 16) && d->y_stride % 16 == 0 && d->y_stride <= kMostStride), "%s: rows of codes begin on 16 bytes (stride %d)", name, d->y_stride);
+    F8Params p = params_of(d, x, x_scale, w_packed, true);
+    p.w_scale = w_scale_gate;
+    p.w_scale_up = w_scale_up;
+    p.bias = bias_gate;
+    p.bias_up = bias_up;
+    p.y_f16 = y_f16;
+    p.y_f8 = y_f8;
+    p.y_scale = y_scale;
+    p.gate = gate;
+    return p.m <= 16 ? launch_rows<4, 1, 4, 2, true>(ctx, p) : launch_rows<4, 4, 4, 1, true>(ctx, p);
+}

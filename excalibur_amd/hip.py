@@ -45,6 +45,8 @@ def lib():
         L.exhip_host_alloc.argtypes = [ctypes.c_size_t]
         L.exhip_host_free.restype = None
         L.exhip_host_free.argtypes = [ctypes.c_void_p]
+        L.exhip_f8_packed_bytes.restype = ctypes.c_size_t
+        L.exhip_log_probabilities_workspace.restype = ctypes.c_size_t
         _lib = L
     return _lib
 
@@ -113,6 +115,27 @@ class _Inside:
         self.ptr = ptr
 
 
+class View:
+    """Device memory that something else owns (another library's tensor), with a shape and dtype: what the calls below need of an operand. It has to
+    outlive the work queued on it."""
+
+    def __init__(self, address, shape, dtype):
+        self.ptr = ctypes.c_void_p(int(address))
+        self.shape = tuple(int(s) for s in shape)
+        self.dtype = np.dtype(dtype)
+
+    @property
+    def size(self):
+        return int(np.prod(self.shape, dtype=np.int64))
+
+
+class F8Desc(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_int) for k in ("m", "n_out", "k_in", "x_stride", "y_stride")]
+
+
+F8_BLOCK = 128  # values that share a scale
+
+
 class Event:
     def __init__(self):
         self.h = ctypes.c_void_p()
@@ -160,6 +183,11 @@ class Ctx:
     def array(self, a, dtype=None):
         a = np.ascontiguousarray(a, dtype if dtype is not None else a.dtype)
         return DevArray(self, a.shape, a.dtype).upload(a)
+
+    @staticmethod
+    def view(address, shape, dtype):
+        """An operand at a device address that the caller owns."""
+        return View(address, shape, dtype)
 
     # ---- layout / precision ----
     def quantize_nchw_to_nhwc_i8(self, x, fs, c_stride, fs_per_channel=None):
@@ -588,6 +616,75 @@ class Ctx:
         y = self.empty((m, n_out, 1, 1), np.uint16)
         _check(lib().exhip_innerproduct_f16(self.h, x.ptr, w.ptr, _ptr(bias), y.ptr, m, n_out, k_in))
         return y
+
+    # ---- inner products in 8-bit floating point ----
+    GATES = {"silu": 0, "gelu": 1, "sigmoid": 2, "relu": 3}
+
+    def quantize_rows_f8(self, x, k=None, y=None, scale=None):
+        """Rows x [m][stride] (float32, or halves as uint16) of k values: (codes [m][k up to 16], scales [k blocks][m])."""
+        m, stride = x.shape
+        k = stride if k is None else k
+        if y is None:
+            y = self.empty((m, pad_to(k, 16)), np.uint8)
+        if scale is None:
+            scale = self.empty((pad_to(k, F8_BLOCK) // F8_BLOCK, m), np.float32)
+        entry = lib().exhip_quantize_rows_f32_to_f8 if x.dtype == np.float32 else lib().exhip_quantize_rows_f16_to_f8
+        _check(entry(self.h, x.ptr, stride, m, k, y.ptr, y.shape[1], scale.ptr))
+        return y, scale
+
+    def quantize_blocks_f8(self, w):
+        """A float32 weight matrix [n][k]: (codes [n][k], scales [n blocks][k blocks])."""
+        n, k = w.shape
+        y = self.empty((n, k), np.uint8)
+        scale = self.empty((pad_to(n, F8_BLOCK) // F8_BLOCK, pad_to(k, F8_BLOCK) // F8_BLOCK), np.float32)
+        _check(lib().exhip_quantize_blocks_f32_to_f8(self.h, w.ptr, n, k, y.ptr, scale.ptr))
+        return y, scale
+
+    @staticmethod
+    def f8_packed_bytes(n_out, k_in, gated=False):
+        nbytes = lib().exhip_f8_packed_bytes(int(n_out), int(k_in), int(gated))
+        if nbytes == 0:
+            raise ExhipError(f"exhip_f8_packed_bytes: {lib().exhip_last_error().decode()}")
+        return nbytes
+
+    def pack_f8_weights(self, n_out, k_in, w, w_up=None, packed=None):
+        """Codes [n_out][k_in] in the product's order; with w_up those of a gated product, w the one in front of the activation."""
+        if packed is None:
+            packed = self.empty((self.f8_packed_bytes(n_out, k_in, w_up is not None),), np.uint8)
+        _check(lib().exhip_f8_pack_weights(self.h, n_out, k_in, w.ptr, _ptr(w_up), packed.ptr))
+        return packed
+
+    @staticmethod
+    def f8_desc(m, n_out, k_in, x_stride=None, y_stride=None):
+        return F8Desc(m, n_out, k_in, pad_to(k_in, 16) if x_stride is None else x_stride, n_out if y_stride is None else y_stride)
+
+    def innerproduct_f8(self, d, x, x_scale, w, w_scale, bias=None, y_f32=None, y_f16=None):
+        _check(lib().exhip_innerproduct_f8(self.h, ctypes.byref(d), x.ptr, x_scale.ptr, w.ptr, w_scale.ptr, _ptr(bias), _ptr(y_f32), _ptr(y_f16)))
+
+    def innerproduct_gated_f8(self, d, x, x_scale, w, w_scale_gate, w_scale_up, gate="silu", bias_gate=None, bias_up=None, y_f16=None, y_f8=None, y_scale=None):
+        _check(lib().exhip_innerproduct_gated_f8(self.h, ctypes.byref(d), self.GATES[gate], x.ptr, x_scale.ptr, w.ptr, w_scale_gate.ptr, w_scale_up.ptr,
+                                                 _ptr(bias_gate), _ptr(bias_up), _ptr(y_f16), _ptr(y_f8), _ptr(y_scale)))
+
+    # ---- answers ----
+    @staticmethod
+    def log_probabilities_workspace(m, c, top=0):
+        nbytes = lib().exhip_log_probabilities_workspace(int(m), int(c), int(top))
+        if nbytes == 0:
+            raise ExhipError(f"exhip_log_probabilities_workspace: {lib().exhip_last_error().decode()}")
+        return nbytes
+
+    def log_probabilities(self, x, c=None, ids=None, top=0, log_p=None, entropy=None, top_ids=None, top_log_p=None, workspace=None):
+        """Of rows x [m][stride] (float32, or halves as uint16) of c values: the log probabilities of ids [m][n], the entropy, the `top` largest classes and
+        their log probabilities, into the given arrays."""
+        m, stride = x.shape
+        c = stride if c is None else c
+        own = self.empty((self.log_probabilities_workspace(m, c, top),), np.uint8) if workspace is None else None
+        entry = lib().exhip_log_probabilities_f32 if x.dtype == np.float32 else lib().exhip_log_probabilities_f16
+        rc = entry(self.h, x.ptr, stride, m, c, _ptr(ids), ids.shape[1] if ids is not None else 0, _ptr(log_p), _ptr(entropy), top, _ptr(top_ids),
+                   _ptr(top_log_p), (workspace or own).ptr)
+        if own is not None:
+            own.free()
+        _check(rc)
 
     def stem_f16(self, d, x, mean, factor, wp, bias, y):
         """The status: 0, or EXHIP_ERR_UNSUPPORTED where the layers run by themselves."""

@@ -527,6 +527,61 @@ int exhip_innerproduct_f32(exhip_ctx* ctx, const float* x, const float* w, const
 /* the same on half rows, as the fp16 wrapper runs it (include/Excalibur/operation.hpp:204-266): sums in float32, results rounded once */
 int exhip_innerproduct_f16(exhip_ctx* ctx, const uint16_t* x, const float* w, const float* bias, uint16_t* y, int m, int n_out, int k_in);
 
+/* ---- inner products in 8-bit floating point (no counterpart in the reference) ---- */
+/* Operands are e4m3 codes (one sign, four exponent and three fraction bits, largest value 448, 0x7F / 0xFF are NaN) with float32 scales: one for each
+ * 128 values of an input row, scale[k block][row], and one for each 128 x 128 block of a weight matrix, scale[n block][k block]. The last blocks
+ * hold what is left. A code stands for its value times its block's scale. Codes' rows begin on 16 bytes (base and stride); what lies between a
+ * row's end and its stride is neither used nor written. */
+#define EXHIP_F8_BLOCK 128
+/* Rows x[m][k] (row stride x_stride elements, at least k) to codes y (row stride y_stride bytes) and scales [ceil(k / 128)][m]:
+ * scale = max(max |x| / 448, 2^-100), code = e4m3(x * (1 / scale)), to nearest even. A NaN becomes a NaN code and does not count in its block's
+ * maximum; a block with an infinity has an infinite scale. */
+int exhip_quantize_rows_f32_to_f8(exhip_ctx* ctx, const float* x, int x_stride, int m, int k, uint8_t* y, int y_stride, float* scale);
+int exhip_quantize_rows_f16_to_f8(exhip_ctx* ctx, const uint16_t* x, int x_stride, int m, int k, uint8_t* y, int y_stride, float* scale);
+/* A float32 weight matrix w[n][k] to codes y[n][k] (dense, like operation_innerproduct's weights, src/Excalibur/operation_innerproduct.cpp:176-224) and
+ * scales [ceil(n / 128)][ceil(k / 128)], a block at a time by the same rule. */
+int exhip_quantize_blocks_f32_to_f8(exhip_ctx* ctx, const float* w, int n, int k, uint8_t* y, float* scale);
+/* Codes w[n_out][k_in] in the order the product reads them, made on the device: exhip_f8_packed_bytes() bytes (0 for bad sizes) at `packed`, on 16 bytes.
+ * With w_up both projections of a gated product, w the one that goes through the activation; `gated` tells the size. */
+size_t exhip_f8_packed_bytes(int n_out, int k_in, int gated);
+int exhip_f8_pack_weights(exhip_ctx* ctx, int n_out, int k_in, const uint8_t* w, const uint8_t* w_up, void* packed);
+typedef struct exhip_f8_desc {
+    int m, n_out, k_in; /* rows, outputs, inputs of a row */
+    int x_stride;       /* bytes between the input's rows, at least k_in, a multiple of 16 */
+    int y_stride;       /* elements between the results' rows, at least n_out; a multiple of 16 for codes */
+} exhip_f8_desc;
+/* y[r][j] = bias[j] + sum over blocks b of x_scale[b][r] * w_scale[j / 128][b] * (the codes' products of that block), sums in float32, rounded once.
+ * bias may be NULL; any non-NULL result is written, columns [0, n_out) only. Products of one row take their time from reading the weights, large
+ * ones from the matrix cores. */
+int exhip_innerproduct_f8(exhip_ctx* ctx, const exhip_f8_desc* d, const uint8_t* x, const float* x_scale, const void* w_packed, const float* w_scale,
+                          const float* bias, float* y_f32, uint16_t* y_f16);
+/* A feed-forward block's first half in one launch: h = act(x w_gate + bias_gate) * (x w_up + bias_up) with act(v) = v / (1 + exp(-v)),
+ * v (1 + erf(v / sqrt 2)) / 2, 1 / (1 + exp(-v)) or max(v, 0). The result is h as halves (y_f16), or the codes (y_f8) and scales (y_scale, both or neither)
+ * that exhip_quantize_rows_f32_to_f8 makes of h in float32; one of the two forms. Biases: both or neither. */
+#define EXHIP_GATE_SILU 0
+#define EXHIP_GATE_GELU 1
+#define EXHIP_GATE_SIGMOID 2
+#define EXHIP_GATE_RELU 3
+int exhip_innerproduct_gated_f8(exhip_ctx* ctx, const exhip_f8_desc* d, int gate, const uint8_t* x, const float* x_scale, const void* w_packed,
+                                const float* w_scale_gate, const float* w_scale_up, const float* bias_gate, const float* bias_up, uint16_t* y_f16,
+                                uint8_t* y_f8, float* y_scale);
+
+/* ---- what a classifier or a language model answers with (no counterpart in the reference; exhip_softmax_channels_f32 stores all of a row) ---- */
+/* For rows x[m][c] (row stride x_stride elements, at least c; any alignment of the element type), in one reading of them:
+ * log_p[m][n_ids]: x[id] - log(sum exp x) of the classes ids[m][n_ids]; a negative id asks nothing and gives 0, one from c on gives NaN;
+ * entropy[m]: -sum p log p, with classes of no probability left out;
+ * top_ids[m][top], top_log_p[m][top]: the largest x in falling order, equal ones by their index, and their log probabilities.
+ * -infinity masks a class. A row with nothing else has log probabilities of -infinity and entropy 0. In a row with a NaN or a +infinity all of these
+ * values are NaN (those of negative ids are 0), and NaN stands above every number in top_ids. log_p, entropy and the top pair may be NULL (with n_ids = 0,
+ * and top = 0). top is at most 64 and at most c. `workspace` (on 16 bytes) is the caller's, exhip_log_probabilities_workspace() bytes of it (0 for bad
+ * sizes); calls that may overlap need one each. */
+#define EXHIP_LOG_PROBABILITIES_TOP 64
+size_t exhip_log_probabilities_workspace(int m, int c, int top);
+int exhip_log_probabilities_f32(exhip_ctx* ctx, const float* x, int x_stride, int m, int c, const int32_t* ids, int n_ids, float* log_p, float* entropy,
+                                int top, int32_t* top_ids, float* top_log_p, void* workspace);
+int exhip_log_probabilities_f16(exhip_ctx* ctx, const uint16_t* x, int x_stride, int m, int c, const int32_t* ids, int n_ids, float* log_p, float* entropy,
+                                int top, int32_t* top_ids, float* top_log_p, void* workspace);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,115 @@
+"""e4m3 codes and the operators that work on them, in 64 bits: what the inner products in 8-bit floating point are tested against.
+
+Error bounds (all per value, |.| summed over what a result sums):
+* a block's 128 products are exact; their sum in float32 is off by at most 128 steps of 2^-23 (a chain of adds, each off by less than one unit of the
+  last place, as an adder that cuts off would be) relative to the sum of absolute values; the multiply-add with the scales adds three roundings a block,
+  the join of waves and the bias fewer than 64 in all: `sum_bound`.
+* a rounding to halves is off by 2^-11 relative, or 2^-25 below the normal range; one to e4m3 by 2^-4 relative, or half a step of 2^-9 times the scale.
+* an activation's value is off by less than 2^-21 max(|v|, 1) (exp and erf within two units, a division, three products), and changes by at most 1.13
+  times what its argument does."""
+import numpy as np
+
+BLOCK = 128
+U = 2.0 ** -23
+
+
+def _values():
+    v = np.empty(256)
+    for code in range(256):
+        e, f = code >> 3 & 15, code & 7
+        mag = np.nan if (e, f) == (15, 7) else (f / 8) * 2.0 ** -6 if e == 0 else (1 + f / 8) * 2.0 ** (e - 7)
+        v[code] = -mag if code & 128 else mag
+    return v
+
+
+VALUES = _values()
+
+
+def encode(v):
+    """float64 to codes, to nearest even; beyond 448 by less than half a step stays 448; NaN is 0x7F (its sign is the input's)."""
+    v = np.asarray(v, np.float64)
+    mag = np.abs(v)
+    step = 2.0 ** (np.floor(np.log2(np.maximum(np.where(np.isfinite(mag), mag, 1.0), 2.0 ** -6))) - 3)
+    r = np.rint(np.where(np.isfinite(mag), mag, 0.0) / step) * step
+    code = np.searchsorted(VALUES[:127], r)  # the non-negative values in rising order
+    code = np.where(np.isfinite(mag), code, 0x7F).astype(np.uint8)
+    return code | (np.signbit(v).astype(np.uint8) << 7)
+
+
+def blocks(v):
+    return -(-v // BLOCK)
+
+
+def quantize_rows(x):
+    """(codes, scales [blocks][m]) of float32 rows, in float32 as it is defined."""
+    m, k = x.shape
+    wide = np.zeros((m, blocks(k) * BLOCK), np.float32)
+    wide[:, :k] = x
+    wide = wide.reshape(m, -1, BLOCK)
+    with np.errstate(all="ignore"):
+        most = np.fmax.reduce(np.abs(wide), axis=2, initial=np.float32(0))
+        scale = np.maximum(most / np.float32(448), np.float32(2.0 ** -100)).astype(np.float32)
+        codes = encode(wide * (np.float32(1) / scale)[:, :, None])
+    return codes.reshape(m, -1)[:, :k], np.ascontiguousarray(scale.T)
+
+
+def quantize_weights(w):
+    n, k = w.shape
+    wide = np.zeros((blocks(n) * BLOCK, blocks(k) * BLOCK), np.float32)
+    wide[:n, :k] = w
+    wide = wide.reshape(blocks(n), BLOCK, blocks(k), BLOCK)
+    scale = np.maximum(np.abs(wide).max(axis=(1, 3)) / np.float32(448), np.float32(2.0 ** -100)).astype(np.float32)
+    codes = encode(wide * (np.float32(1) / scale)[:, None, :, None])
+    return np.ascontiguousarray(codes.reshape(blocks(n) * BLOCK, -1)[:n, :k]), scale
+
+
+def rows_of(codes, scale):
+    return VALUES[codes] * np.repeat(scale.T.astype(np.float64), BLOCK, 1)[:, :codes.shape[1]]
+
+
+def weights_of(codes, scale):
+    n, k = codes.shape
+    return VALUES[codes] * np.repeat(np.repeat(scale.astype(np.float64), BLOCK, 0)[:n], BLOCK, 1)[:, :k]
+
+
+def product(x, x_scale, w, w_scale, bias=None):
+    """(y, bound on a float32 result's error) in 64 bits."""
+    a, b = rows_of(x, x_scale), weights_of(w, w_scale)
+    y, size = a @ b.T, np.abs(a) @ np.abs(b).T
+    if bias is not None:
+        y, size = y + bias, size + np.abs(bias)
+    return y, sum_bound(size, x.shape[1])
+
+
+def sum_bound(size, k):
+    return (BLOCK + 3 * blocks(k) + 64) * U * size
+
+
+def gate(name, v):
+    with np.errstate(over="ignore"):
+        sig = 1 / (1 + np.exp(-v))
+    if name == "silu":
+        return v * sig
+    if name == "sigmoid":
+        return sig
+    if name == "relu":
+        return np.maximum(v, 0)
+    from math import erf
+    return 0.5 * v * (1 + np.vectorize(erf)(v / np.sqrt(2)))
+
+
+def gated(name, g, g_bound, u, u_bound):
+    a = gate(name, g)
+    a_bound = 1.13 * g_bound + 2.0 ** -21 * np.maximum(np.abs(g), 1)
+    h = a * u
+    return h, a_bound * np.abs(u) + np.abs(a) * u_bound + a_bound * u_bound + 2.0 ** -22 * np.abs(h)
+
+
+def half_bound(y, bound):
+    return bound + (np.abs(y) + bound) * 2.0 ** -11 + 2.0 ** -25
+
+
+def code_bound(h, bound, scale):
+    """Of what codes with `scale` [blocks][m] stand for, against h."""
+    s = np.repeat(scale.T.astype(np.float64), BLOCK, 1)[:, :h.shape[1]]
+    return (bound + (np.abs(h) + bound) * 2.0 ** -4 + s * 2.0 ** -10) * (1 + 2.0 ** -20)

@@ -1,0 +1,129 @@
+"""What the 8-bit floating point and log probability entry points refuse: checked on the host, before a device is asked for anything."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from tests import f8ref
+
+ERR_ARG = 10001
+
+
+def _lib():
+    from excalibur_amd import hip
+    return hip.lib()
+
+
+def _status(entry, *args):
+    """For operands that are addresses only: what passes the checks ends in the runtime's own error where there is no GPU."""
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("operands are addresses only")
+    ctx = ctypes.create_string_buffer(4096)
+    return entry(ctx, *[ctypes.c_void_p(a) if isinstance(a, int) and a >= 0x10000 else a for a in args])
+
+
+X, Y, S, W, S2, B, B2, I, P, E = (0x10000 * (i + 1) for i in range(10))
+
+
+@pytest.mark.parametrize("name", ["exhip_quantize_rows_f32_to_f8", "exhip_quantize_rows_f16_to_f8"])
+def test_quantize_rows_refusals(name):
+    entry = getattr(_lib(), name)
+    good = [X, 100, 3, 100, Y, 112, S]
+    assert _status(entry, *good) not in (0, ERR_ARG)
+    for at, bad in ((0, None), (4, None), (6, None), (1, 99), (2, 0), (2, -1), (3, 0), (5, 96), (5, 120), (4, Y + 8), (0, X + 1), (6, S + 2), (5, 1 << 23)):
+        args = list(good)
+        args[at] = bad
+        assert _status(entry, *args) == ERR_ARG, (at, bad)
+
+
+def test_quantize_blocks_and_pack_refusals():
+    L = _lib()
+    assert _status(L.exhip_quantize_blocks_f32_to_f8, X, 5, 7, Y, S) not in (0, ERR_ARG)
+    for args in ((None, 5, 7, Y, S), (X, 0, 7, Y, S), (X, 5, -7, Y, S), (X, 5, 7, None, S), (X, 5, 7, Y, S + 1), (X + 2, 5, 7, Y, S), (X, 1 << 24, 1 << 22, Y, S)):
+        assert _status(L.exhip_quantize_blocks_f32_to_f8, *args) == ERR_ARG, args
+    assert _status(L.exhip_f8_pack_weights, 5, 7, X, W, Y) not in (0, ERR_ARG)
+    for args in ((5, 7, None, W, Y), (0, 7, X, None, Y), (5, 7, X, W, None), (5, 7, X, W, Y + 8), (5, (1 << 22) + 1, X, None, Y), (1 << 24, 1 << 22, X, None, Y)):
+        assert _status(L.exhip_f8_pack_weights, *args) == ERR_ARG, args
+    assert L.exhip_f8_packed_bytes(17, 129, 0) == 2 * 2 * 2048 and L.exhip_f8_packed_bytes(17, 129, 1) == 2 * 2 * 2 * 2048
+    assert L.exhip_f8_packed_bytes(0, 5, 0) == 0 and L.exhip_f8_packed_bytes(5, -1, 0) == 0
+    assert L.exhip_f8_packed_bytes(1 << 24, 1 << 22, 0) == 1 << 46
+
+
+def _desc(**change):
+    from excalibur_amd import hip
+    return ctypes.byref(hip.F8Desc(*[{**dict(m=3, n_out=40, k_in=100, x_stride=112, y_stride=48), **change}[f] for f, _ in hip.F8Desc._fields_]))
+
+
+BAD_DESC = (dict(m=0), dict(n_out=0), dict(k_in=0), dict(m=-1), dict(x_stride=96), dict(x_stride=120), dict(y_stride=39), dict(x_stride=1 << 23), dict(k_in=1 << 23, x_stride=1 << 23),
+            dict(m=1 << 30, n_out=1 << 24, y_stride=1 << 24))
+
+
+def test_product_refusals():
+    entry = _lib().exhip_innerproduct_f8
+    good = [X, S, W, S2, B, Y, None]
+    assert _status(entry, _desc(), *good) not in (0, ERR_ARG)
+    assert _status(entry, _desc(), X, S, W, S2, None, None, Y) not in (0, ERR_ARG)
+    for change in BAD_DESC:
+        assert _status(entry, _desc(**change), *good) == ERR_ARG, change
+    assert _status(entry, None, *good) == ERR_ARG
+    for at, bad in ((0, None), (1, None), (2, None), (3, None), (5, None), (0, X + 8), (1, S + 1), (2, W + 8), (3, S2 + 2), (4, B + 1), (5, Y + 2), (6, Y + 1)):
+        args = list(good)
+        args[at] = bad
+        assert _status(entry, _desc(), *args) == ERR_ARG, (at, bad)
+
+
+def test_gated_product_refusals():
+    entry = _lib().exhip_innerproduct_gated_f8
+    good = [0, X, S, W, S2, S2, B, B2, Y, None, None]
+    codes = [0, X, S, W, S2, S2, B, B2, None, Y, P]
+    assert _status(entry, _desc(), *good) not in (0, ERR_ARG)
+    assert _status(entry, _desc(), *codes) not in (0, ERR_ARG)
+    for change in BAD_DESC:
+        assert _status(entry, _desc(**change), *good) == ERR_ARG, change
+    assert _status(entry, _desc(y_stride=50), *codes) == ERR_ARG  # codes begin on 16 bytes
+    for at, bad in ((0, -1), (0, 4), (1, None), (2, None), (3, None), (4, None), (5, None), (6, None), (7, None), (8, None), (8, Y + 1), (9, P), (10, P), (7, B2 + 2)):
+        args = list(good)
+        args[at] = bad
+        assert _status(entry, _desc(), *args) == ERR_ARG, (at, bad)
+    for at, bad in ((8, E), (9, None), (10, None), (9, Y + 8), (10, P + 2)):
+        args = list(codes)
+        args[at] = bad
+        assert _status(entry, _desc(), *args) == ERR_ARG, (at, bad)
+
+
+@pytest.mark.parametrize("name", ["exhip_log_probabilities_f32", "exhip_log_probabilities_f16"])
+def test_log_probability_refusals(name):
+    entry = getattr(_lib(), name)
+    #       x, x_stride, m, c, ids, n_ids, log_p, entropy, top, top_ids, top_log_p, workspace
+    good = [X, 100, 3, 100, I, 2, P, E, 5, Y, S, W]
+    assert _status(entry, *good) not in (0, ERR_ARG)
+    for at, bad in ((0, None), (0, X + 1), (1, 99), (2, 0), (3, 0), (3, -5), (4, None), (5, -1), (5, 0), (6, None), (8, -1), (8, 0), (8, 65), (9, None), (10, None), (11, None), (11, W + 8),
+                    (4, I + 2), (6, P + 1), (7, E + 2), (9, Y + 1), (10, S + 3)):
+        args = list(good)
+        args[at] = bad
+        assert _status(entry, *args) == ERR_ARG, (at, bad)
+    assert _status(entry, X, 100, 3, 100, None, 0, None, None, 0, None, None, W) == ERR_ARG  # nothing is asked
+    assert _status(entry, X, 100, 3, 4, None, 0, None, E, 5, Y, S, W) == ERR_ARG  # more classes than there are
+    L = _lib()
+    for args in ((0, 5, 0), (5, 0, 0), (5, 5, 6), (5, 100, 65), (5, 5, -1)):
+        assert L.exhip_log_probabilities_workspace(*args) == 0, args
+    assert L.exhip_log_probabilities_workspace(1, 1, 0) > 0
+
+
+def test_a_null_context_is_refused():
+    L = _lib()
+    p = ctypes.c_void_p(0x10000)
+    assert L.exhip_quantize_rows_f32_to_f8(None, p, 16, 1, 16, p, 16, p) == ERR_ARG
+    assert L.exhip_f8_pack_weights(None, 1, 1, p, None, p) == ERR_ARG
+    assert L.exhip_innerproduct_f8(None, _desc(), p, p, p, p, None, p, None) == ERR_ARG
+    assert L.exhip_log_probabilities_f32(None, p, 16, 1, 16, None, 0, None, p, 0, None, None, p) == ERR_ARG
+
+
+def test_codes_of_the_oracle():
+    """The oracle's own codes: every value is its own code, ties go to the even one, the borders of the format."""
+    finite = ~np.isnan(f8ref.VALUES)
+    codes = np.arange(256, dtype=np.uint8)[finite]
+    assert np.array_equal(f8ref.encode(f8ref.VALUES[finite]), codes)
+    assert f8ref.VALUES.max(initial=0, where=finite) == 448 and f8ref.VALUES[1] == 2.0 ** -9 and f8ref.VALUES[8] == 2.0 ** -6
+    assert f8ref.encode([2.0 ** -10, 3 * 2.0 ** -10, 17, 19, 460, -17, np.nan]).tolist() == [0, 2, 0x58, 0x5A, 0x7E, 0xD8, 0x7F]
