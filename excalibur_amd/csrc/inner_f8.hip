@@ -20,7 +20,8 @@ constexpr int kBlk = EXHIP_F8_BLOCK;
 constexpr int kRsrcWord3 = 0x00020000;
 constexpr float kLargest = 448.f;                   // of e4m3
 constexpr float kLeastScale = 0x1p-100f;            // keeps 1 / scale finite and blocks of zeros at zero
-constexpr int kMostStride = 1 << 22;                // of a row of codes: offsets inside a tile's rows stay below 2^31
+constexpr int kMostStride = 1 << 22;                // of a row of codes: offsets inside the 256 rows at most of a group stay below kNoRow
+constexpr int kNoRow = 0x7f000000;                  // beyond every group's rows: loads there give zeros
 
 // What the last block's codes of a row are ANDed with: `left` values of 16 are the row's own.
 __device__ __forceinline__ v4i keep_first(int left) {
@@ -204,6 +205,93 @@ __device__ __forceinline__ void store_outputs(const F8Params& p, int row, int j,
     }
 }
 
+// A wave's sums, TN tiles of outputs from tile0 on and TM tiles of rows from row0 on, of which `rows` exist.
+template <int TN, int TM>
+__device__ __forceinline__ void write_outputs(const F8Params& p, const v4f (&acc)[TN][TM], int tile0, int row0, int rows, int lane) {
+    const int q = lane / 16, col = lane % 16;
+#pragma unroll
+    for (int i = 0; i < TN; ++i) {
+        const int j = (tile0 + i) * 16 + q * 4;
+        if (j >= p.n) continue;
+        v4f bias = {0.f, 0.f, 0.f, 0.f};
+        if (p.bias)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bias[e] = p.bias[min(j + e, p.n - 1)];
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            const int row = 16 * t + col;
+            if (row < rows) store_outputs(p, row0 + row, j, acc[i][t] + bias);
+        }
+    }
+}
+
+// The same of a gated product, whose tiles alternate. Quantized results take the whole group: its WN waves side by side hold one block of the result
+// (WN * TN == 16), WM such rows of waves stand one behind the other. `mine`: this wave has sums to write.
+template <int TN, int TM, int WN, int WM>
+__device__ __forceinline__ void write_gated(const F8Params& p, const v4f (&acc)[TN][TM], int tile0, int group_n, int wn, int wm, int row0, int rows, int lane, bool mine) {
+    static_assert(TN % 2 == 0, "both sides of an output are one wave's");
+    const int q = lane / 16, col = lane % 16;
+    v4f h[TN / 2][TM];
+    if (mine)
+#pragma unroll
+        for (int i = 0; i < TN / 2; ++i) {
+            const int j = (tile0 / 2 + i) * 16 + q * 4;
+            v4f bias = {0.f, 0.f, 0.f, 0.f}, bias_up = bias;
+            if (p.bias)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    bias[e] = p.bias[min(j + e, p.n - 1)];
+                    bias_up[e] = p.bias_up[min(j + e, p.n - 1)];
+                }
+#pragma unroll
+            for (int t = 0; t < TM; ++t) {
+                const v4f g = acc[2 * i][t] + bias, u = acc[2 * i + 1][t] + bias_up;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) h[i][t][e] = j + e < p.n ? gated(p.gate, g[e], u[e]) : 0.f;
+                if (p.y_f16 && j < p.n && 16 * t + col < rows) store_outputs(p, row0 + 16 * t + col, j, h[i][t]);
+            }
+        }
+    if constexpr (WN * TN == 16) {
+        if (!p.y_f8) return;
+        __shared__ float most[WM][WN][16 * TM];
+        if (mine)
+#pragma unroll
+            for (int t = 0; t < TM; ++t) {
+                float a = 0.f;
+#pragma unroll
+                for (int i = 0; i < TN / 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) a = fmaxf(a, fabsf(h[i][t][e]));
+                a = fmaxf(a, __shfl_xor(a, 16));
+                a = fmaxf(a, __shfl_xor(a, 32));
+                if (q == 0) most[wm][wn][16 * t + col] = a;
+            }
+        __syncthreads();
+        if (!mine) return;
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            const int row = 16 * t + col;
+            if (row >= rows) continue;
+            float top = most[wm][0][row];
+#pragma unroll
+            for (int o = 1; o < WN; ++o) top = fmaxf(top, most[wm][o][row]);
+            const float s = scale_of(top), r = 1.f / s;
+            if (wn == 0 && q == 0) p.y_scale[(size_t)group_n * p.m + row0 + row] = s;
+#pragma unroll
+            for (int i = 0; i < TN / 2; ++i) {
+                const int j = (tile0 / 2 + i) * 16 + q * 4;
+                const int code = four_codes(h[i][t][0] * r, h[i][t][1] * r, h[i][t][2] * r, h[i][t][3] * r);
+                uint8_t* const dst = p.y_f8 + (size_t)(row0 + row) * p.y_stride + j;
+                if (j + 4 <= p.n) *reinterpret_cast<int*>(dst) = code;
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (j + e < p.n) dst[e] = (uint8_t)(code >> (8 * e));
+            }
+        }
+    }
+}
+
 // A group of WN x WK waves takes WN * TN tiles of outputs and 16 TM rows; wave (wn, wk) its own TN tiles and every WK-th block. The waves' sums are
 // added in the order of wk.
 template <int TN, int TM, int WN, int WK, bool GATED>
@@ -224,7 +312,7 @@ __global__ __launch_bounds__(64 * WN * WK) void f8_rows_kernel(const F8Params p)
         float xs[TM];
 #pragma unroll
         for (int t = 0; t < TM; ++t) {
-            const int row = 16 * t + col, off = row < rows ? row * p.x_stride + b * kBlk + q * 16 : 0x7fffffff - 64;
+            const int row = 16 * t + col, off = row < rows ? row * p.x_stride + b * kBlk + q * 16 : kNoRow;
             v4i lo = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xr, off, 0, 0));
             v4i hi = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xr, off + 64, 0, 0));
             if (tail && b == p.blocks_k - 1) {
@@ -263,84 +351,129 @@ __global__ __launch_bounds__(64 * WN * WK) void f8_rows_kernel(const F8Params p)
                 for (int i = 0; i < TN * TM; ++i) acc[i / TM][i % TM] += joined[o][wn][i][lane];
     }
     if constexpr (!GATED) {
-        if (wk > 0) return;
+        if (wk == 0) write_outputs<TN, TM>(p, acc, tile0, row0, rows, lane);
+    } else {
+        write_gated<TN, TM, WN, 1>(p, acc, tile0, group_n, wn, 0, row0, rows, lane, wk == 0);
+    }
+}
+
+// Many rows: a group of WN x WM waves takes 64 WN outputs and 16 TM WM rows. A block's rows of the input become halves once for the group, on their way
+// into LDS (two buffers); a wave's weights go from L2 straight into its registers, the next block's while this one's are used.
+template <int WN, int WM, int TM, bool GATED>
+__global__ __launch_bounds__(64 * WN * WM, 2) void f8_tile_kernel(const F8Params p) {
+    constexpr int TN = 4, kRows = 16 * TM * WM, kThreads = 64 * WN * WM, kItems = kRows * 4 / kThreads;
+    static_assert(kItems * kThreads == kRows * 4, "every thread stages the same");
+    // [buffer][row][16 pieces of 16 bytes]: piece 4 s + q of a row is halves_of()'s piece s of lanes of quarter q, at place (4 s + q) ^ (row % 16), so that
+    // eight neighbouring rows' pieces lie in different banks
+    __shared__ v4i staged[2][kRows][16];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, wn = wave % WN, wm = wave / WN;
+    const int q = lane / 16, col = lane % 16;
+    const int group_n = blockIdx.x % p.groups_n, tile0 = (group_n * WN + wn) * TN, row0 = blockIdx.x / p.groups_n * kRows;
+    const int rows = min(kRows, p.m - row0), tail = p.k % kBlk;
+    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.x) + (size_t)row0 * p.x_stride, 0,
+                                                                      (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16, kRsrcWord3);
+    const v4i* wp[TN];
+#pragma unroll
+    for (int i = 0; i < TN; ++i) wp[i] = reinterpret_cast<const v4i*>(p.w) + (size_t)min(tile0 + i, p.tiles - 1) * p.blocks_k * 128 + lane;
+    const int block_n = min(GATED ? tile0 / 2 : tile0, (p.n - 1) / 16) / (kBlk / 16);
+    const float* const ws = p.w_scale + (size_t)block_n * p.blocks_k;
+    const float* const ws_up = GATED ? p.w_scale_up + (size_t)block_n * p.blocks_k : nullptr;
+    const float* xs[TM];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) xs[t] = p.x_scale + row0 + min((wm * TM + t) * 16 + col, rows - 1);
+
+    int off[kItems], at_row[kItems];
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+        const int item = i * kThreads + threadIdx.x;
+        at_row[i] = item / 4;
+        off[i] = at_row[i] < rows ? at_row[i] * p.x_stride + item % 4 * 16 : kNoRow;
+    }
+    const int sq = threadIdx.x % 4;
+    v4i codes[kItems][2];
+    auto request = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            codes[i][0] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xr, off[i] + b * kBlk, 0, 0));
+            codes[i][1] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xr, off[i] + b * kBlk + 64, 0, 0));
+        }
+    };
+    auto stage = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            v4i lo = codes[i][0], hi = codes[i][1];
+            if (tail && b == p.blocks_k - 1) {
+                lo &= keep_first(tail - sq * 16);
+                hi &= keep_first(tail - 64 - sq * 16);
+            }
+            const Halves h = halves_of(lo, hi);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) staged[b & 1][at_row[i]][(4 * s + sq) ^ (at_row[i] & 15)] = __builtin_bit_cast(v4i, h.v[s]);
+        }
+    };
+    v4i w[TN][2];
+    auto request_w = [&](int b) {
 #pragma unroll
         for (int i = 0; i < TN; ++i) {
-            const int j = (tile0 + i) * 16 + q * 4;
-            if (j >= p.n) continue;
-            v4f bias = {0.f, 0.f, 0.f, 0.f};
-            if (p.bias)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) bias[e] = p.bias[min(j + e, p.n - 1)];
-#pragma unroll
-            for (int t = 0; t < TM; ++t) {
-                const int row = 16 * t + col;
-                if (row < rows) store_outputs(p, row0 + row, j, acc[i][t] + bias);
-            }
+            w[i][0] = wp[i][(size_t)b * 128];
+            w[i][1] = wp[i][(size_t)b * 128 + 64];
         }
-    } else {
-        static_assert(TN % 2 == 0, "both sides of an output are one wave's");
-        v4f h[TN / 2][TM];
-        if (wk == 0)
+    };
+    float s_x[TM], s_w, s_w_up = 0.f;
+    auto request_scales = [&](int b) {
 #pragma unroll
-            for (int i = 0; i < TN / 2; ++i) {
-                const int j = (tile0 / 2 + i) * 16 + q * 4;
+        for (int t = 0; t < TM; ++t) s_x[t] = xs[t][(size_t)b * p.m];
+        s_w = ws[b];
+        if constexpr (GATED) s_w_up = ws_up[b];
+    };
+    v4f acc[TN][TM];
 #pragma unroll
-                for (int t = 0; t < TM; ++t)
+    for (int i = 0; i < TN; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float g = acc[2 * i][t][e], u = acc[2 * i + 1][t][e];
-                        if (p.bias) {
-                            g += p.bias[min(j + e, p.n - 1)];
-                            u += p.bias_up[min(j + e, p.n - 1)];
-                        }
-                        h[i][t][e] = j + e < p.n ? gated(p.gate, g, u) : 0.f;
-                    }
-                if (p.y_f16 && j < p.n)
+        for (int t = 0; t < TM; ++t) acc[i][t] = v4f{0.f, 0.f, 0.f, 0.f};
+    request(0);
+    request_w(0);
+    request_scales(0);
+    stage(0);
+    if (p.blocks_k > 1) request(1);
+    __syncthreads();
+    for (int b = 0; b < p.blocks_k; ++b) {
+        Halves wh[TN];
 #pragma unroll
-                    for (int t = 0; t < TM; ++t)
-                        if (16 * t + col < rows) store_outputs(p, row0 + 16 * t + col, j, h[i][t]);
-            }
-        if (!p.y_f8) return;
-        // the group's outputs are one block of the result (WN * TN == 16): its largest value per row
-        __shared__ float most[WN][16 * TM];
-        float a[TM];
-        if (wk == 0)
-#pragma unroll
-            for (int t = 0; t < TM; ++t) {
-                a[t] = 0.f;
-#pragma unroll
-                for (int i = 0; i < TN / 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) a[t] = fmaxf(a[t], fabsf(h[i][t][e]));
-                a[t] = fmaxf(a[t], __shfl_xor(a[t], 16));
-                a[t] = fmaxf(a[t], __shfl_xor(a[t], 32));
-                if (q == 0) most[wn][16 * t + col] = a[t];
-            }
-        __syncthreads();
-        if (wk > 0) return;
+        for (int i = 0; i < TN; ++i) wh[i] = halves_of(w[i][0], w[i][1]);
+        float sc[TM], sc_up[TM];
 #pragma unroll
         for (int t = 0; t < TM; ++t) {
-            const int row = 16 * t + col;
-            if (row >= rows) continue;
-            float top = most[0][row];
-#pragma unroll
-            for (int o = 1; o < WN; ++o) top = fmaxf(top, most[o][row]);
-            const float s = scale_of(top), r = 1.f / s;
-            if (wn == 0 && q == 0) p.y_scale[(size_t)group_n * p.m + row0 + row] = s;
-#pragma unroll
-            for (int i = 0; i < TN / 2; ++i) {
-                const int j = (tile0 / 2 + i) * 16 + q * 4;
-                const int code = four_codes(h[i][t][0] * r, h[i][t][1] * r, h[i][t][2] * r, h[i][t][3] * r);
-                uint8_t* const dst = p.y_f8 + (size_t)(row0 + row) * p.y_stride + j;
-                if (j + 4 <= p.n) *reinterpret_cast<int*>(dst) = code;
-                else
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (j + e < p.n) dst[e] = (uint8_t)(code >> (8 * e));
-            }
+            sc[t] = s_w * s_x[t];
+            sc_up[t] = s_w_up * s_x[t];
         }
+        if (b + 1 < p.blocks_k) {
+            stage(b + 1);
+            if (b + 2 < p.blocks_k) request(b + 2);
+            request_w(b + 1);
+            request_scales(b + 1);
+        }
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            const int row = (wm * TM + t) * 16 + col;
+            v4f part[TN];
+#pragma unroll
+            for (int i = 0; i < TN; ++i) part[i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const v8h x = __builtin_bit_cast(v8h, staged[b & 1][row][(4 * s + q) ^ col]);
+#pragma unroll
+                for (int i = 0; i < TN; ++i) part[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[i].v[s], x, part[i], 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][t][e] = __builtin_fmaf(part[i][e], GATED && i % 2 ? sc_up[t] : sc[t], acc[i][t][e]);
+        }
+        __syncthreads();
     }
+    if constexpr (!GATED) write_outputs<TN, TM>(p, acc, tile0, row0 + wm * TM * 16, min(16 * TM, rows - wm * TM * 16), lane);
+    else write_gated<TN, TM, WN, WM>(p, acc, tile0, group_n, wn, wm, row0 + wm * TM * 16, min(16 * TM, rows - wm * TM * 16), lane, true);
 }
 
 int blocks_of(int v) { return v / kBlk + (v % kBlk != 0); }
@@ -385,17 +518,24 @@ F8Params params_of(const exhip_f8_desc* d, const uint8_t* x, const float* x_scal
     return p;
 }
 
-template <int TN, int TM, int WN, int WK, bool GATED>
-int launch_rows(exhip_ctx* ctx, F8Params p) {
-    constexpr int tiles = TN * WN, rows = 16 * TM, threads = 64 * WN * WK;
+template <typename K>
+int launch(exhip_ctx* ctx, K kernel, F8Params p, int tiles, int rows, int threads) {
     p.groups_n = (p.tiles + tiles - 1) / tiles;
     const long long groups = (long long)p.groups_n * (p.m / rows + (p.m % rows != 0));
     EXHIP_REQUIRE(groups <= 0x7fffffff / threads, "inner product: %d rows of %d outputs are more than one launch takes", p.m, p.n);
     const exhip_on_device on(ctx->device);
     EXHIP_CHECK(on.error);
-    hipLaunchKernelGGL((f8_rows_kernel<TN, TM, WN, WK, GATED>), dim3((unsigned)groups), dim3(threads), 0, ctx->stream, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(threads), 0, ctx->stream, p);
     EXHIP_LAUNCH_CHECK();
     return 0;
+}
+template <int TN, int TM, int WN, int WK, bool GATED>
+int launch_rows(exhip_ctx* ctx, const F8Params& p) {
+    return launch(ctx, f8_rows_kernel<TN, TM, WN, WK, GATED>, p, TN * WN, 16 * TM, 64 * WN * WK);
+}
+template <int WN, int WM, int TM, bool GATED>
+int launch_tile(exhip_ctx* ctx, const F8Params& p) {
+    return launch(ctx, f8_tile_kernel<WN, WM, TM, GATED>, p, 4 * WN, 16 * TM * WM, 64 * WN * WM);
 }
 
 }  // namespace
@@ -452,7 +592,8 @@ extern "C" int exhip_innerproduct_f8(exhip_ctx* ctx, const exhip_f8_desc* d, con
     p.bias = bias;
     p.y_f32 = y_f32;
     p.y_f16 = y_f16;
-    return p.m <= 16 ? launch_rows<4, 1, 1, 4, false>(ctx, p) : launch_rows<4, 4, 1, 2, false>(ctx, p);
+    if (p.m <= 16) return launch_rows<4, 1, 1, 4, false>(ctx, p);
+    return (long long)p.m * p.n >= 256 * 128 * 256 ? launch_tile<4, 2, 4, false>(ctx, p) : launch_tile<2, 2, 2, false>(ctx, p);
 }
 
 extern "C" int exhip_innerproduct_gated_f8(exhip_ctx* ctx, const exhip_f8_desc* d, int gate, const uint8_t* x, const float* x_scale, const void* w_packed,
@@ -475,5 +616,7 @@ extern "C" int exhip_innerproduct_gated_f8(exhip_ctx* ctx, const exhip_f8_desc* 
     p.y_f8 = y_f8;
     p.y_scale = y_scale;
     p.gate = gate;
-    return p.m <= 16 ? launch_rows<4, 1, 4, 2, true>(ctx, p) : launch_rows<4, 4, 4, 1, true>(ctx, p);
+    if (p.m <= 16) return launch_rows<4, 1, 4, 2, true>(ctx, p);
+    if (2ll * p.m * p.n >= 256 * 128 * 256) return launch_tile<4, 2, 4, true>(ctx, p);
+    return p.y_f8 ? launch_tile<4, 1, 4, true>(ctx, p) : launch_tile<2, 2, 2, true>(ctx, p);
 }
