@@ -1,90 +1,379 @@
 // Log probabilities of given classes, the entropy and the largest classes of rows of values.
 //
-// With M = max x, S = sum exp(x - M) and T = sum exp(x - M) (x - M): log p = x - M - log S, and the entropy is log S - T / S.
+// With M = max x, S = sum exp(x - M) and T = sum exp(x - M) (x - M): log p = x - M - log S, and the entropy is log S - T / S. The values are read once: a
+// group holds its slice of a row in registers, so the maximum comes first and every exponential is taken once. Slices of a row are joined in the order of
+// their lanes, whatever order the groups end in.
+#include <float.h>
+
 #include "common.h"
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kMostSlice = 32768;   // values of a row that a group holds in its registers
+constexpr int kCandidates = 512;    // values of a slice that are ranked at once
 typedef unsigned long long u64;
 
-__device__ __forceinline__ float value_of(const float* x, size_t i) { return x[i]; }
-__device__ __forceinline__ float value_of(const uint16_t* x, size_t i) { return exhip_h2f(x[i]); }
+template <typename T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Run {  // neighbouring values at any alignment of their type
+    T v[N];
+};
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(uint16_t v) { return exhip_h2f(v); }
+// The largest of a run, NaN left out.
+__device__ __forceinline__ float run_max(const Run<float, 4>& r) { return fmaxf(fmaxf(r.v[0], r.v[1]), fmaxf(r.v[2], r.v[3])); }
+__device__ __forceinline__ float run_max(const Run<uint16_t, 8>& r) {
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+    struct Pairs { v2h p[4]; };
+    const Pairs h = __builtin_bit_cast(Pairs, r);
+    const v2h m = __builtin_elementwise_max(__builtin_elementwise_max(h.p[0], h.p[1]), __builtin_elementwise_max(h.p[2], h.p[3]));
+    return fmaxf((float)m[0], (float)m[1]);
+}
 
-// Larger for what stands further in front: by value (the zeros alike, NaN above all), then by index.
+__device__ __forceinline__ float masked(float) { return -INFINITY; }
+__device__ __forceinline__ uint16_t masked(uint16_t) { return 0xfc00; }
+
+// f over the values of a wave's 64 lanes, or of each of its rows of 16, in all of them: lanes one and two apart trade within their quads, quads and
+// halves of a row by its mirror images, rows by swaps. Both partners of a trade compute the same, so f has to be symmetric.
+template <int CONTROL>
+__device__ __forceinline__ float traded(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CONTROL, 0xF, 0xF, true));
+}
+template <typename F>
+__device__ __forceinline__ float over_row(float v, F f) {
+    v = f(v, traded<0xB1>(v));   // quad_perm [1, 0, 3, 2]
+    v = f(v, traded<0x4E>(v));   // quad_perm [2, 3, 0, 1]
+    v = f(v, traded<0x141>(v));  // row_half_mirror
+    return f(v, traded<0x140>(v));  // row_mirror
+}
+template <typename F>
+__device__ __forceinline__ float over_wave(float v, F f) {
+    v = over_row(v, f);
+    const auto bits = [](float x) { return __builtin_bit_cast(unsigned, x); };
+    const auto r = __builtin_amdgcn_permlane16_swap(bits(v), bits(v), false, false);
+    const unsigned r0 = r[0], r1 = r[1];
+    v = f(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
+    const auto h = __builtin_amdgcn_permlane32_swap(bits(v), bits(v), false, false);
+    const unsigned h0 = h[0], h1 = h[1];
+    return f(__builtin_bit_cast(float, h0), __builtin_bit_cast(float, h1));
+}
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float sum(float a, float b) { return a + b; }
+// A lane's place among those of a mask.
+__device__ __forceinline__ int place_in(u64 mask) { return __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0)); }
+
+// Larger for what stands further in front: by value (the zeros alike, NaN above all), then by index. Never 0.
 __device__ __forceinline__ unsigned order_of(float v) {
     if (v != v) return 0xffffffffu;
     const unsigned b = __builtin_bit_cast(unsigned, v + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ u64 place_of(float v, int i) { return (u64)order_of(v) << 32 | (unsigned)~i; }
+__device__ __forceinline__ int index_of(u64 place) { return (int)~(unsigned)place; }
+
+// Exponentials are taken as powers of two, logarithms as those to base two.
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
+constexpr float kNoPart = -300.f;  // two to this has no part in a sum; -infinity must not meet a zero in a product
+
+// Maximum, s = sum exp(x - maximum) and t = sum exp(x - maximum) (x - maximum) log2 e of some values; nothing: -infinity, 0, 0.
+struct __attribute__((aligned(16))) Sums {
+    float most, s, t, unused;
+};
+__device__ __forceinline__ float power(float z) { return __builtin_amdgcn_exp2f(z); }
+__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
+    Sums r;
+    r.most = fmaxf(a.most, b.most);
+    const float base = r.most == -INFINITY ? 0.f : r.most;
+    const float da = fmaxf((a.most - base) * kLog2e, kNoPart), db = fmaxf((b.most - base) * kLog2e, kNoPart), ea = power(da), eb = power(db);
+    r.s = a.s * ea + b.s * eb;
+    r.t = (a.t + a.s * da) * ea + (b.t + b.s * db) * eb;
+    r.unused = 0.f;
+    return r;
+}
+template <int CONTROL>
+__device__ __forceinline__ Sums traded(const Sums& a) { return Sums{traded<CONTROL>(a.most), traded<CONTROL>(a.s), traded<CONTROL>(a.t), 0.f}; }
+__device__ __forceinline__ Sums from_lane(const Sums& a, int d) {
+    return Sums{__shfl_xor(a.most, d), __shfl_xor(a.s, d), __shfl_xor(a.t, d), 0.f};
+}
+
+// How many of n places (eight zeros behind them) stand in front of `own`: eight reads under way at a time.
+__device__ __forceinline__ int rank_of(u64 own, const u64* places, int n) {
+    int rank = 0;
+    for (int j = 0; j < n; j += 8) {
+        u64 o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = places[j + e];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rank += o[e] > own;
+    }
+    return rank;
+}
 
 struct LogpParams {
     const int32_t* ids;
     float *log_p, *entropy, *top_log_p;
     int32_t* top_ids;
+    Sums* part;   // [row][slice], of rows in several slices
+    u64* part_top;  // [row][slice][top]: places in falling order, 0 where there are no more
     int m, c, x_stride, n_ids, top;
+    int slices, slice_len;
 };
 
-// What is written for value v of a row with maximum `most` and logarithm `log_s`.
-__device__ __forceinline__ float log_p_of(float v, float most, float log_s) {
-    if (most == -INFINITY) return v != v ? v : -INFINITY;
-    return v - most - log_s;
+// What is written for value v of a row with these sums.
+__device__ __forceinline__ float log_p_of(float v, const Sums& r, float log_s) {
+    if (r.s != r.s) return r.s;
+    if (r.most == -INFINITY) return -INFINITY;
+    return v - r.most - log_s;
 }
 
-template <typename T, typename F>
-__device__ T over_group(T v, T* shared, F f) {
+// The answers of a row, by a group of `threads`, from its sums and the places of its largest.
+template <typename T>
+__device__ void write_row(const T* __restrict__ src, const LogpParams& p, size_t row, const Sums& r, const u64* places, int threads) {
+    const float log_s = __builtin_amdgcn_logf(r.s) * kLn2;
+    if (threadIdx.x == 0 && p.entropy) p.entropy[row] = r.s != r.s ? r.s : r.most == -INFINITY ? 0.f : log_s - r.t / r.s * kLn2;
+    for (int i = threadIdx.x; i < p.n_ids; i += threads) {
+        const int id = p.ids[row * p.n_ids + i];
+        p.log_p[row * p.n_ids + i] = id < 0 ? 0.f : id >= p.c ? NAN : log_p_of(as_float(src[id]), r, log_s);
+    }
+    for (int i = threadIdx.x; i < p.top; i += threads) {
+        const u64 at = places[i];
+        const unsigned o = (unsigned)(at >> 32);
+        p.top_ids[row * p.top + i] = index_of(at);
+        // the value back from its order
+        p.top_log_p[row * p.top + i] = log_p_of(__builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o), r, log_s);
+    }
+}
+
+// A group of W waves a slice of a row, V values a thread, all requested before the first is used.
+template <typename T, int W, int V, bool TOP>
+__global__ __launch_bounds__(64 * W, W == 16 ? 8 : 4) void log_probabilities_kernel(const T* __restrict__ x, const LogpParams p) {
+    constexpr int kThreads = 64 * W, N = 16 / sizeof(T), kRuns = V / N;
+    __shared__ Sums sums[W];
+    __shared__ float bounds[W];
+    __shared__ u64 places[TOP ? kCandidates + 8 : 1], sorted[TOP ? EXHIP_LOG_PROBABILITIES_TOP : 1];
+    __shared__ int count;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const size_t row = blockIdx.x / p.slices;
+    const int slice = blockIdx.x % p.slices, first = slice * p.slice_len, len = min(p.slice_len, p.c - first);
+    const T* const src = x + row * p.x_stride + first;
+    Run<T, N> r[kRuns];
+    auto value = [&](int e) { return as_float(r[e / N].v[e % N]); };
+    auto at = [&](int e) { return (e / N * kThreads + (int)threadIdx.x) * N + e % N; };  // of value e in the slice
+#pragma unroll
+    for (int i = 0; i < kRuns; ++i) {
+        const int k = at(i * N);
+        if (k + N <= len) r[i] = *reinterpret_cast<const Run<T, N>*>(src + k);
+        else
+#pragma unroll
+            for (int e = 0; e < N; ++e) r[i].v[e] = k + e < len ? src[k + e] : masked(T());
+    }
+    float largest[kRuns], mine = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kRuns; ++i) {
+        largest[i] = run_max(r[i]);
+        mine = fmaxf(mine, largest[i]);
+    }
+    const float most = over_wave(mine, larger), base = most == -INFINITY ? 0.f : most;
+    // (x - base) log2 e. Halves, of which a byte costs twice the exponentials, take one multiply-add: base log2 e is scaled + beside exactly, and `beside`
+    // comes in at the end. (Of the largest floats that product is infinite.)
+    constexpr bool kOneStep = sizeof(T) == 2;
+    const float scaled = base * kLog2e, beside = __builtin_fmaf(base, kLog2e, -scaled);
+    float s = 0.f, t = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const float z = kOneStep ? __builtin_fmaf(value(e), kLog2e, -scaled) : (value(e) - base) * kLog2e, w = power(z);  // a NaN goes on into s
+        s += w;
+        t = __builtin_fmaf(w, fmaxf(z, kNoPart), t);
+    }
+    if constexpr (kOneStep) {
+        t = (t - beside * s) * power(-beside);
+        s *= power(-beside);
+    }
+    Sums all = {most, over_wave(s, sum), over_wave(t, sum), 0.f};
+    if constexpr (W > 1) {
+        if (lane == 0) sums[wave] = all;
+    }
+    if constexpr (TOP) {
+        // A bound that at least `top` of the slice reach: the top-th largest of a wave's 64 lanes' largest (to 16 bits, downwards), the highest of the waves'.
+        const unsigned o = order_of(mine);
+        unsigned bound = 0;
+#pragma unroll
+        for (int bit = 31; bit >= 16; --bit) {
+            const unsigned up = bound | 1u << bit;
+            if (__popcll(__ballot(o >= up)) >= p.top) bound = up;
+        }
+        const float least = bound < 0x007fffffu ? -INFINITY : __builtin_bit_cast(float, bound & 0x80000000u ? bound & 0x7fffffffu : ~bound);
+        if (lane == 0) bounds[wave] = least;
+        if (threadIdx.x == 0) count = 0;
+    }
     __syncthreads();
-    shared[threadIdx.x] = v;
-    __syncthreads();
-    for (int d = kThreads / 2; d > 0; d >>= 1) {
-        if ((int)threadIdx.x < d) shared[threadIdx.x] = f(shared[threadIdx.x], shared[threadIdx.x + d]);
+    if constexpr (W > 1) {
+        all = sums[lane % W];
+        all = joined(all, traded<0xB1>(all));
+        all = joined(all, traded<0x4E>(all));
+        if constexpr (W == 16) {
+            all = joined(all, traded<0x141>(all));
+            all = joined(all, traded<0x140>(all));
+        }
+    }
+    if constexpr (TOP) {
+        static_assert(W == 1 || W == 4 || W == 16, "the waves' bounds are joined within rows of lanes");
+        float least = bounds[lane % W];
+        if constexpr (W > 1) least = over_row(least, larger);
+        const bool nan = all.s != all.s;
+        if (!nan) {
+            // a class of no probability is no candidate, whatever the bound
+            const float beyond = fmaxf(least, -FLT_MAX);
+            int wave_count = 0;
+#pragma unroll
+            for (int i = 0; i < kRuns; ++i)
+                if (__ballot(largest[i] >= beyond) != 0)
+#pragma unroll
+                    for (int e = i * N; e < i * N + N; ++e) wave_count += __popcll(__ballot(value(e) >= beyond));
+            if (wave_count > 0) {
+                int slot = 0;
+                if (lane == 0) slot = atomicAdd(&count, wave_count);
+                slot = __builtin_amdgcn_readfirstlane(slot);
+                if (slot + wave_count <= kCandidates)
+#pragma unroll
+                    for (int i = 0; i < kRuns; ++i)
+                        if (__ballot(largest[i] >= beyond) != 0)
+#pragma unroll
+                            for (int e = i * N; e < i * N + N; ++e) {
+                                const bool takes = value(e) >= beyond;
+                                const u64 all_takes = __ballot(takes);
+                                if (takes) places[slot + place_in(all_takes)] = place_of(value(e), first + at(e));
+                                slot += __popcll(all_takes);
+                            }
+            }
+            __syncthreads();
+            const int n = count;
+            if (n < p.top) {  // masked classes too, by their index: they are among the first n + top of the slice
+                __syncthreads();
+                for (int i = threadIdx.x; i < min(n + p.top, len); i += kThreads)
+                    if (as_float(src[i]) == -INFINITY) places[atomicAdd(&count, 1)] = place_of(-INFINITY, first + i);
+                __syncthreads();
+            }
+        }
+        const int n = nan ? kCandidates + 1 : count;
+        if (n <= kCandidates) {
+            if (threadIdx.x < 8) places[n + threadIdx.x] = 0;
+            for (int i = threadIdx.x; i < p.top; i += kThreads)
+                if (i >= n) sorted[i] = 0;
+            __syncthreads();
+            for (int i = threadIdx.x; i < n; i += kThreads) {
+                const u64 own = places[i];
+                const int rank = rank_of(own, places, n);
+                if (rank < p.top) sorted[rank] = own;
+            }
+        } else {
+            // many equal values, or a NaN: the largest behind the last one found, `top` times, each a reading of the slice
+            u64 last = ~0ull;
+            for (int i = 0; i < p.top; ++i) {
+                u64 best = 0;
+                for (int k = threadIdx.x; k < len; k += kThreads) {
+                    const u64 here = place_of(as_float(src[k]), first + k);
+                    if (here < last && here > best) best = here;
+                }
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) {
+                    const u64 other = __shfl_xor(best, d);
+                    best = other > best ? other : best;
+                }
+                __syncthreads();
+                if (lane == 0) places[wave] = best;
+                __syncthreads();
+                last = places[0];
+                for (int w = 1; w < W; ++w) last = places[w] > last ? places[w] : last;
+                if (threadIdx.x == 0) sorted[i] = last;
+                if (last == 0) last = 1;  // nothing is left: none of the places lies beneath
+            }
+        }
         __syncthreads();
     }
-    return shared[0];
+    if (p.slices == 1) {
+        write_row(src, p, row, all, sorted, kThreads);
+    } else {
+        if (threadIdx.x == 0) p.part[blockIdx.x] = all;
+        if constexpr (TOP)
+            for (int i = threadIdx.x; i < p.top; i += kThreads) p.part_top[(size_t)blockIdx.x * p.top + i] = sorted[i];
+    }
 }
 
-// A group a row.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void log_probabilities_kernel(const T* __restrict__ x, const LogpParams p) {
-    __shared__ float fs[kThreads];
-    __shared__ u64 us[kThreads];
-    const size_t row = blockIdx.x;
-    const T* const src = x + row * p.x_stride;
-    float most = -INFINITY;
-    for (int i = threadIdx.x; i < p.c; i += kThreads) most = fmaxf(most, value_of(src, i));
-    most = over_group(most, fs, [](float a, float b) { return fmaxf(a, b); });
-    const float base = most == -INFINITY ? 0.f : most;
-    float s = 0.f, t = 0.f;
-    for (int i = threadIdx.x; i < p.c; i += kThreads) {
-        const float d = value_of(src, i) - base, e = expf(d);
-        s += e;
-        if (e != 0.f) t += e * d;
-    }
-    s = over_group(s, fs, [](float a, float b) { return a + b; });
-    t = over_group(t, fs, [](float a, float b) { return a + b; });
-    const bool empty = most == -INFINITY && s == 0.f;
-    const float log_s = logf(s);
-    if (threadIdx.x == 0 && p.entropy) p.entropy[row] = empty ? 0.f : log_s - t / s;
-    for (int i = threadIdx.x; i < p.n_ids; i += kThreads) {
-        const int id = p.ids[row * p.n_ids + i];
-        p.log_p[row * p.n_ids + i] = id < 0 ? 0.f : id >= p.c ? NAN : s != s ? s : log_p_of(value_of(src, id), most, log_s);
-    }
-    u64 last = ~0ull;
-    for (int n = 0; n < p.top; ++n) {
-        u64 best = 0;
-        for (int i = threadIdx.x; i < p.c; i += kThreads) {
-            const u64 at = place_of(value_of(src, i), i);
-            if (at < last && at > best) best = at;
+// The largest of the slices' lists, `top` of them into sorted, by one wave: a batch of entries is held in registers with those found so far in front, the top-th
+// largest of it is found to 24 bits by halving, and what reaches that is ranked.
+__device__ void join_lists(const u64* __restrict__ from, size_t total, int top, u64* places, u64* sorted) {
+    constexpr int kHeld = 8;
+    const int lane = threadIdx.x;
+    int kept = 0;
+    for (size_t done = 0; done < total;) {
+        u64 held[kHeld];
+#pragma unroll
+        for (int e = 0; e < kHeld; ++e) {
+            const int i = e * 64 + lane;  // the first `kept` of a batch are those found so far
+            held[e] = i < kept ? sorted[i] : done + (i - kept) < total ? from[done + (i - kept)] : 0;
         }
-        last = over_group(best, us, [](u64 a, u64 b) { return a > b ? a : b; });
-        if (threadIdx.x == 0) {
-            const int id = (int)~(unsigned)last;
-            p.top_ids[row * p.top + n] = id;
-            p.top_log_p[row * p.top + n] = s != s ? s : log_p_of(value_of(src, id), most, log_s);
+        done += kHeld * 64 - kept;
+        unsigned bound = 0;
+        for (int bit = 31; bit >= 8; --bit) {
+            const unsigned up = bound | 1u << bit;
+            int reach = 0;
+#pragma unroll
+            for (int e = 0; e < kHeld; ++e) reach += __popcll(__ballot((unsigned)(held[e] >> 32) >= up));
+            if (reach >= top) bound = up;
         }
+        int n = 0;
+#pragma unroll
+        for (int e = 0; e < kHeld; ++e) {
+            const bool takes = held[e] != 0 && (unsigned)(held[e] >> 32) >= bound;
+            const u64 all_takes = __ballot(takes);
+            if (takes) places[n + place_in(all_takes)] = held[e];
+            n += __popcll(all_takes);
+        }
+        if (lane < 8) places[n + lane] = 0;
+        __syncthreads();
+        for (int i = lane; i < n; i += 64) {
+            const u64 own = places[i];
+            const int rank = rank_of(own, places, n);
+            if (rank < top) sorted[rank] = own;
+        }
+        __syncthreads();
+        kept = min(n, top);
     }
 }
+
+// The slices of a row, joined by one wave.
+template <typename T>
+__global__ __launch_bounds__(64) void join_slices_kernel(const T* __restrict__ x, const LogpParams p) {
+    __shared__ u64 places[512 + 8], sorted[EXHIP_LOG_PROBABILITIES_TOP];
+    const int lane = threadIdx.x;
+    const size_t row = blockIdx.x;
+    Sums all = {-INFINITY, 0.f, 0.f, 0.f};
+    for (int i = lane; i < p.slices; i += 64) all = joined(all, p.part[row * p.slices + i]);
+    if (p.top > 0) join_lists(p.part_top + row * p.slices * p.top, (size_t)p.slices * p.top, p.top, places, sorted);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) all = joined(all, from_lane(all, d));
+    write_row(x + row * p.x_stride, p, row, all, sorted, 64);
+}
+
+// How a row is split: slices that a group's registers hold, and more of them where there are few rows.
+void split(int m, int c, int* slices, int* slice_len) {
+    const int least = (c - 1) / kMostSlice + 1, wish = 512 / m, most = (c - 1) / 8192 + 1;
+    *slices = least > wish ? least : wish < most ? wish : most;
+    const int len = (c - 1) / *slices + 1;
+    *slice_len = (len + 7) / 8 * 8;
+    *slices = (c - 1) / *slice_len + 1;
+}
+
+template <typename T, bool TOP>
+void launch_slices(exhip_ctx* ctx, const T* x, const LogpParams& p) {
+    const dim3 grid((unsigned)((size_t)p.m * p.slices));
+    if (p.slice_len <= 512) hipLaunchKernelGGL((log_probabilities_kernel<T, 1, 8, TOP>), grid, dim3(64), 0, ctx->stream, x, p);
+    else if (p.slice_len <= 2048) hipLaunchKernelGGL((log_probabilities_kernel<T, 1, 32, TOP>), grid, dim3(64), 0, ctx->stream, x, p);
+    else if (p.slice_len <= 8192) hipLaunchKernelGGL((log_probabilities_kernel<T, 4, 32, TOP>), grid, dim3(256), 0, ctx->stream, x, p);
+    else hipLaunchKernelGGL((log_probabilities_kernel<T, 16, 32, TOP>), grid, dim3(1024), 0, ctx->stream, x, p);
+}
+
+bool sizes_ok(int m, int c, int top) { return m > 0 && c > 0 && top >= 0 && top <= EXHIP_LOG_PROBABILITIES_TOP && top <= c; }
 
 template <typename T>
 int log_probabilities(exhip_ctx* ctx, const char* name, const T* x, int x_stride, int m, int c, const int32_t* ids, int n_ids, float* log_p, float* entropy, int top,
@@ -92,27 +381,40 @@ int log_probabilities(exhip_ctx* ctx, const char* name, const T* x, int x_stride
     EXHIP_REQUIRE(ctx && x && workspace, "%s: NULL argument", name);
     EXHIP_REQUIRE(m > 0 && c > 0 && x_stride >= c, "%s: %d rows of %d values, %d apart", name, m, c, x_stride);
     EXHIP_REQUIRE(n_ids >= 0 && (n_ids == 0 ? !log_p : ids && log_p), "%s: %d classes asked of a row need ids and log_p, none need neither", name, n_ids);
-    EXHIP_REQUIRE(top >= 0 && top <= EXHIP_LOG_PROBABILITIES_TOP && top <= c && (top == 0 ? !top_ids && !top_log_p : top_ids && top_log_p),
-                  "%s: the %d largest of %d classes: at most %d, with both results", name, top, c, EXHIP_LOG_PROBABILITIES_TOP);
+    EXHIP_REQUIRE(sizes_ok(m, c, top) && (top == 0 ? !top_ids && !top_log_p : top_ids && top_log_p), "%s: the %d largest of %d classes: at most %d, with both results", name,
+                  top, c, EXHIP_LOG_PROBABILITIES_TOP);
     EXHIP_REQUIRE(log_p || entropy || top, "%s: nothing is asked", name);
     EXHIP_REQUIRE((uintptr_t)x % sizeof(T) == 0 && ((uintptr_t)ids | (uintptr_t)log_p | (uintptr_t)entropy | (uintptr_t)top_ids | (uintptr_t)top_log_p) % 4 == 0 && (uintptr_t)workspace % 16 == 0,
                   "%s: an operand's address is not that of its type", name);
-    const LogpParams p = {ids, log_p, entropy, top_log_p, top_ids, m, c, x_stride, n_ids, top};
+    LogpParams p = {ids, log_p, entropy, top_log_p, top_ids, nullptr, nullptr, m, c, x_stride, n_ids, top, 0, 0};
+    split(m, c, &p.slices, &p.slice_len);
+    EXHIP_REQUIRE((size_t)m * p.slices <= 0xffffffffu / 1024, "%s: %d rows of %d values are more than one launch takes", name, m, c);
+    if (p.slices > 1) {
+        p.part = static_cast<Sums*>(workspace);
+        p.part_top = reinterpret_cast<u64*>(p.part + (size_t)m * p.slices);
+    }
     const exhip_on_device on(ctx->device);
     EXHIP_CHECK(on.error);
-    hipLaunchKernelGGL(log_probabilities_kernel<T>, dim3(m), dim3(kThreads), 0, ctx->stream, x, p);
+    if (top) launch_slices<T, true>(ctx, x, p);
+    else launch_slices<T, false>(ctx, x, p);
     EXHIP_LAUNCH_CHECK();
+    if (p.slices > 1) {
+        hipLaunchKernelGGL(join_slices_kernel<T>, dim3(m), dim3(64), 0, ctx->stream, x, p);
+        EXHIP_LAUNCH_CHECK();
+    }
     return 0;
 }
 
 }  // namespace
 
 extern "C" size_t exhip_log_probabilities_workspace(int m, int c, int top) {
-    if (m <= 0 || c <= 0 || top < 0 || top > EXHIP_LOG_PROBABILITIES_TOP || top > c) {
+    if (!sizes_ok(m, c, top)) {
         exhip_set_error("exhip_log_probabilities_workspace: %d rows of %d values, the %d largest", m, c, top);
         return 0;
     }
-    return 16;
+    int slices, slice_len;
+    split(m, c, &slices, &slice_len);
+    return slices > 1 ? (size_t)m * slices * (sizeof(Sums) + 8 * top) : 16;
 }
 
 extern "C" int exhip_log_probabilities_f32(exhip_ctx* ctx, const float* x, int x_stride, int m, int c, const int32_t* ids, int n_ids, float* log_p, float* entropy,
