@@ -147,7 +147,7 @@ struct F8Params {
     int m, n, k, x_stride, y_stride;
     int blocks_k, tiles;  // blocks along k, tiles of 16 outputs (of both projections)
     int gate;
-    int groups_n;  // groups side by side along the outputs
+    int groups_n, groups_m;  // groups side by side along the outputs, and along the rows
 };
 
 __device__ __forceinline__ float gated(int gate, float g, float u) {
@@ -357,6 +357,140 @@ __global__ __launch_bounds__(64 * WN * WK) void f8_rows_kernel(const F8Params p)
     }
 }
 
+// ---- results of the kernels for many rows: through LDS, so that whole lines are stored ----
+// (A lane's four neighbouring outputs of one row, stored as they are, are 32 bytes of each of 16 rows at a time: 1.2 TB/s.)
+template <typename O>
+struct __attribute__((packed, aligned(sizeof(O)))) Piece {  // 16 bytes of results at any alignment of their type
+    O v[16 / sizeof(O)];
+};
+// Row-major results of a group: rows of WIDTH outputs, 16-byte pieces at place piece ^ (row % 8).
+template <typename O, int WIDTH>
+__device__ __forceinline__ char* place_in_rows(char* lds, int row, int j) {
+    const int byte = j * (int)sizeof(O);
+    return lds + row * (WIDTH * (int)sizeof(O)) + ((byte / 16) ^ (row & 7)) * 16 + byte % 16;
+}
+template <typename O, int WIDTH, int ROWS, int THREADS>
+__device__ __forceinline__ void store_rows(const char* lds, O* y, size_t stride, int row0, int rows, int j0, int n) {
+    constexpr int kPer = 16 / sizeof(O), kPieces = WIDTH / kPer;
+    static_assert(ROWS * kPieces % THREADS == 0 && kPieces >= 8, "every thread stores the same, and eight rows' pieces lie in different banks");
+#pragma unroll 4
+    for (int i = 0; i < ROWS * kPieces / THREADS; ++i) {
+        const int at = i * THREADS + threadIdx.x, row = at / kPieces, piece = at % kPieces, j = j0 + piece * kPer;
+        if (row >= rows || j >= n) continue;
+        const Piece<O> v = *reinterpret_cast<const Piece<O>*>(lds + row * (WIDTH * (int)sizeof(O)) + (piece ^ (row & 7)) * 16);
+        O* const dst = y + (size_t)(row0 + row) * stride + j;
+        if (j + kPer <= n) *reinterpret_cast<Piece<O>*>(dst) = v;
+        else
+            for (int e = 0; e < n - j; ++e) dst[e] = v.v[e];
+    }
+}
+__device__ __forceinline__ v4f four_of(const float* v, int j, int n) {
+    v4f r = {0.f, 0.f, 0.f, 0.f};
+    if (v)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = v[min(j + e, n - 1)];
+    return r;
+}
+
+// The sums of a group of WN x WM waves, TN = 4 tiles of outputs and TM tiles of rows each. `lds` is free for at least the group's results as floats (halves
+// where there are no others).
+template <int WN, int WM, int TM, bool FLOATS>
+__device__ __forceinline__ void write_group(const F8Params& p, v4f (&acc)[4][TM], int group_n, int wn, int wm, int row0, int rows, int lane, char* lds) {
+    constexpr int kWidth = 64 * WN, kRows = 16 * TM * WM, kThreads = 64 * WN * WM;
+    const int q = lane / 16, col = lane % 16, j0 = group_n * kWidth;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const v4f bias = four_of(p.bias, j0 + wn * 64 + i * 16 + q * 4, p.n);
+#pragma unroll
+        for (int t = 0; t < TM; ++t) acc[i][t] += bias;
+    }
+    if (FLOATS && p.y_f32) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < TM; ++t) *reinterpret_cast<v4f*>(place_in_rows<float, kWidth>(lds, (wm * TM + t) * 16 + col, wn * 64 + i * 16 + q * 4)) = acc[i][t];
+        __syncthreads();
+        store_rows<float, kWidth, kRows, kThreads>(lds, p.y_f32, p.y_stride, row0, rows, j0, p.n);
+    }
+    if (p.y_f16) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < TM; ++t)
+                *reinterpret_cast<v4h*>(place_in_rows<uint16_t, kWidth>(lds, (wm * TM + t) * 16 + col, wn * 64 + i * 16 + q * 4)) = __builtin_convertvector(acc[i][t], v4h);
+        __syncthreads();
+        store_rows<uint16_t, kWidth, kRows, kThreads>(lds, p.y_f16, p.y_stride, row0, rows, j0, p.n);
+    }
+}
+
+// The same of a gated product, whose tiles alternate: 32 WN outputs. Quantized results need a whole block of them, WN == 4.
+template <int WN, int WM, int TM>
+__device__ __forceinline__ void write_gated_group(const F8Params& p, v4f (&acc)[4][TM], int group_n, int wn, int wm, int row0, int rows, int lane, char* lds) {
+    constexpr int kWidth = 32 * WN, kRows = 16 * TM * WM, kThreads = 64 * WN * WM;
+    const int q = lane / 16, col = lane % 16, j0 = group_n * kWidth;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int j = j0 + wn * 32 + i * 16 + q * 4;
+        const v4f bias = four_of(p.bias, j, p.n), bias_up = four_of(p.bias_up, j, p.n);
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            const v4f g = acc[2 * i][t] + bias, u = acc[2 * i + 1][t] + bias_up;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][t][e] = j + e < p.n ? gated(p.gate, g[e], u[e]) : 0.f;
+        }
+    }
+    __syncthreads();
+    if (p.y_f16) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int t = 0; t < TM; ++t)
+                *reinterpret_cast<v4h*>(place_in_rows<uint16_t, kWidth>(lds, (wm * TM + t) * 16 + col, wn * 32 + i * 16 + q * 4)) = __builtin_convertvector(acc[i][t], v4h);
+        __syncthreads();
+        store_rows<uint16_t, kWidth, kRows, kThreads>(lds, p.y_f16, p.y_stride, row0, rows, j0, p.n);
+    }
+    if constexpr (WN == 4) {
+        if (!p.y_f8) return;
+        float* const most = reinterpret_cast<float*>(lds);  // [wave along the outputs][row]
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            float a = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a = fmaxf(a, fabsf(acc[i][t][e]));
+            a = fmaxf(a, __shfl_xor(a, 16));
+            a = fmaxf(a, __shfl_xor(a, 32));
+            if (q == 0) most[wn * kRows + (wm * TM + t) * 16 + col] = a;
+        }
+        __syncthreads();
+        float s[TM];
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            const int row = (wm * TM + t) * 16 + col;
+            float top = most[row];
+#pragma unroll
+            for (int o = 1; o < WN; ++o) top = fmaxf(top, most[o * kRows + row]);
+            s[t] = scale_of(top);
+            if (wn == 0 && q == 0 && row < rows) p.y_scale[(size_t)group_n * p.m + row0 + row] = s[t];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            const float r = 1.f / s[t];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const v4f v = acc[i][t] * r;
+                *reinterpret_cast<int*>(place_in_rows<uint8_t, kWidth>(lds, (wm * TM + t) * 16 + col, wn * 32 + i * 16 + q * 4)) = four_codes(v[0], v[1], v[2], v[3]);
+            }
+        }
+        __syncthreads();
+        store_rows<uint8_t, kWidth, kRows, kThreads>(lds, p.y_f8, p.y_stride, row0, rows, j0, p.n);
+    }
+}
+
 // Many rows: a group of WN x WM waves takes 64 WN outputs and 16 TM WM rows. A block's rows of the input become halves once for the group, on their way
 // into LDS (two buffers); a wave's weights go from L2 straight into its registers, the next block's while this one's are used.
 template <int WN, int WM, int TM, bool GATED>
@@ -365,7 +499,9 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void f8_tile_kernel(const F8Params
     static_assert(kItems * kThreads == kRows * 4, "every thread stages the same");
     // [buffer][row][16 pieces of 16 bytes]: piece 4 s + q of a row is halves_of()'s piece s of lanes of quarter q, at place (4 s + q) ^ (row % 16), so that
     // eight neighbouring rows' pieces lie in different banks
-    __shared__ v4i staged[2][kRows][16];
+    constexpr int kStaged = 2 * kRows * 256, kResults = kRows * (GATED ? 32 * WN * 2 : 64 * WN * 4);
+    __shared__ __attribute__((aligned(16))) char memory[kStaged > kResults ? kStaged : kResults];
+    auto& staged = *reinterpret_cast<v4i(*)[2][kRows][16]>(memory);
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, wn = wave % WN, wm = wave / WN;
     const int q = lane / 16, col = lane % 16;
     const int group_n = blockIdx.x % p.groups_n, tile0 = (group_n * WN + wn) * TN, row0 = blockIdx.x / p.groups_n * kRows;
@@ -472,8 +608,170 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void f8_tile_kernel(const F8Params
         }
         __syncthreads();
     }
-    if constexpr (!GATED) write_outputs<TN, TM>(p, acc, tile0, row0 + wm * TM * 16, min(16 * TM, rows - wm * TM * 16), lane);
-    else write_gated<TN, TM, WN, WM>(p, acc, tile0, group_n, wn, wm, row0 + wm * TM * 16, min(16 * TM, rows - wm * TM * 16), lane, true);
+    if constexpr (!GATED) write_group<WN, WM, TM, true>(p, acc, group_n, wn, wm, row0, rows, lane, memory);
+    else write_gated_group<WN, WM, TM>(p, acc, group_n, wn, wm, row0, rows, lane, memory);
+}
+
+// ---- many rows with halves as results: the matrix core's own 8-bit products ----
+typedef int v8i __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ v8i both(v4i a, v4i b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+// One 16-byte (4-byte) element per lane from a bounds-checked view straight into LDS, lane l's at lds + 16 l (4 l); lds is the wave's, in M0. vmcnt counts
+// them like any other load. The views and addresses are pinned to scalar registers for the inline assembly.
+__device__ __forceinline__ void load16_to_lds(__amdgpu_buffer_rsrc_t view, int off, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(view) : "m0", "memory");
+}
+__device__ __forceinline__ void load4_to_lds(__amdgpu_buffer_rsrc_t view, int off, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(view) : "m0", "memory");
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t uniform_view(const void* base, unsigned range) {
+    const unsigned long long a = (unsigned long long)(uintptr_t)base;
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)a), hi = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>((uintptr_t)(((unsigned long long)hi << 32) | lo)), 0, __builtin_amdgcn_readfirstlane(range), kRsrcWord3);
+}
+
+// Which tiles a group takes: each of the 8 XCDs a run of neighbouring ones, in bands of eight row tiles, so that the groups that run on an XCD at a time share
+// rows and weights in its L2.
+__device__ __forceinline__ void tile_of(int groups_n, int groups_m, int* n, int* m) {
+    const int total = groups_n * groups_m, xcd = blockIdx.x % 8, per = total / 8, more = total % 8;
+    const int i = xcd * per + min(xcd, more) + blockIdx.x / 8;
+    const int band = i / (8 * groups_n), within = i % (8 * groups_n), high = min(8, groups_m - band * 8);
+    *m = band * 8 + within % high;
+    *n = within / high;
+}
+
+// A group of 4 x 2 waves takes 256 outputs and 256 rows, a wave 64 x 128: 128 of its 256 registers are sums. Rows' codes and their scales come straight into
+// LDS, two blocks ahead in four buffers; weights from L2 straight into registers, a block ahead. Products are issued one by one, and the multiply-adds of the
+// product three places before run while the matrix core works on a new one. A block's one barrier stands in its middle: it says that the next block's rows are
+// there, so that a block's end waits for nothing.
+template <bool GATED>
+__global__ __launch_bounds__(512, 2) void f8_wide_kernel(const F8Params p) {
+    constexpr int WN = 4, TN = 4, TM = 8, kRows = 256, kBuffers = 4, kCodes = kRows * kBlk, kBuffer = kCodes + kRows * 4, kLag = 3;
+    __shared__ __attribute__((aligned(16))) char staged[kBuffers * kBuffer];
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)staged;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wn = wave % WN, wm = wave / WN;
+    const int q = lane / 16, col = lane % 16;
+    int group_n, group_m;
+    tile_of(p.groups_n, p.groups_m, &group_n, &group_m);
+    const int tile0 = (group_n * WN + wn) * TN, row0 = group_m * kRows;
+    const int rows = min(kRows, p.m - row0), tail = p.k % kBlk, blocks = p.blocks_k;
+    const __amdgpu_buffer_rsrc_t xr = uniform_view(p.x + (size_t)row0 * p.x_stride, (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16);
+    // A wave stages 32 rows, eight with a load: lane l holds piece (l % 8) ^ (l / 8) of row l / 8, so that a piece of eight neighbouring rows lies in all banks.
+    // Pieces behind a row's end are zeros.
+    const int piece = (lane % 8) ^ (lane / 8);
+    const bool behind = tail && piece * 16 >= tail;
+    int off[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int row = wave * 32 + j * 8 + lane / 8;
+        off[j] = row < rows ? row * p.x_stride + piece * 16 : kNoRow;
+    }
+    const int scale_off = min(wave % 4 * 64 + lane, rows - 1) * 4;
+    // (Behind the last block that one is staged and requested again, where nothing reads it: every block waits for the same number of loads.)
+    auto stage = [&](int buffer, int j) {  // in five loads
+        const int b = min(buffer, blocks - 1);
+        const unsigned to = lds0 + buffer % kBuffers * kBuffer;
+        if (j < 4) load16_to_lds(xr, behind && b == blocks - 1 ? kNoRow : off[j] + b * kBlk, to + (wave * 32 + j * 8) * kBlk);
+        else load4_to_lds(uniform_view(p.x_scale + (size_t)b * p.m + row0, rows * 4), scale_off, to + kCodes + wave % 4 * 256);
+    };
+    const v4i* wp[TN];
+#pragma unroll
+    for (int i = 0; i < TN; ++i) wp[i] = reinterpret_cast<const v4i*>(p.w) + (size_t)min(tile0 + i, p.tiles - 1) * blocks * 128;
+    const int block_n = min(GATED ? tile0 / 2 : tile0, (p.n - 1) / 16) / (kBlk / 16);
+    // (by scalar loads: a vector load's wait would be one for the rows on their way too)
+    typedef const __attribute__((address_space(4))) float* Constants;
+    const Constants ws = (Constants)(uintptr_t)(p.w_scale + (size_t)block_n * blocks);
+    const Constants ws_up = (Constants)(uintptr_t)(GATED ? p.w_scale_up + (size_t)block_n * blocks : nullptr);
+    struct Weights {
+        v8i v[TN];
+    };
+    auto request = [&](Weights& w, int b, int j) {  // in eight
+        const v4i* const from = wp[j / 2] + (size_t)min(b, blocks - 1) * 128;
+        const v4i got = from[lane + j % 2 * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w.v[j / 2][j % 2 * 4 + e] = got[e];
+    };
+    v4f acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int t = 0; t < TM; ++t) acc[i][t] = v4f{0.f, 0.f, 0.f, 0.f};
+    const int at = (wm * TM * 16 + col) * kBlk + (q ^ (col & 7)) * 16, at_hi = (wm * TM * 16 + col) * kBlk + (q ^ (col & 7) ^ 4) * 16;
+    const int at_scale = kCodes + (wm * TM * 16 + col) * 4;
+    struct Rows {
+        v8i v;
+        float s;
+    };
+    auto rows_from = [&](int b, int t) {
+        const char* const from = staged + b % kBuffers * kBuffer;
+        return Rows{both(*reinterpret_cast<const v4i*>(from + at + t * 16 * kBlk), *reinterpret_cast<const v4i*>(from + at_hi + t * 16 * kBlk)),
+                    *reinterpret_cast<const float*>(from + at_scale + t * 64)};
+    };
+    Rows x[2];
+    float s_w = ws[0], s_up = GATED ? ws_up[0] : 0.f, s_next = 0.f, s_up_next = 0.f;
+    auto block = [&](Weights& w, Weights& next, int b) {
+        if (p.k % 16 && b == blocks - 1) {  // the piece that a row's end cuts
+            if (threadIdx.x < kRows) {
+                v4i* const cut = reinterpret_cast<v4i*>(staged + b % kBuffers * kBuffer + threadIdx.x * kBlk + ((tail / 16) ^ (threadIdx.x & 7)) * 16);
+                *cut &= keep_first(tail % 16);
+            }
+            __syncthreads();
+            x[0] = rows_from(b, 0);
+        }
+        // The weights, requested a block ago, are waited for here: behind the next loads the compiler, which does not see those into LDS, would wait for them too.
+#pragma unroll
+        for (int i = 0; i < TN; ++i) asm volatile("" : "+v"(w.v[i]));
+        v4f part[kLag + 1];
+        float s[2], su[2];
+#pragma unroll
+        for (int u = 0; u < TN * TM + kLag; ++u) {
+            const int t = u / TN, i = u % TN;
+            // A load beside every second product: thirteen in a row would hold the wave up, 16 cycles of the CU's address unit each, eight waves at a time.
+            if (u % 2 == 0 && u / 2 < 5) stage(b + 2, u / 2);
+            else if (u % 2 == 0 && u / 2 < 13) request(next, b + 1, u / 2 - 5);
+            if (u < TN * TM) {
+                if (i == 0) {
+                    if (t == TM / 2) {
+                        // the next block's rows are older than the eight loads of this block so far
+                        asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+                        __builtin_amdgcn_s_barrier();
+                        asm volatile("" ::: "memory");
+                        const int after = min(b + 1, blocks - 1);
+                        s_next = ws[after];
+                        if constexpr (GATED) s_up_next = ws_up[after];
+                    }
+                    s[t % 2] = s_w * x[t % 2].s;
+                    su[t % 2] = s_up * x[t % 2].s;
+                    x[(t + 1) % 2] = t + 1 < TM ? rows_from(b, t + 1) : rows_from(b + 1, 0);
+                }
+                part[u % (kLag + 1)] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v[i], x[t % 2].v, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+            }
+            if (u >= kLag) {
+                const int v = u - kLag, vt = v / TN, vi = v % TN;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[vi][vt][e] = __builtin_fmaf(part[v % (kLag + 1)][e], GATED && vi % 2 ? su[vt % 2] : s[vt % 2], acc[vi][vt][e]);
+                asm volatile("" : "+v"(acc[vi][vt]));  // here, not where the compiler would like them: together at the end, out of registers
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        s_w = s_next;
+        s_up = s_up_next;
+    };
+    Weights w0, w1;
+#pragma unroll
+    for (int j = 0; j < 10; ++j) stage(j / 5, j % 5);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) request(w0, 0, j);
+    asm volatile("s_waitcnt vmcnt(13)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    x[0] = rows_from(0, 0);
+    for (int b = 0; b < blocks; b += 2) {
+        block(w0, w1, b);
+        if (b + 1 < blocks) block(w1, w0, b + 1);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was staged behind the end, in front of the results' barrier
+    if constexpr (!GATED) write_group<WN, 2, TM, false>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
+    else write_gated_group<WN, 2, TM>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
 }
 
 int blocks_of(int v) { return v / kBlk + (v % kBlk != 0); }
@@ -521,13 +819,18 @@ F8Params params_of(const exhip_f8_desc* d, const uint8_t* x, const float* x_scal
 template <typename K>
 int launch(exhip_ctx* ctx, K kernel, F8Params p, int tiles, int rows, int threads) {
     p.groups_n = (p.tiles + tiles - 1) / tiles;
-    const long long groups = (long long)p.groups_n * (p.m / rows + (p.m % rows != 0));
+    p.groups_m = p.m / rows + (p.m % rows != 0);
+    const long long groups = (long long)p.groups_n * p.groups_m;
     EXHIP_REQUIRE(groups <= 0x7fffffff / threads, "inner product: %d rows of %d outputs are more than one launch takes", p.m, p.n);
     const exhip_on_device on(ctx->device);
     EXHIP_CHECK(on.error);
     hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(threads), 0, ctx->stream, p);
     EXHIP_LAUNCH_CHECK();
     return 0;
+}
+template <bool GATED>
+int launch_wide(exhip_ctx* ctx, const F8Params& p) {
+    return launch(ctx, f8_wide_kernel<GATED>, p, 16, 256, 512);
 }
 template <int TN, int TM, int WN, int WK, bool GATED>
 int launch_rows(exhip_ctx* ctx, const F8Params& p) {
@@ -593,6 +896,7 @@ extern "C" int exhip_innerproduct_f8(exhip_ctx* ctx, const exhip_f8_desc* d, con
     p.y_f32 = y_f32;
     p.y_f16 = y_f16;
     if (p.m <= 16) return launch_rows<4, 1, 1, 4, false>(ctx, p);
+    if (!p.y_f32 && (long long)p.m * p.n >= 256ll * 256 * 128) return launch_wide<false>(ctx, p);
     return (long long)p.m * p.n >= 256 * 128 * 256 ? launch_tile<4, 2, 4, false>(ctx, p) : launch_tile<2, 2, 2, false>(ctx, p);
 }
 
@@ -617,6 +921,7 @@ extern "C" int exhip_innerproduct_gated_f8(exhip_ctx* ctx, const exhip_f8_desc* 
     p.y_scale = y_scale;
     p.gate = gate;
     if (p.m <= 16) return launch_rows<4, 1, 4, 2, true>(ctx, p);
+    if (!p.y_f8 && 2ll * p.m * p.n >= 256ll * 256 * 128) return launch_wide<true>(ctx, p);
     if (2ll * p.m * p.n >= 256 * 128 * 256) return launch_tile<4, 2, 4, true>(ctx, p);
     return p.y_f8 ? launch_tile<4, 1, 4, true>(ctx, p) : launch_tile<2, 2, 2, true>(ctx, p);
 }
