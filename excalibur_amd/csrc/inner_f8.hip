@@ -205,156 +205,48 @@ __device__ __forceinline__ void store_outputs(const F8Params& p, int row, int j,
     }
 }
 
-// A wave's sums, TN tiles of outputs from tile0 on and TM tiles of rows from row0 on, of which `rows` exist.
-template <int TN, int TM>
-__device__ __forceinline__ void write_outputs(const F8Params& p, const v4f (&acc)[TN][TM], int tile0, int row0, int rows, int lane) {
-    const int q = lane / 16, col = lane % 16;
-#pragma unroll
-    for (int i = 0; i < TN; ++i) {
-        const int j = (tile0 + i) * 16 + q * 4;
-        if (j >= p.n) continue;
-        v4f bias = {0.f, 0.f, 0.f, 0.f};
-        if (p.bias)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) bias[e] = p.bias[min(j + e, p.n - 1)];
-#pragma unroll
-        for (int t = 0; t < TM; ++t) {
-            const int row = 16 * t + col;
-            if (row < rows) store_outputs(p, row0 + row, j, acc[i][t] + bias);
-        }
-    }
+// ---- loads ----
+typedef int v8i __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ v8i both(v4i a, v4i b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+// One 16-byte (4-byte) element per lane from a bounds-checked view straight into LDS, lane l's at lds + 16 l (4 l); lds is the wave's, in M0. vmcnt counts
+// them like any other load. The views and addresses are pinned to scalar registers for the inline assembly.
+__device__ __forceinline__ void load16_to_lds(__amdgpu_buffer_rsrc_t view, int off, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(view) : "m0", "memory");
+}
+__device__ __forceinline__ void load4_to_lds(__amdgpu_buffer_rsrc_t view, int off, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(view) : "m0", "memory");
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t uniform_view(const void* base, unsigned range) {
+    const unsigned long long a = (unsigned long long)(uintptr_t)base;
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)a), hi = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>((uintptr_t)(((unsigned long long)hi << 32) | lo)), 0, __builtin_amdgcn_readfirstlane(range), kRsrcWord3);
 }
 
-// The same of a gated product, whose tiles alternate. Quantized results take the whole group: its WN waves side by side hold one block of the result
-// (WN * TN == 16), WM such rows of waves stand one behind the other. `mine`: this wave has sums to write.
-template <int TN, int TM, int WN, int WM>
-__device__ __forceinline__ void write_gated(const F8Params& p, const v4f (&acc)[TN][TM], int tile0, int group_n, int wn, int wm, int row0, int rows, int lane, bool mine) {
-    static_assert(TN % 2 == 0, "both sides of an output are one wave's");
-    const int q = lane / 16, col = lane % 16;
-    v4f h[TN / 2][TM];
-    if (mine)
-#pragma unroll
-        for (int i = 0; i < TN / 2; ++i) {
-            const int j = (tile0 / 2 + i) * 16 + q * 4;
-            v4f bias = {0.f, 0.f, 0.f, 0.f}, bias_up = bias;
-            if (p.bias)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    bias[e] = p.bias[min(j + e, p.n - 1)];
-                    bias_up[e] = p.bias_up[min(j + e, p.n - 1)];
-                }
-#pragma unroll
-            for (int t = 0; t < TM; ++t) {
-                const v4f g = acc[2 * i][t] + bias, u = acc[2 * i + 1][t] + bias_up;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) h[i][t][e] = j + e < p.n ? gated(p.gate, g[e], u[e]) : 0.f;
-                if (p.y_f16 && j < p.n && 16 * t + col < rows) store_outputs(p, row0 + 16 * t + col, j, h[i][t]);
-            }
-        }
-    if constexpr (WN * TN == 16) {
-        if (!p.y_f8) return;
-        __shared__ float most[WM][WN][16 * TM];
-        if (mine)
-#pragma unroll
-            for (int t = 0; t < TM; ++t) {
-                float a = 0.f;
-#pragma unroll
-                for (int i = 0; i < TN / 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) a = fmaxf(a, fabsf(h[i][t][e]));
-                a = fmaxf(a, __shfl_xor(a, 16));
-                a = fmaxf(a, __shfl_xor(a, 32));
-                if (q == 0) most[wm][wn][16 * t + col] = a;
-            }
-        __syncthreads();
-        if (!mine) return;
-#pragma unroll
-        for (int t = 0; t < TM; ++t) {
-            const int row = 16 * t + col;
-            if (row >= rows) continue;
-            float top = most[wm][0][row];
-#pragma unroll
-            for (int o = 1; o < WN; ++o) top = fmaxf(top, most[wm][o][row]);
-            const float s = scale_of(top), r = 1.f / s;
-            if (wn == 0 && q == 0) p.y_scale[(size_t)group_n * p.m + row0 + row] = s;
-#pragma unroll
-            for (int i = 0; i < TN / 2; ++i) {
-                const int j = (tile0 / 2 + i) * 16 + q * 4;
-                const int code = four_codes(h[i][t][0] * r, h[i][t][1] * r, h[i][t][2] * r, h[i][t][3] * r);
-                uint8_t* const dst = p.y_f8 + (size_t)(row0 + row) * p.y_stride + j;
-                if (j + 4 <= p.n) *reinterpret_cast<int*>(dst) = code;
-                else
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (j + e < p.n) dst[e] = (uint8_t)(code >> (8 * e));
-            }
-        }
-    }
-}
+// Of a wave's own, by scalar loads: a vector load's wait would be one for what else is on its way too.
+typedef const __attribute__((address_space(4))) float* Constants;
 
-// A group of WN x WK waves takes WN * TN tiles of outputs and 16 TM rows; wave (wn, wk) its own TN tiles and every WK-th block. The waves' sums are
-// added in the order of wk.
-template <int TN, int TM, int WN, int WK, bool GATED>
-__global__ __launch_bounds__(64 * WN * WK) void f8_rows_kernel(const F8Params p) {
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, wn = wave % WN, wk = wave / WN;
-    const int group_n = blockIdx.x % p.groups_n, tile0 = (group_n * WN + wn) * TN, row0 = blockIdx.x / p.groups_n * (16 * TM);
-    const int q = lane / 16, col = lane % 16;
-    const int rows = min(16 * TM, p.m - row0), tail = p.k % kBlk;
-    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.x) + (size_t)row0 * p.x_stride, 0,
-                                                                      (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16, kRsrcWord3);
-    v4f acc[TN][TM];
-#pragma unroll
-    for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int t = 0; t < TM; ++t) acc[i][t] = v4f{0.f, 0.f, 0.f, 0.f};
-    for (int b = wk; b < p.blocks_k; b += WK) {
-        Halves x[TM];
-        float xs[TM];
-#pragma unroll
-        for (int t = 0; t < TM; ++t) {
-            const int row = 16 * t + col, off = row < rows ? row * p.x_stride + b * kBlk + q * 16 : kNoRow;
-            v4i lo = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xr, off, 0, 0));
-            v4i hi = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xr, off + 64, 0, 0));
-            if (tail && b == p.blocks_k - 1) {
-                lo &= keep_first(tail - q * 16);
-                hi &= keep_first(tail - 64 - q * 16);
-            }
-            x[t] = halves_of(lo, hi);
-            xs[t] = p.x_scale[(size_t)b * p.m + row0 + min(row, rows - 1)];
-        }
-#pragma unroll
-        for (int i = 0; i < TN; ++i) {
-            const int tile = min(tile0 + i, p.tiles - 1);
-            const v4i* const wp = reinterpret_cast<const v4i*>(p.w) + ((size_t)tile * p.blocks_k + b) * 128 + lane;
-            const Halves w = halves_of(wp[0], wp[64]);
-            const int block_n = (GATED ? tile / 2 : tile) / (kBlk / 16);
-            const float ws = (GATED && tile % 2 ? p.w_scale_up : p.w_scale)[(size_t)block_n * p.blocks_k + b];
-#pragma unroll
-            for (int t = 0; t < TM; ++t) {
-                const v4f part = block_product(w, x[t]);
-                const float s = ws * xs[t];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][t][e] = __builtin_fmaf(part[e], s, acc[i][t][e]);
-            }
-        }
+// A wave's TN tile rows of the packed weights: a view from the first on, and where in it the i-th begins (the last that exists, for those beyond).
+struct WeightRows {
+    __amdgpu_buffer_rsrc_t view;
+    int first, last, row_bytes, at;
+    __device__ __forceinline__ WeightRows(const F8Params& p, int tile0, int tiles, int lane)
+        : first(min(tile0, p.tiles - 1)), last(p.tiles - 1), row_bytes(p.blocks_k * 2048), at(lane * 16) {
+        view = uniform_view(p.w + (size_t)first * row_bytes, (unsigned)(min(tiles, p.tiles - first) * row_bytes));
     }
-    if constexpr (WK > 1) {
-        __shared__ v4f joined[WK - 1][WN][TN * TM][64];
-        if (wk > 0)
-#pragma unroll
-            for (int i = 0; i < TN * TM; ++i) joined[wk - 1][wn][i][lane] = acc[i / TM][i % TM];
-        __syncthreads();
-        if (wk == 0)
-#pragma unroll
-            for (int o = 0; o < WK - 1; ++o)
-#pragma unroll
-                for (int i = 0; i < TN * TM; ++i) acc[i / TM][i % TM] += joined[o][wn][i][lane];
+    // half h of block b of tile i
+    __device__ __forceinline__ v4i load(int i, int b, int h) const {
+        return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(view, at + h * 1024, min(i, last - first) * row_bytes + b * 2048, 0));
     }
-    if constexpr (!GATED) {
-        if (wk == 0) write_outputs<TN, TM>(p, acc, tile0, row0, rows, lane);
-    } else {
-        write_gated<TN, TM, WN, 1>(p, acc, tile0, group_n, wn, 0, row0, rows, lane, wk == 0);
-    }
+};
+
+// Which tiles a group takes: each of the 8 XCDs a run of neighbouring ones, in bands of eight row tiles, so that the groups that run on an XCD at a time share
+// rows and weights in its L2.
+__device__ __forceinline__ void tile_of(int groups_n, int groups_m, int* n, int* m) {
+    const int total = groups_n * groups_m, xcd = blockIdx.x % 8, per = total / 8, more = total % 8;
+    const int i = xcd * per + min(xcd, more) + blockIdx.x / 8;
+    const int band = i / (8 * groups_n), within = i % (8 * groups_n), high = min(8, groups_m - band * 8);
+    *m = band * 8 + within % high;
+    *n = within / high;
 }
 
 // ---- results of the kernels for many rows: through LDS, so that whole lines are stored ----
@@ -491,154 +383,7 @@ __device__ __forceinline__ void write_gated_group(const F8Params& p, v4f (&acc)[
     }
 }
 
-// Many rows: a group of WN x WM waves takes 64 WN outputs and 16 TM WM rows. A block's rows of the input become halves once for the group, on their way
-// into LDS (two buffers); a wave's weights go from L2 straight into its registers, the next block's while this one's are used.
-template <int WN, int WM, int TM, bool GATED>
-__global__ __launch_bounds__(64 * WN * WM, 2) void f8_tile_kernel(const F8Params p) {
-    constexpr int TN = 4, kRows = 16 * TM * WM, kThreads = 64 * WN * WM, kItems = kRows * 4 / kThreads;
-    static_assert(kItems * kThreads == kRows * 4, "every thread stages the same");
-    // [buffer][row][16 pieces of 16 bytes]: piece 4 s + q of a row is halves_of()'s piece s of lanes of quarter q, at place (4 s + q) ^ (row % 16), so that
-    // eight neighbouring rows' pieces lie in different banks
-    constexpr int kStaged = 2 * kRows * 256, kResults = kRows * (GATED ? 32 * WN * 2 : 64 * WN * 4);
-    __shared__ __attribute__((aligned(16))) char memory[kStaged > kResults ? kStaged : kResults];
-    auto& staged = *reinterpret_cast<v4i(*)[2][kRows][16]>(memory);
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, wn = wave % WN, wm = wave / WN;
-    const int q = lane / 16, col = lane % 16;
-    const int group_n = blockIdx.x % p.groups_n, tile0 = (group_n * WN + wn) * TN, row0 = blockIdx.x / p.groups_n * kRows;
-    const int rows = min(kRows, p.m - row0), tail = p.k % kBlk;
-    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.x) + (size_t)row0 * p.x_stride, 0,
-                                                                      (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16, kRsrcWord3);
-    const v4i* wp[TN];
-#pragma unroll
-    for (int i = 0; i < TN; ++i) wp[i] = reinterpret_cast<const v4i*>(p.w) + (size_t)min(tile0 + i, p.tiles - 1) * p.blocks_k * 128 + lane;
-    const int block_n = min(GATED ? tile0 / 2 : tile0, (p.n - 1) / 16) / (kBlk / 16);
-    const float* const ws = p.w_scale + (size_t)block_n * p.blocks_k;
-    const float* const ws_up = GATED ? p.w_scale_up + (size_t)block_n * p.blocks_k : nullptr;
-    const float* xs[TM];
-#pragma unroll
-    for (int t = 0; t < TM; ++t) xs[t] = p.x_scale + row0 + min((wm * TM + t) * 16 + col, rows - 1);
-
-    int off[kItems], at_row[kItems];
-#pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-        const int item = i * kThreads + threadIdx.x;
-        at_row[i] = item / 4;
-        off[i] = at_row[i] < rows ? at_row[i] * p.x_stride + item % 4 * 16 : kNoRow;
-    }
-    const int sq = threadIdx.x % 4;
-    v4i codes[kItems][2];
-    auto request = [&](int b) {
-#pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-            codes[i][0] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xr, off[i] + b * kBlk, 0, 0));
-            codes[i][1] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xr, off[i] + b * kBlk + 64, 0, 0));
-        }
-    };
-    auto stage = [&](int b) {
-#pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-            v4i lo = codes[i][0], hi = codes[i][1];
-            if (tail && b == p.blocks_k - 1) {
-                lo &= keep_first(tail - sq * 16);
-                hi &= keep_first(tail - 64 - sq * 16);
-            }
-            const Halves h = halves_of(lo, hi);
-#pragma unroll
-            for (int s = 0; s < 4; ++s) staged[b & 1][at_row[i]][(4 * s + sq) ^ (at_row[i] & 15)] = __builtin_bit_cast(v4i, h.v[s]);
-        }
-    };
-    v4i w[TN][2];
-    auto request_w = [&](int b) {
-#pragma unroll
-        for (int i = 0; i < TN; ++i) {
-            w[i][0] = wp[i][(size_t)b * 128];
-            w[i][1] = wp[i][(size_t)b * 128 + 64];
-        }
-    };
-    float s_x[TM], s_w, s_w_up = 0.f;
-    auto request_scales = [&](int b) {
-#pragma unroll
-        for (int t = 0; t < TM; ++t) s_x[t] = xs[t][(size_t)b * p.m];
-        s_w = ws[b];
-        if constexpr (GATED) s_w_up = ws_up[b];
-    };
-    v4f acc[TN][TM];
-#pragma unroll
-    for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int t = 0; t < TM; ++t) acc[i][t] = v4f{0.f, 0.f, 0.f, 0.f};
-    request(0);
-    request_w(0);
-    request_scales(0);
-    stage(0);
-    if (p.blocks_k > 1) request(1);
-    __syncthreads();
-    for (int b = 0; b < p.blocks_k; ++b) {
-        Halves wh[TN];
-#pragma unroll
-        for (int i = 0; i < TN; ++i) wh[i] = halves_of(w[i][0], w[i][1]);
-        float sc[TM], sc_up[TM];
-#pragma unroll
-        for (int t = 0; t < TM; ++t) {
-            sc[t] = s_w * s_x[t];
-            sc_up[t] = s_w_up * s_x[t];
-        }
-        if (b + 1 < p.blocks_k) {
-            stage(b + 1);
-            if (b + 2 < p.blocks_k) request(b + 2);
-            request_w(b + 1);
-            request_scales(b + 1);
-        }
-#pragma unroll
-        for (int t = 0; t < TM; ++t) {
-            const int row = (wm * TM + t) * 16 + col;
-            v4f part[TN];
-#pragma unroll
-            for (int i = 0; i < TN; ++i) part[i] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const v8h x = __builtin_bit_cast(v8h, staged[b & 1][row][(4 * s + q) ^ col]);
-#pragma unroll
-                for (int i = 0; i < TN; ++i) part[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[i].v[s], x, part[i], 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < TN; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][t][e] = __builtin_fmaf(part[i][e], GATED && i % 2 ? sc_up[t] : sc[t], acc[i][t][e]);
-        }
-        __syncthreads();
-    }
-    if constexpr (!GATED) write_group<WN, WM, TM, true>(p, acc, group_n, wn, wm, row0, rows, lane, memory);
-    else write_gated_group<WN, WM, TM>(p, acc, group_n, wn, wm, row0, rows, lane, memory);
-}
-
 // ---- many rows with halves as results: the matrix core's own 8-bit products ----
-typedef int v8i __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ v8i both(v4i a, v4i b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
-// One 16-byte (4-byte) element per lane from a bounds-checked view straight into LDS, lane l's at lds + 16 l (4 l); lds is the wave's, in M0. vmcnt counts
-// them like any other load. The views and addresses are pinned to scalar registers for the inline assembly.
-__device__ __forceinline__ void load16_to_lds(__amdgpu_buffer_rsrc_t view, int off, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(view) : "m0", "memory");
-}
-__device__ __forceinline__ void load4_to_lds(__amdgpu_buffer_rsrc_t view, int off, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(view) : "m0", "memory");
-}
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t uniform_view(const void* base, unsigned range) {
-    const unsigned long long a = (unsigned long long)(uintptr_t)base;
-    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)a), hi = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
-    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>((uintptr_t)(((unsigned long long)hi << 32) | lo)), 0, __builtin_amdgcn_readfirstlane(range), kRsrcWord3);
-}
-
-// Which tiles a group takes: each of the 8 XCDs a run of neighbouring ones, in bands of eight row tiles, so that the groups that run on an XCD at a time share
-// rows and weights in its L2.
-__device__ __forceinline__ void tile_of(int groups_n, int groups_m, int* n, int* m) {
-    const int total = groups_n * groups_m, xcd = blockIdx.x % 8, per = total / 8, more = total % 8;
-    const int i = xcd * per + min(xcd, more) + blockIdx.x / 8;
-    const int band = i / (8 * groups_n), within = i % (8 * groups_n), high = min(8, groups_m - band * 8);
-    *m = band * 8 + within % high;
-    *n = within / high;
-}
-
 // A group of 4 x 2 waves takes 256 outputs and 256 rows, a wave 64 x 128: 128 of its 256 registers are sums. Rows' codes and their scales come straight into
 // LDS, two blocks ahead in four buffers; weights from L2 straight into registers, a block ahead. Products are issued one by one, and the multiply-adds of the
 // product three places before run while the matrix core works on a new one. A block's one barrier stands in its middle: it says that the next block's rows are
@@ -673,20 +418,15 @@ __global__ __launch_bounds__(512, 2) void f8_wide_kernel(const F8Params p) {
         if (j < 4) load16_to_lds(xr, behind && b == blocks - 1 ? kNoRow : off[j] + b * kBlk, to + (wave * 32 + j * 8) * kBlk);
         else load4_to_lds(uniform_view(p.x_scale + (size_t)b * p.m + row0, rows * 4), scale_off, to + kCodes + wave % 4 * 256);
     };
-    const v4i* wp[TN];
-#pragma unroll
-    for (int i = 0; i < TN; ++i) wp[i] = reinterpret_cast<const v4i*>(p.w) + (size_t)min(tile0 + i, p.tiles - 1) * blocks * 128;
+    const WeightRows weights(p, tile0, TN, lane);
     const int block_n = min(GATED ? tile0 / 2 : tile0, (p.n - 1) / 16) / (kBlk / 16);
-    // (by scalar loads: a vector load's wait would be one for the rows on their way too)
-    typedef const __attribute__((address_space(4))) float* Constants;
     const Constants ws = (Constants)(uintptr_t)(p.w_scale + (size_t)block_n * blocks);
     const Constants ws_up = (Constants)(uintptr_t)(GATED ? p.w_scale_up + (size_t)block_n * blocks : nullptr);
     struct Weights {
         v8i v[TN];
     };
     auto request = [&](Weights& w, int b, int j) {  // in eight
-        const v4i* const from = wp[j / 2] + (size_t)min(b, blocks - 1) * 128;
-        const v4i got = from[lane + j % 2 * 64];
+        const v4i got = weights.load(j / 2, min(b, blocks - 1), j % 2);
 #pragma unroll
         for (int e = 0; e < 4; ++e) w.v[j / 2][j % 2 * 4 + e] = got[e];
     };
@@ -774,6 +514,304 @@ __global__ __launch_bounds__(512, 2) void f8_wide_kernel(const F8Params p) {
     else write_gated_group<WN, 2, TM>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
 }
 
+// ---- few rows, or few products ----
+// A group of WN x WK waves takes WN * TN tiles of outputs and 16 TM rows; wave (wn, wk) its own TN tiles and every WK-th block, with nothing between memory and
+// its registers: the codes of D of its blocks are on their way at a time, and no wave waits for another before the sums are joined. Those go through LDS;
+// a wave joins a share of the tiles, always in the order of wk, and writes them.
+template <int TN, int TM, int WN, int WK, int D, bool GATED>
+__global__ __launch_bounds__(64 * WN * WK, 2) void f8_rows_kernel(const F8Params p) {
+    constexpr int kRows = 16 * TM, kSide = GATED ? 2 : 1, kUnits = TN / kSide * TM;  // a unit: a tile, or both sides of one
+    static_assert(TN % kSide == 0, "both sides of an output are one wave's");
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wn = wave % WN, wk = wave / WN;
+    const int q = lane / 16, col = lane % 16;
+    const int group_n = blockIdx.x % p.groups_n, tile0 = (group_n * WN + wn) * TN, row0 = blockIdx.x / p.groups_n * kRows;
+    const int rows = min(kRows, p.m - row0), tail = p.k % kBlk, blocks = p.blocks_k;
+    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.x) + (size_t)row0 * p.x_stride, 0,
+                                                                      (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16, kRsrcWord3);
+    int off[TM];
+    unsigned scale_at[TM];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) {
+        const int row = 16 * t + col;
+        off[t] = row < rows ? row * p.x_stride + q * 16 : kNoRow;
+        scale_at[t] = min(row, rows - 1);
+    }
+    const WeightRows weights(p, tile0, TN, lane);
+    const int block_n = min(tile0 / kSide, (p.n - 1) / 16) / (kBlk / 16);
+    const Constants ws = (Constants)(uintptr_t)(p.w_scale + (size_t)block_n * blocks);
+    const Constants ws_up = (Constants)(uintptr_t)(GATED ? p.w_scale_up + (size_t)block_n * blocks : nullptr);
+    struct Codes {
+        v4i w[TN][2], x[TM][2];
+        float s[TM];
+    } codes[D];
+    auto request_x = [&](Codes& c, int b) {
+        const float* const scales = p.x_scale + (size_t)b * p.m + row0;
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            c.x[t][0] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xr, off[t] + b * kBlk, 0, 0));
+            c.x[t][1] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xr, off[t] + b * kBlk + 64, 0, 0));
+            c.s[t] = scales[scale_at[t]];
+        }
+    };
+    auto request_w = [&](Codes& c, int b, int i) {
+        c.w[i][0] = weights.load(i, b, 0);
+        c.w[i][1] = weights.load(i, b, 1);
+    };
+    v4f acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int t = 0; t < TM; ++t) acc[i][t] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+        if (wk + d * WK < blocks) {
+#pragma unroll
+            for (int i = 0; i < TN; ++i) request_w(codes[d], wk + d * WK, i);
+            request_x(codes[d], wk + d * WK);
+        }
+    for (int first = wk; first < blocks; first += WK * D) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            const int b = first + d * WK, next = b + WK * D;
+            if (b >= blocks) break;
+            Codes& c = codes[d];
+            const float s_w = ws[b], s_up = GATED ? ws_up[b] : 0.f;
+            if (tail && b == blocks - 1)
+#pragma unroll
+                for (int t = 0; t < TM; ++t) {
+                    c.x[t][0] &= keep_first(tail - q * 16);
+                    c.x[t][1] &= keep_first(tail - 64 - q * 16);
+                }
+            Halves x[TM];
+            float s[TM];
+#pragma unroll
+            for (int t = 0; t < TM; ++t) {
+                x[t] = halves_of(c.x[t][0], c.x[t][1]);
+                s[t] = c.s[t];
+            }
+            if (next < blocks) request_x(c, next);
+            if constexpr (TN * TM > 8) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < TN; ++i) {
+                const Halves w = halves_of(c.w[i][0], c.w[i][1]);
+                if (next < blocks) request_w(c, next, i);
+#pragma unroll
+                for (int t = 0; t < TM; ++t) {
+                    const v4f part = block_product(w, x[t]);
+                    const float f = (GATED && i % 2 ? s_up : s_w) * s[t];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][t][e] = __builtin_fmaf(part[e], f, acc[i][t][e]);
+                }
+                if constexpr (TN * TM > 8) __builtin_amdgcn_sched_barrier(0);  // a tile's conversions at a time: all of them together do not fit the registers
+            }
+        }
+    }
+    // unit u (tile i, rows t; both sides of a gated one) is joined by wave u % WK
+    if constexpr (WK > 1) {
+        __shared__ v4f joined[WK][WN][kUnits * kSide][64];
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u)
+            if (u % WK != wk)
+#pragma unroll
+                for (int o = 0; o < kSide; ++o) joined[wk][wn][u * kSide + o][lane] = acc[u / TM * kSide + o][u % TM];
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u)
+            if (u % WK == wk)
+#pragma unroll
+                for (int o = 0; o < kSide; ++o) {
+                    v4f sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < WK; ++k) sum += k == u % WK ? acc[u / TM * kSide + o][u % TM] : joined[k][wn][u * kSide + o][lane];
+                    acc[u / TM * kSide + o][u % TM] = sum;
+                }
+    }
+    if constexpr (!GATED) {
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+            const int j = (tile0 + u / TM) * 16 + q * 4, row = u % TM * 16 + col;
+            if (u % WK == wk && j < p.n && row < rows) store_outputs(p, row0 + row, j, acc[u / TM][u % TM] + four_of(p.bias, j, p.n));
+        }
+    } else {
+        v4f h[kUnits];
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+            const int j = (tile0 / 2 + u / TM) * 16 + q * 4, row = u % TM * 16 + col;
+            h[u] = v4f{0.f, 0.f, 0.f, 0.f};
+            if (u % WK != wk) continue;
+            const v4f g = acc[u / TM * 2][u % TM] + four_of(p.bias, j, p.n), up = acc[u / TM * 2 + 1][u % TM] + four_of(p.bias_up, j, p.n);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[u][e] = j + e < p.n ? gated(p.gate, g[e], up[e]) : 0.f;
+            if (p.y_f16 && j < p.n && row < rows) store_outputs(p, row0 + row, j, h[u]);
+        }
+        if constexpr (WN * TN == 16) {  // the group's outputs are one block of a quantized result
+            if (!p.y_f8) return;
+            __shared__ float most[WN * WK][kRows];
+#pragma unroll
+            for (int t = 0; t < TM; ++t) {
+                float a = 0.f;
+#pragma unroll
+                for (int u = t; u < kUnits; u += TM)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) a = fmaxf(a, fabsf(h[u][e]));
+                a = fmaxf(a, __shfl_xor(a, 16));
+                a = fmaxf(a, __shfl_xor(a, 32));
+                if (q == 0) most[wave][16 * t + col] = a;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int t = 0; t < TM; ++t) {
+                const int row = 16 * t + col;
+                float top = 0.f;
+#pragma unroll
+                for (int o = 0; o < WN * WK; ++o) top = fmaxf(top, most[o][row]);
+                const float scale = scale_of(top), r = 1.f / scale;
+                if (wave == 0 && q == 0 && row < rows) p.y_scale[(size_t)group_n * p.m + row0 + row] = scale;
+#pragma unroll
+                for (int u = t; u < kUnits; u += TM) {
+                    const int j = (tile0 / 2 + u / TM) * 16 + q * 4;
+                    if (u % WK != wk || row >= rows) continue;
+                    const int code = four_codes(h[u][0] * r, h[u][1] * r, h[u][2] * r, h[u][3] * r);
+                    uint8_t* const dst = p.y_f8 + (size_t)(row0 + row) * p.y_stride + j;
+                    if (j + 4 <= p.n) *reinterpret_cast<int*>(dst) = code;
+                    else
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (j + e < p.n) dst[e] = (uint8_t)(code >> (8 * e));
+                }
+            }
+        }
+    }
+}
+
+// ---- many rows, exact products ----
+// A group of WN x WM waves takes 64 WN outputs and 16 TM WM rows, a wave 64 x 16 TM. A block's rows become halves once for the group, on their way into LDS
+// (four buffers); a wave's weights come from L2 as codes, a block ahead, and become halves in its registers. A block is 8 TM steps of two matrix products
+// each (2 x 17 cycles), and what else there is to do has its steps: the multiply-adds of the pair of tiles before, the conversions, the loads one by one. The
+// barrier in the block's middle says that the next block's rows are there.
+template <int WN, int WM, int TM, bool GATED>
+__global__ __launch_bounds__(64 * WN * WM, 2) void f8_tile_kernel(const F8Params p) {
+    constexpr int TN = 4, kRows = 16 * TM * WM, kThreads = 64 * WN * WM, kSteps = 8 * TM, kBuffers = 4, kPitch = 272, kBuffer = kRows * (kPitch + 4);
+    static_assert(kRows * 4 == kThreads, "a thread stages a quarter of a row");
+    // [buffer][row][16 pieces of 16 bytes]: piece 4 s + q of a row is halves_of()'s piece s of lanes of quarter q. A row's pitch is 16 bytes more, so that a
+    // piece of eight neighbouring rows lies in all banks. The rows' scales stand behind them.
+    constexpr int kStaged = kBuffers * kBuffer, kResults = kRows * (GATED ? 32 * WN * 2 : 64 * WN * 4);
+    __shared__ __attribute__((aligned(16))) char memory[kStaged > kResults ? kStaged : kResults];
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wn = wave % WN, wm = wave / WN;
+    const int q = lane / 16, col = lane % 16;
+    int group_n, group_m;
+    tile_of(p.groups_n, p.groups_m, &group_n, &group_m);
+    const int tile0 = (group_n * WN + wn) * TN, row0 = group_m * kRows;
+    const int rows = min(kRows, p.m - row0), tail = p.k % kBlk, blocks = p.blocks_k;
+    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.x) + (size_t)row0 * p.x_stride, 0,
+                                                                      (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16, kRsrcWord3);
+    // what this thread stages
+    const int own_row = threadIdx.x / 4, own_q = threadIdx.x % 4;
+    const int off = own_row < rows ? own_row * p.x_stride + own_q * 16 : kNoRow;
+    const unsigned scale_at = min(own_row, rows - 1);
+    v4i codes[2];
+    float code_scale = 0.f;
+    auto request = [&](int b, int j) {  // in three loads; behind the last block that one again, which nothing reads
+        b = min(b, blocks - 1);
+        if (j < 2) codes[j] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xr, off + b * kBlk + j * 64, 0, 0));
+        else code_scale = (p.x_scale + (size_t)b * p.m + row0)[scale_at];
+    };
+    auto stage = [&](int b, int s) {  // in four pieces
+        if (s == 0 && tail && b == blocks - 1) {
+            codes[0] &= keep_first(tail - own_q * 16);
+            codes[1] &= keep_first(tail - 64 - own_q * 16);
+        }
+        char* const to = memory + b % kBuffers * kBuffer;
+        *reinterpret_cast<v8h*>(to + own_row * kPitch + (4 * s + own_q) * 16) = halves_of(codes[0][s], codes[1][s]);
+        if (s == 0 && own_q == 0) *reinterpret_cast<float*>(to + kRows * kPitch + own_row * 4) = code_scale;
+    };
+    const WeightRows weights(p, tile0, TN, lane);
+    const int block_n = min(GATED ? tile0 / 2 : tile0, (p.n - 1) / 16) / (kBlk / 16);
+    const Constants ws = (Constants)(uintptr_t)(p.w_scale + (size_t)block_n * blocks);
+    const Constants ws_up = (Constants)(uintptr_t)(GATED ? p.w_scale_up + (size_t)block_n * blocks : nullptr);
+    v4i raw[TN][2];
+    auto request_w = [&](int b, int j) { raw[j / 2][j % 2] = weights.load(j / 2, min(b, blocks - 1), j % 2); };  // in eight
+    Halves w[TN];
+    v4f acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int t = 0; t < TM; ++t) acc[i][t] = v4f{0.f, 0.f, 0.f, 0.f};
+    struct Rows {
+        v8h v[4];
+        float s;
+    };
+    auto rows_from = [&](int b, int t) {
+        const char* const from = memory + b % kBuffers * kBuffer;
+        const int row = (wm * TM + t) * 16 + col;
+        Rows r;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) r.v[s] = *reinterpret_cast<const v8h*>(from + row * kPitch + (4 * s + q) * 16);
+        r.s = *reinterpret_cast<const float*>(from + kRows * kPitch + row * 4);
+        return r;
+    };
+#pragma unroll
+    for (int j = 0; j < 3; ++j) request(0, j);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) request_w(0, j);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) stage(0, s);
+#pragma unroll
+    for (int j = 0; j < 3; ++j) request(1, j);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w[i] = halves_of(raw[i][0], raw[i][1]);
+    __syncthreads();
+    Rows x[2];
+    x[0] = rows_from(0, 0);
+    float s_w = ws[0], s_up = GATED ? ws_up[0] : 0.f, s_next = 0.f, s_up_next = 0.f;
+    for (int b = 0; b < blocks; ++b) {
+        v4f part[2][2];
+        float sc[2], sc_up[2];
+#pragma unroll
+        for (int u = 0; u < kSteps + 2; ++u) {
+            const int t = u / 8, pair = u / 4 % 2, s = u % 4;
+            if (u < 4) {
+#pragma unroll
+                for (int i = 2; i < 4; ++i) w[i].v[u] = halves_of(raw[i][0][u], raw[i][1][u]);
+            }
+            if (u < 8) request_w(b + 1, u);  // (those of step u < 4 were used up in the block before)
+            if (u >= kSteps / 4 && u < kSteps / 4 + 4) stage(b + 1, u - kSteps / 4);
+            if (u >= kSteps / 4 + 4 && u < kSteps / 4 + 7) request(b + 2, u - kSteps / 4 - 4);
+            if (u == kSteps / 2) {
+                const int after = min(b + 1, blocks - 1);
+                s_next = ws[after];
+                if constexpr (GATED) s_up_next = ws_up[after];
+                __syncthreads();
+            }
+            if (u >= kSteps - 4 && u < kSteps) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) w[i].v[u % 4] = halves_of(raw[i][0][u % 4], raw[i][1][u % 4]);
+            }
+            if (u < kSteps) {
+                if (u % 8 == 0) {
+                    sc[t % 2] = s_w * x[t % 2].s;
+                    sc_up[t % 2] = s_up * x[t % 2].s;
+                    x[(t + 1) % 2] = t + 1 < TM ? rows_from(b, t + 1) : rows_from(b + 1, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    part[pair][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[2 * pair + i].v[s], x[t % 2].v[s], s == 0 ? v4f{0.f, 0.f, 0.f, 0.f} : part[pair][i], 0, 0, 0);
+            }
+            if (u >= 4 && s < 2) {  // of the pair before, a tile a step
+                const int vt = (u - 4) / 8, vi = (1 - pair) * 2 + s;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[vi][vt][e] = __builtin_fmaf(part[1 - pair][s][e], GATED && s == 1 ? sc_up[vt % 2] : sc[vt % 2], acc[vi][vt][e]);
+                asm volatile("" : "+v"(acc[vi][vt]));  // here, not where the compiler would like them: together at the end, out of registers
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        s_w = s_next;
+        s_up = s_up_next;
+    }
+    if constexpr (!GATED) write_group<WN, WM, TM, true>(p, acc, group_n, wn, wm, row0, rows, lane, memory);
+    else write_gated_group<WN, WM, TM>(p, acc, group_n, wn, wm, row0, rows, lane, memory);
+}
+
 int blocks_of(int v) { return v / kBlk + (v % kBlk != 0); }
 bool aligned(const void* p, uintptr_t to) { return (uintptr_t)p % to == 0; }
 bool sizes_ok(int n, int k) { return n > 0 && k > 0 && n <= (1 << 24) && k <= kMostStride; }
@@ -832,9 +870,9 @@ template <bool GATED>
 int launch_wide(exhip_ctx* ctx, const F8Params& p) {
     return launch(ctx, f8_wide_kernel<GATED>, p, 16, 256, 512);
 }
-template <int TN, int TM, int WN, int WK, bool GATED>
+template <int TN, int TM, int WN, int WK, int D, bool GATED>
 int launch_rows(exhip_ctx* ctx, const F8Params& p) {
-    return launch(ctx, f8_rows_kernel<TN, TM, WN, WK, GATED>, p, TN * WN, 16 * TM, 64 * WN * WK);
+    return launch(ctx, f8_rows_kernel<TN, TM, WN, WK, D, GATED>, p, TN * WN, 16 * TM, 64 * WN * WK);
 }
 template <int WN, int WM, int TM, bool GATED>
 int launch_tile(exhip_ctx* ctx, const F8Params& p) {
@@ -895,9 +933,26 @@ extern "C" int exhip_innerproduct_f8(exhip_ctx* ctx, const exhip_f8_desc* d, con
     p.bias = bias;
     p.y_f32 = y_f32;
     p.y_f16 = y_f16;
-    if (p.m <= 16) return launch_rows<4, 1, 1, 4, false>(ctx, p);
+    switch (g_exhip_options.f8_form) {
+    case 1: return launch_rows<1, 1, 1, 8, 4, false>(ctx, p);
+    case 2: return launch_rows<2, 1, 1, 8, 2, false>(ctx, p);
+    case 3: return launch_rows<4, 1, 1, 8, 2, false>(ctx, p);
+    case 4: return launch_rows<2, 2, 1, 8, 2, false>(ctx, p);
+    case 5: return launch_rows<4, 2, 1, 8, 1, false>(ctx, p);
+    case 6: return launch_rows<4, 4, 1, 8, 1, false>(ctx, p);
+    case 7: return launch_rows<4, 4, 1, 4, 1, false>(ctx, p);
+    case 8: return launch_rows<4, 4, 2, 4, 1, false>(ctx, p);
+    case 9: return launch_tile<2, 2, 2, false>(ctx, p);
+    case 10: return launch_tile<4, 1, 4, false>(ctx, p);
+    case 11: return launch_wide<false>(ctx, p);
+    case 12: return launch_rows<2, 4, 1, 8, 1, false>(ctx, p);
+    case 13: return launch_rows<1, 4, 1, 8, 2, false>(ctx, p);
+    case 14: return launch_rows<1, 2, 1, 8, 2, false>(ctx, p);
+    case 15: return launch_rows<1, 1, 1, 16, 2, false>(ctx, p);
+    }
+    if (p.m <= 16) return launch_rows<1, 1, 1, 8, 4, false>(ctx, p);
     if (!p.y_f32 && (long long)p.m * p.n >= 256ll * 256 * 128) return launch_wide<false>(ctx, p);
-    return (long long)p.m * p.n >= 256 * 128 * 256 ? launch_tile<4, 2, 4, false>(ctx, p) : launch_tile<2, 2, 2, false>(ctx, p);
+    return (long long)p.m * p.n >= 256 * 128 * 256 ? launch_tile<4, 1, 4, false>(ctx, p) : launch_tile<2, 2, 2, false>(ctx, p);
 }
 
 extern "C" int exhip_innerproduct_gated_f8(exhip_ctx* ctx, const exhip_f8_desc* d, int gate, const uint8_t* x, const float* x_scale, const void* w_packed,
@@ -920,8 +975,24 @@ extern "C" int exhip_innerproduct_gated_f8(exhip_ctx* ctx, const exhip_f8_desc* 
     p.y_f8 = y_f8;
     p.y_scale = y_scale;
     p.gate = gate;
-    if (p.m <= 16) return launch_rows<4, 1, 4, 2, true>(ctx, p);
+    switch (g_exhip_options.f8_form) {
+    case 1: return launch_rows<2, 1, 1, 8, 4, true>(ctx, p);
+    case 2: return launch_rows<2, 1, 1, 8, 2, true>(ctx, p);
+    case 3: return launch_rows<4, 1, 1, 8, 2, true>(ctx, p);
+    case 4: return launch_rows<2, 2, 1, 8, 2, true>(ctx, p);
+    case 5: return launch_rows<4, 2, 1, 8, 1, true>(ctx, p);
+    case 6: return launch_rows<4, 4, 1, 8, 1, true>(ctx, p);
+    case 7: return launch_rows<4, 4, 1, 4, 1, true>(ctx, p);
+    case 8: return launch_rows<4, 1, 4, 4, 2, true>(ctx, p);
+    case 9: return launch_tile<2, 2, 2, true>(ctx, p);
+    case 10: return launch_tile<4, 1, 4, true>(ctx, p);
+    case 11: return launch_wide<true>(ctx, p);
+    case 12: return launch_rows<2, 4, 1, 8, 1, true>(ctx, p);
+    case 13: return launch_rows<2, 1, 8, 2, 2, true>(ctx, p);
+    case 14: return launch_rows<4, 4, 4, 2, 1, true>(ctx, p);
+    }
+    if (p.m <= 16) return p.y_f8 ? launch_rows<4, 1, 4, 4, 2, true>(ctx, p) : launch_rows<2, 1, 1, 8, 4, true>(ctx, p);
     if (!p.y_f8 && 2ll * p.m * p.n >= 256ll * 256 * 128) return launch_wide<true>(ctx, p);
-    if (2ll * p.m * p.n >= 256 * 128 * 256) return launch_tile<4, 2, 4, true>(ctx, p);
+    if (2ll * p.m * p.n >= 256 * 128 * 256) return launch_tile<4, 1, 4, true>(ctx, p);
     return p.y_f8 ? launch_tile<4, 1, 4, true>(ctx, p) : launch_tile<2, 2, 2, true>(ctx, p);
 }
