@@ -184,25 +184,18 @@ __device__ __forceinline__ v4f block_product(const Halves& w, const Halves& x) {
     return c;
 }
 
-// Four neighbouring outputs of a row.
-__device__ __forceinline__ void store_outputs(const F8Params& p, int row, int j, v4f v) {
-    const size_t at = (size_t)row * p.y_stride + j;
-    const bool whole = j + 4 <= p.n && p.y_stride % 4 == 0;
-    if (p.y_f32) {
-        if (whole && ((uintptr_t)p.y_f32 & 15) == 0) *reinterpret_cast<v4f*>(p.y_f32 + at) = v;
-        else
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (j + e < p.n) p.y_f32[at + e] = v[e];
-    }
-    if (p.y_f16) {
-        const v4h h = __builtin_convertvector(v, v4h);
-        if (whole && ((uintptr_t)p.y_f16 & 7) == 0) *reinterpret_cast<v4h*>(p.y_f16 + at) = h;
-        else
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (j + e < p.n) p.y_f16[at + e] = exhip_f2h(v[e]);
-    }
+// Four neighbouring outputs of a row at any alignment of their type, and the first of them where the row ends.
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef _Float16 v4h_any __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ void store_cut(float* y, v4f v, int left) {
+    y[0] = v[0];
+    if (left > 1) y[1] = v[1];
+    if (left > 2) y[2] = v[2];
+}
+__device__ __forceinline__ void store_cut(uint16_t* y, v4f v, int left) {
+    y[0] = exhip_f2h(v[0]);
+    if (left > 1) y[1] = exhip_f2h(v[1]);
+    if (left > 2) y[2] = exhip_f2h(v[2]);
 }
 
 // ---- loads ----
@@ -251,29 +244,35 @@ __device__ __forceinline__ void tile_of(int groups_n, int groups_m, int* n, int*
 
 // ---- results of the kernels for many rows: through LDS, so that whole lines are stored ----
 // (A lane's four neighbouring outputs of one row, stored as they are, are 32 bytes of each of 16 rows at a time: 1.2 TB/s.)
-template <typename O>
-struct __attribute__((packed, aligned(sizeof(O)))) Piece {  // 16 bytes of results at any alignment of their type
-    O v[16 / sizeof(O)];
-};
 // Row-major results of a group: rows of WIDTH outputs, 16-byte pieces at place piece ^ (row % 8).
 template <typename O, int WIDTH>
 __device__ __forceinline__ char* place_in_rows(char* lds, int row, int j) {
     const int byte = j * (int)sizeof(O);
     return lds + row * (WIDTH * (int)sizeof(O)) + ((byte / 16) ^ (row & 7)) * 16 + byte % 16;
 }
+typedef int v4i_any __attribute__((ext_vector_type(4), aligned(1)));
+// (Nothing but whole pieces in the loop: code that a group runs once comes from memory line by line, 1 us each where a branch leaves the straight line. With
+// the cut pieces inside it the same loop took 2 to 14 us a group, by the XCD. The stores go past L2: 8192 x 8192 x 4096 263 -> 237 us.)
 template <typename O, int WIDTH, int ROWS, int THREADS>
 __device__ __forceinline__ void store_rows(const char* lds, O* y, size_t stride, int row0, int rows, int j0, int n) {
-    constexpr int kPer = 16 / sizeof(O), kPieces = WIDTH / kPer;
-    static_assert(ROWS * kPieces % THREADS == 0 && kPieces >= 8, "every thread stores the same, and eight rows' pieces lie in different banks");
+    constexpr int kPer = 16 / sizeof(O), kPieces = WIDTH / kPer, kPitch = WIDTH * (int)sizeof(O), kTogether = THREADS / kPieces;
+    static_assert(THREADS % kPieces == 0 && ROWS % kTogether == 0 && kPieces >= 8, "every thread stores one piece of every kTogether-th row; eight rows' pieces lie in different banks");
+    const int piece = threadIdx.x % kPieces, first = threadIdx.x / kPieces, j = j0 + piece * kPer;
+    O* const dst = y + (size_t)(row0 + first) * stride + j;
+    const size_t step = (size_t)kTogether * stride;
+    const bool whole = j + kPer <= n;
 #pragma unroll 4
-    for (int i = 0; i < ROWS * kPieces / THREADS; ++i) {
-        const int at = i * THREADS + threadIdx.x, row = at / kPieces, piece = at % kPieces, j = j0 + piece * kPer;
-        if (row >= rows || j >= n) continue;
-        const Piece<O> v = *reinterpret_cast<const Piece<O>*>(lds + row * (WIDTH * (int)sizeof(O)) + (piece ^ (row & 7)) * 16);
-        O* const dst = y + (size_t)(row0 + row) * stride + j;
-        if (j + kPer <= n) *reinterpret_cast<Piece<O>*>(dst) = v;
-        else
-            for (int e = 0; e < n - j; ++e) dst[e] = v.v[e];
+    for (int i = 0; i < ROWS / kTogether; ++i) {
+        const int row = i * kTogether + first;
+        const v4i v = *reinterpret_cast<const v4i*>(lds + row * kPitch + (piece ^ (row & 7)) * 16);
+        if (whole && row < rows) __builtin_nontemporal_store(v, reinterpret_cast<v4i_any*>(dst + i * step));
+    }
+    if (j0 + WIDTH > n && n % kPer != 0) {
+        const int at = n / kPer * kPer, left = n - at;
+        for (int i = threadIdx.x; i < rows * left; i += THREADS) {
+            const int row = i / left, e = i % left, byte = (at - j0) * (int)sizeof(O);
+            y[(size_t)(row0 + row) * stride + at + e] = reinterpret_cast<const O*>(lds + row * kPitch + ((byte / 16) ^ (row & 7)) * 16)[e];
+        }
     }
 }
 __device__ __forceinline__ v4f four_of(const float* v, int j, int n) {
@@ -390,6 +389,7 @@ __device__ __forceinline__ void write_gated_group(const F8Params& p, v4f (&acc)[
 // there, so that a block's end waits for nothing.
 template <bool GATED>
 __global__ __launch_bounds__(512, 2) void f8_wide_kernel(const F8Params p) {
+    exhip_touch_args(p);
     constexpr int WN = 4, TN = 4, TM = 8, kRows = 256, kBuffers = 4, kCodes = kRows * kBlk, kBuffer = kCodes + kRows * 4, kLag = 3;
     __shared__ __attribute__((aligned(16))) char staged[kBuffers * kBuffer];
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)staged;
@@ -520,7 +520,8 @@ __global__ __launch_bounds__(512, 2) void f8_wide_kernel(const F8Params p) {
 // a wave joins a share of the tiles, always in the order of wk, and writes them.
 template <int TN, int TM, int WN, int WK, int D, bool GATED>
 __global__ __launch_bounds__(64 * WN * WK, 2) void f8_rows_kernel(const F8Params p) {
-    constexpr int kRows = 16 * TM, kSide = GATED ? 2 : 1, kUnits = TN / kSide * TM;  // a unit: a tile, or both sides of one
+    exhip_touch_args(p);
+    constexpr int kRows = 16 * TM, kSide = GATED ? 2 : 1;
     static_assert(TN % kSide == 0, "both sides of an output are one wave's");
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wn = wave % WN, wk = wave / WN;
     const int q = lane / 16, col = lane % 16;
@@ -606,80 +607,54 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void f8_rows_kernel(const F8Params
             }
         }
     }
-    // unit u (tile i, rows t; both sides of a gated one) is joined by wave u % WK
-    if constexpr (WK > 1) {
-        __shared__ v4f joined[WK][WN][kUnits * kSide][64];
+    // The waves' sums meet in LDS, row by row (four floats more a row, for the banks), and every thread joins four neighbouring outputs in the order of wk.
+    constexpr int kWidth = WN * TN * 16, kPitch = kWidth + 4, kThreads = 64 * WN * WK, kQuads = kWidth / 4 / kSide;
+    __shared__ __attribute__((aligned(16))) float joined[WK][kRows][kPitch];
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u)
-            if (u % WK != wk)
+    for (int i = 0; i < TN; ++i)
 #pragma unroll
-                for (int o = 0; o < kSide; ++o) joined[wk][wn][u * kSide + o][lane] = acc[u / TM * kSide + o][u % TM];
-        __syncthreads();
+        for (int t = 0; t < TM; ++t) *reinterpret_cast<v4f*>(&joined[wk][16 * t + col][(wn * TN + i) * 16 + q * 4]) = acc[i][t];
+    __syncthreads();
+    const int j0 = group_n * (kWidth / kSide);
+    static_assert(kThreads % kQuads == 0, "a thread has the same outputs of all its rows");
+    const int quad = threadIdx.x % kQuads, j = j0 + quad * 4;
+    const v4f bias = four_of(p.bias, j, p.n), bias_up = GATED ? four_of(p.bias_up, j, p.n) : bias;
+    for (int row = threadIdx.x / kQuads; row < kRows; row += kThreads / kQuads) {
+        v4f v = {0.f, 0.f, 0.f, 0.f}, up = v;
+        const int at = GATED ? quad / 4 * 32 + quad % 4 * 4 : quad * 4;
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u)
-            if (u % WK == wk)
-#pragma unroll
-                for (int o = 0; o < kSide; ++o) {
-                    v4f sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int k = 0; k < WK; ++k) sum += k == u % WK ? acc[u / TM * kSide + o][u % TM] : joined[k][wn][u * kSide + o][lane];
-                    acc[u / TM * kSide + o][u % TM] = sum;
-                }
-    }
-    if constexpr (!GATED) {
-#pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
-            const int j = (tile0 + u / TM) * 16 + q * 4, row = u % TM * 16 + col;
-            if (u % WK == wk && j < p.n && row < rows) store_outputs(p, row0 + row, j, acc[u / TM][u % TM] + four_of(p.bias, j, p.n));
+        for (int k = 0; k < WK; ++k) {
+            v += *reinterpret_cast<const v4f*>(&joined[k][row][at]);
+            if constexpr (GATED) up += *reinterpret_cast<const v4f*>(&joined[k][row][at + 16]);
         }
-    } else {
-        v4f h[kUnits];
+        v += bias;
+        if constexpr (GATED) {
+            up += bias_up;
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
-            const int j = (tile0 / 2 + u / TM) * 16 + q * 4, row = u % TM * 16 + col;
-            h[u] = v4f{0.f, 0.f, 0.f, 0.f};
-            if (u % WK != wk) continue;
-            const v4f g = acc[u / TM * 2][u % TM] + four_of(p.bias, j, p.n), up = acc[u / TM * 2 + 1][u % TM] + four_of(p.bias_up, j, p.n);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) h[u][e] = j + e < p.n ? gated(p.gate, g[e], up[e]) : 0.f;
-            if (p.y_f16 && j < p.n && row < rows) store_outputs(p, row0 + row, j, h[u]);
+            for (int e = 0; e < 4; ++e) v[e] = j + e < p.n ? gated(p.gate, v[e], up[e]) : 0.f;
         }
-        if constexpr (WN * TN == 16) {  // the group's outputs are one block of a quantized result
-            if (!p.y_f8) return;
-            __shared__ float most[WN * WK][kRows];
+        const size_t to = (size_t)(row0 + row) * p.y_stride + j;
+        const bool here = row < rows && j < p.n, whole = here && j + 4 <= p.n;
+        if constexpr (GATED && kWidth == 256) {  // 32 lanes have a row's whole block of a quantized result
+            if (p.y_f8) {
+                float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
 #pragma unroll
-            for (int t = 0; t < TM; ++t) {
-                float a = 0.f;
-#pragma unroll
-                for (int u = t; u < kUnits; u += TM)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) a = fmaxf(a, fabsf(h[u][e]));
-                a = fmaxf(a, __shfl_xor(a, 16));
-                a = fmaxf(a, __shfl_xor(a, 32));
-                if (q == 0) most[wave][16 * t + col] = a;
+                for (int d = 1; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+                const float scale = scale_of(most), r = 1.f / scale;
+                const int code = four_codes(v[0] * r, v[1] * r, v[2] * r, v[3] * r);
+                if (row < rows && quad == 0) p.y_scale[(size_t)group_n * p.m + row0 + row] = scale;
+                if (whole) *reinterpret_cast<int*>(p.y_f8 + to) = code;
+                else if (here)
+                    for (int e = 0; j + e < p.n; ++e) p.y_f8[to + e] = (uint8_t)(code >> (8 * e));
             }
-            __syncthreads();
-#pragma unroll
-            for (int t = 0; t < TM; ++t) {
-                const int row = 16 * t + col;
-                float top = 0.f;
-#pragma unroll
-                for (int o = 0; o < WN * WK; ++o) top = fmaxf(top, most[o][row]);
-                const float scale = scale_of(top), r = 1.f / scale;
-                if (wave == 0 && q == 0 && row < rows) p.y_scale[(size_t)group_n * p.m + row0 + row] = scale;
-#pragma unroll
-                for (int u = t; u < kUnits; u += TM) {
-                    const int j = (tile0 / 2 + u / TM) * 16 + q * 4;
-                    if (u % WK != wk || row >= rows) continue;
-                    const int code = four_codes(h[u][0] * r, h[u][1] * r, h[u][2] * r, h[u][3] * r);
-                    uint8_t* const dst = p.y_f8 + (size_t)(row0 + row) * p.y_stride + j;
-                    if (j + 4 <= p.n) *reinterpret_cast<int*>(dst) = code;
-                    else
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (j + e < p.n) dst[e] = (uint8_t)(code >> (8 * e));
-                }
-            }
+        }
+        if (!GATED && p.y_f32) {
+            if (whole) *reinterpret_cast<v4f_any*>(p.y_f32 + to) = v;
+            else if (here) store_cut(p.y_f32 + to, v, p.n - j);
+        }
+        if (p.y_f16) {
+            if (whole) *reinterpret_cast<v4h_any*>(p.y_f16 + to) = __builtin_convertvector(v, v4h);
+            else if (here) store_cut(p.y_f16 + to, v, p.n - j);
         }
     }
 }
@@ -691,6 +666,7 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void f8_rows_kernel(const F8Params
 // barrier in the block's middle says that the next block's rows are there.
 template <int WN, int WM, int TM, bool GATED>
 __global__ __launch_bounds__(64 * WN * WM, 2) void f8_tile_kernel(const F8Params p) {
+    exhip_touch_args(p);
     constexpr int TN = 4, kRows = 16 * TM * WM, kThreads = 64 * WN * WM, kSteps = 8 * TM, kBuffers = 4, kPitch = 272, kBuffer = kRows * (kPitch + 4);
     static_assert(kRows * 4 == kThreads, "a thread stages a quarter of a row");
     // [buffer][row][16 pieces of 16 bytes]: piece 4 s + q of a row is halves_of()'s piece s of lanes of quarter q. A row's pitch is 16 bytes more, so that a
@@ -812,6 +788,208 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void f8_tile_kernel(const F8Params
     else write_gated_group<WN, WM, TM>(p, acc, group_n, wn, wm, row0, rows, lane, memory);
 }
 
+// ---- a tile or two for every CU ----
+// Between the two: a group of 2 x 2 waves takes 128 outputs and 128 rows, a wave 64 x 64, and both operands' codes come straight into LDS, three blocks ahead in
+// four buffers (all the LDS that a CU has), so that a CU with one group does not wait for memory block by block. EXACT: codes become halves in registers.
+template <bool EXACT, bool GATED>
+__global__ __launch_bounds__(256, 1) void f8_deep_kernel(const F8Params p) {
+    exhip_touch_args(p);
+    constexpr int WN = 2, WM = 2, TN = 4, TM = 4, kRows = 128, kBuffers = 4, kWeights = 16384, kCodes = kRows * kBlk, kBuffer = kWeights + kCodes + kRows * 4;
+    __shared__ __attribute__((aligned(16))) char staged[kBuffers * kBuffer];
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)staged;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wn = wave % WN, wm = wave / WN;
+    const int q = lane / 16, col = lane % 16;
+    int group_n, group_m;
+    tile_of(p.groups_n, p.groups_m, &group_n, &group_m);
+    const int tile0 = (group_n * WN + wn) * TN, row0 = group_m * kRows;
+    const int rows = min(kRows, p.m - row0), tail = p.k % kBlk, blocks = p.blocks_k;
+    const __amdgpu_buffer_rsrc_t xr = uniform_view(p.x + (size_t)row0 * p.x_stride, (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16);
+    // A wave stages 32 rows, eight with a load (as in f8_wide_kernel), and two of the group's eight tiles of weights, half of one with a load.
+    const int piece = (lane % 8) ^ (lane / 8);
+    const bool behind = tail && piece * 16 >= tail;
+    int off[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int row = wave * 32 + j * 8 + lane / 8;
+        off[j] = row < rows ? row * p.x_stride + piece * 16 : kNoRow;
+    }
+    const int scale_off = min(wave % 2 * 64 + lane, rows - 1) * 4;
+    const WeightRows weights(p, group_n * WN * TN + wave * 2, 2, lane);
+    auto stage = [&](int buffer, int j) {  // in nine loads; behind the last block that one again, which nothing reads
+        const int b = min(buffer, blocks - 1);
+        const unsigned to = lds0 + buffer % kBuffers * kBuffer;
+        if (j < 4) load16_to_lds(weights.view, weights.at + min(j / 2, weights.last - weights.first) * weights.row_bytes + b * 2048 + j % 2 * 1024, to + (wave * 4 + j) * 1024);
+        else if (j < 8) load16_to_lds(xr, behind && b == blocks - 1 ? kNoRow : off[j - 4] + b * kBlk, to + kWeights + (wave * 32 + (j - 4) * 8) * kBlk);
+        else load4_to_lds(uniform_view(p.x_scale + (size_t)b * p.m + row0, rows * 4), scale_off, to + kWeights + kCodes + wave % 2 * 256);
+    };
+    const int block_n = min(GATED ? tile0 / 2 : tile0, (p.n - 1) / 16) / (kBlk / 16);
+    const Constants ws = (Constants)(uintptr_t)(p.w_scale + (size_t)block_n * blocks);
+    const Constants ws_up = (Constants)(uintptr_t)(GATED ? p.w_scale_up + (size_t)block_n * blocks : nullptr);
+    const int at_w = wn * 8192 + lane * 16;
+    auto weights_from = [&](int b, int i) {
+        const char* const from = staged + b % kBuffers * kBuffer + at_w + i * 2048;
+        return both(*reinterpret_cast<const v4i*>(from), *reinterpret_cast<const v4i*>(from + 1024));
+    };
+    const int at = kWeights + (wm * TM * 16 + col) * kBlk + (q ^ (col & 7)) * 16, at_hi = kWeights + (wm * TM * 16 + col) * kBlk + (q ^ (col & 7) ^ 4) * 16;
+    const int at_scale = kWeights + kCodes + (wm * TM * 16 + col) * 4;
+    struct Rows {
+        v8i v;
+        float s;
+    };
+    auto rows_from = [&](int b, int t) {
+        const char* const from = staged + b % kBuffers * kBuffer;
+        return Rows{both(*reinterpret_cast<const v4i*>(from + at + t * 16 * kBlk), *reinterpret_cast<const v4i*>(from + at_hi + t * 16 * kBlk)),
+                    *reinterpret_cast<const float*>(from + at_scale + t * 64)};
+    };
+    v4f acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int t = 0; t < TM; ++t) acc[i][t] = v4f{0.f, 0.f, 0.f, 0.f};
+    auto arrive = [&]() {
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    auto cut_row_end = [&](int b) {  // the piece that a row's end cuts
+        if (p.k % 16 && b == blocks - 1) {
+            if (threadIdx.x < kRows) {
+                v4i* const cut = reinterpret_cast<v4i*>(staged + b % kBuffers * kBuffer + kWeights + threadIdx.x * kBlk + ((tail / 16) ^ (threadIdx.x & 7)) * 16);
+                *cut &= keep_first(tail % 16);
+            }
+            __syncthreads();
+            return true;
+        }
+        return false;
+    };
+#pragma unroll
+    for (int j = 0; j < 27; ++j) stage(j / 9, j % 9);
+    asm volatile("s_waitcnt vmcnt(18)" ::: "memory");
+    arrive();
+    float s_w = ws[0], s_up = GATED ? ws_up[0] : 0.f, s_next = 0.f, s_up_next = 0.f;
+    if constexpr (!EXACT) {
+        struct Weights {
+            v8i v[TN];
+        } w0, w1;
+#pragma unroll
+        for (int i = 0; i < TN; ++i) w0.v[i] = weights_from(0, i);
+        Rows x[2];
+        x[0] = rows_from(0, 0);
+        constexpr int kLag = 3, kSteps = TN * TM;
+        auto block = [&](Weights& w, Weights& next, int b) {
+            if (cut_row_end(b)) x[0] = rows_from(b, 0);
+            v4f part[kLag + 1];
+            float s[2], su[2];
+#pragma unroll
+            for (int u = 0; u < kSteps + kLag; ++u) {
+                const int t = u / TN, i = u % TN;
+                if (u == kSteps / 2) {
+                    asm volatile("s_waitcnt vmcnt(9)" ::: "memory");  // the next block's are there, the one's behind it are on their way
+                    arrive();
+                    const int after = min(b + 1, blocks - 1);
+                    s_next = ws[after];
+                    if constexpr (GATED) s_up_next = ws_up[after];
+                }
+                if (u >= kSteps / 2 && u < kSteps / 2 + 8) {
+                    stage(b + 3, u - kSteps / 2);
+                    if (u == kSteps / 2 + 7) stage(b + 3, 8);
+                }
+                if (u >= kSteps / 2 + 2 && u < kSteps / 2 + 6) next.v[u - kSteps / 2 - 2] = weights_from(b + 1, u - kSteps / 2 - 2);
+                if (u < kSteps) {
+                    if (i == 0) {
+                        s[t % 2] = s_w * x[t % 2].s;
+                        su[t % 2] = s_up * x[t % 2].s;
+                        x[(t + 1) % 2] = t + 1 < TM ? rows_from(b, t + 1) : rows_from(b + 1, 0);
+                    }
+                    part[u % (kLag + 1)] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v[i], x[t % 2].v, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+                }
+                if (u >= kLag) {
+                    const int v = u - kLag, vt = v / TN, vi = v % TN;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[vi][vt][e] = __builtin_fmaf(part[v % (kLag + 1)][e], GATED && vi % 2 ? su[vt % 2] : s[vt % 2], acc[vi][vt][e]);
+                    asm volatile("" : "+v"(acc[vi][vt]));
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            s_w = s_next;
+            s_up = s_up_next;
+        };
+        for (int b = 0; b < blocks; b += 2) {
+            block(w0, w1, b);
+            if (b + 1 < blocks) block(w1, w0, b + 1);
+        }
+    } else {
+        constexpr int kSteps = 8 * TM;
+        v8i raw[TN];
+        Halves w[TN], x[2];
+        Rows next_x;
+        float x_scale[2];
+        auto half_of = [&](const v8i& c, int s) { return halves_of(c[s], c[4 + s]); };
+#pragma unroll
+        for (int i = 0; i < TN; ++i) raw[i] = weights_from(0, i);
+        cut_row_end(0);
+        next_x = rows_from(0, 0);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            w[0].v[s] = half_of(raw[0], s);
+            w[1].v[s] = half_of(raw[1], s);
+            x[0].v[s] = half_of(next_x.v, s);
+        }
+        x_scale[0] = next_x.s;
+        for (int b = 0; b < blocks; ++b) {
+            v4f part[2][2];
+            float sc[2], sc_up[2];
+#pragma unroll
+            for (int u = 0; u < kSteps + 2; ++u) {
+                const int t = u / 8, pair = u / 4 % 2, s = u % 4;
+                if (u < 4) {
+                    w[2].v[u] = half_of(raw[2], u);
+                    w[3].v[u] = half_of(raw[3], u);
+                }
+                if (u == kSteps / 2) {
+                    asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
+                    arrive();
+                    const int after = min(b + 1, blocks - 1);
+                    s_next = ws[after];
+                    if constexpr (GATED) s_up_next = ws_up[after];
+                    cut_row_end(b + 1);
+                }
+                if (u >= kSteps / 2 && u < kSteps / 2 + 9) stage(b + 3, u - kSteps / 2);
+                if (u >= kSteps - 10 && u < kSteps - 6) raw[u - kSteps + 10] = weights_from(b + 1, u - kSteps + 10);
+                if (u >= kSteps - 4 && u < kSteps) {
+                    w[0].v[s] = half_of(raw[0], s);
+                    w[1].v[s] = half_of(raw[1], s);
+                }
+                if (u < kSteps) {
+                    if (u % 8 == 0) {
+                        sc[t % 2] = s_w * x_scale[t % 2];
+                        sc_up[t % 2] = s_up * x_scale[t % 2];
+                        next_x = t + 1 < TM ? rows_from(b, t + 1) : rows_from(b + 1, 0);
+                    }
+                    if (u % 8 >= 4) {
+                        x[(t + 1) % 2].v[s] = half_of(next_x.v, s);
+                        if (s == 0) x_scale[(t + 1) % 2] = next_x.s;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        part[pair][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[2 * pair + i].v[s], x[t % 2].v[s], s == 0 ? v4f{0.f, 0.f, 0.f, 0.f} : part[pair][i], 0, 0, 0);
+                }
+                if (u >= 4 && s < 2) {  // of the pair before, a tile a step
+                    const int vt = (u - 4) / 8, vi = (1 - pair) * 2 + s;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[vi][vt][e] = __builtin_fmaf(part[1 - pair][s][e], GATED && s == 1 ? sc_up[vt % 2] : sc[vt % 2], acc[vi][vt][e]);
+                    asm volatile("" : "+v"(acc[vi][vt]));
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            s_w = s_next;
+            s_up = s_up_next;
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was staged behind the end, in front of the results' barrier
+    if constexpr (!GATED) write_group<WN, WM, TM, EXACT>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
+    else write_gated_group<WN, WM, TM>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
+}
+
 int blocks_of(int v) { return v / kBlk + (v % kBlk != 0); }
 bool aligned(const void* p, uintptr_t to) { return (uintptr_t)p % to == 0; }
 bool sizes_ok(int n, int k) { return n > 0 && k > 0 && n <= (1 << 24) && k <= kMostStride; }
@@ -865,6 +1043,10 @@ int launch(exhip_ctx* ctx, K kernel, F8Params p, int tiles, int rows, int thread
     hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(threads), 0, ctx->stream, p);
     EXHIP_LAUNCH_CHECK();
     return 0;
+}
+template <bool EXACT, bool GATED>
+int launch_deep(exhip_ctx* ctx, const F8Params& p) {
+    return launch(ctx, f8_deep_kernel<EXACT, GATED>, p, 8, 128, 256);
 }
 template <bool GATED>
 int launch_wide(exhip_ctx* ctx, const F8Params& p) {
@@ -949,6 +1131,8 @@ extern "C" int exhip_innerproduct_f8(exhip_ctx* ctx, const exhip_f8_desc* d, con
     case 13: return launch_rows<1, 4, 1, 8, 2, false>(ctx, p);
     case 14: return launch_rows<1, 2, 1, 8, 2, false>(ctx, p);
     case 15: return launch_rows<1, 1, 1, 16, 2, false>(ctx, p);
+    case 16: return launch_deep<true, false>(ctx, p);
+    case 17: return launch_deep<false, false>(ctx, p);
     }
     if (p.m <= 16) return launch_rows<1, 1, 1, 8, 4, false>(ctx, p);
     if (!p.y_f32 && (long long)p.m * p.n >= 256ll * 256 * 128) return launch_wide<false>(ctx, p);
@@ -990,6 +1174,8 @@ extern "C" int exhip_innerproduct_gated_f8(exhip_ctx* ctx, const exhip_f8_desc* 
     case 12: return launch_rows<2, 4, 1, 8, 1, true>(ctx, p);
     case 13: return launch_rows<2, 1, 8, 2, 2, true>(ctx, p);
     case 14: return launch_rows<4, 4, 4, 2, 1, true>(ctx, p);
+    case 16: return launch_deep<true, true>(ctx, p);
+    case 17: return launch_deep<false, true>(ctx, p);
     }
     if (p.m <= 16) return p.y_f8 ? launch_rows<4, 1, 4, 4, 2, true>(ctx, p) : launch_rows<2, 1, 1, 8, 4, true>(ctx, p);
     if (!p.y_f8 && 2ll * p.m * p.n >= 256ll * 256 * 128) return launch_wide<true>(ctx, p);

@@ -146,6 +146,7 @@ __device__ void write_row(const T* __restrict__ src, const LogpParams& p, size_t
 // A group of W waves a slice of a row, V values a thread, all requested before the first is used.
 template <typename T, int W, int V, bool TOP>
 __global__ __launch_bounds__(64 * W, W == 16 ? 8 : 4) void log_probabilities_kernel(const T* __restrict__ x, const LogpParams p) {
+    exhip_touch_args(p);
     constexpr int kThreads = 64 * W, N = 16 / sizeof(T), kRuns = V / N;
     __shared__ Sums sums[W];
     __shared__ float bounds[W];
@@ -344,6 +345,7 @@ __device__ void join_lists(const u64* __restrict__ from, size_t total, int top, 
 // The slices of a row, joined by one wave.
 template <typename T>
 __global__ __launch_bounds__(64) void join_slices_kernel(const T* __restrict__ x, const LogpParams p) {
+    exhip_touch_args(p);
     __shared__ u64 places[512 + 8], sorted[EXHIP_LOG_PROBABILITIES_TOP];
     const int lane = threadIdx.x;
     const size_t row = blockIdx.x;
