@@ -201,18 +201,16 @@ __device__ __forceinline__ void store_cut(uint16_t* y, v4f v, int left) {
 // ---- loads ----
 typedef int v8i __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ v8i both(v4i a, v4i b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
-// One 16-byte (4-byte) element per lane from a bounds-checked view straight into LDS, lane l's at lds + 16 l (4 l); lds is the wave's, in M0. vmcnt counts
-// them like any other load. The views and addresses are pinned to scalar registers for the inline assembly.
-__device__ __forceinline__ void load16_to_lds(__amdgpu_buffer_rsrc_t view, int off, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(view) : "m0", "memory");
+// One 16-byte (4-byte) element per lane from a bounds-checked view straight into LDS, lane l's at lds + 16 l (4 l); lds is the wave's, and so is `more`, an
+// offset beside the lane's. vmcnt counts them like any other load. (The bounds need not see `more`: lanes with nothing to load have kNoRow.)
+__device__ __forceinline__ void load16_to_lds(__amdgpu_buffer_rsrc_t view, int off, int more, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(off), "s"(view), "s"(more) : "m0", "memory");
 }
 __device__ __forceinline__ void load4_to_lds(__amdgpu_buffer_rsrc_t view, int off, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(view) : "m0", "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(view) : "m0", "memory");
 }
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t uniform_view(const void* base, unsigned range) {
-    const unsigned long long a = (unsigned long long)(uintptr_t)base;
-    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)a), hi = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
-    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>((uintptr_t)(((unsigned long long)hi << 32) | lo)), 0, __builtin_amdgcn_readfirstlane(range), kRsrcWord3);
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t uniform_view(const void* base, unsigned range) {  // base and range are the wave's
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, range, kRsrcWord3);
 }
 
 // Of a wave's own, by scalar loads: a vector load's wait would be one for what else is on its way too.
@@ -415,7 +413,7 @@ __global__ __launch_bounds__(512, 2) void f8_wide_kernel(const F8Params p) {
     auto stage = [&](int buffer, int j) {  // in five loads
         const int b = min(buffer, blocks - 1);
         const unsigned to = lds0 + buffer % kBuffers * kBuffer;
-        if (j < 4) load16_to_lds(xr, behind && b == blocks - 1 ? kNoRow : off[j] + b * kBlk, to + (wave * 32 + j * 8) * kBlk);
+        if (j < 4) load16_to_lds(xr, behind && b == blocks - 1 ? kNoRow : off[j], b * kBlk, to + (wave * 32 + j * 8) * kBlk);
         else load4_to_lds(uniform_view(p.x_scale + (size_t)b * p.m + row0, rows * 4), scale_off, to + kCodes + wave % 4 * 256);
     };
     const WeightRows weights(p, tile0, TN, lane);
@@ -789,12 +787,13 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void f8_tile_kernel(const F8Params
 }
 
 // ---- a tile or two for every CU ----
-// Between the two: a group of 2 x 2 waves takes 128 outputs and 128 rows, a wave 64 x 64, and both operands' codes come straight into LDS, three blocks ahead in
-// four buffers (all the LDS that a CU has), so that a CU with one group does not wait for memory block by block. EXACT: codes become halves in registers.
-template <bool EXACT, bool GATED>
-__global__ __launch_bounds__(256, 1) void f8_deep_kernel(const F8Params p) {
+// Between the two: a group of 2 x 4 waves takes 128 outputs and 128 rows, a wave 64 x 32, and both operands' codes come straight into LDS, three blocks ahead in
+// four buffers (all the LDS that a CU has), so that a CU with one group does not wait for memory block by block.
+// (2 x 2 waves of 64 x 64, one for each SIMD, take longer: 330 instructions a block, of which a wave alone issues one in 4.5 cycles.)
+template <bool GATED>
+__global__ __launch_bounds__(512, 2) void f8_deep_kernel(const F8Params p) {
     exhip_touch_args(p);
-    constexpr int WN = 2, WM = 2, TN = 4, TM = 4, kRows = 128, kBuffers = 4, kWeights = 16384, kCodes = kRows * kBlk, kBuffer = kWeights + kCodes + kRows * 4;
+    constexpr int WN = 2, WM = 4, TN = 4, TM = 2, kRows = 128, kLoads = 5, kBuffers = 4, kWeights = 16384, kCodes = kRows * kBlk, kBuffer = kWeights + kCodes + kRows * 4;
     __shared__ __attribute__((aligned(16))) char staged[kBuffers * kBuffer];
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)staged;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wn = wave % WN, wm = wave / WN;
@@ -804,22 +803,22 @@ __global__ __launch_bounds__(256, 1) void f8_deep_kernel(const F8Params p) {
     const int tile0 = (group_n * WN + wn) * TN, row0 = group_m * kRows;
     const int rows = min(kRows, p.m - row0), tail = p.k % kBlk, blocks = p.blocks_k;
     const __amdgpu_buffer_rsrc_t xr = uniform_view(p.x + (size_t)row0 * p.x_stride, (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16);
-    // A wave stages 32 rows, eight with a load (as in f8_wide_kernel), and two of the group's eight tiles of weights, half of one with a load.
+    // A wave stages 16 rows, eight with a load (as in f8_wide_kernel), and one of the group's eight tiles of weights.
     const int piece = (lane % 8) ^ (lane / 8);
     const bool behind = tail && piece * 16 >= tail;
-    int off[4];
+    int off[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int row = wave * 32 + j * 8 + lane / 8;
+    for (int j = 0; j < 2; ++j) {
+        const int row = wave * 16 + j * 8 + lane / 8;
         off[j] = row < rows ? row * p.x_stride + piece * 16 : kNoRow;
     }
     const int scale_off = min(wave % 2 * 64 + lane, rows - 1) * 4;
-    const WeightRows weights(p, group_n * WN * TN + wave * 2, 2, lane);
-    auto stage = [&](int buffer, int j) {  // in nine loads; behind the last block that one again, which nothing reads
+    const WeightRows weights(p, group_n * WN * TN + wave, 1, lane);
+    auto stage = [&](int buffer, int j) {  // in five loads; behind the last block that one again, which nothing reads
         const int b = min(buffer, blocks - 1);
         const unsigned to = lds0 + buffer % kBuffers * kBuffer;
-        if (j < 4) load16_to_lds(weights.view, weights.at + min(j / 2, weights.last - weights.first) * weights.row_bytes + b * 2048 + j % 2 * 1024, to + (wave * 4 + j) * 1024);
-        else if (j < 8) load16_to_lds(xr, behind && b == blocks - 1 ? kNoRow : off[j - 4] + b * kBlk, to + kWeights + (wave * 32 + (j - 4) * 8) * kBlk);
+        if (j < 2) load16_to_lds(weights.view, weights.at, b * 2048 + j * 1024, to + (wave * 2 + j) * 1024);
+        else if (j < 4) load16_to_lds(xr, behind && b == blocks - 1 ? kNoRow : off[j - 2], b * kBlk, to + kWeights + (wave * 16 + (j - 2) * 8) * kBlk);
         else load4_to_lds(uniform_view(p.x_scale + (size_t)b * p.m + row0, rows * 4), scale_off, to + kWeights + kCodes + wave % 2 * 256);
     };
     const int block_n = min(GATED ? tile0 / 2 : tile0, (p.n - 1) / 16) / (kBlk / 16);
@@ -850,7 +849,7 @@ __global__ __launch_bounds__(256, 1) void f8_deep_kernel(const F8Params p) {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    auto cut_row_end = [&](int b) {  // the piece that a row's end cuts
+    auto cut_row_end = [&](int b) {  // the piece that a row's end cuts; whether there is one
         if (p.k % 16 && b == blocks - 1) {
             if (threadIdx.x < kRows) {
                 v4i* const cut = reinterpret_cast<v4i*>(staged + b % kBuffers * kBuffer + kWeights + threadIdx.x * kBlk + ((tail / 16) ^ (threadIdx.x & 7)) * 16);
@@ -862,131 +861,59 @@ __global__ __launch_bounds__(256, 1) void f8_deep_kernel(const F8Params p) {
         return false;
     };
 #pragma unroll
-    for (int j = 0; j < 27; ++j) stage(j / 9, j % 9);
-    asm volatile("s_waitcnt vmcnt(18)" ::: "memory");
+    for (int j = 0; j < 3 * kLoads; ++j) stage(j / kLoads, j % kLoads);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads) : "memory");
     arrive();
     float s_w = ws[0], s_up = GATED ? ws_up[0] : 0.f, s_next = 0.f, s_up_next = 0.f;
-    if constexpr (!EXACT) {
-        struct Weights {
-            v8i v[TN];
-        } w0, w1;
+    struct Weights {
+        v8i v[TN];
+    } w0, w1;
 #pragma unroll
-        for (int i = 0; i < TN; ++i) w0.v[i] = weights_from(0, i);
-        Rows x[2];
-        x[0] = rows_from(0, 0);
-        constexpr int kLag = 3, kSteps = TN * TM;
-        auto block = [&](Weights& w, Weights& next, int b) {
-            if (cut_row_end(b)) x[0] = rows_from(b, 0);
-            v4f part[kLag + 1];
-            float s[2], su[2];
+    for (int i = 0; i < TN; ++i) w0.v[i] = weights_from(0, i);
+    Rows x[2];
+    x[0] = rows_from(0, 0);
+    constexpr int kLag = 3, kSteps = TN * TM;
+    auto block = [&](Weights& w, Weights& next, int b) {
+        if (cut_row_end(b)) x[0] = rows_from(b, 0);
+        v4f part[kLag + 1];
+        float s[2], su[2];
 #pragma unroll
-            for (int u = 0; u < kSteps + kLag; ++u) {
-                const int t = u / TN, i = u % TN;
-                if (u == kSteps / 2) {
-                    asm volatile("s_waitcnt vmcnt(9)" ::: "memory");  // the next block's are there, the one's behind it are on their way
-                    arrive();
-                    const int after = min(b + 1, blocks - 1);
-                    s_next = ws[after];
-                    if constexpr (GATED) s_up_next = ws_up[after];
-                }
-                if (u >= kSteps / 2 && u < kSteps / 2 + 8) {
-                    stage(b + 3, u - kSteps / 2);
-                    if (u == kSteps / 2 + 7) stage(b + 3, 8);
-                }
-                if (u >= kSteps / 2 + 2 && u < kSteps / 2 + 6) next.v[u - kSteps / 2 - 2] = weights_from(b + 1, u - kSteps / 2 - 2);
-                if (u < kSteps) {
-                    if (i == 0) {
-                        s[t % 2] = s_w * x[t % 2].s;
-                        su[t % 2] = s_up * x[t % 2].s;
-                        x[(t + 1) % 2] = t + 1 < TM ? rows_from(b, t + 1) : rows_from(b + 1, 0);
-                    }
-                    part[u % (kLag + 1)] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v[i], x[t % 2].v, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-                }
-                if (u >= kLag) {
-                    const int v = u - kLag, vt = v / TN, vi = v % TN;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[vi][vt][e] = __builtin_fmaf(part[v % (kLag + 1)][e], GATED && vi % 2 ? su[vt % 2] : s[vt % 2], acc[vi][vt][e]);
-                    asm volatile("" : "+v"(acc[vi][vt]));
-                }
-                __builtin_amdgcn_sched_barrier(0);
+        for (int u = 0; u < kSteps + kLag; ++u) {
+            const int t = u / TN, i = u % TN;
+            if (u == kSteps / 2) {
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");  // the next block's are there, the one's behind it are on their way
+                arrive();
+                const int after = min(b + 1, blocks - 1);
+                s_next = ws[after];
+                if constexpr (GATED) s_up_next = ws_up[after];
             }
-            s_w = s_next;
-            s_up = s_up_next;
-        };
-        for (int b = 0; b < blocks; b += 2) {
-            block(w0, w1, b);
-            if (b + 1 < blocks) block(w1, w0, b + 1);
-        }
-    } else {
-        constexpr int kSteps = 8 * TM;
-        v8i raw[TN];
-        Halves w[TN], x[2];
-        Rows next_x;
-        float x_scale[2];
-        auto half_of = [&](const v8i& c, int s) { return halves_of(c[s], c[4 + s]); };
-#pragma unroll
-        for (int i = 0; i < TN; ++i) raw[i] = weights_from(0, i);
-        cut_row_end(0);
-        next_x = rows_from(0, 0);
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            w[0].v[s] = half_of(raw[0], s);
-            w[1].v[s] = half_of(raw[1], s);
-            x[0].v[s] = half_of(next_x.v, s);
-        }
-        x_scale[0] = next_x.s;
-        for (int b = 0; b < blocks; ++b) {
-            v4f part[2][2];
-            float sc[2], sc_up[2];
-#pragma unroll
-            for (int u = 0; u < kSteps + 2; ++u) {
-                const int t = u / 8, pair = u / 4 % 2, s = u % 4;
-                if (u < 4) {
-                    w[2].v[u] = half_of(raw[2], u);
-                    w[3].v[u] = half_of(raw[3], u);
+            if (u >= kSteps / 2 && u < kSteps / 2 + kLoads) stage(b + 3, u - kSteps / 2);
+            if (u >= kSteps / 2 && u < kSteps / 2 + TN) next.v[u - kSteps / 2] = weights_from(b + 1, u - kSteps / 2);
+            if (u < kSteps) {
+                if (i == 0) {
+                    s[t % 2] = s_w * x[t % 2].s;
+                    su[t % 2] = s_up * x[t % 2].s;
+                    x[(t + 1) % 2] = t + 1 < TM ? rows_from(b, t + 1) : rows_from(b + 1, 0);
                 }
-                if (u == kSteps / 2) {
-                    asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
-                    arrive();
-                    const int after = min(b + 1, blocks - 1);
-                    s_next = ws[after];
-                    if constexpr (GATED) s_up_next = ws_up[after];
-                    cut_row_end(b + 1);
-                }
-                if (u >= kSteps / 2 && u < kSteps / 2 + 9) stage(b + 3, u - kSteps / 2);
-                if (u >= kSteps - 10 && u < kSteps - 6) raw[u - kSteps + 10] = weights_from(b + 1, u - kSteps + 10);
-                if (u >= kSteps - 4 && u < kSteps) {
-                    w[0].v[s] = half_of(raw[0], s);
-                    w[1].v[s] = half_of(raw[1], s);
-                }
-                if (u < kSteps) {
-                    if (u % 8 == 0) {
-                        sc[t % 2] = s_w * x_scale[t % 2];
-                        sc_up[t % 2] = s_up * x_scale[t % 2];
-                        next_x = t + 1 < TM ? rows_from(b, t + 1) : rows_from(b + 1, 0);
-                    }
-                    if (u % 8 >= 4) {
-                        x[(t + 1) % 2].v[s] = half_of(next_x.v, s);
-                        if (s == 0) x_scale[(t + 1) % 2] = next_x.s;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        part[pair][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[2 * pair + i].v[s], x[t % 2].v[s], s == 0 ? v4f{0.f, 0.f, 0.f, 0.f} : part[pair][i], 0, 0, 0);
-                }
-                if (u >= 4 && s < 2) {  // of the pair before, a tile a step
-                    const int vt = (u - 4) / 8, vi = (1 - pair) * 2 + s;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[vi][vt][e] = __builtin_fmaf(part[1 - pair][s][e], GATED && s == 1 ? sc_up[vt % 2] : sc[vt % 2], acc[vi][vt][e]);
-                    asm volatile("" : "+v"(acc[vi][vt]));
-                }
-                __builtin_amdgcn_sched_barrier(0);
+                part[u % (kLag + 1)] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v[i], x[t % 2].v, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
             }
-            s_w = s_next;
-            s_up = s_up_next;
+            if (u >= kLag) {
+                const int v = u - kLag, vt = v / TN, vi = v % TN;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[vi][vt][e] = __builtin_fmaf(part[v % (kLag + 1)][e], GATED && vi % 2 ? su[vt % 2] : s[vt % 2], acc[vi][vt][e]);
+                asm volatile("" : "+v"(acc[vi][vt]));
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
+        s_w = s_next;
+        s_up = s_up_next;
+    };
+    for (int b = 0; b < blocks; b += 2) {
+        block(w0, w1, b);
+        if (b + 1 < blocks) block(w1, w0, b + 1);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was staged behind the end, in front of the results' barrier
-    if constexpr (!GATED) write_group<WN, WM, TM, EXACT>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
+    if constexpr (!GATED) write_group<WN, WM, TM, false>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
     else write_gated_group<WN, WM, TM>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
 }
 
@@ -1044,21 +971,66 @@ int launch(exhip_ctx* ctx, K kernel, F8Params p, int tiles, int rows, int thread
     EXHIP_LAUNCH_CHECK();
     return 0;
 }
-template <bool EXACT, bool GATED>
-int launch_deep(exhip_ctx* ctx, const F8Params& p) {
-    return launch(ctx, f8_deep_kernel<EXACT, GATED>, p, 8, 128, 256);
-}
-template <bool GATED>
-int launch_wide(exhip_ctx* ctx, const F8Params& p) {
-    return launch(ctx, f8_wide_kernel<GATED>, p, 16, 256, 512);
-}
+
+// One way to run a product: the tiles of 16 outputs (of both projections) and the rows a group takes, how many groups the chip runs at once, how many waves share
+// a group's blocks, and what a launch takes: `round` us for the groups that run at once, and `block` for each block that one wave of theirs goes through.
+struct Form {
+    int (*run)(exhip_ctx*, const F8Params&);
+    int tiles, rows, at_once, split;
+    float start, round, block;
+};
 template <int TN, int TM, int WN, int WK, int D, bool GATED>
-int launch_rows(exhip_ctx* ctx, const F8Params& p) {
+int run_rows(exhip_ctx* ctx, const F8Params& p) {
     return launch(ctx, f8_rows_kernel<TN, TM, WN, WK, D, GATED>, p, TN * WN, 16 * TM, 64 * WN * WK);
 }
 template <int WN, int WM, int TM, bool GATED>
-int launch_tile(exhip_ctx* ctx, const F8Params& p) {
+int run_tile(exhip_ctx* ctx, const F8Params& p) {
     return launch(ctx, f8_tile_kernel<WN, WM, TM, GATED>, p, 4 * WN, 16 * TM * WM, 64 * WN * WM);
+}
+template <bool GATED>
+int run_deep(exhip_ctx* ctx, const F8Params& p) {
+    return launch(ctx, f8_deep_kernel<GATED>, p, 8, 128, 512);
+}
+template <bool GATED>
+int run_wide(exhip_ctx* ctx, const F8Params& p) {
+    return launch(ctx, f8_wide_kernel<GATED>, p, 16, 256, 512);
+}
+// The times are fits to 380 launches of 1 to 2048 rows and matrices from 256 x 512 to 8192 x 8192, on the GPU's clock: the form they choose takes 2 % longer than
+// the best one for the shape on average, 20 % at most.
+constexpr Form kExact[] = {  // results in float32
+    {run_rows<1, 1, 1, 8, 4, false>, 1, 16, 512, 8, 0.4f, 2.2f, 0.85f}, {run_rows<2, 1, 1, 8, 2, false>, 2, 16, 512, 8, 0.f, 2.9f, 0.86f},
+    {run_rows<2, 2, 1, 8, 2, false>, 2, 32, 256, 8, 1.4f, 1.3f, 1.42f}, {run_rows<4, 2, 1, 8, 1, false>, 4, 32, 256, 8, 0.7f, 2.4f, 1.65f},
+    {run_tile<2, 2, 2, false>, 8, 64, 512, 1, 0.f, 4.0f, 0.80f},        {run_tile<4, 1, 4, false>, 16, 64, 512, 1, 0.f, 4.8f, 1.08f},
+};
+constexpr Form kHalves[] = {
+    kExact[0], kExact[1], kExact[2], kExact[3], {run_deep<false>, 8, 128, 256, 1, 0.7f, 3.5f, 0.47f}, {run_wide<false>, 16, 256, 256, 1, 0.f, 6.0f, 1.18f},
+};
+constexpr Form kGatedHalves[] = {
+    {run_rows<2, 1, 1, 8, 2, true>, 2, 16, 512, 8, 0.f, 2.9f, 1.34f}, {run_rows<2, 2, 1, 8, 2, true>, 2, 32, 256, 8, 1.3f, 2.1f, 1.41f},
+    {run_rows<4, 2, 1, 8, 1, true>, 4, 32, 256, 8, 1.1f, 2.3f, 2.03f}, {run_deep<true>, 8, 128, 256, 1, 0.9f, 5.2f, 0.50f},
+    {run_wide<true>, 16, 256, 256, 1, 0.f, 14.2f, 1.29f},
+};
+constexpr Form kGatedCodes[] = {  // a group has whole blocks of the result: 16 tiles
+    {run_rows<4, 1, 4, 2, 2, true>, 16, 16, 256, 2, 0.f, 4.0f, 0.97f}, {run_rows<4, 2, 4, 2, 1, true>, 16, 32, 256, 2, 0.f, 5.2f, 1.40f},
+    {run_tile<4, 1, 4, true>, 16, 64, 512, 1, 0.f, 9.5f, 1.11f},
+};
+
+template <int N>
+int run_best(exhip_ctx* ctx, const F8Params& p, const Form (&forms)[N]) {
+    const int pinned = g_exhip_options.f8_form;
+    if (pinned > 0) return forms[(pinned < N ? pinned : N) - 1].run(ctx, p);
+    int best = 0;
+    float best_us = 0.f;
+    for (int i = 0; i < N; ++i) {
+        const Form& f = forms[i];
+        const long long groups = (long long)((p.tiles + f.tiles - 1) / f.tiles) * (p.m / f.rows + (p.m % f.rows != 0));
+        const float us = f.start + (float)((groups - 1) / f.at_once + 1) * (f.round + f.block * (float)((p.blocks_k - 1) / f.split + 1));
+        if (i == 0 || us < best_us) {
+            best = i;
+            best_us = us;
+        }
+    }
+    return forms[best].run(ctx, p);
 }
 
 }  // namespace
@@ -1115,28 +1087,7 @@ extern "C" int exhip_innerproduct_f8(exhip_ctx* ctx, const exhip_f8_desc* d, con
     p.bias = bias;
     p.y_f32 = y_f32;
     p.y_f16 = y_f16;
-    switch (g_exhip_options.f8_form) {
-    case 1: return launch_rows<1, 1, 1, 8, 4, false>(ctx, p);
-    case 2: return launch_rows<2, 1, 1, 8, 2, false>(ctx, p);
-    case 3: return launch_rows<4, 1, 1, 8, 2, false>(ctx, p);
-    case 4: return launch_rows<2, 2, 1, 8, 2, false>(ctx, p);
-    case 5: return launch_rows<4, 2, 1, 8, 1, false>(ctx, p);
-    case 6: return launch_rows<4, 4, 1, 8, 1, false>(ctx, p);
-    case 7: return launch_rows<4, 4, 1, 4, 1, false>(ctx, p);
-    case 8: return launch_rows<4, 4, 2, 4, 1, false>(ctx, p);
-    case 9: return launch_tile<2, 2, 2, false>(ctx, p);
-    case 10: return launch_tile<4, 1, 4, false>(ctx, p);
-    case 11: return launch_wide<false>(ctx, p);
-    case 12: return launch_rows<2, 4, 1, 8, 1, false>(ctx, p);
-    case 13: return launch_rows<1, 4, 1, 8, 2, false>(ctx, p);
-    case 14: return launch_rows<1, 2, 1, 8, 2, false>(ctx, p);
-    case 15: return launch_rows<1, 1, 1, 16, 2, false>(ctx, p);
-    case 16: return launch_deep<true, false>(ctx, p);
-    case 17: return launch_deep<false, false>(ctx, p);
-    }
-    if (p.m <= 16) return launch_rows<1, 1, 1, 8, 4, false>(ctx, p);
-    if (!p.y_f32 && (long long)p.m * p.n >= 256ll * 256 * 128) return launch_wide<false>(ctx, p);
-    return (long long)p.m * p.n >= 256 * 128 * 256 ? launch_tile<4, 1, 4, false>(ctx, p) : launch_tile<2, 2, 2, false>(ctx, p);
+    return y_f32 ? run_best(ctx, p, kExact) : run_best(ctx, p, kHalves);
 }
 
 extern "C" int exhip_innerproduct_gated_f8(exhip_ctx* ctx, const exhip_f8_desc* d, int gate, const uint8_t* x, const float* x_scale, const void* w_packed,
@@ -1159,26 +1110,5 @@ extern "C" int exhip_innerproduct_gated_f8(exhip_ctx* ctx, const exhip_f8_desc* 
     p.y_f8 = y_f8;
     p.y_scale = y_scale;
     p.gate = gate;
-    switch (g_exhip_options.f8_form) {
-    case 1: return launch_rows<2, 1, 1, 8, 4, true>(ctx, p);
-    case 2: return launch_rows<2, 1, 1, 8, 2, true>(ctx, p);
-    case 3: return launch_rows<4, 1, 1, 8, 2, true>(ctx, p);
-    case 4: return launch_rows<2, 2, 1, 8, 2, true>(ctx, p);
-    case 5: return launch_rows<4, 2, 1, 8, 1, true>(ctx, p);
-    case 6: return launch_rows<4, 4, 1, 8, 1, true>(ctx, p);
-    case 7: return launch_rows<4, 4, 1, 4, 1, true>(ctx, p);
-    case 8: return launch_rows<4, 1, 4, 4, 2, true>(ctx, p);
-    case 9: return launch_tile<2, 2, 2, true>(ctx, p);
-    case 10: return launch_tile<4, 1, 4, true>(ctx, p);
-    case 11: return launch_wide<true>(ctx, p);
-    case 12: return launch_rows<2, 4, 1, 8, 1, true>(ctx, p);
-    case 13: return launch_rows<2, 1, 8, 2, 2, true>(ctx, p);
-    case 14: return launch_rows<4, 4, 4, 2, 1, true>(ctx, p);
-    case 16: return launch_deep<true, true>(ctx, p);
-    case 17: return launch_deep<false, true>(ctx, p);
-    }
-    if (p.m <= 16) return p.y_f8 ? launch_rows<4, 1, 4, 4, 2, true>(ctx, p) : launch_rows<2, 1, 1, 8, 4, true>(ctx, p);
-    if (!p.y_f8 && 2ll * p.m * p.n >= 256ll * 256 * 128) return launch_wide<true>(ctx, p);
-    if (2ll * p.m * p.n >= 256 * 128 * 256) return launch_tile<4, 1, 4, true>(ctx, p);
-    return p.y_f8 ? launch_tile<4, 1, 4, true>(ctx, p) : launch_tile<2, 2, 2, true>(ctx, p);
+    return y_f8 ? run_best(ctx, p, kGatedCodes) : run_best(ctx, p, kGatedHalves);
 }

@@ -78,6 +78,7 @@ const char* exhip_last_error(void);
  * that stages the input of 3x3 fp16 / int8 layers in LDS (1 by its rule, 2 to 4 its first to third form wherever it can run, 0 never; fp16 sums then run in another
  * order). "f32_tile" pins the float32 convolution's wave tile and split (0 = its rule, n = the n-th of its list;
  * sums then run in another order).
+ * "f8_form" pins the kernel of the products in 8-bit floating point (0 = its rule, n = the n-th of its list for the result's type; other sums then).
  * Process-wide; packed weights depend on the first three, so set them before packing. */
 int exhip_set_option(const char* name, int value);
 unsigned exhip_options_version(void); /* counts the calls above: plans made under other options are made again */

@@ -1,4 +1,6 @@
 """The inner products in 8-bit floating point, their quantizers and what they refuse, against 64 bits (tests/f8ref.py has the bounds)."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -225,6 +227,117 @@ def test_gated_codes_are_the_quantizer_s(ctx):
         assert np.array_equal(f8ref.VALUES[codes.download()[:, :n]], f8ref.VALUES[want])  # (a zero's sign is that of its product)
 
 
+# ---- every kernel, at sizes that its rule would give to another ----
+@pytest.fixture
+def pin():
+    from excalibur_amd import hip
+    yield lambda form: hip.set_option("f8_form", form)
+    hip.set_option("f8_form", 0)
+
+
+FORM_SIZES = [(1, 1, 1), (16, 16, 128), (17, 130, 129), (130, 300, 1531), (257, 520, 384), (300, 257, 1000), (64, 128, 2049)]
+
+
+@pytest.mark.parametrize("m,n,k", FORM_SIZES)
+def test_every_form_of_the_product(ctx, pin, m, n, k):
+    o = Operands(ctx, np.random.default_rng(m + 3 * n + 5 * k), m, n, k, bias=n % 2 == 0, pad=16 * (n % 2))
+    want, bound = o.want()
+    args = (o.dx, o.dx_scale, o.packed, o.dw_scale[0], o.dbias[0])
+    cut = bound + f8ref.cut_bound(o.x, o.x_scale, o.w[0], o.w_scale[0])
+    for form in range(1, 7):
+        pin(form)
+        for extra in (0, 3):
+            y32, y16 = ctx.array(np.full((m + 1, n + extra), 7.25, np.float32)), ctx.array(np.full((m + 1, n + extra), 0x4567, np.uint16))
+            d = o.desc(ctx, n + extra)
+            ctx.innerproduct_f8(d, *args, y_f32=y32)
+            ctx.innerproduct_f8(d, *args, y_f16=y16)
+            y32, y16 = y32.download(), y16.download()
+            _near(y32[:m, :n], want, bound)
+            _near(y16[:m, :n].view(np.float16), want, f8ref.half_bound(want, cut))
+            for y, fill in ((y32, 7.25), (y16, 0x4567)):
+                assert np.all(y[m] == fill) and np.all(y[:, n:] == fill), form
+
+
+@pytest.mark.parametrize("m,n,k", FORM_SIZES)
+def test_every_form_of_the_gated_product(ctx, pin, m, n, k):
+    o = Operands(ctx, np.random.default_rng(m + 3 * n + 7 * k), m, n, k, sides=2, bias=n % 2 == 0, pad=16 * (n % 2))
+    (g, gb), (u, ub) = o.want(0), o.want(1)
+    h, bound = f8ref.gated("silu", g, gb, u, ub)
+    cut = f8ref.gated("silu", g, gb + f8ref.cut_bound(o.x, o.x_scale, o.w[0], o.w_scale[0]), u, ub + f8ref.cut_bound(o.x, o.x_scale, o.w[1], o.w_scale[1]))[1]
+    args = (o.dx, o.dx_scale, o.packed, o.dw_scale[0], o.dw_scale[1], "silu", o.dbias[0], o.dbias[1])
+    for form in range(1, 6):
+        pin(form)
+        y = ctx.array(np.full((m + 1, n + 3), 0x4567, np.uint16))
+        ctx.innerproduct_gated_f8(o.desc(ctx, n + 3), *args, y_f16=y)
+        y = y.download()
+        _near(y[:m, :n].view(np.float16), h, f8ref.half_bound(h, cut))
+        assert np.all(y[m] == 0x4567) and np.all(y[:, n:] == 0x4567), form
+    stride, blocks = (n + 15) // 16 * 16 + 16, f8ref.blocks(n)
+    for form in range(1, 4):
+        pin(form)
+        codes, scale = ctx.array(np.full((m + 1, stride), 0xA5, np.uint8)), ctx.array(np.full((blocks + 1, m), 7.25, np.float32))
+        ctx.innerproduct_gated_f8(o.desc(ctx, stride), *args, y_f8=codes, y_scale=scale)
+        codes, scale = codes.download(), scale.download()
+        assert np.all(codes[m] == 0xA5) and np.all(codes[:, n:] == 0xA5) and np.all(scale[blocks] == 7.25), form
+        _near(f8ref.rows_of(codes[:m, :n], scale[:blocks]), h, f8ref.code_bound(h, bound, scale[:blocks]))
+
+
+def test_every_form_of_whole_numbers_is_exact(ctx, pin):
+    """As test_product_of_whole_numbers_is_exact, of each kernel: values up to 8, so that nothing of eight products lies 13 bits beneath the largest."""
+    rng = np.random.default_rng(61)
+    for m, n, k in ((40, 200, 384), (270, 300, 905)):
+        o = Operands(ctx, rng, m, n, k)
+        o.x, o.w[0] = f8ref.encode(rng.integers(-8, 9, (m, k))), f8ref.encode(rng.integers(-8, 9, (n, k)))
+        o.x_scale = np.ldexp(1.0, rng.integers(-2, 3, o.x_scale.shape)).astype(np.float32)
+        o.w_scale[0] = np.ldexp(1.0, rng.integers(-2, 3, o.w_scale[0].shape)).astype(np.float32)
+        want, _ = o.want()
+        args = (ctx.array(_wide(o.x, o.stride, 0x7F)), ctx.array(o.x_scale), ctx.pack_f8_weights(n, k, ctx.array(o.w[0])), ctx.array(o.w_scale[0]))
+        for form in range(1, 7):
+            pin(form)
+            y32, y16 = ctx.empty((m, n), np.float32), ctx.empty((m, n), np.uint16)
+            ctx.innerproduct_f8(o.desc(ctx), *args, y_f32=y32)
+            ctx.innerproduct_f8(o.desc(ctx), *args, y_f16=y16)
+            assert np.array_equal(y32.download().astype(np.float64), want), form
+            assert np.array_equal(y16.download().view(np.float16), want.astype(np.float16)), form
+
+
+def test_every_form_keeps_a_nan_in_its_row(ctx, pin):
+    rng = np.random.default_rng(62)
+    m, n, k = 140, 150, 203
+    o = Operands(ctx, rng, m, n, k)
+    o.x[m - 1, 3] = 0x7F
+    o.w[0][n - 1, k - 1] = 0xFF
+    args = (ctx.array(_wide(o.x, o.stride, 0x7F)), o.dx_scale, ctx.pack_f8_weights(n, k, ctx.array(o.w[0])), o.dw_scale[0])
+    want = np.zeros((m, n), bool)
+    want[m - 1], want[:, n - 1] = True, True
+    for form in range(1, 7):
+        pin(form)
+        y32, y16 = ctx.empty((m, n), np.float32), ctx.empty((m, n), np.uint16)
+        ctx.innerproduct_f8(o.desc(ctx), *args, y_f32=y32)
+        ctx.innerproduct_f8(o.desc(ctx), *args, y_f16=y16)
+        assert np.array_equal(np.isnan(y32.download()), want) and np.array_equal(np.isnan(y16.download().view(np.float16)), want), form
+
+
+def test_rows_far_into_a_large_tensor(ctx):
+    """Offsets beyond 32 bits: rows of codes 2^22 bytes apart and results behind 4 GiB of others."""
+    rng = np.random.default_rng(63)
+    m, n, k = 1100, 96, 256
+    o = Operands(ctx, rng, m, n, k)
+    stride, y_stride = 1 << 22, 2_000_000
+    x, y = ctx.empty((m, stride), np.uint8), ctx.empty((m, y_stride), np.float32)
+    from excalibur_amd import hip
+    for r in range(m):
+        hip._check(hip.lib().exhip_memcpy_h2d(ctx.h, x.at(r * stride).ptr, ctypes.c_void_p(np.ascontiguousarray(o.x[r]).ctypes.data), ctypes.c_size_t(k)))
+    ctx.innerproduct_f8(ctx.f8_desc(m, n, k, x_stride=stride, y_stride=y_stride), x, o.dx_scale, o.packed, o.dw_scale[0], y_f32=y)
+    want, bound = o.want()
+    got = np.empty((m, n), np.float32)
+    for r in range(m):
+        hip._check(hip.lib().exhip_memcpy_d2h(ctx.h, ctypes.c_void_p(got[r:].ctypes.data), y.at(r * y_stride * 4).ptr, ctypes.c_size_t(n * 4)))
+    _near(got, want, bound)
+    x.free()
+    y.free()
+
+
 # ---- as a program runs them ----
 def _network(ctx, rng, m, hidden, k, classes):
     """rows -> codes -> gated product (codes) -> product (float32) -> log probabilities, all queued before anything is read."""
@@ -276,8 +389,6 @@ def test_rows_to_log_probabilities(ctx, m, hidden, k, classes):
 
 
 def test_recorded_runs_are_the_direct_ones(ctx):
-    import ctypes
-
     from excalibur_amd import hip
     rng = np.random.default_rng(41)
     for m in (1, 70):
