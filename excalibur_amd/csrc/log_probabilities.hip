@@ -56,6 +56,16 @@ __device__ __forceinline__ float over_wave(float v, F f) {
     const unsigned h0 = h[0], h1 = h[1];
     return f(__builtin_bit_cast(float, h0), __builtin_bit_cast(float, h1));
 }
+// The top-th largest of a wave's 64 values at least, by halving (to 24 bits of order_of(), downwards).
+__device__ __forceinline__ unsigned reached_by(unsigned order, int top) {
+    unsigned bound = 0;
+#pragma unroll 1
+    for (int bit = 31; bit >= 8; --bit) {
+        const unsigned up = bound | 1u << bit;
+        bound = __popcll(__ballot(order >= up)) >= top ? up : bound;
+    }
+    return bound;
+}
 __device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ float sum(float a, float b) { return a + b; }
 // A lane's place among those of a mask.
@@ -95,6 +105,13 @@ __device__ __forceinline__ Sums from_lane(const Sums& a, int d) {
     return Sums{__shfl_xor(a.most, d), __shfl_xor(a.s, d), __shfl_xor(a.t, d), 0.f};
 }
 
+// What lanes of a wave have written into LDS is there for the others.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // How many of n places (eight zeros behind them) stand in front of `own`: eight reads under way at a time.
 __device__ __forceinline__ int rank_of(u64 own, const u64* places, int n) {
     int rank = 0;
@@ -125,34 +142,37 @@ __device__ __forceinline__ float log_p_of(float v, const Sums& r, float log_s) {
     return v - r.most - log_s;
 }
 
-// The answers of a row, by a group of `threads`, from its sums and the places of its largest.
+// The answers of a row, by one wave, from its sums and the places of its largest.
 template <typename T>
-__device__ void write_row(const T* __restrict__ src, const LogpParams& p, size_t row, const Sums& r, const u64* places, int threads) {
+__device__ __forceinline__ void write_row(const T* __restrict__ src, const LogpParams& p, size_t row, const Sums& r, const u64* places) {
+    const int lane = threadIdx.x % 64;
     const float log_s = __builtin_amdgcn_logf(r.s) * kLn2;
-    if (threadIdx.x == 0 && p.entropy) p.entropy[row] = r.s != r.s ? r.s : r.most == -INFINITY ? 0.f : log_s - r.t / r.s * kLn2;
-    for (int i = threadIdx.x; i < p.n_ids; i += threads) {
+    if (lane == 0 && p.entropy) p.entropy[row] = r.s != r.s ? r.s : r.most == -INFINITY ? 0.f : log_s - r.t / r.s * kLn2;
+    for (int i = lane; i < p.n_ids; i += 64) {
         const int id = p.ids[row * p.n_ids + i];
         p.log_p[row * p.n_ids + i] = id < 0 ? 0.f : id >= p.c ? NAN : log_p_of(as_float(src[id]), r, log_s);
     }
-    for (int i = threadIdx.x; i < p.top; i += threads) {
-        const u64 at = places[i];
+    if (lane < p.top) {
+        const u64 at = places[lane];
         const unsigned o = (unsigned)(at >> 32);
-        p.top_ids[row * p.top + i] = index_of(at);
+        p.top_ids[row * p.top + lane] = index_of(at);
         // the value back from its order
-        p.top_log_p[row * p.top + i] = log_p_of(__builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o), r, log_s);
+        p.top_log_p[row * p.top + lane] = log_p_of(__builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o), r, log_s);
     }
 }
 
-// A group of W waves a slice of a row, V values a thread, all requested before the first is used.
+// A group of W waves a slice of a row, V values a thread, all requested before the first is used. What one wave can do for the group is wave 0's: the others
+// would only take its turns.
 template <typename T, int W, int V, bool TOP>
 __global__ __launch_bounds__(64 * W, W == 16 ? 8 : 4) void log_probabilities_kernel(const T* __restrict__ x, const LogpParams p) {
     exhip_touch_args(p);
     constexpr int kThreads = 64 * W, N = 16 / sizeof(T), kRuns = V / N;
+    static_assert(W == 1 || W == 4 || W == 16, "64 sets of W neighbouring lanes");
     __shared__ Sums sums[W];
-    __shared__ float bounds[W];
+    __shared__ float sets[64], bound;
     __shared__ u64 places[TOP ? kCandidates + 8 : 1], sorted[TOP ? EXHIP_LOG_PROBABILITIES_TOP : 1];
     __shared__ int count;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const size_t row = blockIdx.x / p.slices;
     const int slice = blockIdx.x % p.slices, first = slice * p.slice_len, len = min(p.slice_len, p.c - first);
     const T* const src = x + row * p.x_stride + first;
@@ -194,78 +214,80 @@ __global__ __launch_bounds__(64 * W, W == 16 ? 8 : 4) void log_probabilities_ker
         if (lane == 0) sums[wave] = all;
     }
     if constexpr (TOP) {
-        // A bound that at least `top` of the slice reach: the top-th largest of a wave's 64 lanes' largest (to 16 bits, downwards), the highest of the waves'.
-        const unsigned o = order_of(mine);
-        unsigned bound = 0;
-#pragma unroll
-        for (int bit = 31; bit >= 16; --bit) {
-            const unsigned up = bound | 1u << bit;
-            if (__popcll(__ballot(o >= up)) >= p.top) bound = up;
-        }
-        const float least = bound < 0x007fffffu ? -INFINITY : __builtin_bit_cast(float, bound & 0x80000000u ? bound & 0x7fffffffu : ~bound);
-        if (lane == 0) bounds[wave] = least;
+        // the largest of each of the group's 64 sets of W neighbouring lanes
+        float m = mine;
+        if constexpr (W > 1) m = fmaxf(m, traded<0xB1>(m)), m = fmaxf(m, traded<0x4E>(m));
+        if constexpr (W > 4) m = fmaxf(m, traded<0x141>(m)), m = fmaxf(m, traded<0x140>(m));
+        if (lane % W == 0) sets[wave * (64 / W) + lane / W] = m;
         if (threadIdx.x == 0) count = 0;
     }
     __syncthreads();
-    if constexpr (W > 1) {
-        all = sums[lane % W];
-        all = joined(all, traded<0xB1>(all));
-        all = joined(all, traded<0x4E>(all));
-        if constexpr (W == 16) {
-            all = joined(all, traded<0x141>(all));
-            all = joined(all, traded<0x140>(all));
+    if (wave == 0) {
+        if constexpr (W > 1) {
+            all = sums[lane % W];
+            all = joined(all, traded<0xB1>(all));
+            all = joined(all, traded<0x4E>(all));
+            if constexpr (W == 16) {
+                all = joined(all, traded<0x141>(all));
+                all = joined(all, traded<0x140>(all));
+            }
+        }
+        if constexpr (TOP) {
+            // `top` sets hold a value that reaches the top-th largest of the sets' largest, so the slice's `top` largest all do. A class of no probability is
+            // no candidate whatever the bound; with a NaN nothing is.
+            const unsigned o = reached_by(order_of(sets[lane]), p.top);
+            const float least = o <= 0x007fffffu ? -FLT_MAX : __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o);
+            if (lane == 0) bound = all.s != all.s ? INFINITY : least;
         }
     }
     if constexpr (TOP) {
-        static_assert(W == 1 || W == 4 || W == 16, "the waves' bounds are joined within rows of lanes");
-        float least = bounds[lane % W];
-        if constexpr (W > 1) least = over_row(least, larger);
-        const bool nan = all.s != all.s;
-        if (!nan) {
-            // a class of no probability is no candidate, whatever the bound
-            const float beyond = fmaxf(least, -FLT_MAX);
+        __syncthreads();
+        const float least = bound;
+        if (__ballot(mine >= least) != 0) {
             int wave_count = 0;
 #pragma unroll
             for (int i = 0; i < kRuns; ++i)
-                if (__ballot(largest[i] >= beyond) != 0)
+                if (__ballot(largest[i] >= least) != 0)
 #pragma unroll
-                    for (int e = i * N; e < i * N + N; ++e) wave_count += __popcll(__ballot(value(e) >= beyond));
-            if (wave_count > 0) {
-                int slot = 0;
-                if (lane == 0) slot = atomicAdd(&count, wave_count);
-                slot = __builtin_amdgcn_readfirstlane(slot);
-                if (slot + wave_count <= kCandidates)
+                    for (int e = i * N; e < i * N + N; ++e) wave_count += __popcll(__ballot(value(e) >= least));
+            int slot = 0;
+            if (lane == 0) slot = atomicAdd(&count, wave_count);
+            slot = __builtin_amdgcn_readfirstlane(slot);
+            if (slot + wave_count <= kCandidates)
 #pragma unroll
-                    for (int i = 0; i < kRuns; ++i)
-                        if (__ballot(largest[i] >= beyond) != 0)
+                for (int i = 0; i < kRuns; ++i)
+                    if (__ballot(largest[i] >= least) != 0)
 #pragma unroll
-                            for (int e = i * N; e < i * N + N; ++e) {
-                                const bool takes = value(e) >= beyond;
-                                const u64 all_takes = __ballot(takes);
-                                if (takes) places[slot + place_in(all_takes)] = place_of(value(e), first + at(e));
-                                slot += __popcll(all_takes);
-                            }
-            }
-            __syncthreads();
-            const int n = count;
-            if (n < p.top) {  // masked classes too, by their index: they are among the first n + top of the slice
-                __syncthreads();
-                for (int i = threadIdx.x; i < min(n + p.top, len); i += kThreads)
-                    if (as_float(src[i]) == -INFINITY) places[atomicAdd(&count, 1)] = place_of(-INFINITY, first + i);
-                __syncthreads();
-            }
+                        for (int e = i * N; e < i * N + N; ++e) {
+                            const bool takes = value(e) >= least;
+                            const u64 all_takes = __ballot(takes);
+                            if (takes) places[slot + place_in(all_takes)] = place_of(value(e), first + at(e));
+                            slot += __popcll(all_takes);
+                        }
         }
-        const int n = nan ? kCandidates + 1 : count;
+        __syncthreads();
+        const bool nan = least == INFINITY;  // (or a +infinity, whose exponential is one)
+        int n = nan ? kCandidates + 1 : count;
         if (n <= kCandidates) {
-            if (threadIdx.x < 8) places[n + threadIdx.x] = 0;
-            for (int i = threadIdx.x; i < p.top; i += kThreads)
-                if (i >= n) sorted[i] = 0;
-            __syncthreads();
-            for (int i = threadIdx.x; i < n; i += kThreads) {
+            if (wave != 0) return;
+            if (n < p.top) {  // masked classes too, by their index: they are among the first n + top of the slice
+                const int reach = min(n + p.top, len);
+                for (int i = lane; i - lane < reach; i += 64) {
+                    const bool takes = i < reach && as_float(src[i]) == -INFINITY;
+                    const u64 all_takes = __ballot(takes);
+                    if (takes) places[n + place_in(all_takes)] = place_of(-INFINITY, first + i);
+                    n += __popcll(all_takes);
+                }
+            }
+            if (lane < 8) places[n + lane] = 0;
+            if (lane >= n && lane < p.top) sorted[lane] = 0;
+            wave_sync();
+            for (int i = lane; i < n; i += 64) {
                 const u64 own = places[i];
                 const int rank = rank_of(own, places, n);
                 if (rank < p.top) sorted[rank] = own;
             }
+            wave_sync();
         } else {
             // many equal values, or a NaN: the largest behind the last one found, `top` times, each a reading of the slice
             u64 last = ~0ull;
@@ -288,40 +310,38 @@ __global__ __launch_bounds__(64 * W, W == 16 ? 8 : 4) void log_probabilities_ker
                 if (threadIdx.x == 0) sorted[i] = last;
                 if (last == 0) last = 1;  // nothing is left: none of the places lies beneath
             }
+            if (wave != 0) return;
+            wave_sync();
         }
-        __syncthreads();
+    } else if (wave != 0) {
+        return;
     }
     if (p.slices == 1) {
-        write_row(src, p, row, all, sorted, kThreads);
+        write_row(src, p, row, all, sorted);
     } else {
-        if (threadIdx.x == 0) p.part[blockIdx.x] = all;
+        if (lane == 0) p.part[blockIdx.x] = all;
         if constexpr (TOP)
-            for (int i = threadIdx.x; i < p.top; i += kThreads) p.part_top[(size_t)blockIdx.x * p.top + i] = sorted[i];
+            if (lane < p.top) p.part_top[(size_t)blockIdx.x * p.top + lane] = sorted[lane];
     }
 }
 
-// The largest of the slices' lists, `top` of them into sorted, by one wave: a batch of entries is held in registers with those found so far in front, the top-th
-// largest of it is found to 24 bits by halving, and what reaches that is ranked.
-__device__ void join_lists(const u64* __restrict__ from, size_t total, int top, u64* places, u64* sorted) {
+// The largest of the slices' lists, `top` of them into sorted, by one wave: a batch of entries is held in registers with those found so far in front, and what
+// reaches the top-th largest of the lanes' largest is ranked.
+__device__ __forceinline__ void join_lists(const u64* __restrict__ from, size_t total, int top, u64* places, u64* sorted) {
     constexpr int kHeld = 8;
     const int lane = threadIdx.x;
     int kept = 0;
     for (size_t done = 0; done < total;) {
-        u64 held[kHeld];
+        u64 held[kHeld], most = 0;
 #pragma unroll
         for (int e = 0; e < kHeld; ++e) {
             const int i = e * 64 + lane;  // the first `kept` of a batch are those found so far
             held[e] = i < kept ? sorted[i] : done + (i - kept) < total ? from[done + (i - kept)] : 0;
         }
-        done += kHeld * 64 - kept;
-        unsigned bound = 0;
-        for (int bit = 31; bit >= 8; --bit) {
-            const unsigned up = bound | 1u << bit;
-            int reach = 0;
 #pragma unroll
-            for (int e = 0; e < kHeld; ++e) reach += __popcll(__ballot((unsigned)(held[e] >> 32) >= up));
-            if (reach >= top) bound = up;
-        }
+        for (int e = 0; e < kHeld; ++e) most = held[e] > most ? held[e] : most;
+        done += kHeld * 64 - kept;
+        const unsigned bound = reached_by((unsigned)(most >> 32), top);
         int n = 0;
 #pragma unroll
         for (int e = 0; e < kHeld; ++e) {
@@ -331,13 +351,13 @@ __device__ void join_lists(const u64* __restrict__ from, size_t total, int top, 
             n += __popcll(all_takes);
         }
         if (lane < 8) places[n + lane] = 0;
-        __syncthreads();
+        wave_sync();
         for (int i = lane; i < n; i += 64) {
             const u64 own = places[i];
             const int rank = rank_of(own, places, n);
             if (rank < top) sorted[rank] = own;
         }
-        __syncthreads();
+        wave_sync();
         kept = min(n, top);
     }
 }
@@ -354,7 +374,7 @@ __global__ __launch_bounds__(64) void join_slices_kernel(const T* __restrict__ x
     if (p.top > 0) join_lists(p.part_top + row * p.slices * p.top, (size_t)p.slices * p.top, p.top, places, sorted);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) all = joined(all, from_lane(all, d));
-    write_row(x + row * p.x_stride, p, row, all, sorted, 64);
+    write_row(x + row * p.x_stride, p, row, all, sorted);
 }
 
 // How a row is split: slices that a group's registers hold, and more of them where there are few rows.
