@@ -9,7 +9,7 @@
 
 namespace {
 
-constexpr int kMostSlice = 32768;   // values of a row that a group holds in its registers
+constexpr int kMostSlice = 32768, kSmallSlice = 8192;  // values of a row that a group of 16, of 4 waves holds in its registers
 constexpr int kCandidates = 512;    // values of a slice that are ranked at once
 typedef unsigned long long u64;
 
@@ -56,11 +56,11 @@ __device__ __forceinline__ float over_wave(float v, F f) {
     const unsigned h0 = h[0], h1 = h[1];
     return f(__builtin_bit_cast(float, h0), __builtin_bit_cast(float, h1));
 }
-// The top-th largest of a wave's 64 values at least, by halving (to 24 bits of order_of(), downwards).
+// A bound that `top` of a wave's 64 values reach: the top-th largest, by halving, to 16 bits of order_of(), downwards.
 __device__ __forceinline__ unsigned reached_by(unsigned order, int top) {
     unsigned bound = 0;
-#pragma unroll 1
-    for (int bit = 31; bit >= 8; --bit) {
+#pragma unroll
+    for (int bit = 31; bit >= 16; --bit) {
         const unsigned up = bound | 1u << bit;
         bound = __popcll(__ballot(order >= up)) >= top ? up : bound;
     }
@@ -223,6 +223,7 @@ __global__ __launch_bounds__(64 * W, W == 16 ? 8 : 4) void log_probabilities_ker
     }
     __syncthreads();
     if (wave == 0) {
+        __builtin_amdgcn_s_setprio(3);  // the group's other waves wait for this one
         if constexpr (W > 1) {
             all = sums[lane % W];
             all = joined(all, traded<0xB1>(all));
@@ -243,28 +244,26 @@ __global__ __launch_bounds__(64 * W, W == 16 ? 8 : 4) void log_probabilities_ker
     if constexpr (TOP) {
         __syncthreads();
         const float least = bound;
-        if (__ballot(mine >= least) != 0) {
-            int wave_count = 0;
+        if (__ballot(mine >= least) != 0)
 #pragma unroll
             for (int i = 0; i < kRuns; ++i)
-                if (__ballot(largest[i] >= least) != 0)
+                if (__ballot(largest[i] >= least) != 0) {
+                    u64 takes[N];
+                    int here = 0, slot = 0;
 #pragma unroll
-                    for (int e = i * N; e < i * N + N; ++e) wave_count += __popcll(__ballot(value(e) >= least));
-            int slot = 0;
-            if (lane == 0) slot = atomicAdd(&count, wave_count);
-            slot = __builtin_amdgcn_readfirstlane(slot);
-            if (slot + wave_count <= kCandidates)
+                    for (int e = 0; e < N; ++e) {
+                        takes[e] = __ballot(value(i * N + e) >= least);
+                        here += __popcll(takes[e]);
+                    }
+                    if (lane == 0) slot = atomicAdd(&count, here);
+                    slot = __builtin_amdgcn_readfirstlane(slot);
 #pragma unroll
-                for (int i = 0; i < kRuns; ++i)
-                    if (__ballot(largest[i] >= least) != 0)
-#pragma unroll
-                        for (int e = i * N; e < i * N + N; ++e) {
-                            const bool takes = value(e) >= least;
-                            const u64 all_takes = __ballot(takes);
-                            if (takes) places[slot + place_in(all_takes)] = place_of(value(e), first + at(e));
-                            slot += __popcll(all_takes);
-                        }
-        }
+                    for (int e = 0; e < N; ++e) {
+                        const int to = slot + place_in(takes[e]);
+                        if (value(i * N + e) >= least && to < kCandidates) places[to] = place_of(value(i * N + e), first + at(i * N + e));
+                        slot += __popcll(takes[e]);
+                    }
+                }
         __syncthreads();
         const bool nan = least == INFINITY;  // (or a +infinity, whose exponential is one)
         int n = nan ? kCandidates + 1 : count;
@@ -377,9 +376,10 @@ __global__ __launch_bounds__(64) void join_slices_kernel(const T* __restrict__ x
     write_row(x + row * p.x_stride, p, row, all, sorted);
 }
 
-// How a row is split: slices that a group's registers hold, and more of them where there are few rows.
-void split(int m, int c, int* slices, int* slice_len) {
-    const int least = (c - 1) / kMostSlice + 1, wish = 512 / m, most = (c - 1) / 8192 + 1;
+// How a row is split: slices that a group's registers hold, and more of them where there are few rows. Where the largest are asked, groups of four waves (they
+// wait for one wave twice: 300 x 100003 halves with the 8 largest 25 us, 30 with groups of 16).
+void split(int m, int c, int top, int* slices, int* slice_len) {
+    const int most = (c - 1) / kSmallSlice + 1, least = top ? most : (c - 1) / kMostSlice + 1, wish = 512 / m;
     *slices = least > wish ? least : wish < most ? wish : most;
     const int len = (c - 1) / *slices + 1;
     *slice_len = (len + 7) / 8 * 8;
@@ -391,8 +391,8 @@ void launch_slices(exhip_ctx* ctx, const T* x, const LogpParams& p) {
     const dim3 grid((unsigned)((size_t)p.m * p.slices));
     if (p.slice_len <= 512) hipLaunchKernelGGL((log_probabilities_kernel<T, 1, 8, TOP>), grid, dim3(64), 0, ctx->stream, x, p);
     else if (p.slice_len <= 2048) hipLaunchKernelGGL((log_probabilities_kernel<T, 1, 32, TOP>), grid, dim3(64), 0, ctx->stream, x, p);
-    else if (p.slice_len <= 8192) hipLaunchKernelGGL((log_probabilities_kernel<T, 4, 32, TOP>), grid, dim3(256), 0, ctx->stream, x, p);
-    else hipLaunchKernelGGL((log_probabilities_kernel<T, 16, 32, TOP>), grid, dim3(1024), 0, ctx->stream, x, p);
+    else if (p.slice_len <= kSmallSlice) hipLaunchKernelGGL((log_probabilities_kernel<T, 4, 32, TOP>), grid, dim3(256), 0, ctx->stream, x, p);
+    else if constexpr (!TOP) hipLaunchKernelGGL((log_probabilities_kernel<T, 16, 32, false>), grid, dim3(1024), 0, ctx->stream, x, p);
 }
 
 bool sizes_ok(int m, int c, int top) { return m > 0 && c > 0 && top >= 0 && top <= EXHIP_LOG_PROBABILITIES_TOP && top <= c; }
@@ -409,7 +409,7 @@ int log_probabilities(exhip_ctx* ctx, const char* name, const T* x, int x_stride
     EXHIP_REQUIRE((uintptr_t)x % sizeof(T) == 0 && ((uintptr_t)ids | (uintptr_t)log_p | (uintptr_t)entropy | (uintptr_t)top_ids | (uintptr_t)top_log_p) % 4 == 0 && (uintptr_t)workspace % 16 == 0,
                   "%s: an operand's address is not that of its type", name);
     LogpParams p = {ids, log_p, entropy, top_log_p, top_ids, nullptr, nullptr, m, c, x_stride, n_ids, top, 0, 0};
-    split(m, c, &p.slices, &p.slice_len);
+    split(m, c, top, &p.slices, &p.slice_len);
     EXHIP_REQUIRE((size_t)m * p.slices <= 0xffffffffu / 1024, "%s: %d rows of %d values are more than one launch takes", name, m, c);
     if (p.slices > 1) {
         p.part = static_cast<Sums*>(workspace);
@@ -435,7 +435,7 @@ extern "C" size_t exhip_log_probabilities_workspace(int m, int c, int top) {
         return 0;
     }
     int slices, slice_len;
-    split(m, c, &slices, &slice_len);
+    split(m, c, top, &slices, &slice_len);
     return slices > 1 ? (size_t)m * slices * (sizeof(Sums) + 8 * top) : 16;
 }
 
