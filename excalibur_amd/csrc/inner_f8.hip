@@ -1,7 +1,7 @@
 // Inner products in 8-bit floating point: the row quantizer, the weights' layout, the product and the gated product.
 //
-// A block of 128 values shares a float32 scale. Its codes become halves, which hold every e4m3 value exactly, and four v_mfma_f32_16x16x32_f16 sum
-// the block's products, 16 outputs x 16 rows, still without scales; the sum goes to the running one with one multiply-add per value, by the product of
+// A block of 128 values shares a float32 scale. Its codes become halves, which hold every e4m3 value exactly, and four v_mfma_f32_16x16x32_f16 (or
+// eight v_mfma_f32_32x32x16_f16) sum the block's products of 16 outputs (32) and as many rows, still without scales; the sum goes to the running one with one multiply-add per value, by the product of
 // the two blocks' scales. Weights are the first operand, rows of the input the second: a lane's four results are then four neighbouring outputs of
 // one row, so the row's scale is one register of the lane and the weights' scale one value of the wave.
 //
@@ -12,6 +12,7 @@
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v2i __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
 typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 
 namespace {
@@ -281,62 +282,77 @@ __device__ __forceinline__ v4f four_of(const float* v, int j, int n) {
     return r;
 }
 
-// The sums of a group of WN x WM waves, TN = 4 tiles of outputs and TM tiles of rows each. `lds` is free for at least the group's results as floats (halves
-// where there are no others).
-template <int WN, int WM, int TM, bool FLOATS>
-__device__ __forceinline__ void write_group(const F8Params& p, v4f (&acc)[4][TM], int group_n, int wn, int wm, int row0, int rows, int lane, char* lds) {
-    constexpr int kWidth = 64 * WN, kRows = 16 * TM * WM, kThreads = 64 * WN * WM;
-    const int q = lane / 16, col = lane % 16, j0 = group_n * kWidth;
+// Where a lane's sums lie: value i of four neighbouring outputs each, of TN, and rows t. After 16 x 16 products a lane has the outputs of a quarter of each tile and
+// one row, after 32 x 32 products those of a half of each eight.
+template <int SIDE>
+struct Lanes {
+    static constexpr int kOutputs = SIDE == 16 ? 4 : 8;  // of a wave's 64, in fours
+    static __device__ __forceinline__ int output(int i, int lane) { return SIDE == 16 ? i * 16 + lane / 16 * 4 : i * 8 + lane / 32 * 4; }
+    static __device__ __forceinline__ int row(int t, int lane) { return t * SIDE + lane % SIDE; }
+    // of a gated product: the four of the gate, those of the other projection, and where the result of both stands among the wave's 32
+    static __device__ __forceinline__ constexpr int gate(int i) { return SIDE == 16 ? 2 * i : i / 2 * 4 + i % 2; }
+    static __device__ __forceinline__ constexpr int up(int i) { return SIDE == 16 ? 2 * i + 1 : i / 2 * 4 + i % 2 + 2; }
+    static __device__ __forceinline__ int result(int i, int lane) { return SIDE == 16 ? i * 16 + lane / 16 * 4 : i * 8 + lane / 32 * 4; }
+};
+
+// The sums of a group of WN x WM waves, 64 outputs and SIDE * TM rows each. `lds` is free for at least the group's results as floats (halves where there are no
+// others).
+template <int SIDE, int WN, int WM, int TM, bool FLOATS>
+__device__ __forceinline__ void write_group(const F8Params& p, v4f (&acc)[Lanes<SIDE>::kOutputs][TM], int group_n, int wn, int wm, int row0, int rows, int lane, char* lds) {
+    typedef Lanes<SIDE> At;
+    constexpr int kWidth = 64 * WN, kRows = SIDE * TM * WM, kThreads = 64 * WN * WM;
+    const int j0 = group_n * kWidth;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const v4f bias = four_of(p.bias, j0 + wn * 64 + i * 16 + q * 4, p.n);
+    for (int i = 0; i < At::kOutputs; ++i) {
+        const v4f bias = four_of(p.bias, j0 + wn * 64 + At::output(i, lane), p.n);
 #pragma unroll
         for (int t = 0; t < TM; ++t) acc[i][t] += bias;
     }
     if (FLOATS && p.y_f32) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < At::kOutputs; ++i)
 #pragma unroll
-            for (int t = 0; t < TM; ++t) *reinterpret_cast<v4f*>(place_in_rows<float, kWidth>(lds, (wm * TM + t) * 16 + col, wn * 64 + i * 16 + q * 4)) = acc[i][t];
+            for (int t = 0; t < TM; ++t) *reinterpret_cast<v4f*>(place_in_rows<float, kWidth>(lds, wm * TM * SIDE + At::row(t, lane), wn * 64 + At::output(i, lane))) = acc[i][t];
         __syncthreads();
         store_rows<float, kWidth, kRows, kThreads>(lds, p.y_f32, p.y_stride, row0, rows, j0, p.n);
     }
     if (p.y_f16) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < At::kOutputs; ++i)
 #pragma unroll
             for (int t = 0; t < TM; ++t)
-                *reinterpret_cast<v4h*>(place_in_rows<uint16_t, kWidth>(lds, (wm * TM + t) * 16 + col, wn * 64 + i * 16 + q * 4)) = __builtin_convertvector(acc[i][t], v4h);
+                *reinterpret_cast<v4h*>(place_in_rows<uint16_t, kWidth>(lds, wm * TM * SIDE + At::row(t, lane), wn * 64 + At::output(i, lane))) = __builtin_convertvector(acc[i][t], v4h);
         __syncthreads();
         store_rows<uint16_t, kWidth, kRows, kThreads>(lds, p.y_f16, p.y_stride, row0, rows, j0, p.n);
     }
 }
 
 // The same of a gated product, whose tiles alternate: 32 WN outputs. Quantized results need a whole block of them, WN == 4.
-template <int WN, int WM, int TM>
-__device__ __forceinline__ void write_gated_group(const F8Params& p, v4f (&acc)[4][TM], int group_n, int wn, int wm, int row0, int rows, int lane, char* lds) {
-    constexpr int kWidth = 32 * WN, kRows = 16 * TM * WM, kThreads = 64 * WN * WM;
-    const int q = lane / 16, col = lane % 16, j0 = group_n * kWidth;
+template <int SIDE, int WN, int WM, int TM>
+__device__ __forceinline__ void write_gated_group(const F8Params& p, v4f (&acc)[Lanes<SIDE>::kOutputs][TM], int group_n, int wn, int wm, int row0, int rows, int lane, char* lds) {
+    typedef Lanes<SIDE> At;
+    constexpr int kWidth = 32 * WN, kRows = SIDE * TM * WM, kThreads = 64 * WN * WM, kResults = At::kOutputs / 2;
+    const int j0 = group_n * kWidth, row_at = wm * TM * SIDE, out_at = wn * 32;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int j = j0 + wn * 32 + i * 16 + q * 4;
+    for (int i = 0; i < kResults; ++i) {
+        const int j = j0 + out_at + At::result(i, lane);
         const v4f bias = four_of(p.bias, j, p.n), bias_up = four_of(p.bias_up, j, p.n);
 #pragma unroll
         for (int t = 0; t < TM; ++t) {
-            const v4f g = acc[2 * i][t] + bias, u = acc[2 * i + 1][t] + bias_up;
+            const v4f g = acc[At::gate(i)][t] + bias, u = acc[At::up(i)][t] + bias_up;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][t][e] = j + e < p.n ? gated(p.gate, g[e], u[e]) : 0.f;
+            for (int e = 0; e < 4; ++e) acc[At::gate(i)][t][e] = j + e < p.n ? gated(p.gate, g[e], u[e]) : 0.f;
         }
     }
     __syncthreads();
     if (p.y_f16) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < kResults; ++i)
 #pragma unroll
             for (int t = 0; t < TM; ++t)
-                *reinterpret_cast<v4h*>(place_in_rows<uint16_t, kWidth>(lds, (wm * TM + t) * 16 + col, wn * 32 + i * 16 + q * 4)) = __builtin_convertvector(acc[i][t], v4h);
+                *reinterpret_cast<v4h*>(place_in_rows<uint16_t, kWidth>(lds, row_at + At::row(t, lane), out_at + At::result(i, lane))) = __builtin_convertvector(acc[At::gate(i)][t], v4h);
         __syncthreads();
         store_rows<uint16_t, kWidth, kRows, kThreads>(lds, p.y_f16, p.y_stride, row0, rows, j0, p.n);
     }
@@ -347,32 +363,32 @@ __device__ __forceinline__ void write_gated_group(const F8Params& p, v4f (&acc)[
         for (int t = 0; t < TM; ++t) {
             float a = 0.f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < kResults; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) a = fmaxf(a, fabsf(acc[i][t][e]));
-            a = fmaxf(a, __shfl_xor(a, 16));
-            a = fmaxf(a, __shfl_xor(a, 32));
-            if (q == 0) most[wn * kRows + (wm * TM + t) * 16 + col] = a;
+                for (int e = 0; e < 4; ++e) a = fmaxf(a, fabsf(acc[At::gate(i)][t][e]));
+#pragma unroll
+            for (int d = SIDE; d < 64; d <<= 1) a = fmaxf(a, __shfl_xor(a, d));
+            if (lane < SIDE) most[wn * kRows + row_at + At::row(t, lane)] = a;
         }
         __syncthreads();
         float s[TM];
 #pragma unroll
         for (int t = 0; t < TM; ++t) {
-            const int row = (wm * TM + t) * 16 + col;
+            const int row = row_at + At::row(t, lane);
             float top = most[row];
 #pragma unroll
             for (int o = 1; o < WN; ++o) top = fmaxf(top, most[o * kRows + row]);
             s[t] = scale_of(top);
-            if (wn == 0 && q == 0 && row < rows) p.y_scale[(size_t)group_n * p.m + row0 + row] = s[t];
+            if (wn == 0 && lane < SIDE && row < rows) p.y_scale[(size_t)group_n * p.m + row0 + row] = s[t];
         }
         __syncthreads();
 #pragma unroll
         for (int t = 0; t < TM; ++t) {
             const float r = 1.f / s[t];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const v4f v = acc[i][t] * r;
-                *reinterpret_cast<int*>(place_in_rows<uint8_t, kWidth>(lds, (wm * TM + t) * 16 + col, wn * 32 + i * 16 + q * 4)) = four_codes(v[0], v[1], v[2], v[3]);
+            for (int i = 0; i < kResults; ++i) {
+                const v4f v = acc[At::gate(i)][t] * r;
+                *reinterpret_cast<int*>(place_in_rows<uint8_t, kWidth>(lds, row_at + At::row(t, lane), out_at + At::result(i, lane))) = four_codes(v[0], v[1], v[2], v[3]);
             }
         }
         __syncthreads();
@@ -508,8 +524,8 @@ __global__ __launch_bounds__(512, 2) void f8_wide_kernel(const F8Params p) {
         if (b + 1 < blocks) block(w1, w0, b + 1);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was staged behind the end, in front of the results' barrier
-    if constexpr (!GATED) write_group<WN, 2, TM, false>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
-    else write_gated_group<WN, 2, TM>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
+    if constexpr (!GATED) write_group<16, WN, 2, TM, false>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
+    else write_gated_group<16, WN, 2, TM>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
 }
 
 // ---- few rows, or few products ----
@@ -658,132 +674,145 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void f8_rows_kernel(const F8Params
 }
 
 // ---- many rows, exact products ----
-// A group of WN x WM waves takes 64 WN outputs and 16 TM WM rows, a wave 64 x 16 TM. A block's rows become halves once for the group, on their way into LDS
-// (four buffers); a wave's weights come from L2 as codes, a block ahead, and become halves in its registers. A block is 8 TM steps of two matrix products
-// each (2 x 17 cycles), and what else there is to do has its steps: the multiply-adds of the pair of tiles before, the conversions, the loads one by one. The
-// barrier in the block's middle says that the next block's rows are there.
+// A group of WN x WM waves takes 64 WN outputs and 32 TM WM rows, a wave 64 x 32 TM, in products of 32 x 32: of the cycles in which a SIMD can issue they leave
+// more to the conversions and multiply-adds than those of 16 x 16 (48 of these beside 32 x 32 x 128 values take 277 cycles, 342 with the smaller ones). A
+// block's rows become halves once for the group, on their way into LDS (four buffers); a wave's weights come from L2 as codes, a block ahead, and become halves
+// in its registers. A block is 2 TM chains of eight products, one chain for 32 outputs and 32 rows, and what else there is to do has its products: the
+// multiply-adds of the chain before, the conversions, the loads one by one, the next chain's rows. Each load's place is the
+// latest that still covers L2's answer, since all of it together takes every register there is; the barrier says that the next block's rows are there.
+// Measured: 8192 x 8192 x 4096 in 465 us, 1.18 PFLOP/s, where the library's product of halves reaches 1.13; the smaller products took 467, the clock gives way
+// under either. 300 x 4096 x 4096 in 24.3 us (27.4), 200 rows of the gated 4096 x 4096 in 37.6 (42.0).
 template <int WN, int WM, int TM, bool GATED>
 __global__ __launch_bounds__(64 * WN * WM, 2) void f8_tile_kernel(const F8Params p) {
     exhip_touch_args(p);
-    constexpr int TN = 4, kRows = 16 * TM * WM, kThreads = 64 * WN * WM, kSteps = 8 * TM, kBuffers = 4, kPitch = 272, kBuffer = kRows * (kPitch + 4);
+    constexpr int TN = 4, kRows = 32 * TM * WM, kThreads = 64 * WN * WM, kSteps = 16 * TM, kBuffers = 4, kPitch = 272, kBuffer = kRows * (kPitch + 4);
     static_assert(kRows * 4 == kThreads, "a thread stages a quarter of a row");
-    // [buffer][row][16 pieces of 16 bytes]: piece 4 s + q of a row is halves_of()'s piece s of lanes of quarter q. A row's pitch is 16 bytes more, so that a
-    // piece of eight neighbouring rows lies in all banks. The rows' scales stand behind them.
+    // [buffer][row][128 halves], a row's pitch 16 bytes more, so that a piece of eight neighbouring rows lies in all banks; the rows' scales behind them
     constexpr int kStaged = kBuffers * kBuffer, kResults = kRows * (GATED ? 32 * WN * 2 : 64 * WN * 4);
     __shared__ __attribute__((aligned(16))) char memory[kStaged > kResults ? kStaged : kResults];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wn = wave % WN, wm = wave / WN;
-    const int q = lane / 16, col = lane % 16;
+    const int side = lane / 32, col = lane % 32;
     int group_n, group_m;
     tile_of(p.groups_n, p.groups_m, &group_n, &group_m);
     const int tile0 = (group_n * WN + wn) * TN, row0 = group_m * kRows;
     const int rows = min(kRows, p.m - row0), tail = p.k % kBlk, blocks = p.blocks_k;
-    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.x) + (size_t)row0 * p.x_stride, 0,
-                                                                      (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16, kRsrcWord3);
+    const __amdgpu_buffer_rsrc_t xr = uniform_view(p.x + (size_t)row0 * p.x_stride, (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16);
     // what this thread stages
     const int own_row = threadIdx.x / 4, own_q = threadIdx.x % 4;
     const int off = own_row < rows ? own_row * p.x_stride + own_q * 16 : kNoRow;
-    const unsigned scale_at = min(own_row, rows - 1);
+    const int scale_at = own_row * 4;
     v4i codes[2];
     float code_scale = 0.f;
     auto request = [&](int b, int j) {  // in three loads; behind the last block that one again, which nothing reads
         b = min(b, blocks - 1);
-        if (j < 2) codes[j] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xr, off + b * kBlk + j * 64, 0, 0));
-        else code_scale = (p.x_scale + (size_t)b * p.m + row0)[scale_at];
+        if (j < 2) codes[j] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xr, off, b * kBlk + j * 64, 0));
+        else code_scale = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(uniform_view(p.x_scale + (size_t)b * p.m + row0, rows * 4), scale_at, 0, 0));
     };
-    auto stage = [&](int b, int s) {  // in four pieces
-        if (s == 0 && tail && b == blocks - 1) {
-            codes[0] &= keep_first(tail - own_q * 16);
-            codes[1] &= keep_first(tail - 64 - own_q * 16);
-        }
+    auto stage = [&](int b, int j) {  // in four pieces of eight values
         char* const to = memory + b % kBuffers * kBuffer;
-        *reinterpret_cast<v8h*>(to + own_row * kPitch + (4 * s + own_q) * 16) = halves_of(codes[0][s], codes[1][s]);
-        if (s == 0 && own_q == 0) *reinterpret_cast<float*>(to + kRows * kPitch + own_row * 4) = code_scale;
+        *reinterpret_cast<v8h*>(to + own_row * kPitch + j / 2 * 128 + own_q * 32 + j % 2 * 16) = halves_of(codes[j / 2][j % 2 * 2], codes[j / 2][j % 2 * 2 + 1]);
+        if (j == 0) *reinterpret_cast<float*>(to + kRows * kPitch + own_row * 4) = code_scale;
     };
+    auto cut = [&] {  // the last block's codes where the row ends
+        int left = tail - own_q * 16;
+        asm volatile("" : "+v"(left));  // or the masks are made before the loop and take eight registers of it
+        codes[0] &= keep_first(left);
+        codes[1] &= keep_first(left - 64);
+    };
+    // A lane's weights are those of output lane % 32 of two tiles: of a tile's [half][quarter][output] the quarters 2 side and 2 side + 1. Product s of a chain takes
+    // values 8 (s % 2) and on of quarter s / 2 % 2 of half s / 4, and the rows' values in the same order.
     const WeightRows weights(p, tile0, TN, lane);
+    int weights_at[2];
+#pragma unroll
+    for (int f = 0; f < 2; ++f) weights_at[f] = min(2 * f + col / 16, weights.last - weights.first) * weights.row_bytes + side * 512 + col % 16 * 16;
     const int block_n = min(GATED ? tile0 / 2 : tile0, (p.n - 1) / 16) / (kBlk / 16);
     const Constants ws = (Constants)(uintptr_t)(p.w_scale + (size_t)block_n * blocks);
     const Constants ws_up = (Constants)(uintptr_t)(GATED ? p.w_scale_up + (size_t)block_n * blocks : nullptr);
-    v4i raw[TN][2];
-    auto request_w = [&](int b, int j) { raw[j / 2][j % 2] = weights.load(j / 2, min(b, blocks - 1), j % 2); };  // in eight
-    Halves w[TN];
-    v4f acc[TN][TM];
+    v4i raw[2][4];
+    auto request_w = [&](int b, int f, int j) {  // in four loads of each of the two
+        raw[f][j] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(weights.view, weights_at[f], min(b, blocks - 1) * 2048 + j / 2 * 1024 + j % 2 * 256, 0));
+    };
+    v8h w[2][8], x[8];
+    auto convert_w = [&](int f, int s) {
+        w[f][s] = halves_of(raw[f][s / 2][s % 2 * 2], raw[f][s / 2][s % 2 * 2 + 1]);
+        asm volatile("" : "+v"(w[f][s]));  // here, not together ahead of the chain that takes them
+    };
+    auto piece_of = [&](int b, int t, int s) {
+        return *reinterpret_cast<const v8h*>(memory + b % kBuffers * kBuffer + ((wm * TM + t) * 32 + col) * kPitch + side * 64 + s / 4 * 128 + s % 4 * 16);
+    };
+    auto scale_of_row = [&](int b, int t) { return *reinterpret_cast<const float*>(memory + b % kBuffers * kBuffer + kRows * kPitch + ((wm * TM + t) * 32 + col) * 4); };
+    v4f acc[8][TM];
 #pragma unroll
-    for (int i = 0; i < TN; ++i)
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int t = 0; t < TM; ++t) acc[i][t] = v4f{0.f, 0.f, 0.f, 0.f};
-    struct Rows {
-        v8h v[4];
-        float s;
-    };
-    auto rows_from = [&](int b, int t) {
-        const char* const from = memory + b % kBuffers * kBuffer;
-        const int row = (wm * TM + t) * 16 + col;
-        Rows r;
+    v16f part[2], none;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) r.v[s] = *reinterpret_cast<const v8h*>(from + row * kPitch + (4 * s + q) * 16);
-        r.s = *reinterpret_cast<const float*>(from + kRows * kPitch + row * 4);
-        return r;
+    for (int e = 0; e < 16; ++e) none[e] = 0.f;
+    part[1] = none;
+    float sc[TM], sc_up[TM], last = 0.f, last_up = 0.f;  // of the block's rows, and of the chain that the block before ended with
+    auto add = [&](int f, int t, int g, float s, float s_up) {  // four of a chain's outputs to their sums
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[f * 4 + g][t][e] = __builtin_fmaf(part[f][g * 4 + e], GATED && g >= 2 ? s_up : s, acc[f * 4 + g][t][e]);
+        asm volatile("" : "+v"(acc[f * 4 + g][t]));  // here, not where the compiler would like them: together at the end, out of registers
     };
 #pragma unroll
     for (int j = 0; j < 3; ++j) request(0, j);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) request_w(0, j);
+    for (int j = 0; j < 8; ++j) request_w(0, j / 4, j % 4);
+    if (tail && blocks == 1) cut();
 #pragma unroll
-    for (int s = 0; s < 4; ++s) stage(0, s);
+    for (int j = 0; j < 4; ++j) stage(0, j);
 #pragma unroll
-    for (int j = 0; j < 3; ++j) request(1, j);
+    for (int j = 0; j < 3; ++j)
+        if (TM == 1) request(1, j);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) w[i] = halves_of(raw[i][0], raw[i][1]);
+    for (int s = 0; s < 8; ++s) convert_w(0, s);
     __syncthreads();
-    Rows x[2];
-    x[0] = rows_from(0, 0);
-    float s_w = ws[0], s_up = GATED ? ws_up[0] : 0.f, s_next = 0.f, s_up_next = 0.f;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) x[s] = piece_of(0, 0, s);
+    float row_scale = scale_of_row(0, 0), s_w = ws[0], s_up = GATED ? ws_up[0] : 0.f, s_next = 0.f, s_up_next = 0.f;
     for (int b = 0; b < blocks; ++b) {
-        v4f part[2][2];
-        float sc[2], sc_up[2];
+        if (TM == 1 && tail && b == blocks - 2) cut();
 #pragma unroll
-        for (int u = 0; u < kSteps + 2; ++u) {
-            const int t = u / 8, pair = u / 4 % 2, s = u % 4;
-            if (u < 4) {
-#pragma unroll
-                for (int i = 2; i < 4; ++i) w[i].v[u] = halves_of(raw[i][0][u], raw[i][1][u]);
-            }
-            if (u < 8) request_w(b + 1, u);  // (those of step u < 4 were used up in the block before)
-            if (u >= kSteps / 4 && u < kSteps / 4 + 4) stage(b + 1, u - kSteps / 4);
-            if (u >= kSteps / 4 + 4 && u < kSteps / 4 + 7) request(b + 2, u - kSteps / 4 - 4);
-            if (u == kSteps / 2) {
+        for (int u = 0; u < kSteps; ++u) {
+            const int t = u / 16, f = u / 8 % 2, s = u % 8;
+            constexpr int kStage = TM == 1 ? 4 : 12, kAsk = TM == 1 ? 8 : 0;
+            if (u == kSteps / 2 - 4) {
                 const int after = min(b + 1, blocks - 1);
                 s_next = ws[after];
                 if constexpr (GATED) s_up_next = ws_up[after];
-                __syncthreads();
             }
-            if (u >= kSteps - 4 && u < kSteps) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) w[i].v[u % 4] = halves_of(raw[i][0][u % 4], raw[i][1][u % 4]);
+            if (u == (TM == 1 ? 8 : 20)) __syncthreads();
+            if (TM > 1 && u == kStage && tail && b == blocks - 2) cut();
+            if (u % 16 == 0) {
+                sc[t] = s_w * row_scale;
+                sc_up[t] = s_up * row_scale;
             }
-            if (u < kSteps) {
-                if (u % 8 == 0) {
-                    sc[t % 2] = s_w * x[t % 2].s;
-                    sc_up[t % 2] = s_up * x[t % 2].s;
-                    x[(t + 1) % 2] = t + 1 < TM ? rows_from(b, t + 1) : rows_from(b + 1, 0);
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    part[pair][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[2 * pair + i].v[s], x[t % 2].v[s], s == 0 ? v4f{0.f, 0.f, 0.f, 0.f} : part[pair][i], 0, 0, 0);
-            }
-            if (u >= 4 && s < 2) {  // of the pair before, a tile a step
-                const int vt = (u - 4) / 8, vi = (1 - pair) * 2 + s;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[vi][vt][e] = __builtin_fmaf(part[1 - pair][s][e], GATED && s == 1 ? sc_up[vt % 2] : sc[vt % 2], acc[vi][vt][e]);
-                asm volatile("" : "+v"(acc[vi][vt]));  // here, not where the compiler would like them: together at the end, out of registers
+            if (u < 8) convert_w(1, s);
+            if (u >= kSteps / 2 - 8 && u < kSteps / 2 - 4) request_w(b + 1, 0, u - (kSteps / 2 - 8));
+            if (u >= kSteps - 8 && u < kSteps - 4) request_w(b + 1, 1, u - (kSteps - 8));
+            if (u >= kStage && u < kStage + 4) stage(b + 1, u - kStage);
+            if (u >= kAsk && u < kAsk + 3) request(TM == 1 ? b + 2 : b + 1, u - kAsk);
+            part[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w[f][s], x[s], s == 0 ? none : part[f], 0, 0, 0);
+            if (f == 1) x[s] = t + 1 < TM ? piece_of(b, t + 1, s) : piece_of(b + 1, 0, s);
+            if (f == 1 && s == 7) row_scale = t + 1 < TM ? scale_of_row(b, t + 1) : scale_of_row(b + 1, 0);
+            if (u >= kSteps - 8) convert_w(0, s);
+            if (s >= 2 && s < 6) {
+                if (u < 8) add(1, TM - 1, s - 2, last, last_up);
+                else add(1 - f, f == 1 ? t : t - 1, s - 2, sc[f == 1 ? t : t - 1 < 0 ? 0 : t - 1], sc_up[f == 1 ? t : t - 1 < 0 ? 0 : t - 1]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        last = sc[TM - 1];
+        last_up = sc_up[TM - 1];
         s_w = s_next;
         s_up = s_up_next;
     }
-    if constexpr (!GATED) write_group<WN, WM, TM, true>(p, acc, group_n, wn, wm, row0, rows, lane, memory);
-    else write_gated_group<WN, WM, TM>(p, acc, group_n, wn, wm, row0, rows, lane, memory);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) add(1, TM - 1, g, last, last_up);
+    if constexpr (!GATED) write_group<32, WN, WM, TM, true>(p, acc, group_n, wn, wm, row0, rows, lane, memory);
+    else write_gated_group<32, WN, WM, TM>(p, acc, group_n, wn, wm, row0, rows, lane, memory);
 }
 
 // ---- a tile or two for every CU ----
@@ -913,8 +942,8 @@ __global__ __launch_bounds__(512, 2) void f8_deep_kernel(const F8Params p) {
         if (b + 1 < blocks) block(w1, w0, b + 1);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was staged behind the end, in front of the results' barrier
-    if constexpr (!GATED) write_group<WN, WM, TM, false>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
-    else write_gated_group<WN, WM, TM>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
+    if constexpr (!GATED) write_group<16, WN, WM, TM, false>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
+    else write_gated_group<16, WN, WM, TM>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
 }
 
 int blocks_of(int v) { return v / kBlk + (v % kBlk != 0); }
@@ -985,7 +1014,7 @@ int run_rows(exhip_ctx* ctx, const F8Params& p) {
 }
 template <int WN, int WM, int TM, bool GATED>
 int run_tile(exhip_ctx* ctx, const F8Params& p) {
-    return launch(ctx, f8_tile_kernel<WN, WM, TM, GATED>, p, 4 * WN, 16 * TM * WM, 64 * WN * WM);
+    return launch(ctx, f8_tile_kernel<WN, WM, TM, GATED>, p, 4 * WN, 32 * TM * WM, 64 * WN * WM);
 }
 template <bool GATED>
 int run_deep(exhip_ctx* ctx, const F8Params& p) {
@@ -1000,7 +1029,7 @@ int run_wide(exhip_ctx* ctx, const F8Params& p) {
 constexpr Form kExact[] = {  // results in float32
     {run_rows<1, 1, 1, 8, 4, false>, 1, 16, 512, 8, 0.4f, 2.2f, 0.85f}, {run_rows<2, 1, 1, 8, 2, false>, 2, 16, 512, 8, 0.f, 2.9f, 0.86f},
     {run_rows<2, 2, 1, 8, 2, false>, 2, 32, 256, 8, 1.4f, 1.3f, 1.42f}, {run_rows<4, 2, 1, 8, 1, false>, 4, 32, 256, 8, 0.7f, 2.4f, 1.65f},
-    {run_tile<2, 2, 2, false>, 8, 64, 512, 1, 0.f, 4.0f, 0.80f},        {run_tile<4, 1, 4, false>, 16, 64, 512, 1, 0.f, 4.8f, 1.08f},
+    {run_tile<2, 2, 1, false>, 8, 64, 512, 1, 0.f, 3.8f, 0.66f},        {run_tile<4, 1, 2, false>, 16, 64, 512, 1, 0.f, 4.4f, 0.90f},
 };
 constexpr Form kHalves[] = {
     kExact[0], kExact[1], kExact[2], kExact[3], {run_deep<false>, 8, 128, 256, 1, 0.7f, 3.5f, 0.47f}, {run_wide<false>, 16, 256, 256, 1, 0.f, 6.0f, 1.18f},
@@ -1012,7 +1041,7 @@ constexpr Form kGatedHalves[] = {
 };
 constexpr Form kGatedCodes[] = {  // a group has whole blocks of the result: 16 tiles
     {run_rows<4, 1, 4, 2, 2, true>, 16, 16, 256, 2, 0.f, 4.0f, 0.97f}, {run_rows<4, 2, 4, 2, 1, true>, 16, 32, 256, 2, 0.f, 5.2f, 1.40f},
-    {run_tile<4, 1, 4, true>, 16, 64, 512, 1, 0.f, 9.5f, 1.11f},
+    {run_tile<4, 1, 2, true>, 16, 64, 512, 1, 0.f, 8.3f, 1.01f},
 };
 
 template <int N>
