@@ -9,8 +9,9 @@
 
 namespace {
 
-constexpr int kMostSlice = 32768, kSmallSlice = 8192;  // values of a row that a group of 16, of 4 waves holds in its registers
-constexpr int kCandidates = 512;    // values of a slice that are ranked at once
+constexpr int kMostSlice = 32768, kSmallSlice = 1 << 13;  // values of a row that a group of 16, of 4 waves holds in its registers
+constexpr int kCandidates = 512;  // places that are held at once
+constexpr int kRanked = 128;      // and that are ranked, each against all; of more, those behind the top-th are left out first
 typedef unsigned long long u64;
 
 template <typename T, int N>
@@ -56,13 +57,17 @@ __device__ __forceinline__ float over_wave(float v, F f) {
     const unsigned h0 = h[0], h1 = h[1];
     return f(__builtin_bit_cast(float, h0), __builtin_bit_cast(float, h1));
 }
-// A bound that `top` of a wave's 64 values reach: the top-th largest, by halving, to 16 bits of order_of(), downwards.
-__device__ __forceinline__ unsigned reached_by(unsigned order, int top) {
+// A bound that `top` of a wave's values, N of each lane, reach: the top-th largest, by halving, to BITS bits of order_of(), downwards.
+template <int BITS, int N>
+__device__ __forceinline__ unsigned reached_by(const unsigned (&order)[N], int top) {
     unsigned bound = 0;
 #pragma unroll
-    for (int bit = 31; bit >= 16; --bit) {
+    for (int bit = 31; bit >= 32 - BITS; --bit) {
         const unsigned up = bound | 1u << bit;
-        bound = __popcll(__ballot(order >= up)) >= top ? up : bound;
+        int reach = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) reach += __popcll(__ballot(order[e] >= up));
+        bound = reach >= top ? up : bound;
     }
     return bound;
 }
@@ -124,6 +129,37 @@ __device__ __forceinline__ int rank_of(u64 own, const u64* places, int n) {
     }
     return rank;
 }
+// The `top` first of n places, in falling order, into sorted, by one wave.
+__device__ __forceinline__ void rank_places(u64* places, int n, int top, u64* sorted) {
+    const int lane = threadIdx.x % 64;
+    if (lane < 8) places[n + lane] = 0;
+    wave_sync();
+    for (int i = lane; i < n; i += 64) {
+        const u64 own = places[i];
+        const int rank = rank_of(own, places, n);
+        if (rank < top) sorted[rank] = own;
+    }
+    wave_sync();
+}
+// Of kHeld places of each lane (0: none) those that reach a bound, into places; how many.
+constexpr int kHeld = kCandidates / 64;
+__device__ __forceinline__ int keep_reaching(const u64 (&held)[kHeld], unsigned bound, u64* places) {
+    int n = 0;
+#pragma unroll
+    for (int e = 0; e < kHeld; ++e) {
+        const bool takes = held[e] != 0 && (unsigned)(held[e] >> 32) >= bound;
+        const u64 all_takes = __ballot(takes);
+        if (takes) places[n + place_in(all_takes)] = held[e];
+        n += __popcll(all_takes);
+    }
+    return n;
+}
+__device__ __forceinline__ unsigned reached_by_all(const u64 (&held)[kHeld], int top) {
+    unsigned order[kHeld];
+#pragma unroll
+    for (int e = 0; e < kHeld; ++e) order[e] = (unsigned)(held[e] >> 32);
+    return reached_by<16>(order, top);
+}
 
 struct LogpParams {
     const int32_t* ids;
@@ -164,14 +200,14 @@ __device__ __forceinline__ void write_row(const T* __restrict__ src, const LogpP
 // A group of W waves a slice of a row, V values a thread, all requested before the first is used. What one wave can do for the group is wave 0's: the others
 // would only take its turns.
 template <typename T, int W, int V, bool TOP>
-__global__ __launch_bounds__(64 * W, W == 16 ? 8 : 4) void log_probabilities_kernel(const T* __restrict__ x, const LogpParams p) {
+__global__ __launch_bounds__(64 * W, 8) void log_probabilities_kernel(const T* __restrict__ x, const LogpParams p) {
     exhip_touch_args(p);
     constexpr int kThreads = 64 * W, N = 16 / sizeof(T), kRuns = V / N;
-    static_assert(W == 1 || W == 4 || W == 16, "64 sets of W neighbouring lanes");
+    static_assert(W == 1 || W == 4 || (W == 16 && !TOP), "128 sets of the slice's values");
     __shared__ Sums sums[W];
-    __shared__ float sets[64], bound;
+    __shared__ float sets[TOP ? 128 : 1], bound;
     __shared__ u64 places[TOP ? kCandidates + 8 : 1], sorted[TOP ? EXHIP_LOG_PROBABILITIES_TOP : 1];
-    __shared__ int count;
+    __shared__ int count, counts[2][W];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const size_t row = blockIdx.x / p.slices;
     const int slice = blockIdx.x % p.slices, first = slice * p.slice_len, len = min(p.slice_len, p.c - first);
@@ -179,6 +215,15 @@ __global__ __launch_bounds__(64 * W, W == 16 ? 8 : 4) void log_probabilities_ker
     Run<T, N> r[kRuns];
     auto value = [&](int e) { return as_float(r[e / N].v[e % N]); };
     auto at = [&](int e) { return (e / N * kThreads + (int)threadIdx.x) * N + e % N; };  // of value e in the slice
+    auto read = [&](int i) {
+        Run<T, N> run;
+        const int k = at(i * N);
+        if (k + N <= len) run = *reinterpret_cast<const Run<T, N>*>(src + k);
+        else
+#pragma unroll
+            for (int e = 0; e < N; ++e) run.v[e] = k + e < len ? src[k + e] : masked(T());
+        return run;
+    };
 #pragma unroll
     for (int i = 0; i < kRuns; ++i) {
         const int k = at(i * N);
@@ -214,11 +259,17 @@ __global__ __launch_bounds__(64 * W, W == 16 ? 8 : 4) void log_probabilities_ker
         if (lane == 0) sums[wave] = all;
     }
     if constexpr (TOP) {
-        // the largest of each of the group's 64 sets of W neighbouring lanes
-        float m = mine;
-        if constexpr (W > 1) m = fmaxf(m, traded<0xB1>(m)), m = fmaxf(m, traded<0x4E>(m));
-        if constexpr (W > 4) m = fmaxf(m, traded<0x141>(m)), m = fmaxf(m, traded<0x140>(m));
-        if (lane % W == 0) sets[wave * (64 / W) + lane / W] = m;
+        // the largest of each of 128 sets: two lanes' values, or one wave's even and odd runs
+        if constexpr (W > 1) {
+            const float m = fmaxf(mine, traded<0xB1>(mine));
+            if (lane % 2 == 0) sets[wave * 32 + lane / 2] = m;
+        } else {
+            float m[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < kRuns; ++i) m[i % 2] = fmaxf(m[i % 2], largest[i]);
+            sets[lane] = m[0];
+            sets[64 + lane] = m[1];
+        }
         if (threadIdx.x == 0) count = 0;
     }
     __syncthreads();
@@ -236,7 +287,8 @@ __global__ __launch_bounds__(64 * W, W == 16 ? 8 : 4) void log_probabilities_ker
         if constexpr (TOP) {
             // `top` sets hold a value that reaches the top-th largest of the sets' largest, so the slice's `top` largest all do. A class of no probability is
             // no candidate whatever the bound; with a NaN nothing is.
-            const unsigned o = reached_by(order_of(sets[lane]), p.top);
+            const unsigned of_sets[2] = {order_of(sets[lane]), order_of(sets[64 + lane])};
+            const unsigned o = reached_by<16>(of_sets, p.top);
             const float least = o <= 0x007fffffu ? -FLT_MAX : __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o);
             if (lane == 0) bound = all.s != all.s ? INFINITY : least;
         }
@@ -265,53 +317,104 @@ __global__ __launch_bounds__(64 * W, W == 16 ? 8 : 4) void log_probabilities_ker
                     }
                 }
         __syncthreads();
-        const bool nan = least == INFINITY;  // (or a +infinity, whose exponential is one)
-        int n = nan ? kCandidates + 1 : count;
-        if (n <= kCandidates) {
-            if (wave != 0) return;
-            if (n < p.top) {  // masked classes too, by their index: they are among the first n + top of the slice
-                const int reach = min(n + p.top, len);
-                for (int i = lane; i - lane < reach; i += 64) {
-                    const bool takes = i < reach && as_float(src[i]) == -INFINITY;
-                    const u64 all_takes = __ballot(takes);
-                    if (takes) places[n + place_in(all_takes)] = place_of(-INFINITY, first + i);
-                    n += __popcll(all_takes);
-                }
-            }
-            if (lane < 8) places[n + lane] = 0;
-            if (lane >= n && lane < p.top) sorted[lane] = 0;
-            wave_sync();
-            for (int i = lane; i < n; i += 64) {
-                const u64 own = places[i];
-                const int rank = rank_of(own, places, n);
-                if (rank < p.top) sorted[rank] = own;
-            }
-            wave_sync();
-        } else {
-            // many equal values, or a NaN: the largest behind the last one found, `top` times, each a reading of the slice
-            u64 last = ~0ull;
-            for (int i = 0; i < p.top; ++i) {
-                u64 best = 0;
-                for (int k = threadIdx.x; k < len; k += kThreads) {
-                    const u64 here = place_of(as_float(src[k]), first + k);
-                    if (here < last && here > best) best = here;
-                }
+        int n = count;
+        const bool many = least == INFINITY || n > kCandidates;  // a NaN (or a +infinity, whose exponential is one), or values close to each other
+        if (many) {
+            // The bound is raised by halves until between `want` and kRanked values reach it; where more are alike (all of a slice, if its classes are masked
+            // with the type's lowest value), as many of these as come first. (300 rows of 100003 equal halves: 71 us with the 8 largest, 156 with 64; a reading of the
+            // slice for each of the largest took 187 and 1375.)
+            const int want = min(p.top, len);
+            int turn = 0;
+            const unsigned of_sets[2] = {order_of(sets[lane]), order_of(sets[64 + lane])};
+            unsigned o = reached_by<32>(of_sets, want), most_o = ~0u;
+            int above = 0;  // the values whose order is more than o
+            auto held = [&](auto takes) {
+                int here = 0, more = 0;
+#pragma unroll 1
+                for (int i = 0; i < kRuns; ++i) {  // read again: what stays of them for this path costs the other one its waves
+                    const Run<T, N> run = read(i);
 #pragma unroll
-                for (int d = 1; d < 64; d <<= 1) {
-                    const u64 other = __shfl_xor(best, d);
-                    best = other > best ? other : best;
+                    for (int e = 0; e < N; ++e) {
+                        const unsigned order = order_of(as_float(run.v[e]));
+                        here += __popcll(__ballot(takes(order, at(i * N + e))));
+                        more += __popcll(__ballot(order > o));
+                    }
                 }
-                __syncthreads();
-                if (lane == 0) places[wave] = best;
-                __syncthreads();
-                last = places[0];
-                for (int w = 1; w < W; ++w) last = places[w] > last ? places[w] : last;
-                if (threadIdx.x == 0) sorted[i] = last;
-                if (last == 0) last = 1;  // nothing is left: none of the places lies beneath
+                if constexpr (W > 1) {
+                    if (lane == 0) counts[turn][wave] = here | more << 16;
+                    __syncthreads();
+                    here = 0;
+#pragma unroll
+                    for (int w = 0; w < W; ++w) here += counts[turn][w];
+                    turn ^= 1;
+                    more = here >> 16;
+                    here &= 0xffff;
+                }
+                above = more;
+                return here;
+            };
+            int reach = held([&](unsigned order, int) { return order >= o; });
+            while (reach > kRanked && above >= want && o < most_o) {
+                const unsigned up = o + (most_o - o) / 2 + 1;
+                const int n_up = held([&](unsigned order, int) { return order >= up; });
+                if (n_up < want) {
+                    most_o = up - 1;
+                } else {
+                    o = up;
+                    reach = n_up;
+                    above = want;  // or more, unless there is nothing above
+                    if (o == most_o) held([&](unsigned, int) { return false; });
+                }
             }
-            if (wave != 0) return;
-            wave_sync();
+            int begin = 0, end = len;  // of those alike, what stands in front of `end`
+            for (int step = 0, n_begin = above, n_end = reach; n_end > kRanked; ++step) {
+                // where they would be spread evenly, and the middle, by turns
+                const int even = (end - begin) * ((want + kRanked) / 2 - n_begin) / (n_end - n_begin), most_to = end - begin > 1 ? end - begin - 1 : 1;
+                const int to = begin + (step % 2 == 0 && even > 0 && even < most_to ? even : (end - begin + 1) / 2);
+                const int here = held([&](unsigned order, int i) { return order == o && i < to; }), n_to = above + here;
+                if (n_to < want) {
+                    begin = to;
+                    n_begin = n_to;
+                } else {
+                    end = to;
+                    n_end = n_to;
+                }
+            }
+            if (threadIdx.x == 0) count = 0;
+            __syncthreads();
+#pragma unroll 1
+            for (int i = 0; i < kRuns; ++i) {
+                const Run<T, N> run = read(i);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const float v = as_float(run.v[e]);
+                    const unsigned order = order_of(v);
+                    const int k = at(i * N + e);
+                    if (order > o || (order == o && k < end)) places[atomicAdd(&count, 1)] = place_of(v, first + k);
+                }
+            }
+            __syncthreads();
+            n = count;  // without what stands behind the slice's end
         }
+        if (wave != 0) return;
+        if (!many && n < p.top) {  // masked classes too, by their index: they are among the first n + top of the slice
+            const int reach = min(n + p.top, len);
+            for (int i = lane; i - lane < reach; i += 64) {
+                const bool takes = i < reach && as_float(src[i]) == -INFINITY;
+                const u64 all_takes = __ballot(takes);
+                if (takes) places[n + place_in(all_takes)] = place_of(-INFINITY, first + i);
+                n += __popcll(all_takes);
+            }
+        }
+        if (lane >= n && lane < p.top) sorted[lane] = 0;
+        wave_sync();
+        if (n > kRanked) {
+            u64 held[kHeld];
+#pragma unroll
+            for (int e = 0; e < kHeld; ++e) held[e] = e * 64 + lane < n ? places[e * 64 + lane] : 0;
+            n = keep_reaching(held, reached_by_all(held, p.top), places);
+        }
+        rank_places(places, n, p.top, sorted);
     } else if (wave != 0) {
         return;
     }
@@ -327,7 +430,6 @@ __global__ __launch_bounds__(64 * W, W == 16 ? 8 : 4) void log_probabilities_ker
 // The largest of the slices' lists, `top` of them into sorted, by one wave: a batch of entries is held in registers with those found so far in front, and what
 // reaches the top-th largest of the lanes' largest is ranked.
 __device__ __forceinline__ void join_lists(const u64* __restrict__ from, size_t total, int top, u64* places, u64* sorted) {
-    constexpr int kHeld = 8;
     const int lane = threadIdx.x;
     int kept = 0;
     for (size_t done = 0; done < total;) {
@@ -340,23 +442,15 @@ __device__ __forceinline__ void join_lists(const u64* __restrict__ from, size_t 
 #pragma unroll
         for (int e = 0; e < kHeld; ++e) most = held[e] > most ? held[e] : most;
         done += kHeld * 64 - kept;
-        const unsigned bound = reached_by((unsigned)(most >> 32), top);
-        int n = 0;
-#pragma unroll
-        for (int e = 0; e < kHeld; ++e) {
-            const bool takes = held[e] != 0 && (unsigned)(held[e] >> 32) >= bound;
-            const u64 all_takes = __ballot(takes);
-            if (takes) places[n + place_in(all_takes)] = held[e];
-            n += __popcll(all_takes);
+        unsigned bound;
+        if (top > 32) {  // of so many the lanes' largest leave hundreds to rank
+            bound = reached_by_all(held, top);
+        } else {
+            const unsigned of_lane[1] = {(unsigned)(most >> 32)};
+            bound = reached_by<16>(of_lane, top);
         }
-        if (lane < 8) places[n + lane] = 0;
-        wave_sync();
-        for (int i = lane; i < n; i += 64) {
-            const u64 own = places[i];
-            const int rank = rank_of(own, places, n);
-            if (rank < top) sorted[rank] = own;
-        }
-        wave_sync();
+        const int n = keep_reaching(held, bound, places);
+        rank_places(places, n, top, sorted);
         kept = min(n, top);
     }
 }
@@ -365,7 +459,7 @@ __device__ __forceinline__ void join_lists(const u64* __restrict__ from, size_t 
 template <typename T>
 __global__ __launch_bounds__(64) void join_slices_kernel(const T* __restrict__ x, const LogpParams p) {
     exhip_touch_args(p);
-    __shared__ u64 places[512 + 8], sorted[EXHIP_LOG_PROBABILITIES_TOP];
+    __shared__ u64 places[kCandidates + 8], sorted[EXHIP_LOG_PROBABILITIES_TOP];
     const int lane = threadIdx.x;
     const size_t row = blockIdx.x;
     Sums all = {-INFINITY, 0.f, 0.f, 0.f};

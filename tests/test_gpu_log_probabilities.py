@@ -184,3 +184,29 @@ def test_many_candidates_of_a_row(ctx):
     rng = np.random.default_rng(13)
     x = _logits(rng, 2, 3001, np.float32)
     _check(ctx, x, rng.integers(0, 3001, (2, 1000)))
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("c", [130, 513, 2049, 8200, 24999])
+@pytest.mark.parametrize("top", [1, 20, 64])
+def test_more_candidates_than_are_ranked(ctx, c, top, dtype):
+    rng = np.random.default_rng(c + top)
+    x = np.zeros((11, c), dtype)
+    low = np.finfo(dtype).min
+    x[0, rng.permutation(c)[:130]] = np.nan              # more than are asked, few others
+    x[1] = rng.standard_normal(c)
+    x[1, rng.permutation(c)[:100]] = np.inf
+    x[2] = np.sort(rng.standard_normal(c)).astype(dtype)
+    x[3] = np.linspace(1, 2, c)                          # close to each other
+    x[4] = rng.integers(0, 40, c)
+    x[5] = low
+    x[5, rng.permutation(c)[:top - 1]] = -1.0            # one of the masked ones is among the largest
+    x[6] = -np.inf
+    x[6, c // 2:] = low
+    x[7] = -np.inf
+    x[7, -1] = 0.0
+    x[8] = np.nan
+    x[9, ::-1] = np.repeat(np.arange(c // 70 + 1), 70)[:c] % 1500  # 70 alike of each
+    x[10] = np.where(np.arange(c) < c - 50, 1.0, 0.5)
+    got = _run(ctx, x, None, top)
+    assert np.array_equal(got["top_ids"], _order(x, top))
