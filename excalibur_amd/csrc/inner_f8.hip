@@ -707,7 +707,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void f8_tile_kernel(const F8Params
     float code_scale = 0.f;
     auto request = [&](int b, int j) {  // in three loads; behind the last block that one again, which nothing reads
         b = min(b, blocks - 1);
-        if (j < 2) codes[j] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xr, off, b * kBlk + j * 64, 0));
+        if (j < 2) codes[j] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xr, off + b * kBlk + j * 64, 0, 0));  // (all in what the bounds see: the last row may end here)
         else code_scale = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(uniform_view(p.x_scale + (size_t)b * p.m + row0, rows * 4), scale_at, 0, 0));
     };
     auto stage = [&](int b, int j) {  // in four pieces of eight values
@@ -956,6 +956,7 @@ template <typename T>
 int quantize_rows(exhip_ctx* ctx, const char* name, const T* x, int x_stride, int m, int k, uint8_t* y, int y_stride, float* scale) {
     EXHIP_REQUIRE(ctx && x && y && scale, "%s: NULL argument", name);
     EXHIP_REQUIRE(m > 0 && k > 0 && k <= kMostStride && x_stride >= k, "%s: %d rows of %d values, %d apart: sizes are positive, a row at most 2^22 values", name, m, k, x_stride);
+    EXHIP_REQUIRE(m <= 1 << 26, "%s: %d rows are more than one launch takes", name, m);
     EXHIP_REQUIRE(y_stride >= k && y_stride % 16 == 0 && y_stride <= kMostStride && aligned(y, 16), "%s: rows of codes begin on 16 bytes and hold the row (stride %d)", name, y_stride);
     EXHIP_REQUIRE(aligned(x, sizeof(T)) && aligned(scale, 4), "%s: an operand's address is not that of its type", name);
     const exhip_on_device on(ctx->device);

@@ -675,7 +675,7 @@ class Ctx:
 
     def log_probabilities(self, x, c=None, ids=None, top=0, log_p=None, entropy=None, top_ids=None, top_log_p=None, workspace=None):
         """Of rows x [m][stride] (float32, or halves as uint16) of c values: the log probabilities of ids [m][n], the entropy, the `top` largest classes and
-        their log probabilities, into the given arrays."""
+        their log probabilities, into the given arrays. Without a workspace it makes one and waits for the results; a recorded run is given one."""
         m, stride = x.shape
         c = stride if c is None else c
         own = self.empty((self.log_probabilities_workspace(m, c, top),), np.uint8) if workspace is None else None

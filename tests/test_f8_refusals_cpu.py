@@ -31,7 +31,7 @@ def test_quantize_rows_refusals(name):
     entry = getattr(_lib(), name)
     good = [X, 100, 3, 100, Y, 112, S]
     assert _status(entry, *good) not in (0, ERR_ARG)
-    for at, bad in ((0, None), (4, None), (6, None), (1, 99), (2, 0), (2, -1), (3, 0), (5, 96), (5, 120), (4, Y + 8), (0, X + 1), (6, S + 2), (5, 1 << 23)):
+    for at, bad in ((0, None), (4, None), (6, None), (1, 99), (2, 0), (2, -1), (3, 0), (5, 96), (5, 120), (4, Y + 8), (0, X + 1), (6, S + 2), (5, 1 << 23), (2, 1 << 27)):
         args = list(good)
         args[at] = bad
         assert _status(entry, *args) == ERR_ARG, (at, bad)
