@@ -210,3 +210,23 @@ def test_more_candidates_than_are_ranked(ctx, c, top, dtype):
     x[10] = np.where(np.arange(c) < c - 50, 1.0, 0.5)
     got = _run(ctx, x, None, top)
     assert np.array_equal(got["top_ids"], _order(x, top))
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("m,c", [(520, 8193), (520, 16384), (300, 16390), (270, 24999)])
+def test_rows_enough_for_long_slices(ctx, m, c, dtype):
+    rng = np.random.default_rng(m + c)
+    x = _logits(rng, m, c, dtype)
+    x[3] = 0.0
+    x[4] = np.finfo(dtype).min
+    x[4, ::c // 5] = 1.0
+    x[5] = np.sort(rng.standard_normal(c)).astype(dtype)
+    x[6, rng.permutation(c)[:200]] = np.nan
+    x[7] = -np.inf
+    x[8] = -np.inf
+    x[8, -3:] = 2.0
+    x[9] = rng.integers(0, 50, c)
+    ids = rng.integers(0, c, (m, 2))
+    _check(ctx, x, ids, 8, c + c % 3)
+    _check(ctx, x, ids, 64)
+    _check(ctx, x, ids)
