@@ -9,7 +9,7 @@
 
 namespace {
 
-constexpr int kMostSlice = 32768, kTopSlice = 16384, kSmallSlice = 8192;  // values of a row that a group of 16, of 8, of 4 waves holds in its registers
+constexpr int kMostSlice = 32768, kLongSlice = 16384, kSlice = 8192;  // values of a row that a group of 16, of 8, of 4 waves holds in its registers
 constexpr int kCandidates = 512;  // places that are held at once
 constexpr int kRanked = 128;      // and that are ranked, each against all; of more, those behind the top-th are left out first
 typedef unsigned long long u64;
@@ -203,7 +203,7 @@ template <typename T, int W, int V, bool TOP>
 __global__ __launch_bounds__(64 * W, 8) void log_probabilities_kernel(const T* __restrict__ x, const LogpParams p) {
     exhip_touch_args(p);
     constexpr int kThreads = 64 * W, N = 16 / sizeof(T), kRuns = V / N;
-    static_assert(W == 1 || W == 4 || (W == 8 && TOP) || (W == 16 && !TOP), "128 sets of the slice's values");
+    static_assert(W == 1 || W == 4 || W == 8 || W == 16, "128 sets of a slice's values; joins of a power of two");
     __shared__ Sums sums[W];
     __shared__ float sets[TOP ? 128 : 1], bound;
     __shared__ u64 places[TOP ? kCandidates + 8 : 1], sorted[TOP ? EXHIP_LOG_PROBABILITIES_TOP : 1];
@@ -263,6 +263,7 @@ __global__ __launch_bounds__(64 * W, 8) void log_probabilities_kernel(const T* _
         if constexpr (W > 1) {
             float m = fmaxf(mine, traded<0xB1>(mine));
             if constexpr (W > 4) m = fmaxf(m, traded<0x4E>(m));
+            if constexpr (W > 8) m = fmaxf(m, traded<0x141>(m));
             if (lane % (W / 2) == 0) sets[wave * (128 / W) + lane / (W / 2)] = m;
         } else {
             float m[2] = {-INFINITY, -INFINITY};
@@ -469,12 +470,14 @@ __global__ __launch_bounds__(64) void join_slices_kernel(const T* __restrict__ x
     write_row(x + row * p.x_stride, p, row, all, sorted);
 }
 
-// How a row is split: slices that a group's registers hold, and more of them where there are few rows. Where the largest are asked, groups of at most eight
-// waves: they wait for one wave twice. 300 x 100003 halves with the 8 largest take 24 us (24 with four waves, 30 with sixteen), with 64 of them 37 (42 with
-// four), 4096 x 32000 with 10 of them 70 (71 with four), 512 x 16000 with 5 of them 9 (13.5 with four and a second launch).
+// How a row is split. What one group holds is not: 64 rows of 32000 halves with the 20 largest take 8.6 us in one launch, 11.2 in slices that a second joins,
+// 4096 of them 70 and 71. Longer rows are in slices of four waves (300 x 100003 halves 17 us, 20 with groups of sixteen). The largest of many slices cost the
+// second launch more than groups of eight waves cost the first one, which all but one wait twice: 300 x 100003 with the 64 largest 36 us (42 with four waves, 40
+// with sixteen), one row of 262144 with 20 of them 10.6 (12.3 with four); of a few rows in 16 slices not yet, 8 x 131072 with 20 of them 11.4 (10.7).
 void split(int m, int c, int top, int* slices, int* slice_len) {
-    const int most = (c - 1) / kSmallSlice + 1, least = (c - 1) / (top ? kTopSlice : kMostSlice) + 1, wish = 512 / m;
-    *slices = least > wish ? least : wish < most ? wish : most;
+    const bool few = top == 0 || (m <= 32 && c <= 16 * kSlice);
+    const int most = c <= kMostSlice ? c : few ? kSlice : kLongSlice;
+    *slices = (c - 1) / most + 1;
     const int len = (c - 1) / *slices + 1;
     *slice_len = (len + 7) / 8 * 8;
     *slices = (c - 1) / *slice_len + 1;
@@ -485,9 +488,9 @@ void launch_slices(exhip_ctx* ctx, const T* x, const LogpParams& p) {
     const dim3 grid((unsigned)((size_t)p.m * p.slices));
     if (p.slice_len <= 512) hipLaunchKernelGGL((log_probabilities_kernel<T, 1, 8, TOP>), grid, dim3(64), 0, ctx->stream, x, p);
     else if (p.slice_len <= 2048) hipLaunchKernelGGL((log_probabilities_kernel<T, 1, 32, TOP>), grid, dim3(64), 0, ctx->stream, x, p);
-    else if (p.slice_len <= kSmallSlice) hipLaunchKernelGGL((log_probabilities_kernel<T, 4, 32, TOP>), grid, dim3(256), 0, ctx->stream, x, p);
-    else if constexpr (TOP) hipLaunchKernelGGL((log_probabilities_kernel<T, 8, 32, true>), grid, dim3(512), 0, ctx->stream, x, p);
-    else hipLaunchKernelGGL((log_probabilities_kernel<T, 16, 32, false>), grid, dim3(1024), 0, ctx->stream, x, p);
+    else if (p.slice_len <= kSlice) hipLaunchKernelGGL((log_probabilities_kernel<T, 4, 32, TOP>), grid, dim3(256), 0, ctx->stream, x, p);
+    else if (p.slice_len <= kLongSlice) hipLaunchKernelGGL((log_probabilities_kernel<T, 8, 32, TOP>), grid, dim3(512), 0, ctx->stream, x, p);
+    else hipLaunchKernelGGL((log_probabilities_kernel<T, 16, 32, TOP>), grid, dim3(1024), 0, ctx->stream, x, p);
 }
 
 bool sizes_ok(int m, int c, int top) { return m > 0 && c > 0 && top >= 0 && top <= EXHIP_LOG_PROBABILITIES_TOP && top <= c; }
