@@ -215,6 +215,7 @@ __global__ __launch_bounds__(64 * W, 8) void log_probabilities_kernel(const T* _
     Run<T, N> r[kRuns];
     auto value = [&](int e) { return as_float(r[e / N].v[e % N]); };
     auto at = [&](int e) { return (e / N * kThreads + (int)threadIdx.x) * N + e % N; };  // of value e in the slice
+    auto has = [&](int i) { return (i * kThreads + wave * 64) * N < len; };  // whether run i of the wave has a value at all
     auto read = [&](int i) {
         Run<T, N> run;
         const int k = at(i * N);
@@ -228,6 +229,9 @@ __global__ __launch_bounds__(64 * W, 8) void log_probabilities_kernel(const T* _
     for (int i = 0; i < kRuns; ++i) {
         const int k = at(i * N);
         if (k + N <= len) r[i] = *reinterpret_cast<const Run<T, N>*>(src + k);
+        else if (!has(i))
+#pragma unroll
+            for (int e = 0; e < N; ++e) r[i].v[e] = masked(T());
         else
 #pragma unroll
             for (int e = 0; e < N; ++e) r[i].v[e] = k + e < len ? src[k + e] : masked(T());
@@ -246,6 +250,7 @@ __global__ __launch_bounds__(64 * W, 8) void log_probabilities_kernel(const T* _
     float s = 0.f, t = 0.f;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
+        if (e % N == 0 && !has(e / N)) break;
         const float z = kOneStep ? __builtin_fmaf(value(e), kLog2e, -scaled) : (value(e) - base) * kLog2e, w = power(z);  // a NaN goes on into s
         s += w;
         t = __builtin_fmaf(w, fmaxf(z, kNoPart), t);
