@@ -243,11 +243,15 @@ __device__ __forceinline__ void tile_of(int groups_n, int groups_m, int* n, int*
 
 // ---- results of the kernels for many rows: through LDS, so that whole lines are stored ----
 // (A lane's four neighbouring outputs of one row, stored as they are, are 32 bytes of each of 16 rows at a time: 1.2 TB/s.)
-// Row-major results of a group: rows of WIDTH outputs, 16-byte pieces at place piece ^ (row % 8).
+// Row-major results of a group: rows of WIDTH outputs, 16-byte pieces at place piece ^ (row % 8), % 4 where there are four.
+template <typename O, int WIDTH>
+__device__ __forceinline__ int byte_in_row(int row, int byte) {
+    constexpr int kPieces = WIDTH * (int)sizeof(O) / 16, kTurn = kPieces < 8 ? kPieces - 1 : 7;
+    return ((byte / 16) ^ (row & kTurn)) * 16 + byte % 16;
+}
 template <typename O, int WIDTH>
 __device__ __forceinline__ char* place_in_rows(char* lds, int row, int j) {
-    const int byte = j * (int)sizeof(O);
-    return lds + row * (WIDTH * (int)sizeof(O)) + ((byte / 16) ^ (row & 7)) * 16 + byte % 16;
+    return lds + row * (WIDTH * (int)sizeof(O)) + byte_in_row<O, WIDTH>(row, j * (int)sizeof(O));
 }
 typedef int v4i_any __attribute__((ext_vector_type(4), aligned(1)));
 // (Nothing but whole pieces in the loop: code that a group runs once comes from memory line by line, 1 us each where a branch leaves the straight line. With
@@ -255,7 +259,7 @@ typedef int v4i_any __attribute__((ext_vector_type(4), aligned(1)));
 template <typename O, int WIDTH, int ROWS, int THREADS>
 __device__ __forceinline__ void store_rows(const char* lds, O* y, size_t stride, int row0, int rows, int j0, int n) {
     constexpr int kPer = 16 / sizeof(O), kPieces = WIDTH / kPer, kPitch = WIDTH * (int)sizeof(O), kTogether = THREADS / kPieces;
-    static_assert(THREADS % kPieces == 0 && ROWS % kTogether == 0 && kPieces >= 8, "every thread stores one piece of every kTogether-th row; eight rows' pieces lie in different banks");
+    static_assert(THREADS % kPieces == 0 && ROWS % kTogether == 0, "every thread stores one piece of every kTogether-th row");
     const int piece = threadIdx.x % kPieces, first = threadIdx.x / kPieces, j = j0 + piece * kPer;
     O* const dst = y + (size_t)(row0 + first) * stride + j;
     const size_t step = (size_t)kTogether * stride;
@@ -263,14 +267,14 @@ __device__ __forceinline__ void store_rows(const char* lds, O* y, size_t stride,
 #pragma unroll 4
     for (int i = 0; i < ROWS / kTogether; ++i) {
         const int row = i * kTogether + first;
-        const v4i v = *reinterpret_cast<const v4i*>(lds + row * kPitch + (piece ^ (row & 7)) * 16);
+        const v4i v = *reinterpret_cast<const v4i*>(lds + row * kPitch + byte_in_row<O, WIDTH>(row, piece * 16));
         if (whole && row < rows) __builtin_nontemporal_store(v, reinterpret_cast<v4i_any*>(dst + i * step));
     }
     if (j0 + WIDTH > n && n % kPer != 0) {
         const int at = n / kPer * kPer, left = n - at;
         for (int i = threadIdx.x; i < rows * left; i += THREADS) {
             const int row = i / left, e = i % left, byte = (at - j0) * (int)sizeof(O);
-            y[(size_t)(row0 + row) * stride + at + e] = reinterpret_cast<const O*>(lds + row * kPitch + ((byte / 16) ^ (row & 7)) * 16)[e];
+            y[(size_t)(row0 + row) * stride + at + e] = reinterpret_cast<const O*>(lds + row * kPitch + byte_in_row<O, WIDTH>(row, byte))[e];
         }
     }
 }
@@ -286,7 +290,7 @@ __device__ __forceinline__ v4f four_of(const float* v, int j, int n) {
 // one row, after 32 x 32 products those of a half of each eight.
 template <int SIDE>
 struct Lanes {
-    static constexpr int kOutputs = SIDE == 16 ? 4 : 8;  // of a wave's 64, in fours
+    static constexpr int kOfAFour = SIDE == 16 ? 16 : 8;  // the wave's outputs for each four of a lane
     static __device__ __forceinline__ int output(int i, int lane) { return SIDE == 16 ? i * 16 + lane / 16 * 4 : i * 8 + lane / 32 * 4; }
     static __device__ __forceinline__ int row(int t, int lane) { return t * SIDE + lane % SIDE; }
     // of a gated product: the four of the gate, those of the other projection, and where the result of both stands among the wave's 32
@@ -295,46 +299,46 @@ struct Lanes {
     static __device__ __forceinline__ int result(int i, int lane) { return SIDE == 16 ? i * 16 + lane / 16 * 4 : i * 8 + lane / 32 * 4; }
 };
 
-// The sums of a group of WN x WM waves, 64 outputs and SIDE * TM rows each. `lds` is free for at least the group's results as floats (halves where there are no
+// The sums of a group of WN x WM waves, FOURS x 4 outputs a lane and SIDE * TM rows each. `lds` is free for at least the group's results as floats (halves where there are no
 // others).
-template <int SIDE, int WN, int WM, int TM, bool FLOATS>
-__device__ __forceinline__ void write_group(const F8Params& p, v4f (&acc)[Lanes<SIDE>::kOutputs][TM], int group_n, int wn, int wm, int row0, int rows, int lane, char* lds) {
+template <int SIDE, int WN, int WM, bool FLOATS, int FOURS, int TM>
+__device__ __forceinline__ void write_group(const F8Params& p, v4f (&acc)[FOURS][TM], int group_n, int wn, int wm, int row0, int rows, int lane, char* lds) {
     typedef Lanes<SIDE> At;
-    constexpr int kWidth = 64 * WN, kRows = SIDE * TM * WM, kThreads = 64 * WN * WM;
+    constexpr int kOwn = FOURS * At::kOfAFour, kWidth = kOwn * WN, kRows = SIDE * TM * WM, kThreads = 64 * WN * WM;
     const int j0 = group_n * kWidth;
 #pragma unroll
-    for (int i = 0; i < At::kOutputs; ++i) {
-        const v4f bias = four_of(p.bias, j0 + wn * 64 + At::output(i, lane), p.n);
+    for (int i = 0; i < FOURS; ++i) {
+        const v4f bias = four_of(p.bias, j0 + wn * kOwn + At::output(i, lane), p.n);
 #pragma unroll
         for (int t = 0; t < TM; ++t) acc[i][t] += bias;
     }
     if (FLOATS && p.y_f32) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < At::kOutputs; ++i)
+        for (int i = 0; i < FOURS; ++i)
 #pragma unroll
-            for (int t = 0; t < TM; ++t) *reinterpret_cast<v4f*>(place_in_rows<float, kWidth>(lds, wm * TM * SIDE + At::row(t, lane), wn * 64 + At::output(i, lane))) = acc[i][t];
+            for (int t = 0; t < TM; ++t) *reinterpret_cast<v4f*>(place_in_rows<float, kWidth>(lds, wm * TM * SIDE + At::row(t, lane), wn * kOwn + At::output(i, lane))) = acc[i][t];
         __syncthreads();
         store_rows<float, kWidth, kRows, kThreads>(lds, p.y_f32, p.y_stride, row0, rows, j0, p.n);
     }
     if (p.y_f16) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < At::kOutputs; ++i)
+        for (int i = 0; i < FOURS; ++i)
 #pragma unroll
             for (int t = 0; t < TM; ++t)
-                *reinterpret_cast<v4h*>(place_in_rows<uint16_t, kWidth>(lds, wm * TM * SIDE + At::row(t, lane), wn * 64 + At::output(i, lane))) = __builtin_convertvector(acc[i][t], v4h);
+                *reinterpret_cast<v4h*>(place_in_rows<uint16_t, kWidth>(lds, wm * TM * SIDE + At::row(t, lane), wn * kOwn + At::output(i, lane))) = __builtin_convertvector(acc[i][t], v4h);
         __syncthreads();
         store_rows<uint16_t, kWidth, kRows, kThreads>(lds, p.y_f16, p.y_stride, row0, rows, j0, p.n);
     }
 }
 
-// The same of a gated product, whose tiles alternate: 32 WN outputs. Quantized results need a whole block of them, WN == 4.
-template <int SIDE, int WN, int WM, int TM>
-__device__ __forceinline__ void write_gated_group(const F8Params& p, v4f (&acc)[Lanes<SIDE>::kOutputs][TM], int group_n, int wn, int wm, int row0, int rows, int lane, char* lds) {
+// The same of a gated product, whose tiles alternate: half as many outputs. Quantized results need a whole block of them.
+template <int SIDE, int WN, int WM, int FOURS, int TM>
+__device__ __forceinline__ void write_gated_group(const F8Params& p, v4f (&acc)[FOURS][TM], int group_n, int wn, int wm, int row0, int rows, int lane, char* lds) {
     typedef Lanes<SIDE> At;
-    constexpr int kWidth = 32 * WN, kRows = SIDE * TM * WM, kThreads = 64 * WN * WM, kResults = At::kOutputs / 2;
-    const int j0 = group_n * kWidth, row_at = wm * TM * SIDE, out_at = wn * 32;
+    constexpr int kResults = FOURS / 2, kOwn = kResults * At::kOfAFour, kWidth = kOwn * WN, kRows = SIDE * TM * WM, kThreads = 64 * WN * WM;
+    const int j0 = group_n * kWidth, row_at = wm * TM * SIDE, out_at = wn * kOwn;
 #pragma unroll
     for (int i = 0; i < kResults; ++i) {
         const int j = j0 + out_at + At::result(i, lane);
@@ -356,7 +360,7 @@ __device__ __forceinline__ void write_gated_group(const F8Params& p, v4f (&acc)[
         __syncthreads();
         store_rows<uint16_t, kWidth, kRows, kThreads>(lds, p.y_f16, p.y_stride, row0, rows, j0, p.n);
     }
-    if constexpr (WN == 4) {
+    if constexpr (kWidth == kBlk) {
         if (!p.y_f8) return;
         float* const most = reinterpret_cast<float*>(lds);  // [wave along the outputs][row]
 #pragma unroll
@@ -524,8 +528,8 @@ __global__ __launch_bounds__(512, 2) void f8_wide_kernel(const F8Params p) {
         if (b + 1 < blocks) block(w1, w0, b + 1);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was staged behind the end, in front of the results' barrier
-    if constexpr (!GATED) write_group<16, WN, 2, TM, false>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
-    else write_gated_group<16, WN, 2, TM>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
+    if constexpr (!GATED) write_group<16, WN, 2, false>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
+    else write_gated_group<16, WN, 2>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
 }
 
 // ---- few rows, or few products ----
@@ -813,18 +817,20 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void f8_tile_kernel(const F8Params
     }
 #pragma unroll
     for (int g = 0; g < 4; ++g) add(1, TM - 1, g, last, last_up);
-    if constexpr (!GATED) write_group<32, WN, WM, TM, true>(p, acc, group_n, wn, wm, row0, rows, lane, memory);
-    else write_gated_group<32, WN, WM, TM>(p, acc, group_n, wn, wm, row0, rows, lane, memory);
+    if constexpr (!GATED) write_group<32, WN, WM, true>(p, acc, group_n, wn, wm, row0, rows, lane, memory);
+    else write_gated_group<32, WN, WM>(p, acc, group_n, wn, wm, row0, rows, lane, memory);
 }
 
 // ---- a tile or two for every CU ----
-// Between the two: a group of 2 x 4 waves takes 128 outputs and 128 rows, a wave 64 x 32, and both operands' codes come straight into LDS, three blocks ahead in
-// four buffers (all the LDS that a CU has), so that a CU with one group does not wait for memory block by block.
-// (2 x 2 waves of 64 x 64, one for each SIMD, take longer: 330 instructions a block, of which a wave alone issues one in 4.5 cycles.)
-template <bool GATED>
-__global__ __launch_bounds__(512, 2) void f8_deep_kernel(const F8Params p) {
+// Between the two: a group of 2 x WM waves takes 32 WM outputs and 32 WM rows, a wave 16 WM x 32, and both operands' codes come straight into LDS, three blocks
+// ahead in four buffers, so that a CU with one group does not wait for memory block by block. WM = 4 takes all the LDS that a CU has. What bounds it is what a CU
+// draws from L2, some 27 bytes a cycle: where 128 x 128 leaves CUs without a group, 64 x 64 (WM = 2, two groups a CU) has the others draw too: 128 x 8192 x 8192 in
+// 20 us (32), 256 x 4096 x 4096 in 12 (18), 64 rows of the gated 8192 x 4096 in 15 (21); 1024 x 4096 x 4096 in 23 us with WM = 4.
+// (2 x 2 waves of 64 x 64, one for each SIMD, take longer than 2 x 4: 330 instructions a block, of which a wave alone issues one in 4.5 cycles.)
+template <int WM, bool GATED>
+__global__ __launch_bounds__(128 * WM, 2) void f8_deep_kernel(const F8Params p) {
     exhip_touch_args(p);
-    constexpr int WN = 2, WM = 4, TN = 4, TM = 2, kRows = 128, kLoads = 5, kBuffers = 4, kWeights = 16384, kCodes = kRows * kBlk, kBuffer = kWeights + kCodes + kRows * 4;
+    constexpr int WN = 2, TN = WM, TM = WN, kRows = 16 * TM * WM, kLoads = 5, kBuffers = 4, kWeights = 2048 * TN * WN, kCodes = kRows * kBlk, kBuffer = kWeights + kCodes + kRows * 4;
     __shared__ __attribute__((aligned(16))) char staged[kBuffers * kBuffer];
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)staged;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wn = wave % WN, wm = wave / WN;
@@ -834,7 +840,7 @@ __global__ __launch_bounds__(512, 2) void f8_deep_kernel(const F8Params p) {
     const int tile0 = (group_n * WN + wn) * TN, row0 = group_m * kRows;
     const int rows = min(kRows, p.m - row0), tail = p.k % kBlk, blocks = p.blocks_k;
     const __amdgpu_buffer_rsrc_t xr = uniform_view(p.x + (size_t)row0 * p.x_stride, (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16);
-    // A wave stages 16 rows, eight with a load (as in f8_wide_kernel), and one of the group's eight tiles of weights.
+    // A wave stages 16 rows, eight with a load (as in f8_wide_kernel), and one of the group's tiles of weights.
     const int piece = (lane % 8) ^ (lane / 8);
     const bool behind = tail && piece * 16 >= tail;
     int off[2];
@@ -843,19 +849,19 @@ __global__ __launch_bounds__(512, 2) void f8_deep_kernel(const F8Params p) {
         const int row = wave * 16 + j * 8 + lane / 8;
         off[j] = row < rows ? row * p.x_stride + piece * 16 : kNoRow;
     }
-    const int scale_off = min(wave % 2 * 64 + lane, rows - 1) * 4;
+    const int scale_part = wave % (kRows / 64) * 64, scale_off = min(scale_part + lane, rows - 1) * 4;
     const WeightRows weights(p, group_n * WN * TN + wave, 1, lane);
     auto stage = [&](int buffer, int j) {  // in five loads; behind the last block that one again, which nothing reads
         const int b = min(buffer, blocks - 1);
         const unsigned to = lds0 + buffer % kBuffers * kBuffer;
         if (j < 2) load16_to_lds(weights.view, weights.at, b * 2048 + j * 1024, to + (wave * 2 + j) * 1024);
         else if (j < 4) load16_to_lds(xr, behind && b == blocks - 1 ? kNoRow : off[j - 2], b * kBlk, to + kWeights + (wave * 16 + (j - 2) * 8) * kBlk);
-        else load4_to_lds(uniform_view(p.x_scale + (size_t)b * p.m + row0, rows * 4), scale_off, to + kWeights + kCodes + wave % 2 * 256);
+        else load4_to_lds(uniform_view(p.x_scale + (size_t)b * p.m + row0, rows * 4), scale_off, to + kWeights + kCodes + scale_part * 4);
     };
     const int block_n = min(GATED ? tile0 / 2 : tile0, (p.n - 1) / 16) / (kBlk / 16);
     const Constants ws = (Constants)(uintptr_t)(p.w_scale + (size_t)block_n * blocks);
     const Constants ws_up = (Constants)(uintptr_t)(GATED ? p.w_scale_up + (size_t)block_n * blocks : nullptr);
-    const int at_w = wn * 8192 + lane * 16;
+    const int at_w = wn * TN * 2048 + lane * 16;
     auto weights_from = [&](int b, int i) {
         const char* const from = staged + b % kBuffers * kBuffer + at_w + i * 2048;
         return both(*reinterpret_cast<const v4i*>(from), *reinterpret_cast<const v4i*>(from + 1024));
@@ -944,8 +950,8 @@ __global__ __launch_bounds__(512, 2) void f8_deep_kernel(const F8Params p) {
         if (b + 1 < blocks) block(w1, w0, b + 1);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was staged behind the end, in front of the results' barrier
-    if constexpr (!GATED) write_group<16, WN, WM, TM, false>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
-    else write_gated_group<16, WN, WM, TM>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
+    if constexpr (!GATED) write_group<16, WN, WM, false>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
+    else write_gated_group<16, WN, WM>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
 }
 
 int blocks_of(int v) { return v / kBlk + (v % kBlk != 0); }
@@ -1019,28 +1025,29 @@ template <int WN, int WM, int TM, bool GATED>
 int run_tile(exhip_ctx* ctx, const F8Params& p) {
     return launch(ctx, f8_tile_kernel<WN, WM, TM, GATED>, p, 4 * WN, 32 * TM * WM, 64 * WN * WM);
 }
-template <bool GATED>
+template <int WM, bool GATED>
 int run_deep(exhip_ctx* ctx, const F8Params& p) {
-    return launch(ctx, f8_deep_kernel<GATED>, p, 8, 128, 512);
+    return launch(ctx, f8_deep_kernel<WM, GATED>, p, 2 * WM, 32 * WM, 128 * WM);
 }
 template <bool GATED>
 int run_wide(exhip_ctx* ctx, const F8Params& p) {
     return launch(ctx, f8_wide_kernel<GATED>, p, 16, 256, 512);
 }
-// The times are fits to 380 launches of 1 to 2048 rows and matrices from 256 x 512 to 8192 x 8192, on the GPU's clock: the form they choose takes 2 % longer than
-// the best one for the shape on average, 20 % at most.
+// The times are fits to 1700 launches of 1 to 2048 rows and matrices from 256 x 512 to 8192 x 8192, on the GPU's clock: the form they choose takes 1 % longer than
+// the best one for the shape on average, 12 % at most.
 constexpr Form kExact[] = {  // results in float32
-    {run_rows<1, 1, 1, 8, 4, false>, 1, 16, 512, 8, 0.4f, 2.2f, 0.85f}, {run_rows<2, 1, 1, 8, 2, false>, 2, 16, 512, 8, 0.f, 2.9f, 0.86f},
-    {run_rows<2, 2, 1, 8, 2, false>, 2, 32, 256, 8, 1.4f, 1.3f, 1.42f}, {run_rows<4, 2, 1, 8, 1, false>, 4, 32, 256, 8, 0.7f, 2.4f, 1.65f},
-    {run_tile<2, 2, 1, false>, 8, 64, 512, 1, 0.f, 3.8f, 0.66f},        {run_tile<4, 1, 2, false>, 16, 64, 512, 1, 0.f, 4.4f, 0.90f},
+    {run_rows<1, 1, 1, 8, 4, false>, 1, 16, 512, 8, 1.5f, 1.9f, 0.69f}, {run_rows<2, 1, 1, 8, 2, false>, 2, 16, 512, 8, 0.2f, 3.2f, 0.74f},
+    {run_rows<2, 2, 1, 8, 2, false>, 2, 32, 256, 8, 1.7f, 1.4f, 1.37f}, {run_rows<4, 2, 1, 8, 1, false>, 4, 32, 256, 8, 1.0f, 2.6f, 1.63f},
+    {run_tile<2, 2, 1, false>, 8, 64, 512, 1, 0.2f, 3.7f, 0.65f},       {run_tile<4, 1, 2, false>, 16, 64, 512, 1, 0.f, 4.5f, 0.87f},
 };
 constexpr Form kHalves[] = {
-    kExact[0], kExact[1], kExact[2], kExact[3], {run_deep<false>, 8, 128, 256, 1, 0.7f, 3.5f, 0.47f}, {run_wide<false>, 16, 256, 256, 1, 0.f, 6.0f, 1.18f},
+    kExact[0], kExact[1], kExact[2], kExact[3], {run_deep<2, false>, 4, 64, 512, 1, 0.1f, 3.4f, 0.27f}, {run_deep<4, false>, 8, 128, 256, 1, 0.7f, 4.1f, 0.42f},
+    {run_wide<false>, 16, 256, 256, 1, 0.f, 6.4f, 1.16f},
 };
 constexpr Form kGatedHalves[] = {
-    {run_rows<2, 1, 1, 8, 2, true>, 2, 16, 512, 8, 0.f, 2.9f, 1.34f}, {run_rows<2, 2, 1, 8, 2, true>, 2, 32, 256, 8, 1.3f, 2.1f, 1.41f},
-    {run_rows<4, 2, 1, 8, 1, true>, 4, 32, 256, 8, 1.1f, 2.3f, 2.03f}, {run_deep<true>, 8, 128, 256, 1, 0.9f, 5.2f, 0.50f},
-    {run_wide<true>, 16, 256, 256, 1, 0.f, 14.2f, 1.29f},
+    {run_rows<2, 1, 1, 8, 2, true>, 2, 16, 512, 8, 2.3f, 1.7f, 0.83f}, {run_rows<2, 2, 1, 8, 2, true>, 2, 32, 256, 8, 1.3f, 2.5f, 1.31f},
+    {run_rows<4, 2, 1, 8, 1, true>, 4, 32, 256, 8, 1.6f, 2.5f, 1.83f}, {run_deep<2, true>, 4, 64, 512, 1, 0.5f, 3.8f, 0.35f},
+    {run_deep<4, true>, 8, 128, 256, 1, 0.9f, 5.5f, 0.49f},            {run_wide<true>, 16, 256, 256, 1, 0.2f, 14.4f, 1.26f},
 };
 constexpr Form kGatedCodes[] = {  // a group has whole blocks of the result: 16 tiles
     {run_rows<4, 1, 4, 4, 1, true>, 16, 16, 256, 4, 0.9f, 3.0f, 2.12f}, {run_rows<4, 2, 4, 2, 1, true>, 16, 32, 256, 2, 0.f, 5.2f, 1.40f},
@@ -1055,8 +1062,13 @@ int run_best(exhip_ctx* ctx, const F8Params& p, const Form (&forms)[N]) {
     float best_us = 0.f;
     for (int i = 0; i < N; ++i) {
         const Form& f = forms[i];
-        const long long groups = (long long)((p.tiles + f.tiles - 1) / f.tiles) * (p.m / f.rows + (p.m % f.rows != 0));
-        const float us = f.start + (float)((groups - 1) / f.at_once + 1) * (f.round + f.block * (float)((p.blocks_k - 1) / f.split + 1));
+        const int groups_n = (p.tiles + f.tiles - 1) / f.tiles, groups_m = p.m / f.rows + (p.m % f.rows != 0);
+        const long long rounds = ((long long)groups_n * groups_m - 1) / f.at_once + 1;
+        float us = f.start + (float)rounds * (f.round + f.block * (float)((p.blocks_k - 1) / f.split + 1));
+        if (f.split > 1) {  // all loads together: the weights once from memory, what groups read again, weights and rows, from L2
+            const float weights = (float)p.tiles * (float)p.blocks_k * 2048.f, again = (float)(groups_m - 1) * weights + (float)groups_n * (float)p.m * (float)p.blocks_k * 128.f;
+            us = fmaxf(us, f.start + weights / 6.4e6f + again / 15e6f);
+        }
         if (i == 0 || us < best_us) {
             best = i;
             best_us = us;

@@ -244,7 +244,7 @@ def test_every_form_of_the_product(ctx, pin, m, n, k):
     want, bound = o.want()
     args = (o.dx, o.dx_scale, o.packed, o.dw_scale[0], o.dbias[0])
     cut = bound + f8ref.cut_bound(o.x, o.x_scale, o.w[0], o.w_scale[0])
-    for form in range(1, 7):
+    for form in range(1, 8):
         pin(form)
         for extra in (0, 3):
             y32, y16 = ctx.array(np.full((m + 1, n + extra), 7.25, np.float32)), ctx.array(np.full((m + 1, n + extra), 0x4567, np.uint16))
@@ -265,7 +265,7 @@ def test_every_form_of_the_gated_product(ctx, pin, m, n, k):
     h, bound = f8ref.gated("silu", g, gb, u, ub)
     cut = f8ref.gated("silu", g, gb + f8ref.cut_bound(o.x, o.x_scale, o.w[0], o.w_scale[0]), u, ub + f8ref.cut_bound(o.x, o.x_scale, o.w[1], o.w_scale[1]))[1]
     args = (o.dx, o.dx_scale, o.packed, o.dw_scale[0], o.dw_scale[1], "silu", o.dbias[0], o.dbias[1])
-    for form in range(1, 6):
+    for form in range(1, 7):
         pin(form)
         y = ctx.array(np.full((m + 1, n + 3), 0x4567, np.uint16))
         ctx.innerproduct_gated_f8(o.desc(ctx, n + 3), *args, y_f16=y)
@@ -292,7 +292,7 @@ def test_every_form_of_whole_numbers_is_exact(ctx, pin):
         o.w_scale[0] = np.ldexp(1.0, rng.integers(-2, 3, o.w_scale[0].shape)).astype(np.float32)
         want, _ = o.want()
         args = (ctx.array(_wide(o.x, o.stride, 0x7F)), ctx.array(o.x_scale), ctx.pack_f8_weights(n, k, ctx.array(o.w[0])), ctx.array(o.w_scale[0]))
-        for form in range(1, 7):
+        for form in range(1, 8):
             pin(form)
             y32, y16 = ctx.empty((m, n), np.float32), ctx.empty((m, n), np.uint16)
             ctx.innerproduct_f8(o.desc(ctx), *args, y_f32=y32)
@@ -310,7 +310,7 @@ def test_every_form_keeps_a_nan_in_its_row(ctx, pin):
     args = (ctx.array(_wide(o.x, o.stride, 0x7F)), o.dx_scale, ctx.pack_f8_weights(n, k, ctx.array(o.w[0])), o.dw_scale[0])
     want = np.zeros((m, n), bool)
     want[m - 1], want[:, n - 1] = True, True
-    for form in range(1, 7):
+    for form in range(1, 8):
         pin(form)
         y32, y16 = ctx.empty((m, n), np.float32), ctx.empty((m, n), np.uint16)
         ctx.innerproduct_f8(o.desc(ctx), *args, y_f32=y32)
