@@ -10,6 +10,9 @@
 #include "common.h"
 
 typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v4i_any __attribute__((ext_vector_type(4), aligned(1)));  // at any address, and at any of their type's
+typedef int int_any __attribute__((aligned(1)));
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef int v2i __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -94,26 +97,44 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
     if (threadIdx.x % 16 == 0) scale[(size_t)b * m + row] = s;
 }
 
-// One 128 x 128 block of a weight matrix a group. Runs once for a model: two readings of the block.
+// One 128 x 128 block of a weight matrix a group: 16 rows of four values a thread, held between the maximum and the codes. (8192 x 4096 in 26 us;
+// with a second reading of single values 53.)
 __global__ __launch_bounds__(256) void quantize_blocks_kernel(const float* __restrict__ w, int n, int k, int blocks_k, uint8_t* __restrict__ y,
                                                               float* __restrict__ scale) {
     const int bn = blockIdx.x / blocks_k, bk = blockIdx.x % blocks_k;
-    const int col = bk * kBlk + threadIdx.x % kBlk, row0 = bn * kBlk + threadIdx.x / kBlk;
-    __shared__ float part[256];
-    float a = 0.f;
-    if (col < k)
-        for (int r = 0; r < kBlk && row0 + r < n; r += 2) a = fmaxf(a, fabsf(w[(size_t)(row0 + r) * k + col]));
-    part[threadIdx.x] = a;
-    __syncthreads();
-    for (int d = 128; d > 0; d >>= 1) {
-        if ((int)threadIdx.x < d) part[threadIdx.x] = fmaxf(part[threadIdx.x], part[threadIdx.x + d]);
-        __syncthreads();
+    const int col = bk * kBlk + threadIdx.x % 32 * 4, row0 = bn * kBlk + threadIdx.x / 32;
+    __shared__ float part[4];
+    v4f v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int row = row0 + 8 * i;
+        const float* const src = w + (size_t)row * k + col;
+        v[i] = v4f{0.f, 0.f, 0.f, 0.f};
+        if (row < n && col + 4 <= k) v[i] = *reinterpret_cast<const v4f_any*>(src);
+        else if (row < n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (col + e < k) v[i][e] = src[e];
     }
-    const float s = scale_of(part[0]), inv = 1.f / s;
+    float a = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) a = fmaxf(fmaxf(a, fmaxf(fabsf(v[i][0]), fabsf(v[i][1]))), fmaxf(fabsf(v[i][2]), fabsf(v[i][3])));
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) a = fmaxf(a, __shfl_xor(a, d));
+    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = a;
+    __syncthreads();
+    const float s = scale_of(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]))), inv = 1.f / s;
     if (threadIdx.x == 0) scale[blockIdx.x] = s;
-    if (col < k)
-        for (int r = 0; r < kBlk && row0 + r < n; r += 2)
-            y[(size_t)(row0 + r) * k + col] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(w[(size_t)(row0 + r) * k + col] * inv, 0.f, 0, false);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int row = row0 + 8 * i, code = four_codes(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+        uint8_t* const dst = y + (size_t)row * k + col;
+        if (row < n && col + 4 <= k) *reinterpret_cast<int_any*>(dst) = code;
+        else if (row < n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (col + e < k) dst[e] = (uint8_t)(code >> (8 * e));
+    }
 }
 
 // ---- the weights' layout ----
@@ -129,8 +150,13 @@ __global__ __launch_bounds__(256) void pack_f8_kernel(const uint8_t* __restrict_
     const int block = tile_block % blocks_k, tile = tile_block / blocks_k;
     const uint8_t* const from = w_up && tile % 2 ? w_up : w;
     const int row = (w_up ? tile / 2 : tile) * 16 + lane % 16, col = block * kBlk + half * 64 + lane / 16 * 16;
+    const uint8_t* const src = from + (size_t)row * k + col;
+    if (row < n && col + 16 <= k) {
+        packed[i] = *reinterpret_cast<const v4i_any*>(src);
+        return;
+    }
     union { uint8_t b[16]; v4i v; } u;
-    for (int e = 0; e < 16; ++e) u.b[e] = row < n && col + e < k ? from[(size_t)row * k + col + e] : 0;
+    for (int e = 0; e < 16; ++e) u.b[e] = row < n && col + e < k ? src[e] : 0;
     packed[i] = u.v;
 }
 
@@ -186,7 +212,6 @@ __device__ __forceinline__ v4f block_product(const Halves& w, const Halves& x) {
 }
 
 // Four neighbouring outputs of a row at any alignment of their type, and the first of them where the row ends.
-typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef _Float16 v4h_any __attribute__((ext_vector_type(4), aligned(2)));
 __device__ __forceinline__ void store_cut(float* y, v4f v, int left) {
     y[0] = v[0];
@@ -253,7 +278,6 @@ template <typename O, int WIDTH>
 __device__ __forceinline__ char* place_in_rows(char* lds, int row, int j) {
     return lds + row * (WIDTH * (int)sizeof(O)) + byte_in_row<O, WIDTH>(row, j * (int)sizeof(O));
 }
-typedef int v4i_any __attribute__((ext_vector_type(4), aligned(1)));
 // (Nothing but whole pieces in the loop: code that a group runs once comes from memory line by line, 1 us each where a branch leaves the straight line. With
 // the cut pieces inside it the same loop took 2 to 14 us a group, by the XCD. The stores go past L2: 8192 x 8192 x 4096 263 -> 237 us.)
 template <typename O, int WIDTH, int ROWS, int THREADS>
