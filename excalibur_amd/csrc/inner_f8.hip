@@ -1034,12 +1034,14 @@ int launch(exhip_ctx* ctx, K kernel, F8Params p, int tiles, int rows, int thread
     return 0;
 }
 
-// One way to run a product: the tiles of 16 outputs (of both projections) and the rows a group takes, how many groups the chip runs at once, how many waves share
-// a group's blocks, and what a launch takes: `round` us for the groups that run at once, and `block` for each block that one wave of theirs goes through.
+// One way to run a product: the tiles of 16 outputs (of both projections) and the rows a group takes, how many groups a CU runs at once, how many waves share a
+// group's blocks, and what a launch takes: `start` us, and for each time that all CUs are given groups `round` and, for each block that one wave goes through,
+// `block`; `alone` where a CU that could run two groups has one.
 struct Form {
     int (*run)(exhip_ctx*, const F8Params&);
     int tiles, rows, at_once, split;
-    float start, round, block;
+    float start, round, block, alone;
+    bool drawn;  // whether its loads may be what bounds it
 };
 template <int TN, int TM, int WN, int WK, int D, bool GATED>
 int run_rows(exhip_ctx* ctx, const F8Params& p) {
@@ -1057,26 +1059,29 @@ template <bool GATED>
 int run_wide(exhip_ctx* ctx, const F8Params& p) {
     return launch(ctx, f8_wide_kernel<GATED>, p, 16, 256, 512);
 }
-// The times are fits to 1700 launches of 1 to 2048 rows and matrices from 256 x 512 to 8192 x 8192, on the GPU's clock: the form they choose takes 1 % longer than
-// the best one for the shape on average, 12 % at most.
+// The times are fits to 3000 launches of 1 to 2048 rows and matrices from 256 x 512 to 8192 x 8192 and 32000 x 4096, on the GPU's clock: the form they choose takes
+// 0.3 % longer than the best one for the shape on average, 9 % at most.
 constexpr Form kExact[] = {  // results in float32
-    {run_rows<1, 1, 1, 8, 4, false>, 1, 16, 512, 8, 1.5f, 1.9f, 0.69f}, {run_rows<2, 1, 1, 8, 2, false>, 2, 16, 512, 8, 0.2f, 3.2f, 0.74f},
-    {run_rows<2, 2, 1, 8, 2, false>, 2, 32, 256, 8, 1.7f, 1.4f, 1.37f}, {run_rows<4, 2, 1, 8, 1, false>, 4, 32, 256, 8, 1.0f, 2.6f, 1.63f},
-    {run_tile<2, 2, 1, false>, 8, 64, 512, 1, 0.2f, 3.7f, 0.65f},       {run_tile<4, 1, 2, false>, 16, 64, 512, 1, 0.f, 4.5f, 0.87f},
+    {run_rows<1, 1, 1, 8, 4, false>, 1, 16, 2, 8, 1.5f, 1.9f, 0.97f, 0.58f, true}, {run_rows<2, 1, 1, 8, 2, false>, 2, 16, 2, 8, 0.3f, 3.1f, 1.74f, 0.64f, true},
+    {run_rows<2, 2, 1, 8, 2, false>, 2, 32, 1, 8, 1.7f, 1.5f, 1.37f, 0.f, true},   {run_rows<4, 2, 1, 8, 1, false>, 4, 32, 1, 8, 1.0f, 2.5f, 1.80f, 0.f, true},
+    {run_tile<2, 2, 1, false>, 8, 64, 2, 1, 0.3f, 4.4f, 1.01f, 0.61f, false},      {run_tile<4, 1, 2, false>, 16, 64, 2, 1, 0.2f, 5.0f, 1.72f, 0.87f, false},
 };
 constexpr Form kHalves[] = {
-    kExact[0], kExact[1], kExact[2], kExact[3], {run_deep<2, false>, 4, 64, 512, 1, 0.1f, 3.4f, 0.27f}, {run_deep<4, false>, 8, 128, 256, 1, 0.7f, 4.1f, 0.42f},
-    {run_wide<false>, 16, 256, 256, 1, 0.f, 6.4f, 1.16f},
+    kExact[0], kExact[1], kExact[2], kExact[3],
+    {run_deep<2, false>, 4, 64, 2, 1, 0.3f, 3.3f, 0.30f, 0.26f, true}, {run_deep<4, false>, 8, 128, 1, 1, 0.5f, 3.7f, 0.50f, 0.f, true},
+    {run_wide<false>, 16, 256, 1, 1, 0.f, 7.4f, 1.17f, 0.f, false},
 };
 constexpr Form kGatedHalves[] = {
-    {run_rows<2, 1, 1, 8, 2, true>, 2, 16, 512, 8, 2.3f, 1.7f, 0.83f}, {run_rows<2, 2, 1, 8, 2, true>, 2, 32, 256, 8, 1.3f, 2.5f, 1.31f},
-    {run_rows<4, 2, 1, 8, 1, true>, 4, 32, 256, 8, 1.6f, 2.5f, 1.83f}, {run_deep<2, true>, 4, 64, 512, 1, 0.5f, 3.8f, 0.35f},
-    {run_deep<4, true>, 8, 128, 256, 1, 0.9f, 5.5f, 0.49f},            {run_wide<true>, 16, 256, 256, 1, 0.2f, 14.4f, 1.26f},
+    {run_rows<2, 1, 1, 8, 2, true>, 2, 16, 2, 8, 2.5f, 1.5f, 1.95f, 0.85f, true}, {run_rows<2, 2, 1, 8, 2, true>, 2, 32, 1, 8, 1.4f, 2.4f, 1.34f, 0.f, true},
+    {run_rows<4, 2, 1, 8, 1, true>, 4, 32, 1, 8, 1.3f, 2.6f, 1.90f, 0.f, true},   {run_deep<2, true>, 4, 64, 2, 1, 2.0f, 2.9f, 0.39f, 0.27f, true},
+    {run_deep<4, true>, 8, 128, 1, 1, 1.6f, 4.3f, 0.55f, 0.f, true},              {run_wide<true>, 16, 256, 1, 1, 0.1f, 15.2f, 1.33f, 0.f, false},
 };
 constexpr Form kGatedCodes[] = {  // a group has whole blocks of the result: 16 tiles
-    {run_rows<4, 1, 4, 4, 1, true>, 16, 16, 256, 4, 0.9f, 3.0f, 2.12f}, {run_rows<4, 2, 4, 2, 1, true>, 16, 32, 256, 2, 0.f, 5.2f, 1.40f},
-    {run_tile<4, 1, 2, true>, 16, 64, 512, 1, 0.f, 8.3f, 1.01f},
+    {run_rows<4, 1, 4, 4, 1, true>, 16, 16, 1, 4, 0.9f, 3.0f, 2.12f, 0.f, true}, {run_rows<4, 2, 4, 2, 1, true>, 16, 32, 1, 2, 0.f, 5.2f, 1.40f, 0.f, true},
+    {run_tile<4, 1, 2, true>, 16, 64, 2, 1, 0.f, 8.7f, 1.68f, 0.92f, false},
 };
+
+constexpr int kCus = 256;
 
 template <int N>
 int run_best(exhip_ctx* ctx, const F8Params& p, const Form (&forms)[N]) {
@@ -1087,11 +1092,11 @@ int run_best(exhip_ctx* ctx, const F8Params& p, const Form (&forms)[N]) {
     for (int i = 0; i < N; ++i) {
         const Form& f = forms[i];
         const int groups_n = (p.tiles + f.tiles - 1) / f.tiles, groups_m = p.m / f.rows + (p.m % f.rows != 0);
-        const long long rounds = ((long long)groups_n * groups_m - 1) / f.at_once + 1;
-        float us = f.start + (float)rounds * (f.round + f.block * (float)((p.blocks_k - 1) / f.split + 1));
-        if (f.split > 1) {  // all loads together: the weights once from memory, what groups read again, weights and rows, from L2
+        const long long times = ((long long)groups_n * groups_m - 1) / kCus + 1, full = times / f.at_once, rest = times % f.at_once;
+        float us = f.start + (float)(full + rest) * f.round + ((float)full * f.block + (float)rest * f.alone) * (float)((p.blocks_k - 1) / f.split + 1);
+        if (f.drawn) {  // all loads together, in bytes a us: the weights once from memory, what groups read again, weights and rows, from L2
             const float weights = (float)p.tiles * (float)p.blocks_k * 2048.f, again = (float)(groups_m - 1) * weights + (float)groups_n * (float)p.m * (float)p.blocks_k * 128.f;
-            us = fmaxf(us, f.start + weights / 6.4e6f + again / 15e6f);
+            us = fmaxf(us, f.start + weights / 7.9e6f + again / 19e6f);
         }
         if (i == 0 || us < best_us) {
             best = i;
