@@ -203,6 +203,10 @@ __device__ __forceinline__ Halves halves_of(v4i lo, v4i hi) {
     for (int s = 0; s < 4; ++s) h.v[s] = halves_of(lo[s], hi[s]);
     return h;
 }
+typedef int v8i __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ Halves halves_of(const v8i& c) {
+    return halves_of(__builtin_shufflevector(c, c, 0, 1, 2, 3), __builtin_shufflevector(c, c, 4, 5, 6, 7));
+}
 // One block's products of 16 outputs and 16 rows.
 __device__ __forceinline__ v4f block_product(const Halves& w, const Halves& x) {
     v4f c = {0.f, 0.f, 0.f, 0.f};
@@ -225,7 +229,6 @@ __device__ __forceinline__ void store_cut(uint16_t* y, v4f v, int left) {
 }
 
 // ---- loads ----
-typedef int v8i __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ v8i both(v4i a, v4i b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 // One 16-byte (4-byte) element per lane from a bounds-checked view straight into LDS, lane l's at lds + 16 l (4 l); lds is the wave's, and so is `more`, an
 // offset beside the lane's. vmcnt counts them like any other load. (The bounds need not see `more`: lanes with nothing to load have kNoRow.)
@@ -704,23 +707,22 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void f8_rows_kernel(const F8Params
 }
 
 // ---- many rows, exact products ----
-// A group of WN x WM waves takes 64 WN outputs and 32 TM WM rows, a wave 64 x 32 TM, in products of 32 x 32: of the cycles in which a SIMD can issue they leave
+// A group of four waves takes 256 outputs and 64 rows, a wave 64 x 64, in products of 32 x 32: of the cycles in which a SIMD can issue they leave
 // more to the conversions and multiply-adds than those of 16 x 16 (48 of these beside 32 x 32 x 128 values take 277 cycles, 342 with the smaller ones). A
 // block's rows become halves once for the group, on their way into LDS (four buffers); a wave's weights come from L2 as codes, a block ahead, and become halves
-// in its registers. A block is 2 TM chains of eight products, one chain for 32 outputs and 32 rows, and what else there is to do has its products: the
+// in its registers. A block is four chains of eight products, one chain for 32 outputs and 32 rows, and what else there is to do has its products: the
 // multiply-adds of the chain before, the conversions, the loads one by one, the next chain's rows. Each load's place is the
 // latest that still covers L2's answer, since all of it together takes every register there is; the barrier says that the next block's rows are there.
 // Measured: 8192 x 8192 x 4096 in 465 us, 1.18 PFLOP/s, where the library's product of halves reaches 1.13; the smaller products took 467, the clock gives way
-// under either. 300 x 4096 x 4096 in 24.3 us (27.4), 200 rows of the gated 4096 x 4096 in 37.6 (42.0).
-template <int WN, int WM, int TM, bool GATED>
-__global__ __launch_bounds__(64 * WN * WM, 2) void f8_tile_kernel(const F8Params p) {
+// under either. 1024 x 4096 x 4096 in 39 us, 200 rows of the gated 4096 x 4096 in 38 (42 with the smaller products).
+template <bool GATED>
+__global__ __launch_bounds__(256, 2) void f8_tile_kernel(const F8Params p) {
     exhip_touch_args(p);
-    constexpr int TN = 4, kRows = 32 * TM * WM, kThreads = 64 * WN * WM, kSteps = 16 * TM, kBuffers = 4, kPitch = 272, kBuffer = kRows * (kPitch + 4);
-    static_assert(kRows * 4 == kThreads, "a thread stages a quarter of a row");
+    constexpr int WN = 4, TN = 4, TM = 2, kRows = 32 * TM, kSteps = 16 * TM, kBuffers = 4, kPitch = 272, kBuffer = kRows * (kPitch + 4);
     // [buffer][row][128 halves], a row's pitch 16 bytes more, so that a piece of eight neighbouring rows lies in all banks; the rows' scales behind them
     constexpr int kStaged = kBuffers * kBuffer, kResults = kRows * (GATED ? 32 * WN * 2 : 64 * WN * 4);
     __shared__ __attribute__((aligned(16))) char memory[kStaged > kResults ? kStaged : kResults];
-    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wn = wave % WN, wm = wave / WN;
+    const int lane = threadIdx.x % 64, wn = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int side = lane / 32, col = lane % 32;
     int group_n, group_m;
     tile_of(p.groups_n, p.groups_m, &group_n, &group_m);
@@ -768,9 +770,9 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void f8_tile_kernel(const F8Params
         asm volatile("" : "+v"(w[f][s]));  // here, not together ahead of the chain that takes them
     };
     auto piece_of = [&](int b, int t, int s) {
-        return *reinterpret_cast<const v8h*>(memory + b % kBuffers * kBuffer + ((wm * TM + t) * 32 + col) * kPitch + side * 64 + s / 4 * 128 + s % 4 * 16);
+        return *reinterpret_cast<const v8h*>(memory + b % kBuffers * kBuffer + (t * 32 + col) * kPitch + side * 64 + s / 4 * 128 + s % 4 * 16);
     };
-    auto scale_of_row = [&](int b, int t) { return *reinterpret_cast<const float*>(memory + b % kBuffers * kBuffer + kRows * kPitch + ((wm * TM + t) * 32 + col) * 4); };
+    auto scale_of_row = [&](int b, int t) { return *reinterpret_cast<const float*>(memory + b % kBuffers * kBuffer + kRows * kPitch + (t * 32 + col) * 4); };
     v4f acc[8][TM];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -794,40 +796,35 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void f8_tile_kernel(const F8Params
 #pragma unroll
     for (int j = 0; j < 4; ++j) stage(0, j);
 #pragma unroll
-    for (int j = 0; j < 3; ++j)
-        if (TM == 1) request(1, j);
-#pragma unroll
     for (int s = 0; s < 8; ++s) convert_w(0, s);
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < 8; ++s) x[s] = piece_of(0, 0, s);
     float row_scale = scale_of_row(0, 0), s_w = ws[0], s_up = GATED ? ws_up[0] : 0.f, s_next = 0.f, s_up_next = 0.f;
     for (int b = 0; b < blocks; ++b) {
-        if (TM == 1 && tail && b == blocks - 2) cut();
 #pragma unroll
         for (int u = 0; u < kSteps; ++u) {
             const int t = u / 16, f = u / 8 % 2, s = u % 8;
-            constexpr int kStage = TM == 1 ? 4 : 12, kAsk = TM == 1 ? 8 : 0;
-            if (u == kSteps / 2 - 4) {
+            if (u == 12) {
                 const int after = min(b + 1, blocks - 1);
                 s_next = ws[after];
                 if constexpr (GATED) s_up_next = ws_up[after];
             }
-            if (u == (TM == 1 ? 8 : 20)) __syncthreads();
-            if (TM > 1 && u == kStage && tail && b == blocks - 2) cut();
+            if (u == 20) __syncthreads();
+            if (u == 12 && tail && b == blocks - 2) cut();
             if (u % 16 == 0) {
                 sc[t] = s_w * row_scale;
                 sc_up[t] = s_up * row_scale;
             }
             if (u < 8) convert_w(1, s);
-            if (u >= kSteps / 2 - 8 && u < kSteps / 2 - 4) request_w(b + 1, 0, u - (kSteps / 2 - 8));
-            if (u >= kSteps - 8 && u < kSteps - 4) request_w(b + 1, 1, u - (kSteps - 8));
-            if (u >= kStage && u < kStage + 4) stage(b + 1, u - kStage);
-            if (u >= kAsk && u < kAsk + 3) request(TM == 1 ? b + 2 : b + 1, u - kAsk);
+            if (u >= 8 && u < 12) request_w(b + 1, 0, u - 8);
+            if (u >= 24 && u < 28) request_w(b + 1, 1, u - 24);
+            if (u >= 12 && u < 16) stage(b + 1, u - 12);
+            if (u < 3) request(b + 1, u);
             part[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w[f][s], x[s], s == 0 ? none : part[f], 0, 0, 0);
             if (f == 1) x[s] = t + 1 < TM ? piece_of(b, t + 1, s) : piece_of(b + 1, 0, s);
             if (f == 1 && s == 7) row_scale = t + 1 < TM ? scale_of_row(b, t + 1) : scale_of_row(b + 1, 0);
-            if (u >= kSteps - 8) convert_w(0, s);
+            if (u >= 24) convert_w(0, s);
             if (s >= 2 && s < 6) {
                 if (u < 8) add(1, TM - 1, s - 2, last, last_up);
                 else add(1 - f, f == 1 ? t : t - 1, s - 2, sc[f == 1 ? t : t - 1 < 0 ? 0 : t - 1], sc_up[f == 1 ? t : t - 1 < 0 ? 0 : t - 1]);
@@ -841,8 +838,8 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void f8_tile_kernel(const F8Params
     }
 #pragma unroll
     for (int g = 0; g < 4; ++g) add(1, TM - 1, g, last, last_up);
-    if constexpr (!GATED) write_group<32, WN, WM, true>(p, acc, group_n, wn, wm, row0, rows, lane, memory);
-    else write_gated_group<32, WN, WM>(p, acc, group_n, wn, wm, row0, rows, lane, memory);
+    if constexpr (!GATED) write_group<32, WN, 1, true>(p, acc, group_n, wn, 0, row0, rows, lane, memory);
+    else write_gated_group<32, WN, 1>(p, acc, group_n, wn, 0, row0, rows, lane, memory);
 }
 
 // ---- a tile or two for every CU ----
@@ -851,7 +848,9 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void f8_tile_kernel(const F8Params
 // draws from L2, some 27 bytes a cycle: where 128 x 128 leaves CUs without a group, 64 x 64 (WM = 2, two groups a CU) has the others draw too: 128 x 8192 x 8192 in
 // 20 us (32), 256 x 4096 x 4096 in 12 (18), 64 rows of the gated 8192 x 4096 in 15 (21); 1024 x 4096 x 4096 in 23 us with WM = 4.
 // (2 x 2 waves of 64 x 64, one for each SIMD, take longer than 2 x 4: 330 instructions a block, of which a wave alone issues one in 4.5 cycles.)
-template <int WM, bool GATED>
+// EXACT converts each wave's codes to halves, 64 conversions beside 16 products a block: 512 x 4096 x 4096 in float32 takes 25 us, 33 on the larger tiles of
+// f8_tile_kernel and 35 on f8_rows_kernel's, 64 x 32000 x 4096 27 (35, 45), 1024 x 4096 x 4096 47 (39).
+template <int WM, bool GATED, bool EXACT>
 __global__ __launch_bounds__(128 * WM, 2) void f8_deep_kernel(const F8Params p) {
     exhip_touch_args(p);
     constexpr int WN = 2, TN = WM, TM = WN, kRows = 16 * TM * WM, kLoads = 5, kBuffers = 4, kWeights = 2048 * TN * WN, kCodes = kRows * kBlk, kBuffer = kWeights + kCodes + kRows * 4;
@@ -938,9 +937,14 @@ __global__ __launch_bounds__(128 * WM, 2) void f8_deep_kernel(const F8Params p) 
         if (cut_row_end(b)) x[0] = rows_from(b, 0);
         v4f part[kLag + 1];
         float s[2], su[2];
+        Halves weights_h[EXACT ? TN : 1], rows_h;
 #pragma unroll
         for (int u = 0; u < kSteps + kLag; ++u) {
             const int t = u / TN, i = u % TN;
+            if constexpr (EXACT) {
+                if (u < kSteps && i == 0) rows_h = halves_of(x[t % 2].v);
+                if (u < TN) weights_h[u] = halves_of(w.v[u]);
+            }
             if (u == kSteps / 2) {
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");  // the next block's are there, the one's behind it are on their way
                 arrive();
@@ -956,7 +960,8 @@ __global__ __launch_bounds__(128 * WM, 2) void f8_deep_kernel(const F8Params p) 
                     su[t % 2] = s_up * x[t % 2].s;
                     x[(t + 1) % 2] = t + 1 < TM ? rows_from(b, t + 1) : rows_from(b + 1, 0);
                 }
-                part[u % (kLag + 1)] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v[i], x[t % 2].v, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+                if constexpr (EXACT) part[u % (kLag + 1)] = block_product(weights_h[i], rows_h);
+                else part[u % (kLag + 1)] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v[i], x[t % 2].v, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
             }
             if (u >= kLag) {
                 const int v = u - kLag, vt = v / TN, vi = v % TN;
@@ -974,7 +979,7 @@ __global__ __launch_bounds__(128 * WM, 2) void f8_deep_kernel(const F8Params p) 
         if (b + 1 < blocks) block(w1, w0, b + 1);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was staged behind the end, in front of the results' barrier
-    if constexpr (!GATED) write_group<16, WN, WM, false>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
+    if constexpr (!GATED) write_group<16, WN, WM, EXACT>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
     else write_gated_group<16, WN, WM>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
 }
 
@@ -1047,38 +1052,38 @@ template <int TN, int TM, int WN, int WK, int D, bool GATED>
 int run_rows(exhip_ctx* ctx, const F8Params& p) {
     return launch(ctx, f8_rows_kernel<TN, TM, WN, WK, D, GATED>, p, TN * WN, 16 * TM, 64 * WN * WK);
 }
-template <int WN, int WM, int TM, bool GATED>
+template <bool GATED>
 int run_tile(exhip_ctx* ctx, const F8Params& p) {
-    return launch(ctx, f8_tile_kernel<WN, WM, TM, GATED>, p, 4 * WN, 32 * TM * WM, 64 * WN * WM);
+    return launch(ctx, f8_tile_kernel<GATED>, p, 16, 64, 256);
 }
-template <int WM, bool GATED>
+template <int WM, bool GATED, bool EXACT>
 int run_deep(exhip_ctx* ctx, const F8Params& p) {
-    return launch(ctx, f8_deep_kernel<WM, GATED>, p, 2 * WM, 32 * WM, 128 * WM);
+    return launch(ctx, f8_deep_kernel<WM, GATED, EXACT>, p, 2 * WM, 32 * WM, 128 * WM);
 }
 template <bool GATED>
 int run_wide(exhip_ctx* ctx, const F8Params& p) {
     return launch(ctx, f8_wide_kernel<GATED>, p, 16, 256, 512);
 }
-// The times are fits to 3000 launches of 1 to 2048 rows and matrices from 256 x 512 to 8192 x 8192 and 32000 x 4096, on the GPU's clock: the form they choose takes
+// The times are fits to 3500 launches of 1 to 2048 rows and matrices from 256 x 512 to 8192 x 8192 and 32000 x 4096, on the GPU's clock: the form they choose takes
 // 0.3 % longer than the best one for the shape on average, 9 % at most.
 constexpr Form kExact[] = {  // results in float32
     {run_rows<1, 1, 1, 8, 4, false>, 1, 16, 2, 8, 1.5f, 1.9f, 0.97f, 0.58f, true}, {run_rows<2, 1, 1, 8, 2, false>, 2, 16, 2, 8, 0.3f, 3.1f, 1.74f, 0.64f, true},
     {run_rows<2, 2, 1, 8, 2, false>, 2, 32, 1, 8, 1.7f, 1.5f, 1.37f, 0.f, true},   {run_rows<4, 2, 1, 8, 1, false>, 4, 32, 1, 8, 1.0f, 2.5f, 1.80f, 0.f, true},
-    {run_tile<2, 2, 1, false>, 8, 64, 2, 1, 0.3f, 4.4f, 1.01f, 0.61f, false},      {run_tile<4, 1, 2, false>, 16, 64, 2, 1, 0.2f, 5.0f, 1.72f, 0.87f, false},
+    {run_deep<2, false, true>, 4, 64, 2, 1, 2.2f, 1.8f, 0.64f, 0.46f, true},       {run_tile<false>, 16, 64, 2, 1, 0.f, 5.0f, 1.69f, 0.89f, false},
 };
 constexpr Form kHalves[] = {
     kExact[0], kExact[1], kExact[2], kExact[3],
-    {run_deep<2, false>, 4, 64, 2, 1, 0.3f, 3.3f, 0.30f, 0.26f, true}, {run_deep<4, false>, 8, 128, 1, 1, 0.5f, 3.7f, 0.50f, 0.f, true},
+    {run_deep<2, false, false>, 4, 64, 2, 1, 0.3f, 3.3f, 0.30f, 0.26f, true}, {run_deep<4, false, false>, 8, 128, 1, 1, 0.5f, 3.7f, 0.50f, 0.f, true},
     {run_wide<false>, 16, 256, 1, 1, 0.f, 7.4f, 1.17f, 0.f, false},
 };
 constexpr Form kGatedHalves[] = {
     {run_rows<2, 1, 1, 8, 2, true>, 2, 16, 2, 8, 2.5f, 1.5f, 1.95f, 0.85f, true}, {run_rows<2, 2, 1, 8, 2, true>, 2, 32, 1, 8, 1.4f, 2.4f, 1.34f, 0.f, true},
-    {run_rows<4, 2, 1, 8, 1, true>, 4, 32, 1, 8, 1.3f, 2.6f, 1.90f, 0.f, true},   {run_deep<2, true>, 4, 64, 2, 1, 2.0f, 2.9f, 0.39f, 0.27f, true},
-    {run_deep<4, true>, 8, 128, 1, 1, 1.6f, 4.3f, 0.55f, 0.f, true},              {run_wide<true>, 16, 256, 1, 1, 0.1f, 15.2f, 1.33f, 0.f, false},
+    {run_rows<4, 2, 1, 8, 1, true>, 4, 32, 1, 8, 1.3f, 2.6f, 1.90f, 0.f, true},   {run_deep<2, true, false>, 4, 64, 2, 1, 2.0f, 2.9f, 0.39f, 0.27f, true},
+    {run_deep<4, true, false>, 8, 128, 1, 1, 1.6f, 4.3f, 0.55f, 0.f, true},              {run_wide<true>, 16, 256, 1, 1, 0.1f, 15.2f, 1.33f, 0.f, false},
 };
 constexpr Form kGatedCodes[] = {  // a group has whole blocks of the result: 16 tiles
     {run_rows<4, 1, 4, 4, 1, true>, 16, 16, 1, 4, 0.9f, 3.0f, 2.12f, 0.f, true}, {run_rows<4, 2, 4, 2, 1, true>, 16, 32, 1, 2, 0.f, 5.2f, 1.40f, 0.f, true},
-    {run_tile<4, 1, 2, true>, 16, 64, 2, 1, 0.f, 8.7f, 1.68f, 0.92f, false},
+    {run_tile<true>, 16, 64, 2, 1, 0.f, 8.7f, 1.68f, 0.92f, false},
 };
 
 constexpr int kCus = 256;
