@@ -74,23 +74,6 @@ int exhip_static_scratch_setup(int device);
         }                                 \
     } while (0)
 
-// Entry points work on the context's device whatever device the calling thread is on.
-struct exhip_on_device {
-    int before = -1;
-    hipError_t error = hipSuccess;
-    explicit exhip_on_device(int device) {
-        int now = device;
-        error = hipGetDevice(&now);
-        if (error == hipSuccess && now != device) {
-            error = hipSetDevice(device);
-            if (error == hipSuccess) before = now;
-        }
-    }
-    ~exhip_on_device() {
-        if (before >= 0) (void)hipSetDevice(before);
-    }
-};
-
 // Kernel launch check: launch errors are reported at once, execution errors at the next sync.
 #define EXHIP_LAUNCH_CHECK() EXHIP_CHECK(hipGetLastError())
 

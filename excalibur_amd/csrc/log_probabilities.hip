@@ -6,6 +6,7 @@
 #include <float.h>
 
 #include "common.h"
+#include "on_device.h"
 
 namespace {
 
