@@ -532,7 +532,7 @@ int exhip_innerproduct_f16(exhip_ctx* ctx, const uint16_t* x, const float* w, co
 /* Operands are e4m3 codes (one sign, four exponent and three fraction bits, largest value 448, 0x7F / 0xFF are NaN) with float32 scales: one for each
  * 128 values of an input row, scale[k block][row], and one for each 128 x 128 block of a weight matrix, scale[n block][k block]. The last blocks
  * hold what is left. A code stands for its value times its block's scale. Codes' rows begin on 16 bytes (base and stride); what lies between a
- * row's end and its stride is neither used nor written. */
+ * row's end and its stride is neither used nor written. Results may not overlap operands. */
 #define EXHIP_F8_BLOCK 128
 /* Rows x[m][k] (row stride x_stride elements, at least k) to codes y (row stride y_stride bytes) and scales [ceil(k / 128)][m]:
  * scale = max(max |x| / 448, 2^-100), code = e4m3(x * (1 / scale)), to nearest even. A NaN becomes a NaN code and does not count in its block's
