@@ -175,7 +175,8 @@ struct F8Params {
     int m, n, k, x_stride, y_stride;
     int blocks_k, tiles;  // blocks along k, tiles of 16 outputs (of both projections)
     int gate;
-    int groups_n, groups_m;  // groups side by side along the outputs, and along the rows
+    int first, last;         // the rows of this launch
+    int groups_n, groups_m;  // its groups side by side along the outputs, and along the rows
 };
 
 __device__ __forceinline__ float gated(int gate, float g, float u) {
@@ -443,8 +444,8 @@ __global__ __launch_bounds__(512, 2) void f8_wide_kernel(const F8Params p) {
     const int q = lane / 16, col = lane % 16;
     int group_n, group_m;
     tile_of(p.groups_n, p.groups_m, &group_n, &group_m);
-    const int tile0 = (group_n * WN + wn) * TN, row0 = group_m * kRows;
-    const int rows = min(kRows, p.m - row0), tail = p.k % kBlk, blocks = p.blocks_k;
+    const int tile0 = (group_n * WN + wn) * TN, row0 = p.first + group_m * kRows;
+    const int rows = min(kRows, p.last - row0), tail = p.k % kBlk, blocks = p.blocks_k;
     const __amdgpu_buffer_rsrc_t xr = uniform_view(p.x + (size_t)row0 * p.x_stride, (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16);
     // A wave stages 32 rows, eight with a load: lane l holds piece (l % 8) ^ (l / 8) of row l / 8, so that a piece of eight neighbouring rows lies in all banks.
     // Pieces behind a row's end are zeros.
@@ -573,8 +574,8 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void f8_rows_kernel(const F8Params
     static_assert(TN % kSide == 0, "both sides of an output are one wave's");
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wn = wave % WN, wk = wave / WN;
     const int q = lane / 16, col = lane % 16;
-    const int group_n = blockIdx.x % p.groups_n, tile0 = (group_n * WN + wn) * TN, row0 = blockIdx.x / p.groups_n * kRows;
-    const int rows = min(kRows, p.m - row0), tail = p.k % kBlk, blocks = p.blocks_k;
+    const int group_n = blockIdx.x % p.groups_n, tile0 = (group_n * WN + wn) * TN, row0 = p.first + blockIdx.x / p.groups_n * kRows;
+    const int rows = min(kRows, p.last - row0), tail = p.k % kBlk, blocks = p.blocks_k;
     const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.x) + (size_t)row0 * p.x_stride, 0,
                                                                       (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16, kRsrcWord3);
     int off[TM];
@@ -727,8 +728,8 @@ __global__ __launch_bounds__(256, 2) void f8_tile_kernel(const F8Params p) {
     const int side = lane / 32, col = lane % 32;
     int group_n, group_m;
     tile_of(p.groups_n, p.groups_m, &group_n, &group_m);
-    const int tile0 = (group_n * WN + wn) * TN, row0 = group_m * kRows;
-    const int rows = min(kRows, p.m - row0), tail = p.k % kBlk, blocks = p.blocks_k;
+    const int tile0 = (group_n * WN + wn) * TN, row0 = p.first + group_m * kRows;
+    const int rows = min(kRows, p.last - row0), tail = p.k % kBlk, blocks = p.blocks_k;
     const __amdgpu_buffer_rsrc_t xr = uniform_view(p.x + (size_t)row0 * p.x_stride, (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16);
     // what this thread stages
     const int own_row = threadIdx.x / 4, own_q = threadIdx.x % 4;
@@ -861,8 +862,8 @@ __global__ __launch_bounds__(128 * WM, 2) void f8_deep_kernel(const F8Params p) 
     const int q = lane / 16, col = lane % 16;
     int group_n, group_m;
     tile_of(p.groups_n, p.groups_m, &group_n, &group_m);
-    const int tile0 = (group_n * WN + wn) * TN, row0 = group_m * kRows;
-    const int rows = min(kRows, p.m - row0), tail = p.k % kBlk, blocks = p.blocks_k;
+    const int tile0 = (group_n * WN + wn) * TN, row0 = p.first + group_m * kRows;
+    const int rows = min(kRows, p.last - row0), tail = p.k % kBlk, blocks = p.blocks_k;
     const __amdgpu_buffer_rsrc_t xr = uniform_view(p.x + (size_t)row0 * p.x_stride, (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16);
     // A wave stages 16 rows, eight with a load (as in f8_wide_kernel), and one of the group's tiles of weights.
     const int piece = (lane % 8) ^ (lane / 8);
@@ -1017,7 +1018,7 @@ F8Params params_of(const exhip_f8_desc* d, const uint8_t* x, const float* x_scal
     p.x = x;
     p.x_scale = x_scale;
     p.w = static_cast<const uint8_t*>(w);
-    p.m = d->m;
+    p.m = p.last = d->m;
     p.n = d->n_out;
     p.k = d->k_in;
     p.x_stride = d->x_stride;
@@ -1030,9 +1031,9 @@ F8Params params_of(const exhip_f8_desc* d, const uint8_t* x, const float* x_scal
 template <typename K>
 int launch(exhip_ctx* ctx, K kernel, F8Params p, int tiles, int rows, int threads) {
     p.groups_n = (p.tiles + tiles - 1) / tiles;
-    p.groups_m = p.m / rows + (p.m % rows != 0);
+    p.groups_m = (p.last - p.first - 1) / rows + 1;
     const long long groups = (long long)p.groups_n * p.groups_m;
-    EXHIP_REQUIRE(groups <= 0x7fffffff / threads, "inner product: %d rows of %d outputs are more than one launch takes", p.m, p.n);
+    EXHIP_REQUIRE(groups <= 0x7fffffff / threads, "inner product: %d rows of %d outputs are more than one launch takes", p.last - p.first, p.n);
     const exhip_on_device on(ctx->device);
     EXHIP_CHECK(on.error);
     hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(threads), 0, ctx->stream, p);
@@ -1089,27 +1090,66 @@ constexpr Form kGatedCodes[] = {  // a group has whole blocks of the result: 16 
 
 constexpr int kCus = 256;
 
+// What a launch of a form takes for some rows, in us.
+float time_of(const Form& f, const F8Params& p, int rows) {
+    const int groups_n = (p.tiles + f.tiles - 1) / f.tiles, groups_m = (rows - 1) / f.rows + 1;
+    const long long times = ((long long)groups_n * groups_m - 1) / kCus + 1, full = times / f.at_once, rest = times % f.at_once;
+    const float us = f.start + (float)(full + rest) * f.round + ((float)full * f.block + (float)rest * f.alone) * (float)((p.blocks_k - 1) / f.split + 1);
+    if (!f.drawn) return us;
+    // all loads together, in bytes a us: the weights once from memory, what groups read again, weights and rows, from L2
+    const float weights = (float)p.tiles * (float)p.blocks_k * 2048.f, again = (float)(groups_m - 1) * weights + (float)groups_n * (float)rows * (float)p.blocks_k * 128.f;
+    return fmaxf(us, f.start + weights / 7.9e6f + again / 19e6f);
+}
 template <int N>
-int run_best(exhip_ctx* ctx, const F8Params& p, const Form (&forms)[N]) {
-    const int pinned = g_exhip_options.f8_form;
-    if (pinned > 0) return forms[(pinned < N ? pinned : N) - 1].run(ctx, p);
+int best_of(const Form (&forms)[N], const F8Params& p, int rows, float* us) {
     int best = 0;
-    float best_us = 0.f;
     for (int i = 0; i < N; ++i) {
-        const Form& f = forms[i];
-        const int groups_n = (p.tiles + f.tiles - 1) / f.tiles, groups_m = p.m / f.rows + (p.m % f.rows != 0);
-        const long long times = ((long long)groups_n * groups_m - 1) / kCus + 1, full = times / f.at_once, rest = times % f.at_once;
-        float us = f.start + (float)(full + rest) * f.round + ((float)full * f.block + (float)rest * f.alone) * (float)((p.blocks_k - 1) / f.split + 1);
-        if (f.drawn) {  // all loads together, in bytes a us: the weights once from memory, what groups read again, weights and rows, from L2
-            const float weights = (float)p.tiles * (float)p.blocks_k * 2048.f, again = (float)(groups_m - 1) * weights + (float)groups_n * (float)p.m * (float)p.blocks_k * 128.f;
-            us = fmaxf(us, f.start + weights / 7.9e6f + again / 19e6f);
-        }
-        if (i == 0 || us < best_us) {
+        const float t = time_of(forms[i], p, rows);
+        if (i == 0 || t < *us) {
             best = i;
-            best_us = us;
+            *us = t;
         }
     }
-    return forms[best].run(ctx, p);
+    return best;
+}
+
+// One launch, or two where the last rows would have a few CUs work while the others are done, and a kernel of smaller tiles takes them: 3 us, less than nothing
+// for short launches, then 20 % and more for some shapes (1657 x 2920 x 5785 in halves 60 -> 48 us, 2711 x 3052 x 2961 in float32 68 -> 56).
+// (Quantized results stay in one: their kernels for few rows take what two launches win.)
+template <int N>
+int run_best(exhip_ctx* ctx, const F8Params& p, const Form (&forms)[N], bool in_two = true) {
+    const int pinned = g_exhip_options.f8_form;
+    if (pinned > 0) return forms[(pinned < N ? pinned : N) - 1].run(ctx, p);
+    float us = 0.f;
+    int best = best_of(forms, p, p.m, &us), behind = 0, rows = p.m;
+    if (in_two && us > 12.f) {
+        us = us * 0.97f - 3.f;
+        for (int i = 0; i < N; ++i) {
+            const Form& f = forms[i];
+            const int groups_n = (p.tiles + f.tiles - 1) / f.tiles, at_once = kCus * f.at_once;
+            const int whole = p.m / f.rows, filled = (int)((long long)groups_n * whole / at_once * at_once / groups_n);  // in tiles of rows
+            for (const int some : {whole, filled}) {
+                const int front = some * f.rows;
+                if (some == 0 || front == p.m) continue;
+                float rest = 0.f;
+                const int next = best_of(forms, p, p.m - front, &rest);
+                const float both = time_of(f, p, front) + rest;
+                if (both < us) {
+                    us = both;
+                    best = i;
+                    behind = next;
+                    rows = front;
+                }
+            }
+        }
+    }
+    F8Params part = p;
+    part.last = rows;
+    const int rc = forms[best].run(ctx, part);
+    if (rc != 0 || rows == p.m) return rc;
+    part.first = rows;
+    part.last = p.m;
+    return forms[behind].run(ctx, part);
 }
 
 }  // namespace
@@ -1189,5 +1229,5 @@ extern "C" int exhip_innerproduct_gated_f8(exhip_ctx* ctx, const exhip_f8_desc* 
     p.y_f8 = y_f8;
     p.y_scale = y_scale;
     p.gate = gate;
-    return y_f8 ? run_best(ctx, p, kGatedCodes) : run_best(ctx, p, kGatedHalves);
+    return y_f8 ? run_best(ctx, p, kGatedCodes, false) : run_best(ctx, p, kGatedHalves);
 }

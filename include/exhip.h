@@ -558,7 +558,7 @@ typedef struct exhip_f8_desc {
  * a half's own rounding is 2e-4 of them. */
 int exhip_innerproduct_f8(exhip_ctx* ctx, const exhip_f8_desc* d, const uint8_t* x, const float* x_scale, const void* w_packed, const float* w_scale,
                           const float* bias, float* y_f32, uint16_t* y_f16);
-/* A feed-forward block's first half in one launch: h = act(x w_gate + bias_gate) * (x w_up + bias_up) with act(v) = v / (1 + exp(-v)),
+/* A feed-forward block's first half, with nothing stored in between: h = act(x w_gate + bias_gate) * (x w_up + bias_up) with act(v) = v / (1 + exp(-v)),
  * v (1 + erf(v / sqrt 2)) / 2, 1 / (1 + exp(-v)) or max(v, 0). The result is h as halves (y_f16), or the codes (y_f8) and scales (y_scale, both or neither)
  * that exhip_quantize_rows_f32_to_f8 makes of h in float32; one of the two forms, summed like halves and like float32 above. Biases: both or neither. */
 #define EXHIP_GATE_SILU 0

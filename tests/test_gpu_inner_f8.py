@@ -432,3 +432,25 @@ def test_two_contexts_at_once(ctx):
         for name in want:
             assert np.array_equal(got[name], want[name]), name
     other.close()
+
+
+@pytest.mark.parametrize("what,m,n,k", [("f32", 2060, 4087, 442), ("f16", 2895, 5799, 332), ("gated", 2076, 3892, 201)])
+def test_last_rows_by_a_launch_of_their_own(ctx, what, m, n, k):
+    o = Operands(ctx, np.random.default_rng(m + n + k), m, n, k, sides=2 if what == "gated" else 1, bias=True, pad=16)
+    y = ctx.array(np.full((m + 1, n + 3), 7.25, np.float32) if what == "f32" else np.full((m + 1, n + 3), 0x4567, np.uint16))
+    d, args = o.desc(ctx, n + 3), (o.dx, o.dx_scale, o.packed)
+    some = np.r_[0:40, m // 2:m // 2 + 40, m - 300:m]  # the launches meet among the last rows
+    x, x_scale = o.x[some], o.x_scale[:, some]
+    want, bound = f8ref.product(x, x_scale, o.w[0], o.w_scale[0], o.bias[0])
+    cut = bound + f8ref.cut_bound(x, x_scale, o.w[0], o.w_scale[0])
+    if what == "gated":
+        ctx.innerproduct_gated_f8(d, *args, *o.dw_scale, "silu", *o.dbias, y_f16=y)
+        up, up_bound = f8ref.product(x, x_scale, o.w[1], o.w_scale[1], o.bias[1])
+        want, bound = f8ref.gated("silu", want, cut, up, up_bound + f8ref.cut_bound(x, x_scale, o.w[1], o.w_scale[1]))
+        bound = f8ref.half_bound(want, bound)
+    else:
+        ctx.innerproduct_f8(d, *args, o.dw_scale[0], o.dbias[0], **{"y_" + what: y})
+        bound = bound if what == "f32" else f8ref.half_bound(want, cut)
+    got, fill = y.download(), 7.25 if what == "f32" else 0x4567
+    assert np.all(got[m] == fill) and np.all(got[:, n:] == fill) and not np.any(np.all(got[:m, :n] == fill, axis=1))
+    _near((got if what == "f32" else got.view(np.float16))[some, :n], want, bound)
