@@ -6,11 +6,13 @@
 #include <float.h>
 
 #include "common.h"
+#include "largest.h"
 #include "on_device.h"
 
 namespace {
 
 constexpr int kMostSlice = 32768, kLongSlice = 16384, kSlice = 8192;  // values of a row that a group of 16, of 8, of 4 waves holds in its registers
+static_assert(kMostSlice <= kMostCounted, "a count of a slice's values is half a word");
 constexpr int kCandidates = 512;  // places that are held at once
 constexpr int kRanked = 128;      // and that are ranked, each against all; of more, those behind the top-th are left out first
 typedef unsigned long long u64;
@@ -208,7 +210,8 @@ __global__ __launch_bounds__(64 * W, 8) void log_probabilities_kernel(const T* _
     __shared__ Sums sums[W];
     __shared__ float sets[TOP ? 128 : 1], bound;
     __shared__ u64 places[TOP ? kCandidates + 8 : 1], sorted[TOP ? EXHIP_LOG_PROBABILITIES_TOP : 1];
-    __shared__ int count, counts[2][W];
+    __shared__ int count;
+    __shared__ unsigned counts[2][W];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const size_t row = blockIdx.x / p.slices;
     const int slice = blockIdx.x % p.slices, first = slice * p.slice_len, len = min(p.slice_len, p.c - first);
@@ -332,9 +335,7 @@ __global__ __launch_bounds__(64 * W, 8) void log_probabilities_kernel(const T* _
             const int want = min(p.top, len);
             int turn = 0;
             const unsigned of_sets[2] = {order_of(sets[lane]), order_of(sets[64 + lane])};
-            unsigned o = reached_by<32>(of_sets, want), most_o = ~0u;
-            int above = 0;  // the values whose order is more than o
-            auto held = [&](auto takes) {
+            const Cut cut = find_cut(reached_by<32>(of_sets, want), want, kRanked, len, [&](unsigned o, auto takes) {
                 int here = 0, more = 0;
 #pragma unroll 1
                 for (int i = 0; i < kRuns; ++i) {  // read again: what stays of them for this path costs the other one its waves
@@ -346,46 +347,17 @@ __global__ __launch_bounds__(64 * W, 8) void log_probabilities_kernel(const T* _
                         more += __popcll(__ballot(order > o));
                     }
                 }
+                unsigned two = two_counts(here, more);
                 if constexpr (W > 1) {
-                    if (lane == 0) counts[turn][wave] = here | more << 16;
+                    if (lane == 0) counts[turn][wave] = two;
                     __syncthreads();
-                    here = 0;
+                    two = 0;
 #pragma unroll
-                    for (int w = 0; w < W; ++w) here += counts[turn][w];
+                    for (int w = 0; w < W; ++w) two += counts[turn][w];
                     turn ^= 1;
-                    more = here >> 16;
-                    here &= 0xffff;
                 }
-                above = more;
-                return here;
-            };
-            int reach = held([&](unsigned order, int) { return order >= o; });
-            while (reach > kRanked && above >= want && o < most_o) {
-                const unsigned up = o + (most_o - o) / 2 + 1;
-                const int n_up = held([&](unsigned order, int) { return order >= up; });
-                if (n_up < want) {
-                    most_o = up - 1;
-                } else {
-                    o = up;
-                    reach = n_up;
-                    above = want;  // or more, unless there is nothing above
-                    if (o == most_o) held([&](unsigned, int) { return false; });
-                }
-            }
-            int begin = 0, end = len;  // of those alike, what stands in front of `end`
-            for (int step = 0, n_begin = above, n_end = reach; n_end > kRanked; ++step) {
-                // where they would be spread evenly, and the middle, by turns
-                const int even = (end - begin) * ((want + kRanked) / 2 - n_begin) / (n_end - n_begin), most_to = end - begin > 1 ? end - begin - 1 : 1;
-                const int to = begin + (step % 2 == 0 && even > 0 && even < most_to ? even : (end - begin + 1) / 2);
-                const int here = held([&](unsigned order, int i) { return order == o && i < to; }), n_to = above + here;
-                if (n_to < want) {
-                    begin = to;
-                    n_begin = n_to;
-                } else {
-                    end = to;
-                    n_end = n_to;
-                }
-            }
+                return two;
+            });
             if (threadIdx.x == 0) count = 0;
             __syncthreads();
 #pragma unroll 1
@@ -396,11 +368,14 @@ __global__ __launch_bounds__(64 * W, 8) void log_probabilities_kernel(const T* _
                     const float v = as_float(run.v[e]);
                     const unsigned order = order_of(v);
                     const int k = at(i * N + e);
-                    if (order > o || (order == o && k < end)) places[atomicAdd(&count, 1)] = place_of(v, first + k);
+                    if (order > cut.order || (order == cut.order && k < cut.end)) {
+                        const int to = atomicAdd(&count, 1);
+                        if (to < kCandidates) places[to] = place_of(v, first + k);
+                    }
                 }
             }
             __syncthreads();
-            n = count;  // without what stands behind the slice's end
+            n = min(count, kCandidates);  // without what stands behind the slice's end
         }
         if (wave != 0) return;
         if (!many && n < p.top) {  // masked classes too, by their index: they are among the first n + top of the slice

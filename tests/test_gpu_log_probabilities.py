@@ -230,3 +230,22 @@ def test_rows_enough_for_long_slices(ctx, m, c, dtype):
     _check(ctx, x, ids, 8, c + c % 3)
     _check(ctx, x, ids, 64)
     _check(ctx, x, ids)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("c", [8192, 16384, 32760, 32767, 32768, 65536])
+@pytest.mark.parametrize("top", [1, 20, 64])
+def test_the_largest_of_a_whole_group_s_values(ctx, c, top, dtype):
+    """As many values as a group holds and nearly so, every one of them above what the search begins with: rows of NaN, and of NaN but for a few."""
+    rng = np.random.default_rng(c + top)
+    x = np.full((6, c), np.nan, dtype)
+    x[1, rng.permutation(c)[:5]] = 1.0
+    x[2, -1] = -3.0
+    x[3] = np.inf
+    x[3, ::9] = np.nan
+    x[4] = np.where(np.arange(c) % 2, rng.standard_normal(c), np.nan)
+    x[5] = -np.inf
+    x[5, c // 2:] = np.nan
+    got = _run(ctx, x, None, top)
+    assert np.array_equal(got["top_ids"], _order(x, top))
+    assert np.all(np.isnan(got["top_log_p"])) and np.all(np.isnan(got["entropy"]))
