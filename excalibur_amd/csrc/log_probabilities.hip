@@ -475,6 +475,7 @@ void launch_slices(exhip_ctx* ctx, const T* x, const LogpParams& p) {
 }
 
 bool sizes_ok(int m, int c, int top) { return m > 0 && c > 0 && top >= 0 && top <= EXHIP_LOG_PROBABILITIES_TOP && top <= c; }
+bool one_launch(int m, int slices) { return (size_t)m * slices <= 0xffffffffu / 1024; }
 
 template <typename T>
 int log_probabilities(exhip_ctx* ctx, const char* name, const T* x, int x_stride, int m, int c, const int32_t* ids, int n_ids, float* log_p, float* entropy, int top,
@@ -489,7 +490,7 @@ int log_probabilities(exhip_ctx* ctx, const char* name, const T* x, int x_stride
                   "%s: an operand's address is not that of its type", name);
     LogpParams p = {ids, log_p, entropy, top_log_p, top_ids, nullptr, nullptr, m, c, x_stride, n_ids, top, 0, 0};
     split(m, c, top, &p.slices, &p.slice_len);
-    EXHIP_REQUIRE((size_t)m * p.slices <= 0xffffffffu / 1024, "%s: %d rows of %d values are more than one launch takes", name, m, c);
+    EXHIP_REQUIRE(one_launch(m, p.slices), "%s: %d rows of %d values are more than one launch takes", name, m, c);
     if (p.slices > 1) {
         p.part = static_cast<Sums*>(workspace);
         p.part_top = reinterpret_cast<u64*>(p.part + (size_t)m * p.slices);
@@ -515,7 +516,12 @@ extern "C" size_t exhip_log_probabilities_workspace(int m, int c, int top) {
     }
     int slices, slice_len;
     split(m, c, top, &slices, &slice_len);
-    return slices > 1 ? (size_t)m * slices * (sizeof(Sums) + 8 * top) : 16;
+    if (!one_launch(m, slices)) {
+        exhip_set_error("exhip_log_probabilities_workspace: %d rows of %d values are more than one launch takes", m, c);
+        return 0;
+    }
+    // Of the shortest slices that a row is ever split into, so that it is enough for fewer rows, classes or largest, whatever their own slices are.
+    return c > kMostSlice ? (size_t)m * ((c - 1) / kSlice + 1) * (sizeof(Sums) + 8 * top) : 16;
 }
 
 extern "C" int exhip_log_probabilities_f32(exhip_ctx* ctx, const float* x, int x_stride, int m, int c, const int32_t* ids, int n_ids, float* log_p, float* entropy,

@@ -576,8 +576,8 @@ int exhip_innerproduct_gated_f8(exhip_ctx* ctx, const exhip_f8_desc* d, int gate
  * top_ids[m][top], top_log_p[m][top]: the largest x in falling order, equal ones by their index, and their log probabilities.
  * -infinity masks a class. A row with nothing else has log probabilities of -infinity and entropy 0. In a row with a NaN or a +infinity all of these
  * values are NaN (those of negative ids are 0), and NaN stands above every number in top_ids. log_p, entropy and the top pair may be NULL (with n_ids = 0,
- * and top = 0). top is at most 64 and at most c. `workspace` (on 16 bytes) is the caller's, exhip_log_probabilities_workspace() bytes of it (0 for bad
- * sizes); calls that may overlap need one each. Values that are close or equal cost more to order than values that are spread, a few readings of them. */
+ * and top = 0). top is at most 64 and at most c. `workspace` (on 16 bytes) is the caller's, exhip_log_probabilities_workspace() bytes of it (0 for sizes
+ * that are refused), which are enough for fewer rows, classes or largest too; calls that may overlap need one each. Values that are close or equal cost more to order than values that are spread, a few readings of them. */
 #define EXHIP_LOG_PROBABILITIES_TOP 64
 size_t exhip_log_probabilities_workspace(int m, int c, int top);
 int exhip_log_probabilities_f32(exhip_ctx* ctx, const float* x, int x_stride, int m, int c, const int32_t* ids, int n_ids, float* log_p, float* entropy,

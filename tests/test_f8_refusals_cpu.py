@@ -127,3 +127,27 @@ def test_codes_of_the_oracle():
     assert np.array_equal(f8ref.encode(f8ref.VALUES[finite]), codes)
     assert f8ref.VALUES.max(initial=0, where=finite) == 448 and f8ref.VALUES[1] == 2.0 ** -9 and f8ref.VALUES[8] == 2.0 ** -6
     assert f8ref.encode([2.0 ** -10, 3 * 2.0 ** -10, 17, 19, 460, -17, np.nan]).tolist() == [0, 2, 0x58, 0x5A, 0x7E, 0xD8, 0x7F]
+
+
+def test_a_log_probability_workspace_is_enough_for_smaller_calls():
+    """A server has one for its largest batch: the size never falls as rows, classes or the largest asked grow, and what is refused has none."""
+    size = _lib().exhip_log_probabilities_workspace
+    rows, classes, tops = (1, 2, 16, 17, 31, 32, 33, 48, 300, 4096), (64, 8192, 8193, 32767, 32768, 32769, 49153, 65536, 100003, 131071, 131072, 131073, 262144, 1000000), (0, 1, 2, 20, 64)
+    sizes = np.array([[[size(m, c, top) for top in tops] for c in classes] for m in rows], np.int64)
+    assert sizes.min() >= 16
+    for axis in range(3):
+        assert np.diff(sizes, axis=axis).min() >= 0, axis
+    entry = _lib().exhip_log_probabilities_f32
+    for m, c, top in ((1 << 22, 64, 0), (1 << 22, 64, 5), (1 << 19, 100000, 0), (1 << 20, 100000, 5)):
+        assert size(m, c, top) == 0, (m, c, top)
+        assert _status(entry, X, c, m, c, None, 0, None, E, top, Y if top else None, S if top else None, W) == ERR_ARG
+        assert size(m // 16, c, top) > 0
+
+
+def test_a_log_probability_workspace_holds_every_row_s_slices():
+    """What the slices of a row need, counted from what a group holds: at least 8192 values of a row of more than 32768, sums of 16 bytes and 8 for each of the largest."""
+    size = _lib().exhip_log_probabilities_workspace
+    for m in (1, 32, 33, 700):
+        for c in (32769, 40000, 65537, 131072, 131073, 500001):
+            for top in (0, 1, 20, 64):
+                assert size(m, c, top) >= m * -(-c // 8192) * (16 + 8 * top), (m, c, top)

@@ -249,3 +249,31 @@ def test_the_largest_of_a_whole_group_s_values(ctx, c, top, dtype):
     got = _run(ctx, x, None, top)
     assert np.array_equal(got["top_ids"], _order(x, top))
     assert np.all(np.isnan(got["top_log_p"])) and np.all(np.isnan(got["entropy"]))
+
+
+@pytest.mark.parametrize("m,c,top", [(48, 131072, 20), (300, 65537, 5), (33, 140000, 64)])
+def test_one_workspace_for_smaller_calls(ctx, m, c, top):
+    """A workspace of the largest call takes smaller ones, and nothing behind it or behind any result changes."""
+    rng = np.random.default_rng(m + c)
+    x = (rng.standard_normal((m, c)) * 2.5).astype(np.float16)
+    ids = rng.integers(0, c, (m, 2)).astype(np.int32)
+    dx, d_ids = ctx.array(x.view(np.uint16)), ctx.array(ids)
+    nbytes = ctx.log_probabilities_workspace(m, c, top)
+    for rows, classes, largest in ((m, c, top), (32, c, top), (17, c, top), (m, c, 1), (m, c, 0), (20, c - 9000, top), (3, 999, top)):
+        work = ctx.array(np.full(nbytes + 4096, 0xA5, np.uint8))
+        out = dict(entropy=ctx.array(np.full(rows + 64, 7.25, np.float32)), log_p=ctx.array(np.full((rows + 8, 2), 7.25, np.float32)))
+        if largest:
+            out.update(top_ids=ctx.array(np.full((rows + 8, largest), 77, np.int32)), top_log_p=ctx.array(np.full((rows + 8, largest), 7.25, np.float32)))
+        ctx.log_probabilities(ctx.view(dx.ptr.value, (rows, c), np.uint16), classes, ids=ctx.view(d_ids.ptr.value, (rows, 2), np.int32), top=largest, workspace=work, **out)
+        got = {name: a.download() for name, a in out.items()}
+        assert np.all(work.download()[nbytes:] == 0xA5), (rows, classes, largest)
+        for name, a in got.items():
+            assert np.all(a[rows:] == (77 if name == "top_ids" else 7.25)), (name, rows, classes, largest)
+        log_p, entropy, b, be = _reference(x[:rows, :classes])
+        _same(got["entropy"][:rows], entropy, be)
+        if largest:
+            assert np.array_equal(got["top_ids"][:rows], _order(x[:rows, :classes], largest))
+        for a in [work, *out.values()]:
+            a.free()
+    dx.free()
+    d_ids.free()
