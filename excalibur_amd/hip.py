@@ -4,6 +4,8 @@ This is the Python face of the product library: it loads excalibur_amd/lib/libex
 loudly if that library or a gfx950 device is missing. There is no CPU fallback.
 """
 import ctypes
+import functools
+import math
 import os
 
 import numpy as np
@@ -75,14 +77,12 @@ class DevArray:
         self.ctx = ctx
         self.shape = tuple(int(s) for s in shape)
         self.dtype = np.dtype(dtype)
-        self.nbytes = int(np.prod(self.shape, dtype=np.int64)) * self.dtype.itemsize
+        self.char = self.dtype.char
+        self.size = math.prod(self.shape)
+        self.nbytes = self.size * self.dtype.itemsize
         p = ctypes.c_void_p()
         _check(lib().exhip_malloc(ctx.h, ctypes.c_size_t(self.nbytes), ctypes.byref(p)))
         self.ptr = p
-
-    @property
-    def size(self):
-        return self.nbytes // self.dtype.itemsize
 
     def upload(self, a):
         a = np.ascontiguousarray(a, self.dtype)
@@ -111,6 +111,8 @@ class DevArray:
 
 
 class _Inside:
+    char, size = "", math.inf
+
     def __init__(self, ptr):
         self.ptr = ptr
 
@@ -123,14 +125,26 @@ class View:
         self.ptr = ctypes.c_void_p(int(address))
         self.shape = tuple(int(s) for s in shape)
         self.dtype = np.dtype(dtype)
-
-    @property
-    def size(self):
-        return int(np.prod(self.shape, dtype=np.int64))
+        self.char = self.dtype.char
+        self.size = math.prod(self.shape)
 
 
 class F8Desc(ctypes.Structure):
     _fields_ = [(k, ctypes.c_int) for k in ("m", "n_out", "k_in", "x_stride", "y_stride")]
+    _counts = None
+
+    def __setattr__(self, name, value):
+        super().__setattr__(name, value)
+        if name != "_counts":
+            self._counts = None
+
+    def counts(self):
+        """How many values the products' operands have: rows, their scales, packed bytes of one projection, its scales, a bias, a result, a quantized one's
+        scales. Counted once: a call that checks its operands is made for every row of a serving program."""
+        m, n, k = self.m, self.n_out, self.k_in
+        bn, bk = _blocks(n), _blocks(k)
+        self._counts = (m - 1) * self.x_stride + k, bk * m, -(-n // 16) * bk * 2048, bn * bk, n, (m - 1) * self.y_stride + n, bn * m
+        return self._counts
 
 
 F8_BLOCK = 128  # values that share a scale
@@ -157,6 +171,34 @@ class Event:
 
 def _ptr(a):
     return a.ptr if a is not None else None
+
+
+_FLOATS, _HALVES, _ROWS, _CODES, _IDS = "f", "He", "fHe", "Bb", "i"  # numpy's characters of the types that an operand may have
+
+
+def _refused(*operands):
+    """Says which operand (its name, itself, the values that the call reads or writes, its types) is of another type or too small."""
+    for name, a, count, types in operands:
+        if a is not None and a.char not in types:
+            raise ExhipError(f"{name} is {a.dtype}, not {' or '.join(np.dtype(t).name for t in types)}")
+        if a is not None and a.size < count:
+            raise ExhipError(f"{name} has {a.size} values, the call takes {count}")
+
+
+def _holds(a, count, types):
+    """Whether an operand that is there has values of one of the types, and enough. (An address alone, DevArray.at(), says neither.)"""
+    return a is None or (a.size >= count and a.char in types)
+
+
+_MOST = 2 ** 31 - 1  # of a C int; ctypes would cut larger ones
+
+
+def _size_refused(*sizes):
+    raise ExhipError(f"{sizes}: more than a size of the library holds")
+
+
+def _blocks(v):
+    return -(-v // F8_BLOCK)
 
 
 class Ctx:
@@ -621,27 +663,39 @@ class Ctx:
     GATES = {"silu": 0, "gelu": 1, "sigmoid": 2, "relu": 3}
 
     def quantize_rows_f8(self, x, k=None, y=None, scale=None):
-        """Rows x [m][stride] (float32, or halves as uint16) of k values: (codes [m][k up to 16], scales [k blocks][m])."""
+        """Rows x [m][stride] (float32, or halves as uint16 or float16) of k values: (codes [m][k up to 16], scales [k blocks][m])."""
         m, stride = x.shape
         k = stride if k is None else k
+        if m > _MOST or stride > _MOST or k > _MOST:
+            _size_refused(m, stride, k)
         if y is None:
             y = self.empty((m, pad_to(k, 16)), np.uint8)
         if scale is None:
-            scale = self.empty((pad_to(k, F8_BLOCK) // F8_BLOCK, m), np.float32)
-        entry = lib().exhip_quantize_rows_f32_to_f8 if x.dtype == np.float32 else lib().exhip_quantize_rows_f16_to_f8
-        _check(entry(self.h, x.ptr, stride, m, k, y.ptr, y.shape[1], scale.ptr))
+            scale = self.empty((_blocks(k), m), np.float32)
+        y_stride, scales = y.shape[1], -(-k // F8_BLOCK) * m
+        if not (x.size >= (m - 1) * stride + k and x.char in _ROWS and y.size >= (m - 1) * y_stride + k and y.char in _CODES and scale.size >= scales and scale.char in _FLOATS):
+            _refused(("x", x, (m - 1) * stride + k, _ROWS), ("y", y, (m - 1) * y_stride + k, _CODES), ("scale", scale, scales, _FLOATS))
+        entry = (_lib or lib()).exhip_quantize_rows_f32_to_f8 if x.char == "f" else (_lib or lib()).exhip_quantize_rows_f16_to_f8
+        rc = entry(self.h, x.ptr, stride, m, k, y.ptr, y_stride, scale.ptr)
+        if rc:
+            _check(rc)
         return y, scale
 
     def quantize_blocks_f8(self, w):
         """A float32 weight matrix [n][k]: (codes [n][k], scales [n blocks][k blocks])."""
         n, k = w.shape
+        if n > _MOST or k > _MOST:
+            _size_refused(n, k)
+        _refused(("w", w, n * k, _FLOATS))
         y = self.empty((n, k), np.uint8)
-        scale = self.empty((pad_to(n, F8_BLOCK) // F8_BLOCK, pad_to(k, F8_BLOCK) // F8_BLOCK), np.float32)
+        scale = self.empty((_blocks(n), _blocks(k)), np.float32)
         _check(lib().exhip_quantize_blocks_f32_to_f8(self.h, w.ptr, n, k, y.ptr, scale.ptr))
         return y, scale
 
     @staticmethod
     def f8_packed_bytes(n_out, k_in, gated=False):
+        if n_out > _MOST or k_in > _MOST:
+            _size_refused(n_out, k_in)
         nbytes = lib().exhip_f8_packed_bytes(int(n_out), int(k_in), int(gated))
         if nbytes == 0:
             raise ExhipError(f"exhip_f8_packed_bytes: {lib().exhip_last_error().decode()}")
@@ -649,39 +703,76 @@ class Ctx:
 
     def pack_f8_weights(self, n_out, k_in, w, w_up=None, packed=None):
         """Codes [n_out][k_in] in the product's order; with w_up those of a gated product, w the one in front of the activation."""
+        nbytes = self.f8_packed_bytes(n_out, k_in, w_up is not None)
+        _refused(("w", w, n_out * k_in, _CODES), ("w_up", w_up, n_out * k_in, _CODES), ("packed", packed, nbytes, _CODES))
         if packed is None:
-            packed = self.empty((self.f8_packed_bytes(n_out, k_in, w_up is not None),), np.uint8)
+            packed = self.empty((nbytes,), np.uint8)
         _check(lib().exhip_f8_pack_weights(self.h, n_out, k_in, w.ptr, _ptr(w_up), packed.ptr))
         return packed
 
     @staticmethod
     def f8_desc(m, n_out, k_in, x_stride=None, y_stride=None):
-        return F8Desc(m, n_out, k_in, pad_to(k_in, 16) if x_stride is None else x_stride, n_out if y_stride is None else y_stride)
+        x_stride, y_stride = pad_to(k_in, 16) if x_stride is None else x_stride, n_out if y_stride is None else y_stride
+        if max(m, n_out, k_in, x_stride, y_stride) > _MOST:
+            _size_refused(m, n_out, k_in, x_stride, y_stride)
+        return F8Desc(m, n_out, k_in, x_stride, y_stride)
 
     def innerproduct_f8(self, d, x, x_scale, w, w_scale, bias=None, y_f32=None, y_f16=None):
-        _check(lib().exhip_innerproduct_f8(self.h, ctypes.byref(d), x.ptr, x_scale.ptr, w.ptr, w_scale.ptr, _ptr(bias), _ptr(y_f32), _ptr(y_f16)))
+        rows, scales, packed, w_scales, n, result, _ = d._counts or d.counts()
+        if not (x.size >= rows and x.char in _CODES and x_scale.size >= scales and x_scale.char in _FLOATS and w.size >= packed and w.char in _CODES
+                and w_scale.size >= w_scales and w_scale.char in _FLOATS and (bias is None or bias.size >= n and bias.char in _FLOATS)
+                and (y_f32 is None or y_f32.size >= result and y_f32.char in _FLOATS) and (y_f16 is None or y_f16.size >= result and y_f16.char in _HALVES)):
+            _refused(("x", x, rows, _CODES), ("x_scale", x_scale, scales, _FLOATS), ("w", w, packed, _CODES), ("w_scale", w_scale, w_scales, _FLOATS), ("bias", bias, n, _FLOATS),
+                     ("y_f32", y_f32, result, _FLOATS), ("y_f16", y_f16, result, _HALVES))
+        rc = (_lib or lib()).exhip_innerproduct_f8(self.h, ctypes.byref(d), x.ptr, x_scale.ptr, w.ptr, w_scale.ptr, bias and bias.ptr, y_f32 and y_f32.ptr, y_f16 and y_f16.ptr)
+        if rc:
+            _check(rc)
 
     def innerproduct_gated_f8(self, d, x, x_scale, w, w_scale_gate, w_scale_up, gate="silu", bias_gate=None, bias_up=None, y_f16=None, y_f8=None, y_scale=None):
-        _check(lib().exhip_innerproduct_gated_f8(self.h, ctypes.byref(d), self.GATES[gate], x.ptr, x_scale.ptr, w.ptr, w_scale_gate.ptr, w_scale_up.ptr,
-                                                 _ptr(bias_gate), _ptr(bias_up), _ptr(y_f16), _ptr(y_f8), _ptr(y_scale)))
+        rows, scales, packed, w_scales, n, result, result_scales = d._counts or d.counts()
+        if not (x.size >= rows and x.char in _CODES and x_scale.size >= scales and x_scale.char in _FLOATS and w.size >= 2 * packed and w.char in _CODES
+                and w_scale_gate.size >= w_scales and w_scale_gate.char in _FLOATS and w_scale_up.size >= w_scales and w_scale_up.char in _FLOATS
+                and _holds(bias_gate, n, _FLOATS) and _holds(bias_up, n, _FLOATS) and _holds(y_f16, result, _HALVES) and _holds(y_f8, result, _CODES)
+                and _holds(y_scale, result_scales, _FLOATS)):
+            _refused(("x", x, rows, _CODES), ("x_scale", x_scale, scales, _FLOATS), ("w", w, 2 * packed, _CODES), ("w_scale_gate", w_scale_gate, w_scales, _FLOATS),
+                     ("w_scale_up", w_scale_up, w_scales, _FLOATS), ("bias_gate", bias_gate, n, _FLOATS), ("bias_up", bias_up, n, _FLOATS), ("y_f16", y_f16, result, _HALVES),
+                     ("y_f8", y_f8, result, _CODES), ("y_scale", y_scale, result_scales, _FLOATS))
+        rc = (_lib or lib()).exhip_innerproduct_gated_f8(self.h, ctypes.byref(d), self.GATES[gate], x.ptr, x_scale.ptr, w.ptr, w_scale_gate.ptr, w_scale_up.ptr,
+                                                         bias_gate and bias_gate.ptr, bias_up and bias_up.ptr, y_f16 and y_f16.ptr, y_f8 and y_f8.ptr, y_scale and y_scale.ptr)
+        if rc:
+            _check(rc)
 
     # ---- answers ----
     @staticmethod
+    @functools.lru_cache(maxsize=256)
     def log_probabilities_workspace(m, c, top=0):
+        if m > _MOST or c > _MOST or top > _MOST:
+            _size_refused(m, c, top)
         nbytes = lib().exhip_log_probabilities_workspace(int(m), int(c), int(top))
         if nbytes == 0:
             raise ExhipError(f"exhip_log_probabilities_workspace: {lib().exhip_last_error().decode()}")
         return nbytes
 
     def log_probabilities(self, x, c=None, ids=None, top=0, log_p=None, entropy=None, top_ids=None, top_log_p=None, workspace=None):
-        """Of rows x [m][stride] (float32, or halves as uint16) of c values: the log probabilities of ids [m][n], the entropy, the `top` largest classes and
-        their log probabilities, into the given arrays. Without a workspace it makes one and waits for the results; a recorded run is given one."""
+        """Of rows x [m][stride] (float32, or halves as uint16 or float16) of c values: the log probabilities of ids [m][n] (int32), the entropy, the `top`
+        largest classes and their log probabilities, into the given arrays. Without a workspace it makes one and waits for the results; a recorded run is
+        given one."""
         m, stride = x.shape
         c = stride if c is None else c
-        own = self.empty((self.log_probabilities_workspace(m, c, top),), np.uint8) if workspace is None else None
-        entry = lib().exhip_log_probabilities_f32 if x.dtype == np.float32 else lib().exhip_log_probabilities_f16
-        rc = entry(self.h, x.ptr, stride, m, c, _ptr(ids), ids.shape[1] if ids is not None else 0, _ptr(log_p), _ptr(entropy), top, _ptr(top_ids),
-                   _ptr(top_log_p), (workspace or own).ptr)
+        n_ids = ids.shape[1] if ids is not None else 0
+        if stride > _MOST or n_ids > _MOST:
+            _size_refused(stride, n_ids)
+        nbytes = self.log_probabilities_workspace(m, c, top)
+        if not (_holds(x, (m - 1) * stride + c, _ROWS) and _holds(ids, m * n_ids, _IDS) and _holds(log_p, m * n_ids, _FLOATS) and _holds(entropy, m, _FLOATS)
+                and _holds(top_ids, m * top, _IDS) and _holds(top_log_p, m * top, _FLOATS)):
+            _refused(("x", x, (m - 1) * stride + c, _ROWS), ("ids", ids, m * n_ids, _IDS), ("log_p", log_p, m * n_ids, _FLOATS), ("entropy", entropy, m, _FLOATS),
+                     ("top_ids", top_ids, m * top, _IDS), ("top_log_p", top_log_p, m * top, _FLOATS))
+        if workspace is not None and not isinstance(workspace, _Inside) and workspace.size * workspace.dtype.itemsize < nbytes:
+            raise ExhipError(f"workspace has {workspace.size * workspace.dtype.itemsize} bytes, the call takes {nbytes}")
+        own = self.empty((nbytes,), np.uint8) if workspace is None else None
+        entry = lib().exhip_log_probabilities_f32 if x.char == "f" else lib().exhip_log_probabilities_f16
+        rc = entry(self.h, x.ptr, stride, m, c, _ptr(ids), n_ids, _ptr(log_p), _ptr(entropy), top, _ptr(top_ids), _ptr(top_log_p),
+                   (own if workspace is None else workspace).ptr)
         if own is not None:
             own.free()
         _check(rc)

@@ -151,3 +151,89 @@ def test_a_log_probability_workspace_holds_every_row_s_slices():
         for c in (32769, 40000, 65537, 131072, 131073, 500001):
             for top in (0, 1, 20, 64):
                 assert size(m, c, top) >= m * -(-c // 8192) * (16 + 8 * top), (m, c, top)
+
+
+# ---- the Python face: operands of another type, or too small, never reach the library ----
+def _face():
+    from excalibur_amd import hip
+    ctx = object.__new__(hip.Ctx)  # without a device: what passes the checks here is refused by the library for its missing context
+    ctx.h = None
+    return hip, ctx
+
+
+def _refused(match, call, *args, **kw):
+    hip, _ = _face()
+    with pytest.raises(hip.ExhipError, match=match):
+        call(*args, **kw)
+
+
+PASSES = "NULL argument"  # the library's first check
+OTHER_ROWS = (np.float64, np.int16, np.int32, np.uint8)
+
+
+def test_face_refuses_other_rows_for_the_quantizers():
+    hip, ctx = _face()
+    view = lambda shape, dtype: hip.View(X, shape, dtype)
+    y, scale = view((3, 112), np.uint8), view((1, 3), np.float32)
+    for dtype in (np.float32, np.float16, np.uint16):
+        _refused(PASSES, ctx.quantize_rows_f8, view((3, 100), dtype), y=y, scale=scale)
+    for dtype in OTHER_ROWS:
+        _refused("x is", ctx.quantize_rows_f8, view((3, 100), dtype), y=y, scale=scale)
+    x = view((3, 100), np.float32)
+    _refused("y is", ctx.quantize_rows_f8, x, y=view((3, 112), np.float32), scale=scale)
+    _refused("y has", ctx.quantize_rows_f8, x, y=view((2, 112), np.uint8), scale=scale)
+    _refused("scale is", ctx.quantize_rows_f8, x, y=y, scale=view((1, 3), np.float64))
+    _refused("scale has", ctx.quantize_rows_f8, x, y=y, scale=view((1, 2), np.float32))
+    _refused("x has", ctx.quantize_rows_f8, x, k=101, y=y, scale=scale)
+    _refused("w is", ctx.quantize_blocks_f8, view((3, 100), np.float16))
+    _refused("w is", ctx.pack_f8_weights, 3, 100, view((3, 100), np.float32))
+    _refused("w has", ctx.pack_f8_weights, 4, 100, view((3, 100), np.uint8))
+    _refused("w_up has", ctx.pack_f8_weights, 3, 100, view((3, 100), np.uint8), view((3, 99), np.uint8))
+    _refused("packed has", ctx.pack_f8_weights, 3, 100, view((3, 100), np.uint8), packed=view((2047,), np.uint8))
+    _refused(PASSES, ctx.pack_f8_weights, 3, 100, view((3, 100), np.uint8), packed=view((2048,), np.uint8))
+
+
+def test_face_refuses_other_operands_of_the_products():
+    hip, ctx = _face()
+    view = lambda count, dtype: hip.View(X, (count,), dtype)
+    d = ctx.f8_desc(3, 40, 100, y_stride=48)  # rows of 112 codes
+    good = dict(x=view(2 * 112 + 100, np.uint8), x_scale=view(3, np.float32), w=view(3 * 2048, np.uint8), w_scale=view(1, np.float32), bias=view(40, np.float32),
+                y_f32=view(2 * 48 + 40, np.float32), y_f16=view(2 * 48 + 40, np.float16))
+    _refused(PASSES, ctx.innerproduct_f8, d, **good)
+    _refused(PASSES, ctx.innerproduct_f8, d, **dict(good, y_f16=view(2 * 48 + 40, np.uint16)))
+    for name, a in good.items():
+        _refused(name + " has", ctx.innerproduct_f8, d, **dict(good, **{name: view(a.size - 1, a.dtype)}))
+        _refused(name + " is", ctx.innerproduct_f8, d, **dict(good, **{name: view(a.size, np.int64)}))
+    d.m = 4  # what a description says now counts
+    _refused("x has", ctx.innerproduct_f8, d, **good)
+    d.m = 3
+    gated = dict(x=good["x"], x_scale=good["x_scale"], w=view(2 * 3 * 2048, np.uint8), w_scale_gate=good["w_scale"], w_scale_up=good["w_scale"], bias_gate=good["bias"], bias_up=good["bias"])
+    for results in (dict(y_f16=view(2 * 48 + 40, np.uint16)), dict(y_f8=view(2 * 48 + 40, np.uint8), y_scale=view(3, np.float32))):
+        call = dict(gated, **results)
+        _refused(PASSES, ctx.innerproduct_gated_f8, d, **call)
+        for name, a in call.items():
+            _refused(" has", ctx.innerproduct_gated_f8, d, **dict(call, **{name: view(a.size - 1, a.dtype)}))
+            _refused(" is", ctx.innerproduct_gated_f8, d, **dict(call, **{name: view(a.size, np.int64)}))
+    _refused("more than a size of", ctx.f8_desc, 2 ** 32 + 3, 40, 100)
+    _refused("more than a size of", ctx.f8_packed_bytes, 40, 2 ** 32 + 100)
+
+
+def test_face_refuses_other_operands_of_the_log_probabilities():
+    hip, ctx = _face()
+    view = lambda shape, dtype: hip.View(X, shape, dtype)
+    m, c, top = 3, 40000, 5
+    good = dict(x=view((m, c), np.uint16), ids=view((m, 2), np.int32), log_p=view((m, 2), np.float32), entropy=view((m,), np.float32), top_ids=view((m, top), np.int32),
+                top_log_p=view((m, top), np.float32), workspace=view((ctx.log_probabilities_workspace(m, c, top),), np.uint8))
+    for dtype in (np.float32, np.float16, np.uint16):
+        _refused(PASSES, ctx.log_probabilities, top=top, **dict(good, x=view((m, c), dtype)))
+    for dtype in OTHER_ROWS:
+        _refused("x is", ctx.log_probabilities, top=top, **dict(good, x=view((m, c), dtype)))
+    _refused("ids is int64", ctx.log_probabilities, top=top, **dict(good, ids=view((m, 2), np.int64)))
+    _refused("top_ids is", ctx.log_probabilities, top=top, **dict(good, top_ids=view((m, top), np.int64)))
+    _refused("entropy is", ctx.log_probabilities, top=top, **dict(good, entropy=view((m,), np.float16)))
+    for name in ("ids", "log_p", "top_ids", "top_log_p"):
+        _refused(" has", ctx.log_probabilities, top=top, **dict(good, **{name: view((m - 1,) + good[name].shape[1:], good[name].dtype)}))
+    _refused("entropy has", ctx.log_probabilities, top=top, **dict(good, entropy=view((m - 1,), np.float32)))
+    _refused("workspace has", ctx.log_probabilities, top=top, **dict(good, workspace=view((good["workspace"].size - 1,), np.uint8)))
+    _refused(PASSES, ctx.log_probabilities, top=top, **dict(good, workspace=view((-(-good["workspace"].size // 4),), np.float32)))
+    _refused("x has", ctx.log_probabilities, c=c + 1, top=top, **good)
