@@ -717,18 +717,25 @@ class Ctx:
             _size_refused(m, n_out, k_in, x_stride, y_stride)
         return F8Desc(m, n_out, k_in, x_stride, y_stride)
 
-    def innerproduct_f8(self, d, x, x_scale, w, w_scale, bias=None, y_f32=None, y_f16=None):
+    def innerproduct_f8(self, d, x, x_scale, w, w_scale, bias=None, y_f32=None, y_f16=None, cut_sums=False):
+        """cut_sums: the faster sums that keep 13 bits beneath the largest of eight products (exhip_innerproduct_cut_f8), for results in halves alone."""
         rows, scales, packed, w_scales, n, result, _ = d._counts or d.counts()
         if not (x.size >= rows and x.char in _CODES and x_scale.size >= scales and x_scale.char in _FLOATS and w.size >= packed and w.char in _CODES
                 and w_scale.size >= w_scales and w_scale.char in _FLOATS and (bias is None or bias.size >= n and bias.char in _FLOATS)
                 and (y_f32 is None or y_f32.size >= result and y_f32.char in _FLOATS) and (y_f16 is None or y_f16.size >= result and y_f16.char in _HALVES)):
             _refused(("x", x, rows, _CODES), ("x_scale", x_scale, scales, _FLOATS), ("w", w, packed, _CODES), ("w_scale", w_scale, w_scales, _FLOATS), ("bias", bias, n, _FLOATS),
                      ("y_f32", y_f32, result, _FLOATS), ("y_f16", y_f16, result, _HALVES))
+        if cut_sums:
+            if y_f32:
+                raise ExhipError("cut sums are for results in halves alone")
+            return _check(lib().exhip_innerproduct_cut_f8(self.h, ctypes.byref(d), x.ptr, x_scale.ptr, w.ptr, w_scale.ptr, _ptr(bias), _ptr(y_f16)))
         rc = (_lib or lib()).exhip_innerproduct_f8(self.h, ctypes.byref(d), x.ptr, x_scale.ptr, w.ptr, w_scale.ptr, bias and bias.ptr, y_f32 and y_f32.ptr, y_f16 and y_f16.ptr)
         if rc:
             _check(rc)
 
-    def innerproduct_gated_f8(self, d, x, x_scale, w, w_scale_gate, w_scale_up, gate="silu", bias_gate=None, bias_up=None, y_f16=None, y_f8=None, y_scale=None):
+    def innerproduct_gated_f8(self, d, x, x_scale, w, w_scale_gate, w_scale_up, gate="silu", bias_gate=None, bias_up=None, y_f16=None, y_f8=None, y_scale=None,
+                              cut_sums=False):
+        """cut_sums: as of innerproduct_f8."""
         rows, scales, packed, w_scales, n, result, result_scales = d._counts or d.counts()
         if not (x.size >= rows and x.char in _CODES and x_scale.size >= scales and x_scale.char in _FLOATS and w.size >= 2 * packed and w.char in _CODES
                 and w_scale_gate.size >= w_scales and w_scale_gate.char in _FLOATS and w_scale_up.size >= w_scales and w_scale_up.char in _FLOATS
@@ -737,6 +744,11 @@ class Ctx:
             _refused(("x", x, rows, _CODES), ("x_scale", x_scale, scales, _FLOATS), ("w", w, 2 * packed, _CODES), ("w_scale_gate", w_scale_gate, w_scales, _FLOATS),
                      ("w_scale_up", w_scale_up, w_scales, _FLOATS), ("bias_gate", bias_gate, n, _FLOATS), ("bias_up", bias_up, n, _FLOATS), ("y_f16", y_f16, result, _HALVES),
                      ("y_f8", y_f8, result, _CODES), ("y_scale", y_scale, result_scales, _FLOATS))
+        if cut_sums:
+            if y_f8 or y_scale:
+                raise ExhipError("cut sums are for results in halves alone")
+            return _check(lib().exhip_innerproduct_gated_cut_f8(self.h, ctypes.byref(d), self.GATES[gate], x.ptr, x_scale.ptr, w.ptr, w_scale_gate.ptr, w_scale_up.ptr,
+                                                                _ptr(bias_gate), _ptr(bias_up), _ptr(y_f16)))
         rc = (_lib or lib()).exhip_innerproduct_gated_f8(self.h, ctypes.byref(d), self.GATES[gate], x.ptr, x_scale.ptr, w.ptr, w_scale_gate.ptr, w_scale_up.ptr,
                                                          bias_gate and bias_gate.ptr, bias_up and bias_up.ptr, y_f16 and y_f16.ptr, y_f8 and y_f8.ptr, y_scale and y_scale.ptr)
         if rc:

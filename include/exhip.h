@@ -78,7 +78,8 @@ const char* exhip_last_error(void);
  * that stages the input of 3x3 fp16 / int8 layers in LDS (1 by its rule, 2 to 4 its first to third form wherever it can run, 0 never; fp16 sums then run in another
  * order). "f32_tile" pins the float32 convolution's wave tile and split (0 = its rule, n = the n-th of its list;
  * sums then run in another order).
- * "f8_form" pins the kernel of the products in 8-bit floating point (0 = its rule, n = the n-th of its list for the result's type; other sums then).
+ * "f8_form" pins the kernel of the products in 8-bit floating point (0 = its rule, n = the n-th of the entry point's list for the result's type; sums
+ * then run in another order).
  * Process-wide; packed weights depend on the first three, so set them before packing. */
 int exhip_set_option(const char* name, int value);
 unsigned exhip_options_version(void); /* counts the calls above: plans made under other options are made again */
@@ -552,15 +553,18 @@ typedef struct exhip_f8_desc {
     int y_stride;       /* elements between the results' rows, at least n_out; a multiple of 16 for codes */
 } exhip_f8_desc;
 /* y[r][j] = bias[j] + sum over blocks b of x_scale[b][r] * w_scale[j / 128][b] * (the codes' products of that block), sums in float32, rounded once.
- * bias may be NULL; any non-NULL result is written, columns [0, n_out) only. Products of one row take their time from reading the weights, large
- * ones from the matrix cores. Where y_f32 is asked, the codes' products are summed exactly but for float32's roundings. Where halves alone are, sums of
- * many rows may come from the matrix core's 8-bit products, which keep 13 bits beneath the largest of eight products: 3e-5 of normal rows' results, where
- * a half's own rounding is 2e-4 of them. */
+ * bias may be NULL; any non-NULL result is written, columns [0, n_out) only. The codes' products are summed exactly but for float32's roundings, whatever
+ * the number of rows and the result's type. Products of one row take their time from reading the weights, large ones from the matrix cores. */
 int exhip_innerproduct_f8(exhip_ctx* ctx, const exhip_f8_desc* d, const uint8_t* x, const float* x_scale, const void* w_packed, const float* w_scale,
                           const float* bias, float* y_f32, uint16_t* y_f16);
+/* The same for results in halves, where sums of many rows may come from the matrix core's 8-bit products, which are up to twice as fast and keep 13 bits beneath the
+ * largest of eight neighbouring products: what is smaller is cut off. Of normal rows' results that is 3e-5, where a half's own rounding is 2e-4; where large
+ * products cancel, what they leave may be lost. Which kernel takes a call depends on its sizes, so a row may have other sums alone than among others. */
+int exhip_innerproduct_cut_f8(exhip_ctx* ctx, const exhip_f8_desc* d, const uint8_t* x, const float* x_scale, const void* w_packed, const float* w_scale,
+                              const float* bias, uint16_t* y_f16);
 /* A feed-forward block's first half, with nothing stored in between: h = act(x w_gate + bias_gate) * (x w_up + bias_up) with act(v) = v / (1 + exp(-v)),
  * v (1 + erf(v / sqrt 2)) / 2, 1 / (1 + exp(-v)) or max(v, 0). The result is h as halves (y_f16), or the codes (y_f8) and scales (y_scale, both or neither)
- * that exhip_quantize_rows_f32_to_f8 makes of h in float32; one of the two forms, summed like halves and like float32 above. Biases: both or neither. */
+ * that exhip_quantize_rows_f32_to_f8 makes of h in float32; one of the two forms. Sums are those of exhip_innerproduct_f8. Biases: both or neither. */
 #define EXHIP_GATE_SILU 0
 #define EXHIP_GATE_GELU 1
 #define EXHIP_GATE_SIGMOID 2
@@ -568,6 +572,9 @@ int exhip_innerproduct_f8(exhip_ctx* ctx, const exhip_f8_desc* d, const uint8_t*
 int exhip_innerproduct_gated_f8(exhip_ctx* ctx, const exhip_f8_desc* d, int gate, const uint8_t* x, const float* x_scale, const void* w_packed,
                                 const float* w_scale_gate, const float* w_scale_up, const float* bias_gate, const float* bias_up, uint16_t* y_f16,
                                 uint8_t* y_f8, float* y_scale);
+/* The same for results in halves, with the sums of exhip_innerproduct_cut_f8. */
+int exhip_innerproduct_gated_cut_f8(exhip_ctx* ctx, const exhip_f8_desc* d, int gate, const uint8_t* x, const float* x_scale, const void* w_packed,
+                                    const float* w_scale_gate, const float* w_scale_up, const float* bias_gate, const float* bias_up, uint16_t* y_f16);
 
 /* ---- what a classifier or a language model answers with (no counterpart in the reference; exhip_softmax_channels_f32 stores all of a row) ---- */
 /* For rows x[m][c] (row stride x_stride elements, at least c; any alignment of the element type), in one reading of them:

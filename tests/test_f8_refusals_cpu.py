@@ -153,6 +153,27 @@ def test_a_log_probability_workspace_holds_every_row_s_slices():
                 assert size(m, c, top) >= m * -(-c // 8192) * (16 + 8 * top), (m, c, top)
 
 
+def test_refusals_of_the_products_with_cut_sums():
+    entry = _lib().exhip_innerproduct_cut_f8
+    good = [X, S, W, S2, B, Y]
+    assert _status(entry, _desc(), *good) not in (0, ERR_ARG)
+    for change in BAD_DESC:
+        assert _status(entry, _desc(**change), *good) == ERR_ARG, change
+    for at, bad in ((0, None), (1, None), (2, None), (3, None), (5, None), (0, X + 8), (1, S + 1), (2, W + 8), (3, S2 + 2), (4, B + 1), (5, Y + 1)):
+        args = list(good)
+        args[at] = bad
+        assert _status(entry, _desc(), *args) == ERR_ARG, (at, bad)
+    entry = _lib().exhip_innerproduct_gated_cut_f8
+    good = [0, X, S, W, S2, S2, B, B2, Y]
+    assert _status(entry, _desc(), *good) not in (0, ERR_ARG)
+    for change in BAD_DESC:
+        assert _status(entry, _desc(**change), *good) == ERR_ARG, change
+    for at, bad in ((0, -1), (0, 4), (1, None), (2, None), (3, None), (4, None), (5, None), (6, None), (7, None), (8, None), (8, Y + 1), (7, B2 + 2)):
+        args = list(good)
+        args[at] = bad
+        assert _status(entry, _desc(), *args) == ERR_ARG, (at, bad)
+
+
 # ---- the Python face: operands of another type, or too small, never reach the library ----
 def _face():
     from excalibur_amd import hip
