@@ -363,8 +363,8 @@ __device__ __forceinline__ void write_group(const F8Params& p, v4f (&acc)[FOURS]
     }
 }
 
-// The same of a gated product, whose tiles alternate: half as many outputs. Quantized results need a whole block of them.
-template <int SIDE, int WN, int WM, int FOURS, int TM>
+// The same of a gated product, whose tiles alternate: half as many outputs. Quantized results (CODES) need a whole block of them in a group, and exact sums.
+template <int SIDE, int WN, int WM, bool CODES, int FOURS, int TM>
 __device__ __forceinline__ void write_gated_group(const F8Params& p, v4f (&acc)[FOURS][TM], int group_n, int wn, int wm, int row0, int rows, int lane, char* lds) {
     typedef Lanes<SIDE> At;
     constexpr int kResults = FOURS / 2, kOwn = kResults * At::kOfAFour, kWidth = kOwn * WN, kRows = SIDE * TM * WM, kThreads = 64 * WN * WM;
@@ -390,7 +390,8 @@ __device__ __forceinline__ void write_gated_group(const F8Params& p, v4f (&acc)[
         __syncthreads();
         store_rows<uint16_t, kWidth, kRows, kThreads>(lds, p.y_f16, p.y_stride, row0, rows, j0, p.n);
     }
-    if constexpr (kWidth == kBlk) {
+    if constexpr (CODES) {
+        static_assert(kWidth == kBlk, "a row's maximum is that of a block");
         if (!p.y_f8) return;
         float* const most = reinterpret_cast<float*>(lds);  // [wave along the outputs][row]
 #pragma unroll
@@ -559,7 +560,7 @@ __global__ __launch_bounds__(512, 2) void f8_wide_kernel(const F8Params p) {
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was staged behind the end, in front of the results' barrier
     if constexpr (!GATED) write_group<16, WN, 2, false>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
-    else write_gated_group<16, WN, 2>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
+    else write_gated_group<16, WN, 2, false>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
 }
 
 // ---- few rows, or few products ----
@@ -842,7 +843,7 @@ __global__ __launch_bounds__(256, 2) void f8_tile_kernel(const F8Params p) {
 #pragma unroll
     for (int g = 0; g < 4; ++g) add(1, TM - 1, g, last, last_up);
     if constexpr (!GATED) write_group<32, WN, 1, true>(p, acc, group_n, wn, 0, row0, rows, lane, memory);
-    else write_gated_group<32, WN, 1>(p, acc, group_n, wn, 0, row0, rows, lane, memory);
+    else write_gated_group<32, WN, 1, true>(p, acc, group_n, wn, 0, row0, rows, lane, memory);
 }
 
 // ---- a tile or two for every CU ----
@@ -983,7 +984,7 @@ __global__ __launch_bounds__(128 * WM, 2) void f8_deep_kernel(const F8Params p) 
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was staged behind the end, in front of the results' barrier
     if constexpr (!GATED) write_group<16, WN, WM, EXACT>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
-    else write_gated_group<16, WN, WM>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
+    else write_gated_group<16, WN, WM, false>(p, acc, group_n, wn, wm, row0, rows, lane, staged);
 }
 
 int blocks_of(int v) { return v / kBlk + (v % kBlk != 0); }
