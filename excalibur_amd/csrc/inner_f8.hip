@@ -520,7 +520,7 @@ __global__ __launch_bounds__(512, 2) void f8_wide_kernel(const F8Params p) {
             if (u < TN * TM) {
                 if (i == 0) {
                     if (t == TM / 2) {
-                        // the next block's rows are older than the eight loads of this block so far
+                        // The next block's rows are older than all nine loads of this block so far; the eight youngest may be on their way.
                         asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
                         __builtin_amdgcn_s_barrier();
                         asm volatile("" ::: "memory");
