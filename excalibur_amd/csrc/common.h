@@ -107,6 +107,7 @@ struct exhip_options {
     int bottleneck = 1;      // pointwise + depthwise + pointwise fp16 blocks in one kernel: 1 by its rule, 16 * rows + columns of a tile (up to 15 each) wherever it can run, + 256 with eight waves a group, 0 never
     int pw_split = 1;        // that kernel's split form (several waves to a tile): 1 by its rule, 2 wherever it can run, 0 never
     int f8_form = 0;         // the 8-bit inner products' kernel: 0 by its rule, n = the n-th of its list (the last for more)
+    int f8_front = 0;        // the rows of the first of two launches of such a product: 0 by its rule, which may also be one launch
     int pw = 1;              // 1x1 stride-1 fp16 and int8 layers with NHWC results: 1 the pointwise kernel where it measured faster, 2 wherever it can run, 0 never
 };
 extern exhip_options g_exhip_options;

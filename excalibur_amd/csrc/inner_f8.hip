@@ -1124,11 +1124,12 @@ int best_of(const Form (&forms)[N], const F8Params& p, int rows, float* us) {
 // (Quantized results stay in one: their kernels for few rows take what two launches win.)
 template <int N>
 int run_best(exhip_ctx* ctx, const F8Params& p, const Form (&forms)[N], bool in_two = true) {
-    const int pinned = g_exhip_options.f8_form;
-    if (pinned > 0) return forms[(pinned < N ? pinned : N) - 1].run(ctx, p);
+    const int pinned = g_exhip_options.f8_form, pinned_front = g_exhip_options.f8_front;
     float us = 0.f;
-    int best = best_of(forms, p, p.m, &us), behind = 0, rows = p.m;
-    if (in_two && us > 12.f) {
+    int best = best_of(forms, p, p.m, &us), behind = best, rows = p.m;
+    if (pinned > 0) best = behind = (pinned < N ? pinned : N) - 1;
+    if (pinned_front > 0) rows = pinned_front < p.m ? pinned_front : p.m;
+    if (in_two && us > 12.f && pinned <= 0 && pinned_front <= 0) {
         us = us * 0.97f - 3.f;
         for (int i = 0; i < N; ++i) {
             const Form& f = forms[i];

@@ -46,6 +46,7 @@ extern "C" int exhip_set_option(const char* name, int value) {
     else if (!strcmp(name, "bottleneck")) o.bottleneck = value;
     else if (!strcmp(name, "f32_tile")) o.f32_tile = value;
     else if (!strcmp(name, "f8_form")) o.f8_form = value;
+    else if (!strcmp(name, "f8_front")) o.f8_front = value;
     else if (!strcmp(name, "lean_f16")) o.lean_f16 = value;
     else if (!strcmp(name, "lean_groups")) o.lean_groups = value;
     else if (!strcmp(name, "lean_wres")) o.lean_wres = value;

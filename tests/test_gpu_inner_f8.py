@@ -456,6 +456,45 @@ def test_last_rows_by_a_launch_of_their_own(ctx, what, m, n, k):
     _near((got if what == "f32" else got.view(np.float16))[some, :n], want, bound)
 
 
+@pytest.fixture
+def front(pin):
+    from excalibur_amd import hip
+    yield lambda rows: hip.set_option("f8_front", rows)
+    hip.set_option("f8_front", 0)
+
+
+@pytest.mark.parametrize("m,n,k,rows", [(5, 130, 129, 1), (97, 300, 260, 40), (300, 257, 1000, 129), (300, 140, 203, 299), (40, 64, 300, 40)])
+def test_every_form_in_two_launches(ctx, pin, front, m, n, k, rows):
+    """The first rows in a launch and the others in one: the results of one launch, whatever row the second begins with (a kernel's sums of a row do not depend on
+    where it stands)."""
+    o = Operands(ctx, np.random.default_rng(m + n + k), m, n, k, sides=2, bias=True, pad=16)
+    args, single = (o.dx, o.dx_scale, o.packed), ctx.pack_f8_weights(n, k, ctx.array(o.w[0]))
+    stride, blocks = (n + 15) // 16 * 16 + 16, f8ref.blocks(n)
+
+    def calls():
+        out = []
+        for kw in (dict(y_f32=ctx.array(np.full((m + 1, n + 3), 7.25, np.float32))), dict(y_f16=ctx.array(np.full((m + 1, n + 3), 0x4567, np.uint16))),
+                   dict(y_f16=ctx.array(np.full((m + 1, n + 3), 0x4567, np.uint16)), cut_sums=True)):
+            ctx.innerproduct_f8(o.desc(ctx, n + 3), *args[:2], single, o.dw_scale[0], o.dbias[0], **kw)
+            out += [a.download() for a in kw.values() if a is not True]
+        for kw in (dict(y_f16=ctx.array(np.full((m + 1, n + 3), 0x4567, np.uint16))), dict(y_f16=ctx.array(np.full((m + 1, n + 3), 0x4567, np.uint16)), cut_sums=True)):
+            ctx.innerproduct_gated_f8(o.desc(ctx, n + 3), *args, *o.dw_scale, "gelu", *o.dbias, **kw)
+            out += [a.download() for a in kw.values() if a is not True]
+        codes, scale = ctx.array(np.full((m + 1, stride), 0xA5, np.uint8)), ctx.array(np.full((blocks + 1, m), 7.25, np.float32))
+        ctx.innerproduct_gated_f8(o.desc(ctx, stride), *args, *o.dw_scale, "gelu", *o.dbias, y_f8=codes, y_scale=scale)
+        return out + [codes.download(), scale.download()]
+
+    for form in range(1, 8):
+        pin(form)
+        front(0)
+        one = calls()
+        front(rows)
+        for i, (a, b) in enumerate(zip(one, calls())):
+            assert np.array_equal(a, b), (form, i)
+    pin(0)
+    calls()  # the rule's kernels for both
+
+
 # ---- what sums keep ----
 def _cancelling(rng, rows, k):
     """(values, the same with the large ones of every other group of eight negated): one of 448 in each of an even number of groups of eight of a block of
