@@ -185,8 +185,9 @@ __device__ __forceinline__ float log_p_of(float v, const Sums& r, float log_s) {
 template <typename T>
 __device__ __forceinline__ void write_row(const T* __restrict__ src, const LogpParams& p, size_t row, const Sums& r, const u64* places) {
     const int lane = threadIdx.x % 64;
-    const float log_s = __builtin_amdgcn_logf(r.s) * kLn2;
-    if (lane == 0 && p.entropy) p.entropy[row] = r.s != r.s ? r.s : r.most == -INFINITY ? 0.f : log_s - r.t / r.s * kLn2;
+    // The largest has a part of one in s, and none in t has another sign: what rounding leaves below one, or below an entropy of zero, is not there.
+    const float log_s = r.s < 1.f ? 0.f : __builtin_amdgcn_logf(r.s) * kLn2;
+    if (lane == 0 && p.entropy) p.entropy[row] = r.s != r.s ? r.s : r.most == -INFINITY ? 0.f : fmaxf(log_s - r.t / r.s * kLn2, 0.f);
     for (int i = lane; i < p.n_ids; i += 64) {
         const int id = p.ids[row * p.n_ids + i];
         p.log_p[row * p.n_ids + i] = id < 0 ? 0.f : id >= p.c ? NAN : log_p_of(as_float(src[id]), r, log_s);

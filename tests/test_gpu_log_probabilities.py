@@ -277,3 +277,18 @@ def test_one_workspace_for_smaller_calls(ctx, m, c, top):
             a.free()
     dx.free()
     d_ids.free()
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("c", [1, 40, 3000, 40000])
+def test_no_probability_above_one(ctx, c, dtype):
+    """Rows that are sure of one class, at values all over the type's range: log probabilities are not above 0 and entropies not below, whatever is rounded."""
+    rng = np.random.default_rng(c)
+    m = 3000 if c <= 40 else 60
+    sure = rng.uniform(-6e4, 6e4, m)
+    x = np.full((m, c), -np.inf, dtype)
+    x[:, 1::2] = (sure[:, None] - rng.uniform(0, 40, (m, c // 2))).astype(dtype)
+    at = rng.integers(0, c, m)
+    x[np.arange(m), at] = sure
+    out = _run(ctx, x, at[:, None], top=1)
+    assert np.all(out["log_p"] <= 0) and np.all(out["top_log_p"] <= 0) and np.all(out["entropy"] >= 0)
