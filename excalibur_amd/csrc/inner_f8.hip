@@ -849,11 +849,12 @@ __global__ __launch_bounds__(256, 2) void f8_tile_kernel(const F8Params p) {
 // ---- a tile or two for every CU ----
 // Between the two: a group of 2 x WM waves takes 32 WM outputs and 32 WM rows, a wave 16 WM x 32, and both operands' codes come straight into LDS, three blocks
 // ahead in four buffers, so that a CU with one group does not wait for memory block by block. WM = 4 takes all the LDS that a CU has. What bounds it is what a CU
-// draws from L2, some 27 bytes a cycle: where 128 x 128 leaves CUs without a group, 64 x 64 (WM = 2, two groups a CU) has the others draw too: 128 x 8192 x 8192 in
-// 20 us (32), 256 x 4096 x 4096 in 12 (18), 64 rows of the gated 8192 x 4096 in 15 (21); 1024 x 4096 x 4096 in 23 us with WM = 4.
+// draws from L2, some 27 bytes a cycle: where 128 x 128 leaves CUs without a group, 64 x 64 (WM = 2, two groups a CU) has the others draw too: 128 x 8192 x 8192 with
+// cut sums in 20 us (32), 256 x 4096 x 4096 in 12 (18), 64 rows of the gated 8192 x 4096 in 15 (21); 1024 x 4096 x 4096 in 23 us with WM = 4.
 // (2 x 2 waves of 64 x 64, one for each SIMD, take longer than 2 x 4: 330 instructions a block, of which a wave alone issues one in 4.5 cycles.)
 // EXACT converts each wave's codes to halves, 64 conversions beside 16 products a block: 512 x 4096 x 4096 in float32 takes 25 us, 33 on the larger tiles of
-// f8_tile_kernel and 35 on f8_rows_kernel's, 64 x 32000 x 4096 27 (35, 45), 1024 x 4096 x 4096 47 (39).
+// f8_tile_kernel and 35 on f8_rows_kernel's, 64 x 32000 x 4096 27 (35, 45), 1024 x 4096 x 4096 47 (39); 128 rows of the gated
+// 8192 x 4096 in halves 27 (37, 48).
 template <int WM, bool GATED, bool EXACT>
 __global__ __launch_bounds__(128 * WM, 2) void f8_deep_kernel(const F8Params p) {
     exhip_touch_args(p);
@@ -1068,8 +1069,8 @@ template <bool GATED>
 int run_wide(exhip_ctx* ctx, const F8Params& p) {
     return launch(ctx, f8_wide_kernel<GATED>, p, 16, 256, 512);
 }
-// The times are fits to 3500 launches of 1 to 2048 rows and matrices from 256 x 512 to 8192 x 8192 and 32000 x 4096, on the GPU's clock: the form they choose takes
-// 0.3 % longer than the best one for the shape on average, 9 % at most. (The exact gated forms' are fits to 90 launches of 1 to 2048 rows and six matrices: 0.8 % and 13 %.)
+// The times are fits to launches of 1 to 2048 rows and matrices from 256 x 512 to 8192 x 8192 and 32000 x 4096, on the GPU's clock. Over 94 to 96 shapes a list the
+// launch that they choose takes 0.1 to 0.7 % longer than the best form on average, 12 % at most (profiles/inner_f8_forms.txt).
 constexpr Form kExact[] = {  // results in float32 or halves
     {run_rows<1, 1, 1, 8, 4, false>, 1, 16, 2, 8, 1.5f, 1.9f, 0.97f, 0.58f, true}, {run_rows<2, 1, 1, 8, 2, false>, 2, 16, 2, 8, 0.3f, 3.1f, 1.74f, 0.64f, true},
     {run_rows<2, 2, 1, 8, 2, false>, 2, 32, 1, 8, 1.7f, 1.5f, 1.37f, 0.f, true},   {run_rows<4, 2, 1, 8, 1, false>, 4, 32, 1, 8, 1.0f, 2.5f, 1.80f, 0.f, true},
@@ -1120,7 +1121,8 @@ int best_of(const Form (&forms)[N], const F8Params& p, int rows, float* us) {
 }
 
 // One launch, or two where the last rows would have a few CUs work while the others are done, and a kernel of smaller tiles takes them: 3 us, less than nothing
-// for short launches, then 20 % and more for some shapes (1657 x 2920 x 5785 in halves 60 -> 48 us, 2711 x 3052 x 2961 in float32 68 -> 56).
+// for short launches, then 20 % and more for some shapes (1657 x 2920 x 5785 with cut sums 60 -> 48 us, 2711 x 3052 x 2961 in float32 68 -> 56). Over 60 shapes of a list
+// for which two are chosen, one launch takes 10 to 17 % longer on average; where the choice is wrong it costs 9 % at most.
 // (Quantized results stay in one: their kernels for few rows take what two launches win.)
 template <int N>
 int run_best(exhip_ctx* ctx, const F8Params& p, const Form (&forms)[N], bool in_two = true) {

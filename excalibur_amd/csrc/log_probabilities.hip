@@ -331,8 +331,8 @@ __global__ __launch_bounds__(64 * W, 8) void log_probabilities_kernel(const T* _
         const bool many = least == INFINITY || n > kCandidates;  // a NaN (or a +infinity, whose exponential is one), or values close to each other
         if (many) {
             // The bound is raised by halves until between `want` and kRanked values reach it; where more are alike (all of a slice, if its classes are masked
-            // with the type's lowest value), as many of these as come first. (300 rows of 100003 equal halves: 71 us with the 8 largest, 156 with 64; a reading of the
-            // slice for each of the largest took 187 and 1375.)
+            // with the type's lowest value), as many of these as come first. (300 rows of 100003 equal halves: 75 us with the 8 largest, 117 with 64, of NaN, which the bound
+            // reaches last, 404 and 447; a reading of the slice for each of the largest took 187 and 1375.)
             const int want = min(p.top, len);
             int turn = 0;
             const unsigned of_sets[2] = {order_of(sets[lane]), order_of(sets[64 + lane])};
