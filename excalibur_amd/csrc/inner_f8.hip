@@ -1070,7 +1070,7 @@ int run_wide(exhip_ctx* ctx, const F8Params& p) {
     return launch(ctx, f8_wide_kernel<GATED>, p, 16, 256, 512);
 }
 // The times are fits to launches of 1 to 2048 rows and matrices from 256 x 512 to 8192 x 8192 and 32000 x 4096, on the GPU's clock. Over 94 to 96 shapes a list the
-// launch that they choose takes 0.1 to 0.7 % longer than the best form on average, 12 % at most (profiles/inner_f8_forms.txt).
+// launch that they choose takes up to 0.7 % longer than the best form on average, 12 % at most (profiles/inner_f8_forms.txt).
 constexpr Form kExact[] = {  // results in float32 or halves
     {run_rows<1, 1, 1, 8, 4, false>, 1, 16, 2, 8, 1.5f, 1.9f, 0.97f, 0.58f, true}, {run_rows<2, 1, 1, 8, 2, false>, 2, 16, 2, 8, 0.3f, 3.1f, 1.74f, 0.64f, true},
     {run_rows<2, 2, 1, 8, 2, false>, 2, 32, 1, 8, 1.7f, 1.5f, 1.37f, 0.f, true},   {run_rows<4, 2, 1, 8, 1, false>, 4, 32, 1, 8, 1.0f, 2.5f, 1.80f, 0.f, true},
@@ -1122,7 +1122,7 @@ int best_of(const Form (&forms)[N], const F8Params& p, int rows, float* us) {
 
 // One launch, or two where the last rows would have a few CUs work while the others are done, and a kernel of smaller tiles takes them: 3 us, less than nothing
 // for short launches, then 20 % and more for some shapes (1657 x 2920 x 5785 with cut sums 60 -> 48 us, 2711 x 3052 x 2961 in float32 68 -> 56). Over 60 shapes of a list
-// for which two are chosen, one launch takes 10 to 17 % longer on average; where the choice is wrong it costs 9 % at most.
+// for which two are chosen, one launch takes 10 to 18 % longer on average; where the choice is wrong it costs 9 % at most.
 // (Quantized results stay in one: their kernels for few rows take what two launches win.)
 template <int N>
 int run_best(exhip_ctx* ctx, const F8Params& p, const Form (&forms)[N], bool in_two = true) {
