@@ -77,7 +77,7 @@ class DevArray:
         self.ctx = ctx
         self.shape = tuple(int(s) for s in shape)
         self.dtype = np.dtype(dtype)
-        self.char = self.dtype.char
+        self.char = self.dtype.char if self.dtype.isnative else self.dtype.str
         self.size = math.prod(self.shape)
         self.nbytes = self.size * self.dtype.itemsize
         p = ctypes.c_void_p()
@@ -125,7 +125,7 @@ class View:
         self.ptr = ctypes.c_void_p(int(address))
         self.shape = tuple(int(s) for s in shape)
         self.dtype = np.dtype(dtype)
-        self.char = self.dtype.char
+        self.char = self.dtype.char if self.dtype.isnative else self.dtype.str
         self.size = math.prod(self.shape)
 
 

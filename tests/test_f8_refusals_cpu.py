@@ -189,7 +189,7 @@ def _refused(match, call, *args, **kw):
 
 
 PASSES = "NULL argument"  # the library's first check
-OTHER_ROWS = (np.float64, np.int16, np.int32, np.uint8)
+OTHER_ROWS = (np.float64, np.int16, np.int32, np.uint8, np.dtype(">f4"), np.dtype(">f2"))
 
 
 def test_face_refuses_other_rows_for_the_quantizers():
