@@ -48,6 +48,7 @@ def lib():
         L.exhip_host_free.restype = None
         L.exhip_host_free.argtypes = [ctypes.c_void_p]
         L.exhip_f8_packed_bytes.restype = ctypes.c_size_t
+        L.exhip_i8_packed_bytes.restype = ctypes.c_size_t
         L.exhip_log_probabilities_workspace.restype = ctypes.c_size_t
         _lib = L
     return _lib
@@ -145,6 +146,10 @@ class F8Desc(ctypes.Structure):
         bn, bk = _blocks(n), _blocks(k)
         self._counts = (m - 1) * self.x_stride + k, bk * m, -(-n // 16) * bk * 2048, bn * bk, n, (m - 1) * self.y_stride + n, bn * m
         return self._counts
+
+
+class I8Desc(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_int) for k in ("m", "n_out", "k_in", "x_stride", "y_stride")]
 
 
 F8_BLOCK = 128  # values that share a scale
@@ -751,6 +756,131 @@ class Ctx:
                                                                 _ptr(bias_gate), _ptr(bias_up), _ptr(y_f16)))
         rc = (_lib or lib()).exhip_innerproduct_gated_f8(self.h, ctypes.byref(d), self.GATES[gate], x.ptr, x_scale.ptr, w.ptr, w_scale_gate.ptr, w_scale_up.ptr,
                                                          bias_gate and bias_gate.ptr, bias_up and bias_up.ptr, y_f16 and y_f16.ptr, y_f8 and y_f8.ptr, y_scale and y_scale.ptr)
+        if rc:
+            _check(rc)
+
+    # ---- inner products in 8-bit integers ----
+    def quantize_rows_i8(self, x, k=None, y=None, scale=None):
+        """Rows x [m][stride] (float32, or halves as uint16 or float16) of k values: (codes [m][k up to 16], scales [m])."""
+        m, stride = x.shape
+        k = stride if k is None else k
+        if m > _MOST or stride > _MOST or k > _MOST:
+            _size_refused(m, stride, k)
+        if y is None:
+            y = self.empty((m, pad_to(k, 16)), np.int8)
+        if scale is None:
+            scale = self.empty((m,), np.float32)
+        y_stride = y.shape[1]
+        if not (_holds(x, (m - 1) * stride + k, _ROWS) and _holds(y, (m - 1) * y_stride + k, _CODES) and _holds(scale, m, _FLOATS)):
+            _refused(("x", x, (m - 1) * stride + k, _ROWS), ("y", y, (m - 1) * y_stride + k, _CODES), ("scale", scale, m, _FLOATS))
+        entry = (_lib or lib()).exhip_quantize_rows_f32_to_i8 if x.char == "f" else (_lib or lib()).exhip_quantize_rows_f16_to_i8
+        rc = entry(self.h, x.ptr, stride, m, k, y.ptr, y_stride, scale.ptr)
+        if rc:
+            _check(rc)
+        return y, scale
+
+    @staticmethod
+    @functools.lru_cache(maxsize=256)
+    def i8_packed_bytes(n_out, k_in, gated=False, experts=1):
+        if n_out > _MOST or k_in > _MOST or experts > _MOST:
+            _size_refused(n_out, k_in, experts)
+        nbytes = lib().exhip_i8_packed_bytes(int(experts), int(n_out), int(k_in), int(gated))
+        if nbytes == 0:
+            raise ExhipError(f"exhip_i8_packed_bytes: {lib().exhip_last_error().decode()}")
+        return nbytes
+
+    def pack_i8_weights(self, n_out, k_in, w, w_up=None, packed=None, experts=1):
+        """Codes [experts][n_out][k_in] in the products' order; with w_up those of a gated product, w the one in front of the activation."""
+        nbytes, count = self.i8_packed_bytes(n_out, k_in, w_up is not None, experts), experts * n_out * k_in
+        _refused(("w", w, count, _CODES), ("w_up", w_up, count, _CODES), ("packed", packed, nbytes, _CODES))
+        if packed is None:
+            packed = self.empty((nbytes,), np.uint8)
+        _check(lib().exhip_i8_pack_weights(self.h, experts, n_out, k_in, w.ptr, _ptr(w_up), packed.ptr))
+        return packed
+
+    @staticmethod
+    def i8_desc(m, n_out, k_in, x_stride=None, y_stride=None):
+        x_stride, y_stride = pad_to(k_in, 16) if x_stride is None else x_stride, n_out if y_stride is None else y_stride
+        if max(m, n_out, k_in, x_stride, y_stride) > _MOST:
+            _size_refused(m, n_out, k_in, x_stride, y_stride)
+        return I8Desc(m, n_out, k_in, x_stride, y_stride)
+
+    def _check_i8(self, d, experts, gated, x_rows, offsets, rows, x, x_scale, w, w_scale, w_scale_up, bias, bias_up, y_f32, y_f16):
+        """Operands of the products in 8-bit integers: their types, and that they hold what the call reads and writes."""
+        m, n, k = d.m, d.n_out, d.k_in
+        source = m if rows is None else x_rows
+        codes, packed, result, outputs = (source - 1) * d.x_stride + k, self.i8_packed_bytes(n, k, gated, experts), (m - 1) * d.y_stride + n, experts * n
+        if not (_holds(x, codes, _CODES) and _holds(x_scale, source, _FLOATS) and _holds(w, packed, _CODES) and _holds(w_scale, outputs, _FLOATS)
+                and _holds(w_scale_up, outputs, _FLOATS) and _holds(bias, outputs, _FLOATS) and _holds(bias_up, outputs, _FLOATS) and _holds(y_f32, result, _FLOATS)
+                and _holds(y_f16, result, _HALVES) and _holds(offsets, experts + 1, _IDS) and _holds(rows, m, _IDS)):
+            scale, b = ("w_scale_gate", "bias_gate") if gated else ("w_scale", "bias")
+            _refused(("x", x, codes, _CODES), ("x_scale", x_scale, source, _FLOATS), ("w", w, packed, _CODES), (scale, w_scale, outputs, _FLOATS),
+                     ("w_scale_up", w_scale_up, outputs, _FLOATS), (b, bias, outputs, _FLOATS), ("bias_up", bias_up, outputs, _FLOATS), ("y_f32", y_f32, result, _FLOATS),
+                     ("y_f16", y_f16, result, _HALVES), ("offsets", offsets, experts + 1, _IDS), ("rows", rows, m, _IDS))
+
+    def innerproduct_i8(self, d, x, x_scale, w, w_scale, bias=None, y_f32=None, y_f16=None):
+        self._check_i8(d, 1, False, 0, None, None, x, x_scale, w, w_scale, None, bias, None, y_f32, y_f16)
+        rc = (_lib or lib()).exhip_innerproduct_i8(self.h, ctypes.byref(d), x.ptr, x_scale.ptr, w.ptr, w_scale.ptr, _ptr(bias), _ptr(y_f32), _ptr(y_f16))
+        if rc:
+            _check(rc)
+
+    def innerproduct_gated_i8(self, d, x, x_scale, w, w_scale_gate, w_scale_up, gate="silu", bias_gate=None, bias_up=None, y_f32=None, y_f16=None):
+        self._check_i8(d, 1, True, 0, None, None, x, x_scale, w, w_scale_gate, w_scale_up, bias_gate, bias_up, y_f32, y_f16)
+        rc = (_lib or lib()).exhip_innerproduct_gated_i8(self.h, ctypes.byref(d), self.GATES[gate], x.ptr, x_scale.ptr, w.ptr, w_scale_gate.ptr, w_scale_up.ptr,
+                                                         _ptr(bias_gate), _ptr(bias_up), _ptr(y_f32), _ptr(y_f16))
+        if rc:
+            _check(rc)
+
+    # ---- by experts ----
+    WEIGHTS = {"plain": 0, "log": 1, "log_normalized": 2}
+
+    def group_rows(self, ids, experts, offsets=None, rows=None, places=None):
+        """The choices ids [m][each] (int32) in order by expert: (offsets [experts + 1], rows [m * each], places [m][each])."""
+        m, each = ids.shape
+        if m > _MOST or each > _MOST or experts > _MOST:
+            _size_refused(m, each, experts)
+        offsets = self.empty((experts + 1,), np.int32) if offsets is None else offsets
+        rows = self.empty((m * each,), np.int32) if rows is None else rows
+        places = self.empty((m, each), np.int32) if places is None else places
+        if not (_holds(ids, m * each, _IDS) and _holds(offsets, experts + 1, _IDS) and _holds(rows, m * each, _IDS) and _holds(places, m * each, _IDS)):
+            _refused(("ids", ids, m * each, _IDS), ("offsets", offsets, experts + 1, _IDS), ("rows", rows, m * each, _IDS), ("places", places, m * each, _IDS))
+        rc = (_lib or lib()).exhip_group_rows(self.h, ids.ptr, m, each, experts, offsets.ptr, rows.ptr, places.ptr)
+        if rc:
+            _check(rc)
+        return offsets, rows, places
+
+    def innerproduct_grouped_i8(self, d, experts, offsets, x, x_scale, w, w_scale, bias=None, rows=None, x_rows=0, y_f32=None, y_f16=None):
+        """d.m rows in order by expert; with `rows` they are those of the x_rows rows of x."""
+        self._check_i8(d, experts, False, x_rows, offsets, rows, x, x_scale, w, w_scale, None, bias, None, y_f32, y_f16)
+        rc = (_lib or lib()).exhip_innerproduct_grouped_i8(self.h, ctypes.byref(d), experts, offsets.ptr, _ptr(rows), x_rows, x.ptr, x_scale.ptr, w.ptr, w_scale.ptr,
+                                                           _ptr(bias), _ptr(y_f32), _ptr(y_f16))
+        if rc:
+            _check(rc)
+
+    def innerproduct_grouped_gated_i8(self, d, experts, offsets, x, x_scale, w, w_scale_gate, w_scale_up, gate="silu", bias_gate=None, bias_up=None, rows=None, x_rows=0,
+                                      y_f32=None, y_f16=None):
+        """d.m rows in order by expert; with `rows` they are those of the x_rows rows of x."""
+        self._check_i8(d, experts, True, x_rows, offsets, rows, x, x_scale, w, w_scale_gate, w_scale_up, bias_gate, bias_up, y_f32, y_f16)
+        rc = (_lib or lib()).exhip_innerproduct_grouped_gated_i8(self.h, ctypes.byref(d), self.GATES[gate], experts, offsets.ptr, _ptr(rows), x_rows, x.ptr, x_scale.ptr, w.ptr,
+                                                                 w_scale_gate.ptr, w_scale_up.ptr, _ptr(bias_gate), _ptr(bias_up), _ptr(y_f32), _ptr(y_f16))
+        if rc:
+            _check(rc)
+
+    def combine_rows(self, z, places, weights, n=None, kind="plain", y_f32=None, y_f16=None):
+        """For each row of places [m][each] the weighted sum of those rows of the halves z [rows][stride] of n values, into y_f32 or y_f16 [m][stride]."""
+        (m, each), (z_rows, z_stride) = places.shape, z.shape
+        n = z_stride if n is None else n
+        if (y_f32 is None) == (y_f16 is None):
+            raise ExhipError("one result: y_f32 or y_f16")
+        y = y_f16 if y_f32 is None else y_f32
+        y_stride = y.shape[1] if len(y.shape) > 1 else n
+        if max(m, each, z_rows, z_stride, n, y_stride) > _MOST:
+            _size_refused(m, each, z_rows, z_stride, n, y_stride)
+        source, result, types = (z_rows - 1) * z_stride + n, (m - 1) * y_stride + n, _FLOATS if y_f16 is None else _HALVES
+        if not (_holds(z, source, _HALVES) and _holds(places, m * each, _IDS) and _holds(weights, m * each, _FLOATS) and _holds(y, result, types)):
+            _refused(("z", z, source, _HALVES), ("places", places, m * each, _IDS), ("weights", weights, m * each, _FLOATS), ("y_f32" if y_f16 is None else "y_f16", y, result, types))
+        entry = (_lib or lib()).exhip_combine_rows_f32 if y_f16 is None else (_lib or lib()).exhip_combine_rows_f16
+        rc = entry(self.h, z.ptr, z_stride, z_rows, places.ptr, weights.ptr, self.WEIGHTS[kind], m, each, n, y.ptr, y_stride)
         if rc:
             _check(rc)
 

@@ -578,6 +578,56 @@ int exhip_innerproduct_gated_f8(exhip_ctx* ctx, const exhip_f8_desc* d, int gate
 int exhip_innerproduct_gated_cut_f8(exhip_ctx* ctx, const exhip_f8_desc* d, int gate, const uint8_t* x, const float* x_scale, const void* w_packed,
                                     const float* w_scale_gate, const float* w_scale_up, const float* bias_gate, const float* bias_up, uint16_t* y_f16);
 
+/* ---- inner products in 8-bit integers, alone and by experts (no counterpart in the reference) ---- */
+/* Operands are codes from -128 to 127 with float32 scales, one for each row of the input and one for each output of the weights: a code stands for its value times
+ * its row's (its output's) scale. Codes' rows begin on 16 bytes (base and stride); what lies between a row's end and its stride is neither used nor written.
+ * Results may not overlap operands.
+ * Rows x[m][k] (row stride x_stride elements, at least k; any alignment of the element type) to codes y (row stride y_stride bytes) and scales [m]:
+ * scale = max(max |x| / 127, 2^-100), code = the whole number nearest to x / scale, ties to the even one. A row with a NaN or an infinity has codes 0 and
+ * the scale NaN, so that all its results are NaN. A weight matrix w[n][k], row by row, is quantized by the same call. */
+int exhip_quantize_rows_f32_to_i8(exhip_ctx* ctx, const float* x, int x_stride, int m, int k, int8_t* y, int y_stride, float* scale);
+int exhip_quantize_rows_f16_to_i8(exhip_ctx* ctx, const uint16_t* x, int x_stride, int m, int k, int8_t* y, int y_stride, float* scale);
+/* Codes w[experts][n_out][k_in] (dense; experts = 1 for a product without) in the order the products read them, made on the device: exhip_i8_packed_bytes() bytes
+ * (0 for sizes that are refused) at `packed`, on 16 bytes. With w_up both projections of a gated product, w the one that goes through the activation; `gated`
+ * tells the size. */
+size_t exhip_i8_packed_bytes(int experts, int n_out, int k_in, int gated);
+int exhip_i8_pack_weights(exhip_ctx* ctx, int experts, int n_out, int k_in, const int8_t* w, const int8_t* w_up, void* packed);
+typedef struct exhip_i8_desc {
+    int m, n_out, k_in; /* rows, outputs, inputs of a row (at most 131071: their sums fit 32 bits) */
+    int x_stride;       /* bytes between the input's rows, at least k_in, a multiple of 16 */
+    int y_stride;       /* elements between the results' rows, at least n_out */
+} exhip_i8_desc;
+/* y[r][j] = (float(sum of the codes' products) * x_scale[r]) * w_scale[j] + bias[j], the last two steps in one multiply-add; the sum is exact, so a row has the same
+ * result alone as among others. bias may be NULL; any non-NULL result is written, halves rounded once from the float32 value, columns [0, n_out) only. */
+int exhip_innerproduct_i8(exhip_ctx* ctx, const exhip_i8_desc* d, const int8_t* x, const float* x_scale, const void* w_packed, const float* w_scale, const float* bias,
+                          float* y_f32, uint16_t* y_f16);
+/* A feed-forward block's first half, with nothing stored in between: h = act(x w_gate + bias_gate) * (x w_up + bias_up), activations as of
+ * exhip_innerproduct_gated_f8, each side as above and the rest in float32. Biases: both or neither. */
+int exhip_innerproduct_gated_i8(exhip_ctx* ctx, const exhip_i8_desc* d, int gate, const int8_t* x, const float* x_scale, const void* w_packed, const float* w_scale_gate,
+                                const float* w_scale_up, const float* bias_gate, const float* bias_up, float* y_f32, uint16_t* y_f16);
+/* The choices ids[m][each] (each at most 64, of at most 1024 experts; at most 2^28 choices) put in order by expert, and within one by row: expert e's are those from offsets[e] to
+ * offsets[e + 1] (offsets[experts + 1], from 0), rows[i] is the row of the i-th, places[m][each] where each choice stands. An id below 0 or from `experts` on chooses nothing:
+ * its place is -1, and as many of the last rows[m * each] are -1. */
+int exhip_group_rows(exhip_ctx* ctx, const int32_t* ids, int m, int each, int experts, int32_t* offsets, int32_t* rows, int32_t* places);
+/* The two products by experts, for d->m rows in order by expert as exhip_group_rows leaves them: rows i from offsets[e] to offsets[e + 1] (device memory; rising, between 0 and
+ * d->m) have expert e's weights, scales w_scale[experts][n_out] and biases. The i-th row of the input is x's and x_scale's rows[i] of x_rows (x_rows * x_stride below 2^31),
+ * or its i-th where rows is NULL (x_rows is not used then); one that x does not have gives NaN. Result rows before the first expert's and behind the last's stay as they are. */
+int exhip_innerproduct_grouped_i8(exhip_ctx* ctx, const exhip_i8_desc* d, int experts, const int32_t* offsets, const int32_t* rows, int x_rows, const int8_t* x,
+                                  const float* x_scale, const void* w_packed, const float* w_scale, const float* bias, float* y_f32, uint16_t* y_f16);
+int exhip_innerproduct_grouped_gated_i8(exhip_ctx* ctx, const exhip_i8_desc* d, int gate, int experts, const int32_t* offsets, const int32_t* rows, int x_rows,
+                                        const int8_t* x, const float* x_scale, const void* w_packed, const float* w_scale_gate, const float* w_scale_up,
+                                        const float* bias_gate, const float* bias_up, float* y_f32, uint16_t* y_f16);
+/* What the experts of each row answered, added up: y[r] = sum over its choices, in their order, of weight * z[places[r][choice]] (halves z[z_rows][n], row stride z_stride;
+ * y's row stride y_stride, both in elements and at least n), sums in float32. A place below 0 adds nothing, one from z_rows on gives NaN. weights[m][each] are taken as they are,
+ * as logarithms, or as logarithms of weights that are divided by their sum over all of the row's choices; where all of these are -infinity the row is 0. */
+#define EXHIP_WEIGHTS_PLAIN 0
+#define EXHIP_WEIGHTS_LOG 1
+#define EXHIP_WEIGHTS_LOG_NORMALIZED 2
+int exhip_combine_rows_f32(exhip_ctx* ctx, const uint16_t* z, int z_stride, int z_rows, const int32_t* places, const float* weights, int kind, int m, int each, int n,
+                           float* y, int y_stride);
+int exhip_combine_rows_f16(exhip_ctx* ctx, const uint16_t* z, int z_stride, int z_rows, const int32_t* places, const float* weights, int kind, int m, int each, int n,
+                           uint16_t* y, int y_stride);
+
 /* ---- what a classifier or a language model answers with (no counterpart in the reference; exhip_softmax_channels_f32 stores all of a row) ---- */
 /* For rows x[m][c] (row stride x_stride elements, at least c; any alignment of the element type), in one reading of them:
  * log_p[m][n_ids]: x[id] - log(sum exp x) of the classes ids[m][n_ids]; a negative id asks nothing and gives 0, one from c on gives NaN;
