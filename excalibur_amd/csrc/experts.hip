@@ -7,82 +7,161 @@ constexpr int kMostExperts = 1024;
 constexpr int kMostEach = 64;
 constexpr int kMostChoices = 1 << 28;
 
-__device__ __forceinline__ int ones(unsigned long long v) { return __popcll(v); }
-
 // An expert a group: its waves count, each in its own stretch of the choices, those of earlier experts and those of this one, and go over the stretch again to
-// write where they stand. No count depends on another group, so one launch does it and the order is that of the choices.
+// write where they stand. No count depends on another group, so one launch does it and the order is that of the choices. Four choices a lane and 256 a wave at a
+// time, of which HELD stay in registers between the counting and the writing; where a stretch has more they are read again.
+typedef int v4i_of_four __attribute__((ext_vector_type(4), aligned(4)));
+
+template <int HELD>
 __global__ __launch_bounds__(1024) void group_rows_kernel(const int* __restrict__ ids, int choices, int each, int experts, int* __restrict__ offsets, int* __restrict__ rows,
                                                           int* __restrict__ places) {
     constexpr int kWaves = 16;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, expert = blockIdx.x;
-    const int stretch = ((choices + kWaves - 1) / kWaves + 63) / 64 * 64;
+    const int stretch = ((choices + kWaves - 1) / kWaves + 255) / 256 * 256;
     const long long from = (long long)wave * stretch;
-    const int begin = from < choices ? (int)from : choices, end = min(choices - begin, stretch) + begin;
+    const int begin = from < choices ? (int)from : choices, end = min(choices - begin, stretch) + begin, pieces = (end - begin + 255) / 256;
     __shared__ int before[kWaves], own[kWaves];
+    auto four = [&](int piece) {  // -1 behind the end
+        const int at = begin + piece * 256 + lane * 4;
+        v4i v = {-1, -1, -1, -1};
+        if (at + 4 <= end) v = *reinterpret_cast<const v4i_of_four*>(ids + at);
+        else
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+                if (at + e < end) v[e] = ids[at + e];
+        return v;
+    };
     int less = 0, equal = 0;
-    for (int at = begin; at < end; at += 64) {
-        const int id = at + lane < end ? ids[at + lane] : -1;
-        less += ones(__ballot(id >= 0 && id < expert));
-        equal += ones(__ballot(id == expert));
-    }
+    auto count = [&](const v4i& v) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            less += __popcll(__ballot((unsigned)v[e] < (unsigned)expert));
+            equal += __popcll(__ballot(v[e] == expert));
+        }
+    };
+    v4i held[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) held[i] = four(i);
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) count(held[i]);
+    for (int i = HELD; i < pieces; ++i) count(four(i));
     if (lane == 0) {
         before[wave] = less;
         own[wave] = equal;
     }
     __syncthreads();
-    int first = 0, all = 0, at_wave = 0;
+    int first = 0, all = 0, place = 0;
+#pragma unroll
     for (int w = 0; w < kWaves; ++w) {
         first += before[w];
-        if (w < wave) at_wave += own[w];
+        if (w < wave) place += own[w];
         all += own[w];
     }
+    place += first;
     if (threadIdx.x == 0) {
         offsets[expert] = first;
         if (expert == experts - 1) offsets[experts] = first + all;
     }
-    int place = first + at_wave;
-    for (int at = begin; at < end; at += 64) {
-        const int i = at + lane, id = i < end ? ids[i] : -1;
-        const unsigned long long here = __ballot(i < end && id == expert);
-        if (i < end && id == expert) {
-            const int to = place + ones(here & ((1ull << lane) - 1));
-            rows[to] = i / each;
-            places[i] = to;
+    auto write = [&](int piece, const v4i& v) {
+        const int at = begin + piece * 256 + lane * 4;
+        unsigned long long mask[4], any = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) any |= mask[e] = __ballot(v[e] == expert);
+        if (any) {
+            const unsigned long long earlier = (1ull << lane) - 1;
+            int to = place;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to += __popcll(mask[e] & earlier);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (v[e] == expert) {
+                    rows[to] = (at + e) / each;
+                    places[at + e] = to++;
+                }
+                place += __popcll(mask[e]);
+            }
         }
-        if (expert == 0 && i < end && (id < 0 || id >= experts)) places[i] = -1;
-        place += ones(here);
-    }
+        if (expert == 0) {  // those that chose nothing
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if ((unsigned)v[e] >= (unsigned)experts && at + e < end) places[at + e] = -1;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) write(i, held[i]);
+    for (int i = HELD; i < pieces; ++i) write(i, four(i));
     if (expert == experts - 1)
         for (int i = first + all + threadIdx.x; i < choices; i += 1024) rows[i] = -1;
 }
 
-// A row and a run of 1024 outputs a group.
-template <typename O>
+// ---- the sum of the answers ----
+// A row's weights: a choice's own, in a lane each.
+__device__ __forceinline__ float weight_of(const float* weights, int kind, int each, int j) {
+    const float given = j < each ? weights[j] : -__builtin_inff();
+    if (kind == EXHIP_WEIGHTS_PLAIN) return given;
+    if (kind == EXHIP_WEIGHTS_LOG) return expf(given);
+    float top = given;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float own = j < each ? expf(given - (top == -__builtin_inff() ? 0.f : top)) : 0.f;
+    float total = own;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+    return total == 0.f ? 0.f : own / total;
+}
+
+// A wave takes a row and eight outputs a lane; its lanes hold the row's places and weights, which the sum takes from them one choice at a time, always in the
+// choices' order. AHEAD answers are on their way at a time. Every answer is read once: what bounds it is the memory.
+template <typename O, int AHEAD>
 __global__ __launch_bounds__(256) void combine_rows_kernel(const uint16_t* __restrict__ z, int z_stride, int z_rows, const int* __restrict__ places, const float* __restrict__ weights,
-                                                           int kind, int each, int n, O* __restrict__ y, int y_stride) {
-    const int row = blockIdx.x;
-    const int* const place = places + (size_t)row * each;
-    const float* const weight = weights + (size_t)row * each;
-    float top = 0.f, total = 1.f;
-    if (kind == EXHIP_WEIGHTS_LOG_NORMALIZED) {
-        top = -__builtin_inff();
-        for (int j = 0; j < each; ++j) top = fmaxf(top, weight[j]);
-        if (top == -__builtin_inff()) top = 0.f;
-        total = 0.f;
-        for (int j = 0; j < each; ++j) total += expf(weight[j] - top);
-    }
-    for (int at = blockIdx.y * 1024 + threadIdx.x; at < min(n, (int)(blockIdx.y + 1) * 1024); at += 256) {
-        float sum = 0.f;
-        for (int j = 0; j < each; ++j) {
-            const int from = place[j];
-            if (from < 0) continue;
-            const float w = kind == EXHIP_WEIGHTS_PLAIN ? weight[j] : total == 0.f ? 0.f : expf(weight[j] - top) / total;
-            const float v = from < z_rows ? exhip_h2f(z[(size_t)from * z_stride + at]) : __builtin_nanf("");
-            sum = __builtin_fmaf(w, v, sum);
+                                                           int kind, int each, int n, O* __restrict__ y, int y_stride, int waves_a_row, size_t waves) {
+    const size_t wave = (size_t)blockIdx.x * 4 + threadIdx.x / 64;
+    if (wave >= waves) return;
+    const int lane = threadIdx.x % 64;
+    const size_t row = wave / waves_a_row;
+    const int at = (int)(wave % waves_a_row) * 512 + lane * 8;
+    const int place = lane < each ? places[row * each + lane] : -1;
+    const float weight = weight_of(weights + row * each, kind, each, lane);
+    const bool whole = at + 8 <= n;
+    float sum[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+    for (int first = 0; first < each; first += AHEAD) {
+        Eight<uint16_t> got[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            const int from = first + a < each ? __builtin_amdgcn_readlane(place, first + a) : -1;
+            const uint16_t* const src = z + (size_t)max(from, 0) * z_stride + at;
+            if (from >= 0 && from < z_rows) {
+                if (whole) got[a] = *reinterpret_cast<const Eight<uint16_t>*>(src);
+                else
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) got[a].v[e] = at + e < n ? src[e] : 0;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) got[a].v[e] = 0x7E00;  // not a number: there is no such row
+            }
         }
-        if constexpr (sizeof(O) == 4) y[(size_t)row * y_stride + at] = sum;
-        else y[(size_t)row * y_stride + at] = exhip_f2h(sum);
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            if (first + a >= each || __builtin_amdgcn_readlane(place, first + a) < 0) continue;
+            const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), first + a));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] = __builtin_fmaf(w, exhip_h2f(got[a].v[e]), sum[e]);
+        }
     }
+    O* const to = y + row * y_stride + at;
+    Eight<O> out;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if constexpr (sizeof(O) == 4) out.v[e] = sum[e];
+        else out.v[e] = exhip_f2h(sum[e]);
+    }
+    if (whole) *reinterpret_cast<Eight<O>*>(to) = out;
+    else
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (at + e < n) to[e] = out.v[e];
 }
 
 template <typename O>
@@ -95,10 +174,12 @@ int combine_rows(exhip_ctx* ctx, const char* name, const uint16_t* z, int z_stri
     EXHIP_REQUIRE(z_stride >= n && y_stride >= n, "%s: rows of %d values are %d and %d apart", name, n, z_stride, y_stride);
     EXHIP_REQUIRE(kind >= EXHIP_WEIGHTS_PLAIN && kind <= EXHIP_WEIGHTS_LOG_NORMALIZED, "%s: unknown kind of weights %d", name, kind);
     EXHIP_REQUIRE(aligned(z, 2) && aligned(places, 4) && aligned(weights, 4) && aligned(y, sizeof(O)), "%s: an operand's address is not that of its type", name);
-    EXHIP_REQUIRE(m <= 0x7fffffff / 256, "%s: %d rows are more than one launch takes", name, m);
+    const int waves_a_row = (n + 511) / 512;
+    const size_t waves = (size_t)m * waves_a_row, groups = (waves + 3) / 4;
+    EXHIP_REQUIRE(groups <= 0x7fffffff / 256, "%s: %d rows of %d outputs are more than one launch takes", name, m, n);
     const exhip_on_device on(ctx->device);
     EXHIP_CHECK(on.error);
-    hipLaunchKernelGGL(combine_rows_kernel<O>, dim3(m, (n + 1023) / 1024), dim3(256), 0, ctx->stream, z, z_stride, z_rows, places, weights, kind, each, n, y, y_stride);
+    hipLaunchKernelGGL((combine_rows_kernel<O, 4>), dim3((unsigned)groups), dim3(256), 0, ctx->stream, z, z_stride, z_rows, places, weights, kind, each, n, y, y_stride, waves_a_row, waves);
     EXHIP_LAUNCH_CHECK();
     return 0;
 }
@@ -113,7 +194,9 @@ extern "C" int exhip_group_rows(exhip_ctx* ctx, const int32_t* ids, int m, int e
     EXHIP_REQUIRE(aligned(ids, 4) && aligned(offsets, 4) && aligned(rows, 4) && aligned(places, 4), "exhip_group_rows: an operand's address is not that of its type");
     const exhip_on_device on(ctx->device);
     EXHIP_CHECK(on.error);
-    hipLaunchKernelGGL(group_rows_kernel, dim3(experts), dim3(1024), 0, ctx->stream, ids, m * each, each, experts, offsets, rows, places);
+    const int choices = m * each;
+    const auto kernel = choices <= 16 * 256 ? group_rows_kernel<1> : choices <= 16 * 1024 ? group_rows_kernel<4> : group_rows_kernel<16>;
+    hipLaunchKernelGGL(kernel, dim3(experts), dim3(1024), 0, ctx->stream, ids, choices, each, experts, offsets, rows, places);
     EXHIP_LAUNCH_CHECK();
     return 0;
 }

@@ -19,39 +19,117 @@ constexpr unsigned kNoRow = 0x80000000u;  // beyond every view of rows: loads th
 
 // ---- the quantizer ----
 // x / scale to the nearest whole number, ties to the even one, exactly: the product with 1 / scale is less than one off, and what it leaves, x - r scale, is
-// a multiple of the last place of scale / 2 and has no more bits than a float.
-__device__ __forceinline__ int code_of(float x, float scale, float inverse, float half) {
-    float r = __builtin_rintf(x * inverse);
-    const float left = __builtin_fmaf(-r, scale, x), off = fabsf(left);
-    if (off > half || (off == half && ((int)r & 1))) r += left > 0.f ? 1.f : -1.f;
-    return (int)r;
+// a multiple of the last place of scale / 2 and has no more bits than a float. A sum with 1.5 * 2^23 rounds to a whole number and has it in its low bits.
+constexpr float kWhole = 0x1.8p23f;
+__device__ __forceinline__ float nearly(float x, float inverse) { return __builtin_fmaf(x, inverse, kWhole); }
+__device__ __forceinline__ float left_of(float x, float near, float scale) { return __builtin_fmaf(kWhole - near, scale, x); }
+__device__ __forceinline__ float nearest(float x, float scale, float inverse) {
+    const float near = nearly(x, inverse), left = left_of(x, near, scale), off = fabsf(left), half = 0.5f * scale;
+    return off > half || (off == half && (__builtin_bit_cast(int, near) & 1)) ? near + (left > 0.f ? 1.f : -1.f) : near;
 }
-__device__ __forceinline__ int four_codes(int a, int b, int c, int d) { return (a & 255) | (b & 255) << 8 | (c & 255) << 16 | d << 24; }
+__device__ __forceinline__ int low_bytes(float a, float b, float c, float d) {
+    const unsigned ab = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x0c0c0400);
+    const unsigned cd = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, d), __builtin_bit_cast(unsigned, c), 0x0c0c0400);
+    return (int)__builtin_amdgcn_perm(cd, ab, 0x05040100);
+}
 
-// A row a group. Rows are read twice, the second time from L2.
+// 16 bytes of a row a lane at a time, at any alignment of their type.
 template <typename T>
-__global__ __launch_bounds__(256) void quantize_rows_i8_kernel(const T* __restrict__ x, int x_stride, int k, int8_t* __restrict__ y, int y_stride, float* __restrict__ scale) {
-    const T* const row = x + (size_t)blockIdx.x * x_stride;
-    int8_t* const codes = y + (size_t)blockIdx.x * y_stride;
-    __shared__ float part[4];
-    __shared__ int odd[4];
+struct Piece {
+    static constexpr int kValues = 16 / sizeof(T);
+    struct __attribute__((packed, aligned(sizeof(T)))) Packed {
+        T v[kValues];
+    };
+    T v[kValues];
+    __device__ __forceinline__ void load(const T* row, int at, int k) {  // zeros behind the row's end
+        if (at + kValues <= k) {
+            const Packed p = *reinterpret_cast<const Packed*>(row + at);
+#pragma unroll
+            for (int e = 0; e < kValues; ++e) v[e] = p.v[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < kValues; ++e) v[e] = at + e < k ? row[at + e] : T(0);
+        }
+    }
+    __device__ __forceinline__ float most(float so_far) const {  // NaN stays, as the largest of all
+#pragma unroll
+        for (int e = 0; e < kValues; ++e) {
+            const float a = fabsf(as_float(v[e]));
+            so_far = so_far >= a || so_far != so_far ? so_far : a;
+        }
+        return so_far;
+    }
+    __device__ __forceinline__ void store(int8_t* row, int at, int k, float scale, float inverse) const {
+        float near[kValues], off = 0.f;
+#pragma unroll
+        for (int e = 0; e < kValues; ++e) {
+            near[e] = nearly(as_float(v[e]), inverse);
+            off = fmaxf(off, fabsf(left_of(as_float(v[e]), near[e], scale)));
+        }
+        if (off >= 0.5f * scale)  // a tie, or a neighbour of one: 2 % of a wave's pieces
+#pragma unroll
+            for (int e = 0; e < kValues; ++e) near[e] = nearest(as_float(v[e]), scale, inverse);
+        int codes[kValues / 4];
+#pragma unroll
+        for (int e = 0; e < kValues / 4; ++e) codes[e] = low_bytes(near[4 * e], near[4 * e + 1], near[4 * e + 2], near[4 * e + 3]);
+        if (at + kValues <= k) {
+            if constexpr (kValues == 8) *reinterpret_cast<v2i*>(row + at) = v2i{codes[0], codes[1]};
+            else *reinterpret_cast<int*>(row + at) = codes[0];
+        } else {
+#pragma unroll
+            for (int e = 0; e < kValues; ++e)
+                if (at + e < k) row[at + e] = (int8_t)(codes[e / 4] >> (8 * (e % 4)));
+        }
+    }
+};
+
+// WAVES waves a row (a wave takes its own row where that is one), HELD pieces a lane that stay in registers between the largest value and the codes; what a longer
+// row has behind them is read again.
+template <typename T, int WAVES, int HELD>
+__global__ __launch_bounds__(256) void quantize_rows_i8_kernel(const T* __restrict__ x, int x_stride, int m, int k, int8_t* __restrict__ y, int y_stride, float* __restrict__ scale) {
+    constexpr int kStep = 64 * WAVES * Piece<T>::kValues;
+    const int wave = threadIdx.x / 64, row = blockIdx.x * (4 / WAVES) + wave / WAVES;
+    if (row >= m) return;  // a whole wave, and a whole group where several have a row
+    const T* const from = x + (size_t)row * x_stride;
+    const int first = threadIdx.x % (64 * WAVES) * Piece<T>::kValues;
+    Piece<T> held[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) held[i].load(from, first + i * kStep, k);
     float most = 0.f;
-    bool special = false;
-    for (int at = threadIdx.x; at < k; at += 256) {
-        const float a = fabsf(as_float(row[at]));
-        special |= !(a < __builtin_inff());
-        most = fmaxf(most, a);
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) most = held[i].most(most);
+    for (int at = first + HELD * kStep; at < k; at += kStep) {
+        Piece<T> p;
+        p.load(from, at, k);
+        most = p.most(most);
+    }
+    // as whole numbers the bits of values that are not negative are in their order, and those of NaN above all
+    int bits = __builtin_bit_cast(int, most);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) bits = max(bits, __shfl_xor(bits, d));
+    if constexpr (WAVES > 1) {
+        __shared__ int part[WAVES];
+        if (threadIdx.x % 64 == 0) part[wave] = bits;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) bits = max(bits, part[w]);
+    }
+    const bool fine = bits < 0x7f800000;
+    const float s = fine ? fmaxf(__builtin_bit_cast(float, bits) / kLargest, kLeastScale) : __builtin_inff(), inverse = 1.f / s;
+    if (threadIdx.x % (64 * WAVES) == 0) scale[row] = fine ? s : __builtin_nanf("");
+    int8_t* const to = y + (size_t)row * y_stride;
+    if (!fine) {
+        for (int at = threadIdx.x % (64 * WAVES); at < k; at += 64 * WAVES) to[at] = 0;
+        return;
     }
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
-    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = most;
-    odd[threadIdx.x / 64] = 0;
-    if (__any(special)) odd[threadIdx.x / 64] = 1;
-    __syncthreads();
-    const bool none = odd[0] | odd[1] | odd[2] | odd[3];
-    const float s = fmaxf(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) / kLargest, kLeastScale), inverse = 1.f / s;
-    if (threadIdx.x == 0) scale[blockIdx.x] = none ? __builtin_nanf("") : s;
-    for (int at = threadIdx.x; at < k; at += 256) codes[at] = none ? 0 : (int8_t)code_of(as_float(row[at]), s, inverse, 0.5f * s);
+    for (int i = 0; i < HELD; ++i)
+        if (first + i * kStep < k) held[i].store(to, first + i * kStep, k, s, inverse);
+    for (int at = first + HELD * kStep; at < k; at += kStep) {
+        Piece<T> p;
+        p.load(from, at, k);
+        p.store(to, at, k, s, inverse);
+    }
 }
 
 // ---- the weights' layout ----
@@ -266,6 +344,162 @@ __global__ __launch_bounds__(64 * WK, 2) void i8_rows_kernel(const I8Params p) {
     }
 }
 
+// ---- many rows ----
+// Results of a group of WN x WM waves, 32 TN outputs (of both projections) and 32 TM rows a wave, from products of 32 x 32: a lane's sums are runs of four neighbouring
+// outputs, output 8 run + 4 (lane / 32) and on of each 32, of row lane % 32. They go through LDS, so that whole lines are stored: all rows at once, or those of half of
+// the waves after the other's where float32 results of all of them do not fit.
+typedef int v16i __attribute__((ext_vector_type(16)));
+
+template <int WIDTH>
+struct Scales {  // of a group's rows and outputs, in LDS
+    float output[WIDTH], output_up[WIDTH], bias[WIDTH], bias_up[WIDTH];
+    float row[1];  // as many as the group has
+};
+
+template <typename O, int WN, int WM, int TM, int FOURS, int ROOM>
+__device__ __forceinline__ void store_group(O* y, size_t stride, const v4f (&v)[FOURS][TM], const Part& part, int j0, int n, int wn, int wm, int lane, char* lds) {
+    constexpr int kOwn = FOURS * 8, kWidth = kOwn * WN, kAll = 32 * TM * WM, kPasses = kAll * kWidth * (int)sizeof(O) > ROOM ? 2 : 1, kRows = kAll / kPasses;
+    static_assert(kRows * kWidth * sizeof(O) <= ROOM);
+#pragma unroll
+    for (int pass = 0; pass < kPasses; ++pass) {
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            const int row = (wm * TM + t) * 32 - pass * kRows;  // 32 rows lie in one pass
+            if (row < 0 || row >= kRows) continue;
+#pragma unroll
+            for (int i = 0; i < FOURS; ++i) {
+                char* const to = place_in_rows<O, kWidth>(lds, row + lane % 32, wn * kOwn + i * 8 + lane / 32 * 4);
+                if constexpr (sizeof(O) == 4) *reinterpret_cast<v4f*>(to) = v[i][t];
+                else *reinterpret_cast<v4h*>(to) = __builtin_convertvector(v[i][t], v4h);
+            }
+        }
+        __syncthreads();
+        store_rows<O, kWidth, kRows, 64 * WN * WM>(lds, y, stride, part.row0 + pass * kRows, part.rows - pass * kRows, j0, n);
+    }
+}
+
+template <int WN, int WM, int TN, int TM, bool GATED, int ROOM, int WIDTH>
+__device__ __forceinline__ void write_group(const I8Params& p, const Part& part, const v16i (&acc)[TN][TM], int wn, int wm, int lane, char* lds, const Scales<WIDTH>& scales) {
+    constexpr int kFours = TN * (GATED ? 2 : 4), kOwn = kFours * 8;
+    static_assert(kOwn * WN == WIDTH);
+    const int at = wn * kOwn + lane / 32 * 4, row = wm * TM * 32 + lane % 32;
+    v4f v[kFours][TM];
+#pragma unroll
+    for (int i = 0; i < kFours; ++i) {
+        const v4f output = *reinterpret_cast<const v4f*>(scales.output + at + i * 8), bias = *reinterpret_cast<const v4f*>(scales.bias + at + i * 8);
+        v4f output_up = output, bias_up = bias;
+        if constexpr (GATED) {
+            output_up = *reinterpret_cast<const v4f*>(scales.output_up + at + i * 8);
+            bias_up = *reinterpret_cast<const v4f*>(scales.bias_up + at + i * 8);
+        }
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            const float x_scale = scales.row[row + t * 32];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (GATED) {
+                    const float g = result_of(acc[i / 2][t][i % 2 * 4 + e], x_scale, output[e], bias[e]);
+                    v[i][t][e] = gated(p.gate, g, result_of(acc[i / 2][t][i % 2 * 4 + 8 + e], x_scale, output_up[e], bias_up[e]));
+                } else {
+                    v[i][t][e] = result_of(acc[i / 4][t][i % 4 * 4 + e], x_scale, output[e], bias[e]);
+                }
+            }
+        }
+    }
+    const int j0 = part.group_n * WIDTH;
+    if (p.y_f32) store_group<float, WN, WM, TM, kFours, ROOM>(p.y_f32, p.y_stride, v, part, j0, p.n, wn, wm, lane, lds);
+    if (p.y_f16) store_group<uint16_t, WN, WM, TM, kFours, ROOM>(p.y_f16, p.y_stride, v, part, j0, p.n, wn, wm, lane, lds);
+}
+
+// A group of WN x WM waves takes 32 TN WN outputs and 32 TM WM rows. Rows' codes come straight into LDS, three blocks ahead in four buffers; a wave's weights from
+// L2 straight into registers, those of a step of 32 values as soon as the same step of the block before is done with them. Every step's rows are read from LDS while the
+// products of the step before run, and loads stand between the products one by one. A block's one barrier, at its start, says that the next block's rows are there and that
+// the last block's buffer may be filled.
+template <int TN, int TM, int WN, int WM, bool GATED, bool GROUPED>
+__global__ __launch_bounds__(64 * WN * WM, 2) void i8_wide_kernel(const I8Params p) {
+    exhip_touch_args(p);
+    constexpr int kWaves = WN * WM, kRows = 32 * TM * WM, kBuffers = 4, kBuffer = kRows * kBlk, kLoads = kRows / 8 / kWaves, kWidth = TN * WN * (GATED ? 16 : 32), kProducts = TN * TM;
+    constexpr int kResults = kRows * kWidth * 2, kRoom = kBuffers * kBuffer > kResults ? kBuffers * kBuffer : kResults;
+    __shared__ __attribute__((aligned(16))) char staged[kRoom];
+    __shared__ __attribute__((aligned(16))) char scale_room[sizeof(Scales<kWidth>) + kRows * 4];
+    Scales<kWidth>& scales = *reinterpret_cast<Scales<kWidth>*>(scale_room);
+    Part part;
+    if (!part_of<GROUPED, kRows>(p, &part)) return;
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)staged;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wn = wave % WN, wm = wave / WN;
+    const int blocks = p.blocks, row_bytes = blocks * kTileBlock, tile0 = (part.group_n * WN + wn) * TN, first = min(tile0, p.tiles - 1);
+    const __amdgpu_buffer_rsrc_t weights = uniform_view(p.w + ((size_t)part.expert * p.tiles + first) * row_bytes, (unsigned)(min(TN, p.tiles - first) * row_bytes));
+    const Rows<GROUPED> rows(p, part);
+    // A wave stages 8 kLoads rows, eight with a load: lane l holds piece (l % 8) ^ (l / 8) of row l / 8, so that a piece of eight neighbouring rows lies in all banks.
+    unsigned off[kLoads];
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) off[j] = rows.begin(rows.source((wave * kLoads + j) * 8 + lane / 8)) + ((lane % 8) ^ (lane / 8)) * 16;
+    auto stage = [&](int buffer, int j) {  // behind the last block that one again, which nothing reads
+        load16_to_lds(rows.view, off[j], min(buffer, blocks - 1) * kBlk, lds0 + buffer % kBuffers * kBuffer + (wave * kLoads + j) * 1024);
+    };
+    v4i w[4][TN];
+    auto request = [&](int b, int s, int i) {
+        w[s][i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(weights, lane * 16, min(i, p.tiles - 1 - first) * row_bytes + min(b, blocks - 1) * kTileBlock + s * 1024, 0));
+    };
+    // scales and biases, for the end
+    for (int r = threadIdx.x; r < kRows; r += 64 * kWaves) scales.row[r] = rows.scale(rows.source(r));
+    for (int r = threadIdx.x; r < kWidth; r += 64 * kWaves) {
+        const size_t j = (size_t)part.expert * p.n + min(part.group_n * kWidth + r, p.n - 1);
+        scales.output[r] = p.w_scale[j];
+        scales.bias[r] = p.bias ? p.bias[j] : 0.f;
+        if constexpr (GATED) {
+            scales.output_up[r] = p.w_scale_up[j];
+            scales.bias_up[r] = p.bias_up ? p.bias_up[j] : 0.f;
+        }
+    }
+    v16i acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int t = 0; t < TM; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][t][e] = 0;
+#pragma unroll
+    for (int j = 0; j < 3 * kLoads; ++j) stage(j / kLoads, j % kLoads);
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int i = 0; i < TN; ++i) request(0, s, i);
+    auto arrive = [&] {
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads + 4 * TN) : "memory");
+    arrive();
+    const int at = (wm * TM * 32 + lane % 32) * kBlk + ((lane / 32) ^ (lane % 8)) * 16;
+    auto rows_from = [&](int b, int s, int t) { return *reinterpret_cast<const v4i*>(staged + b % kBuffers * kBuffer + (at ^ (s * 32)) + t * 32 * kBlk); };
+    v4i x[2][TM];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) x[0][t] = rows_from(0, 0, t);
+    for (int b = 0; b < blocks; ++b) {
+        // all but the loads of the block before
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLoads + 4 * TN) : "memory");
+        arrive();
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+#pragma unroll
+            for (int u = 0; u < kProducts; ++u) {
+                const int t = u / TN, i = u % TN;
+                if (i == 0) x[(s + 1) % 2][t] = s < 3 ? rows_from(b, s + 1, t) : rows_from(b + 1, 0, t);
+                if (u == kProducts / 4)
+#pragma unroll
+                    for (int j = s * kLoads / 4; j < (s + 1) * kLoads / 4; ++j) stage(b + 3, j);
+                acc[i][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[s][i], x[s % 2][t], acc[i][t], 0, 0, 0);
+                if (u >= kProducts - TN) request(b + 1, s, u - (kProducts - TN));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was staged behind the end, in front of the results' barrier
+    write_group<WN, WM, TN, TM, GATED, kRoom>(p, part, acc, wn, wm, lane, staged, scales);
+}
+
 int blocks_of(int v) { return v / kBlk + (v % kBlk != 0); }
 int tiles_of(int n, bool gated_product) { return gated_product ? (n + 15) / 16 : (n + 31) / 32; }
 bool sizes_ok(int n, int k) { return n > 0 && k > 0 && n <= (1 << 24) && k <= kMostInputs; }
@@ -280,7 +514,13 @@ int quantize_rows(exhip_ctx* ctx, const char* name, const T* x, int x_stride, in
     EXHIP_REQUIRE(aligned(x, sizeof(T)) && aligned(scale, 4), "%s: an operand's address is not that of its type", name);
     const exhip_on_device on(ctx->device);
     EXHIP_CHECK(on.error);
-    hipLaunchKernelGGL(quantize_rows_i8_kernel<T>, dim3(m), dim3(256), 0, ctx->stream, x, x_stride, k, y, y_stride, scale);
+    constexpr int kWave = 64 * Piece<T>::kValues;
+    auto run = [&](auto kernel, int rows) { hipLaunchKernelGGL(kernel, dim3((m - 1) / rows + 1), dim3(256), 0, ctx->stream, x, x_stride, m, k, y, y_stride, scale); };
+    if (k <= kWave) run(quantize_rows_i8_kernel<T, 1, 1>, 4);
+    else if (k <= 4 * kWave) run(quantize_rows_i8_kernel<T, 4, 1>, 1);
+    else if (k <= 8 * kWave) run(quantize_rows_i8_kernel<T, 4, 2>, 1);
+    else if (k <= 16 * kWave) run(quantize_rows_i8_kernel<T, 4, 4>, 1);
+    else run(quantize_rows_i8_kernel<T, 4, 8>, 1);
     EXHIP_LAUNCH_CHECK();
     return 0;
 }
@@ -302,6 +542,9 @@ int launch(exhip_ctx* ctx, K kernel, I8Params p, int tiles, int rows, int thread
 
 template <bool GATED, bool GROUPED>
 int run_best(exhip_ctx* ctx, const I8Params& p) {
+    const int form = g_exhip_options.i8_form > 0 ? g_exhip_options.i8_form : p.m <= 64 ? 1 : (long long)p.m * p.tiles <= 1 << 17 ? 2 : 3;
+    if (form >= 3) return launch(ctx, i8_wide_kernel<2, 4, 4, 1, GATED, GROUPED>, p, 8, 128, 256);
+    if (form == 2) return launch(ctx, i8_wide_kernel<2, 2, 4, 1, GATED, GROUPED>, p, 8, 64, 256);
     return launch(ctx, i8_rows_kernel<2, 1, 8, 2, GATED, GROUPED>, p, 1, 16, 512);
 }
 
