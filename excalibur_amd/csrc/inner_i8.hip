@@ -176,48 +176,69 @@ struct I8Params {
 struct Part {
     int expert, row0, rows, group_n;
 };
-__device__ __forceinline__ int rows_before(const I8Params& p, int expert) { return min(max(p.offsets[expert], 0), p.m); }
 
-// The group's part; false where there is none for it. By experts every wave counts the tiles of rows of all of them.
+// The tiles of ROWS rows. By experts each one's rows are cut by themselves, and every lane of a wave holds an expert, or a run of them where there are more than 64: the
+// tiles of its own and of all up to them. (Offsets that do not rise count rows twice; the bound, beyond every launch, keeps the sums of such ones in range.)
 template <bool GROUPED, int ROWS>
-__device__ __forceinline__ bool part_of(const I8Params& p, Part* part) {
-    int group_m;
-    if constexpr (!GROUPED) {
-        tile_of(p.groups_n, p.groups_m, &part->group_n, &group_m);
-        part->expert = 0;
-        part->row0 = group_m * ROWS;
-        part->rows = min(ROWS, p.m - part->row0);
-        return true;
-    } else {
-        const int lane = threadIdx.x % 64, each = (p.experts + 63) / 64;
-        int own = 0;
-        // (Offsets that do not rise count rows twice; the bound, beyond every launch, keeps the sums of such ones in range.)
-        for (int e = lane * each; e < min((lane + 1) * each, p.experts); ++e)
-            own = min(own + (max(rows_before(p, e + 1) - rows_before(p, e), 0) + ROWS - 1) / ROWS, 1 << 24);
-        int upto = own;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int before = __shfl_up(upto, d);
-            if (lane >= d) upto += before;
-        }
-        const int total = min(__builtin_amdgcn_readlane(upto, 63), p.groups_m);
-        if ((int)blockIdx.x >= p.groups_n * total) return false;
-        tile_of(p.groups_n, total, &part->group_n, &group_m);
-        const int of = __builtin_ctzll(__ballot(upto > group_m));
-        int left = group_m - (__builtin_amdgcn_readlane(upto, of) - __builtin_amdgcn_readlane(own, of));
-        for (int e = of * each; e < min((of + 1) * each, p.experts); ++e) {
-            const int from = rows_before(p, e), count = max(rows_before(p, e + 1) - from, 0), tiles = (count + ROWS - 1) / ROWS;
-            if (left < tiles) {
-                part->expert = __builtin_amdgcn_readfirstlane(e);
-                part->row0 = __builtin_amdgcn_readfirstlane(from + left * ROWS);
-                part->rows = __builtin_amdgcn_readfirstlane(min(ROWS, count - left * ROWS));
-                return true;
+struct Tiles {
+    int total;  // along the rows
+    int own, upto, from, count;
+    static __device__ __forceinline__ int offset(const I8Params& p, int expert) { return min(max(p.offsets[expert], 0), p.m); }
+    static __device__ __forceinline__ int tiles_of(int rows) { return (int)(((unsigned)rows + ROWS - 1) / ROWS); }
+    __device__ __forceinline__ explicit Tiles(const I8Params& p) {
+        if constexpr (!GROUPED) {
+            total = p.groups_m;
+        } else {
+            const int lane = threadIdx.x % 64, each = (p.experts + 63) / 64;
+            own = from = count = 0;
+            for (int e = lane * each; e < min((lane + 1) * each, p.experts); ++e) {
+                from = offset(p, e);
+                count = max(offset(p, e + 1) - from, 0);
+                own = min(own + tiles_of(count), 1 << 24);
             }
-            left -= tiles;
+            upto = own;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int before = __shfl_up(upto, d);
+                if (lane >= d) upto += before;
+            }
+            total = min(__builtin_amdgcn_readlane(upto, 63), p.groups_m);
         }
-        return false;
     }
-}
+    // the part that is the `at`-th in the order in which the groups of an XCD share rows and weights; at < groups_n * total
+    __device__ __forceinline__ Part part(const I8Params& p, int at) const {
+        Part part;
+        int group_m;
+        tile_of(at, p.groups_n, total, &part.group_n, &group_m);
+        if constexpr (!GROUPED) {
+            part.expert = 0;
+            part.row0 = group_m * ROWS;
+            part.rows = min(ROWS, p.m - part.row0);
+        } else {
+            const int of = __builtin_ctzll(__ballot(upto > group_m));
+            int left = group_m - (__builtin_amdgcn_readlane(upto, of) - __builtin_amdgcn_readlane(own, of));
+            int begin = __builtin_amdgcn_readlane(from, of), rows = __builtin_amdgcn_readlane(count, of);
+            part.expert = of;
+            if (p.experts > 64) {
+                const int each = (p.experts + 63) / 64;
+                for (int e = of * each; e < min((of + 1) * each, p.experts); ++e) {
+                    begin = offset(p, e);
+                    rows = max(offset(p, e + 1) - begin, 0);
+                    part.expert = e;
+                    if (left < tiles_of(rows)) break;
+                    left -= tiles_of(rows);
+                }
+                begin = __builtin_amdgcn_readfirstlane(begin);
+                rows = __builtin_amdgcn_readfirstlane(rows);
+                left = __builtin_amdgcn_readfirstlane(left);
+                part.expert = __builtin_amdgcn_readfirstlane(part.expert);
+            }
+            part.row0 = begin + left * ROWS;
+            part.rows = min(ROWS, rows - left * ROWS);
+        }
+        return part;
+    }
+};
 
 // The input's rows that a group reads: a view, where each row begins in it, and each row's scale.
 template <bool GROUPED>
@@ -250,6 +271,23 @@ struct Rows {
 
 __device__ __forceinline__ float result_of(int sum, float row, float output, float bias) { return __builtin_fmaf((float)sum * row, output, bias); }
 
+// The activation of one side times the other, from the hardware's 2^x and 1 / x (one unit of the last place each). What 2^x makes of the rounding of its argument, 2^-24 of
+// that, counts where the activation is near 0 alone: less than 2^-23 of max(|g|, 1) in all. erf is Abramowitz and Stegun's 7.1.26, off by 1.5e-7 at most; on the side where
+// 1 + erf is small it is what is computed. (The library's expf, erff and divisions took 10 us of 4096 x 8 of 64 x 1536 x 2048's 260.)
+__device__ __forceinline__ float gated_value(int gate, float g, float u) {
+    if (gate == EXHIP_GATE_RELU) return (g > 0.f ? g : g != g ? g : 0.f) * u;
+    if (gate == EXHIP_GATE_GELU) {
+        const float x = fabsf(g) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
+        float tail = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
+        tail = __builtin_fmaf(t, tail, 1.421413741f);
+        tail = __builtin_fmaf(t, tail, -0.284496736f);
+        tail = __builtin_fmaf(t, tail, 0.254829592f) * t * __builtin_amdgcn_exp2f(x * x * -1.44269504088896341f);  // 1 - erf(x)
+        return 0.5f * g * (g < 0.f ? tail : 2.f - tail) * u;
+    }
+    const float sigmoid = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504088896341f));
+    return (gate == EXHIP_GATE_SILU ? g * sigmoid : sigmoid) * u;
+}
+
 // ---- few rows, or few products ----
 // A group takes TN x 16 outputs (of both projections) and 16 TM rows; its WK waves every WK-th block, with nothing between memory and their registers: the codes of
 // D of a wave's blocks are on their way at a time. The sums meet in LDS, and every thread finishes four neighbouring outputs of a row.
@@ -258,8 +296,9 @@ __global__ __launch_bounds__(64 * WK, 2) void i8_rows_kernel(const I8Params p) {
     exhip_touch_args(p);
     constexpr int kRows = 16 * TM, kSide = GATED ? 2 : 1;
     static_assert(TN % 2 == 0, "whole tiles");
-    Part part;
-    if (!part_of<GROUPED, kRows>(p, &part)) return;
+    const Tiles<GROUPED, kRows> tiles(p);
+    if ((int)blockIdx.x >= p.groups_n * tiles.total) return;
+    const Part part = tiles.part(p, blockIdx.x);
     const int lane = threadIdx.x % 64, wk = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), q = lane / 16, col = lane % 16;
     const int blocks = p.blocks, row_bytes = blocks * kTileBlock, tile0 = part.group_n * (TN / 2), last = p.tiles - 1;
     const __amdgpu_buffer_rsrc_t weights = uniform_view(p.w + ((size_t)part.expert * p.tiles + tile0) * row_bytes, (unsigned)(min(TN / 2, p.tiles - tile0) * row_bytes));
@@ -330,7 +369,7 @@ __global__ __launch_bounds__(64 * WK, 2) void i8_rows_kernel(const I8Params p) {
     if constexpr (GATED) {
         const v4f w_scale_up = four_of(p.w_scale_up + own, j, p.n), bias_up = four_of(p.bias_up ? p.bias_up + own : nullptr, j, p.n);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = gated(p.gate, v[e], result_of(sum_up[e], x_scale, w_scale_up[e], bias_up[e]));
+        for (int e = 0; e < 4; ++e) v[e] = gated_value(p.gate, v[e], result_of(sum_up[e], x_scale, w_scale_up[e], bias_up[e]));
     }
     const size_t to = (size_t)(part.row0 + row) * p.y_stride + j;
     const bool whole = j + 4 <= p.n;
@@ -400,7 +439,7 @@ __device__ __forceinline__ void write_group(const I8Params& p, const Part& part,
             for (int e = 0; e < 4; ++e) {
                 if constexpr (GATED) {
                     const float g = result_of(acc[i / 2][t][i % 2 * 4 + e], x_scale, output[e], bias[e]);
-                    v[i][t][e] = gated(p.gate, g, result_of(acc[i / 2][t][i % 2 * 4 + 8 + e], x_scale, output_up[e], bias_up[e]));
+                    v[i][t][e] = gated_value(p.gate, g, result_of(acc[i / 2][t][i % 2 * 4 + 8 + e], x_scale, output_up[e], bias_up[e]));
                 } else {
                     v[i][t][e] = result_of(acc[i / 4][t][i % 4 * 4 + e], x_scale, output[e], bias[e]);
                 }
@@ -424,8 +463,9 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void i8_wide_kernel(const I8Params
     __shared__ __attribute__((aligned(16))) char staged[kRoom];
     __shared__ __attribute__((aligned(16))) char scale_room[sizeof(Scales<kWidth>) + kRows * 4];
     Scales<kWidth>& scales = *reinterpret_cast<Scales<kWidth>*>(scale_room);
-    Part part;
-    if (!part_of<GROUPED, kRows>(p, &part)) return;
+    const Tiles<GROUPED, kRows> tiles(p);
+    if ((int)blockIdx.x >= p.groups_n * tiles.total) return;
+    const Part part = tiles.part(p, blockIdx.x);
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)staged;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wn = wave % WN, wm = wave / WN;
     const int blocks = p.blocks, row_bytes = blocks * kTileBlock, tile0 = (part.group_n * WN + wn) * TN, first = min(tile0, p.tiles - 1);
@@ -500,6 +540,8 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void i8_wide_kernel(const I8Params
     write_group<WN, WM, TN, TM, GATED, kRoom>(p, part, acc, wn, wm, lane, staged, scales);
 }
 
+constexpr int kCus = 256;
+
 int blocks_of(int v) { return v / kBlk + (v % kBlk != 0); }
 int tiles_of(int n, bool gated_product) { return gated_product ? (n + 15) / 16 : (n + 31) / 32; }
 bool sizes_ok(int n, int k) { return n > 0 && k > 0 && n <= (1 << 24) && k <= kMostInputs; }
@@ -542,7 +584,7 @@ int launch(exhip_ctx* ctx, K kernel, I8Params p, int tiles, int rows, int thread
 
 template <bool GATED, bool GROUPED>
 int run_best(exhip_ctx* ctx, const I8Params& p) {
-    const int form = g_exhip_options.i8_form > 0 ? g_exhip_options.i8_form : p.m <= 64 ? 1 : (long long)p.m * p.tiles <= 1 << 17 ? 2 : 3;
+    const int form = p.blocks < 4 ? 1 : g_exhip_options.i8_form > 0 ? g_exhip_options.i8_form : p.m <= 64 ? 1 : (long long)p.m * p.tiles <= 1 << 17 ? 2 : 3;
     if (form >= 3) return launch(ctx, i8_wide_kernel<2, 4, 4, 1, GATED, GROUPED>, p, 8, 128, 256);
     if (form == 2) return launch(ctx, i8_wide_kernel<2, 2, 4, 1, GATED, GROUPED>, p, 8, 64, 256);
     return launch(ctx, i8_rows_kernel<2, 1, 8, 2, GATED, GROUPED>, p, 1, 16, 512);
