@@ -60,13 +60,16 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t uniform_view(const void* base,
 
 // Which tiles a group takes: each of the 8 XCDs a run of neighbouring ones, in bands of eight row tiles, so that the groups that run on an XCD at a time share
 // rows and weights in its L2.
-__device__ __forceinline__ void tile_of(int group, int groups_n, int groups_m, int* n, int* m) {
-    const int total = groups_n * groups_m, xcd = group % 8, per = total / 8, more = total % 8;
-    const int i = xcd * per + min(xcd, more) + group / 8;
+__device__ __forceinline__ int place_of(int group, int total) {
+    const int xcd = group % 8, per = total / 8, more = total % 8;
+    return xcd * per + min(xcd, more) + group / 8;
+}
+__device__ __forceinline__ void tile_at(int i, int groups_n, int groups_m, int* n, int* m) {
     const int band = i / (8 * groups_n), within = i % (8 * groups_n), high = min(8, groups_m - band * 8);
     *m = band * 8 + within % high;
     *n = within / high;
 }
+__device__ __forceinline__ void tile_of(int groups_n, int groups_m, int* n, int* m) { tile_at(place_of(blockIdx.x, groups_n * groups_m), groups_n, groups_m, n, m); }
 
 // ---- results of the kernels for many rows: through LDS, so that whole lines are stored ----
 // (A lane's four neighbouring outputs of one row, stored as they are, are 32 bytes of each of 16 rows at a time: 1.2 TB/s.)

@@ -326,7 +326,7 @@ __global__ __launch_bounds__(512, 2) void f8_wide_kernel(const F8Params p) {
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wn = wave % WN, wm = wave / WN;
     const int q = lane / 16, col = lane % 16;
     int group_n, group_m;
-    tile_of(blockIdx.x, p.groups_n, p.groups_m, &group_n, &group_m);
+    tile_of(p.groups_n, p.groups_m, &group_n, &group_m);
     const int tile0 = (group_n * WN + wn) * TN, row0 = p.first + group_m * kRows;
     const int rows = min(kRows, p.last - row0), tail = p.k % kBlk, blocks = p.blocks_k;
     const __amdgpu_buffer_rsrc_t xr = uniform_view(p.x + (size_t)row0 * p.x_stride, (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16);
@@ -610,7 +610,7 @@ __global__ __launch_bounds__(256, 2) void f8_tile_kernel(const F8Params p) {
     const int lane = threadIdx.x % 64, wn = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int side = lane / 32, col = lane % 32;
     int group_n, group_m;
-    tile_of(blockIdx.x, p.groups_n, p.groups_m, &group_n, &group_m);
+    tile_of(p.groups_n, p.groups_m, &group_n, &group_m);
     const int tile0 = (group_n * WN + wn) * TN, row0 = p.first + group_m * kRows;
     const int rows = min(kRows, p.last - row0), tail = p.k % kBlk, blocks = p.blocks_k;
     const __amdgpu_buffer_rsrc_t xr = uniform_view(p.x + (size_t)row0 * p.x_stride, (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16);
@@ -745,7 +745,7 @@ __global__ __launch_bounds__(128 * WM, 2) void f8_deep_kernel(const F8Params p) 
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wn = wave % WN, wm = wave / WN;
     const int q = lane / 16, col = lane % 16;
     int group_n, group_m;
-    tile_of(blockIdx.x, p.groups_n, p.groups_m, &group_n, &group_m);
+    tile_of(p.groups_n, p.groups_m, &group_n, &group_m);
     const int tile0 = (group_n * WN + wn) * TN, row0 = p.first + group_m * kRows;
     const int rows = min(kRows, p.last - row0), tail = p.k % kBlk, blocks = p.blocks_k;
     const __amdgpu_buffer_rsrc_t xr = uniform_view(p.x + (size_t)row0 * p.x_stride, (rows - 1) * p.x_stride + (p.k + 15) / 16 * 16);

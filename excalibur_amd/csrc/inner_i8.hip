@@ -205,36 +205,37 @@ struct Tiles {
             total = min(__builtin_amdgcn_readlane(upto, 63), p.groups_m);
         }
     }
-    // the part that is the `at`-th in the order in which the groups of an XCD share rows and weights; at < groups_n * total
-    __device__ __forceinline__ Part part(const I8Params& p, int at) const {
+    // the group's part; where there are groups_n * total of them. The tiles of an expert follow each other, so that its weights are read from memory once.
+    __device__ __forceinline__ Part part(const I8Params& p) const {
         Part part;
-        int group_m;
-        tile_of(at, p.groups_n, total, &part.group_n, &group_m);
+        int at = place_of(blockIdx.x, p.groups_n * total), group_m;
         if constexpr (!GROUPED) {
+            tile_at(at, p.groups_n, total, &part.group_n, &group_m);
             part.expert = 0;
             part.row0 = group_m * ROWS;
             part.rows = min(ROWS, p.m - part.row0);
         } else {
-            const int of = __builtin_ctzll(__ballot(upto > group_m));
-            int left = group_m - (__builtin_amdgcn_readlane(upto, of) - __builtin_amdgcn_readlane(own, of));
+            const int of = __builtin_ctzll(__ballot(upto > at / p.groups_n));
             int begin = __builtin_amdgcn_readlane(from, of), rows = __builtin_amdgcn_readlane(count, of);
+            at -= (__builtin_amdgcn_readlane(upto, of) - __builtin_amdgcn_readlane(own, of)) * p.groups_n;
             part.expert = of;
-            if (p.experts > 64) {
+            if (p.experts > 64) {  // which one of the lane's
                 const int each = (p.experts + 63) / 64;
                 for (int e = of * each; e < min((of + 1) * each, p.experts); ++e) {
                     begin = offset(p, e);
                     rows = max(offset(p, e + 1) - begin, 0);
                     part.expert = e;
-                    if (left < tiles_of(rows)) break;
-                    left -= tiles_of(rows);
+                    if (at < tiles_of(rows) * p.groups_n) break;
+                    at -= tiles_of(rows) * p.groups_n;
                 }
                 begin = __builtin_amdgcn_readfirstlane(begin);
                 rows = __builtin_amdgcn_readfirstlane(rows);
-                left = __builtin_amdgcn_readfirstlane(left);
+                at = __builtin_amdgcn_readfirstlane(at);
                 part.expert = __builtin_amdgcn_readfirstlane(part.expert);
             }
-            part.row0 = begin + left * ROWS;
-            part.rows = min(ROWS, rows - left * ROWS);
+            tile_at(at, p.groups_n, tiles_of(rows), &part.group_n, &group_m);
+            part.row0 = begin + group_m * ROWS;
+            part.rows = min(ROWS, rows - group_m * ROWS);
         }
         return part;
     }
@@ -298,7 +299,7 @@ __global__ __launch_bounds__(64 * WK, 2) void i8_rows_kernel(const I8Params p) {
     static_assert(TN % 2 == 0, "whole tiles");
     const Tiles<GROUPED, kRows> tiles(p);
     if ((int)blockIdx.x >= p.groups_n * tiles.total) return;
-    const Part part = tiles.part(p, blockIdx.x);
+    const Part part = tiles.part(p);
     const int lane = threadIdx.x % 64, wk = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), q = lane / 16, col = lane % 16;
     const int blocks = p.blocks, row_bytes = blocks * kTileBlock, tile0 = part.group_n * (TN / 2), last = p.tiles - 1;
     const __amdgpu_buffer_rsrc_t weights = uniform_view(p.w + ((size_t)part.expert * p.tiles + tile0) * row_bytes, (unsigned)(min(TN / 2, p.tiles - tile0) * row_bytes));
@@ -465,7 +466,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void i8_wide_kernel(const I8Params
     Scales<kWidth>& scales = *reinterpret_cast<Scales<kWidth>*>(scale_room);
     const Tiles<GROUPED, kRows> tiles(p);
     if ((int)blockIdx.x >= p.groups_n * tiles.total) return;
-    const Part part = tiles.part(p, blockIdx.x);
+    const Part part = tiles.part(p);
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)staged;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wn = wave % WN, wm = wave / WN;
     const int blocks = p.blocks, row_bytes = blocks * kTileBlock, tile0 = (part.group_n * WN + wn) * TN, first = min(tile0, p.tiles - 1);
