@@ -85,19 +85,30 @@ __device__ __forceinline__ char* place_in_rows(char* lds, int row, int j) {
 }
 // (Nothing but whole pieces in the loop: code that a group runs once comes from memory line by line, 1 us each where a branch leaves the straight line. With
 // the cut pieces inside it the same loop took 2 to 14 us a group, by the XCD. The stores go past L2: 8192 x 8192 x 4096 263 -> 237 us.)
+// `past_l2` is for rows that begin on lines: lines that two groups write parts of are put together in L2 (8192 x 5003 in halves 68 us past it, 61 through it).
 template <typename O, int WIDTH, int ROWS, int THREADS>
-__device__ __forceinline__ void store_rows(const char* lds, O* y, size_t stride, int row0, int rows, int j0, int n) {
+__device__ __forceinline__ void store_rows(const char* lds, O* y, size_t stride, int row0, int rows, int j0, int n, bool past_l2 = true) {
     constexpr int kPer = 16 / sizeof(O), kPieces = WIDTH / kPer, kPitch = WIDTH * (int)sizeof(O), kTogether = THREADS / kPieces;
     static_assert(THREADS % kPieces == 0 && ROWS % kTogether == 0, "every thread stores one piece of every kTogether-th row");
     const int piece = threadIdx.x % kPieces, first = threadIdx.x / kPieces, j = j0 + piece * kPer;
     O* const dst = y + (size_t)(row0 + first) * stride + j;
     const size_t step = (size_t)kTogether * stride;
     const bool whole = j + kPer <= n;
+    auto held = [&](int row) { return *reinterpret_cast<const v4i*>(lds + row * kPitch + byte_in_row<O, WIDTH>(row, piece * 16)); };
+    if (past_l2) {
 #pragma unroll 4
-    for (int i = 0; i < ROWS / kTogether; ++i) {
-        const int row = i * kTogether + first;
-        const v4i v = *reinterpret_cast<const v4i*>(lds + row * kPitch + byte_in_row<O, WIDTH>(row, piece * 16));
-        if (whole && row < rows) __builtin_nontemporal_store(v, reinterpret_cast<v4i_any*>(dst + i * step));
+        for (int i = 0; i < ROWS / kTogether; ++i) {
+            const int row = i * kTogether + first;
+            const v4i v = held(row);
+            if (whole && row < rows) __builtin_nontemporal_store(v, reinterpret_cast<v4i_any*>(dst + i * step));
+        }
+    } else {
+#pragma unroll 4
+        for (int i = 0; i < ROWS / kTogether; ++i) {
+            const int row = i * kTogether + first;
+            const v4i v = held(row);
+            if (whole && row < rows) *reinterpret_cast<v4i_any*>(dst + i * step) = v;
+        }
     }
     if (j0 + WIDTH > n && n % kPer != 0) {
         const int at = n / kPer * kPer, left = n - at;

@@ -415,7 +415,7 @@ __device__ __forceinline__ void store_group(O* y, size_t stride, const v4f (&v)[
             }
         }
         __syncthreads();
-        store_rows<O, kWidth, kRows, 64 * WN * WM>(lds, y, stride, part.row0 + pass * kRows, part.rows - pass * kRows, j0, n);
+        store_rows<O, kWidth, kRows, 64 * WN * WM>(lds, y, stride, part.row0 + pass * kRows, part.rows - pass * kRows, j0, n, ((uintptr_t)y | stride * sizeof(O)) % 128 == 0);
     }
 }
 
@@ -456,10 +456,14 @@ __device__ __forceinline__ void write_group(const I8Params& p, const Part& part,
 // L2 straight into registers, those of a step of 32 values as soon as the same step of the block before is done with them. Every step's rows are read from LDS while the
 // products of the step before run, and loads stand between the products one by one. A block's one barrier, at its start, says that the next block's rows are there and that
 // the last block's buffer may be filled.
-template <int TN, int TM, int WN, int WM, bool GATED, bool GROUPED>
+constexpr int most_on_their_way(int loads) { return loads < 63 ? loads : 63; }  // as many as a wait can name
+
+template <int TN, int TM, int WN, int WM, int BUFFERS, int D, bool GATED, bool GROUPED>
 __global__ __launch_bounds__(64 * WN * WM, 2) void i8_wide_kernel(const I8Params p) {
     exhip_touch_args(p);
-    constexpr int kWaves = WN * WM, kRows = 32 * TM * WM, kBuffers = 4, kBuffer = kRows * kBlk, kLoads = kRows / 8 / kWaves, kWidth = TN * WN * (GATED ? 16 : 32), kProducts = TN * TM;
+    constexpr int kWaves = WN * WM, kRows = 32 * TM * WM, kBuffers = BUFFERS, kBuffer = kRows * kBlk, kLoads = kRows / 8 / kWaves, kWidth = TN * WN * (GATED ? 16 : 32), kProducts = TN * TM;
+    constexpr int kAhead = kProducts < 4 ? 4 * TM : TM;  // pieces of rows on their way from LDS: a step's, or a block's where a step's products are too few to wait behind
+    static_assert(D * 4 * TM % (2 * kAhead) == 0 && D >= kBuffers - 3);
     constexpr int kResults = kRows * kWidth * 2, kRoom = kBuffers * kBuffer > kResults ? kBuffers * kBuffer : kResults;
     __shared__ __attribute__((aligned(16))) char staged[kRoom];
     __shared__ __attribute__((aligned(16))) char scale_room[sizeof(Scales<kWidth>) + kRows * 4];
@@ -476,12 +480,12 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void i8_wide_kernel(const I8Params
     unsigned off[kLoads];
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) off[j] = rows.begin(rows.source((wave * kLoads + j) * 8 + lane / 8)) + ((lane % 8) ^ (lane / 8)) * 16;
-    auto stage = [&](int buffer, int j) {  // behind the last block that one again, which nothing reads
-        load16_to_lds(rows.view, off[j], min(buffer, blocks - 1) * kBlk, lds0 + buffer % kBuffers * kBuffer + (wave * kLoads + j) * 1024);
+    auto stage = [&](int buffer, int j) {  // behind the last block zeros, which nothing reads
+        load16_to_lds(rows.view, buffer < blocks ? off[j] : kNoRow, buffer * kBlk, lds0 + buffer % kBuffers * kBuffer + (wave * kLoads + j) * 1024);
     };
-    v4i w[4][TN];
-    auto request = [&](int b, int s, int i) {
-        w[s][i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(weights, lane * 16, min(i, p.tiles - 1 - first) * row_bytes + min(b, blocks - 1) * kTileBlock + s * 1024, 0));
+    v4i w[D][4][TN];
+    auto request = [&](v4i (&w)[4][TN], int b, int s, int i) {
+        w[s][i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(weights, b < blocks ? lane * 16 : kNoRow, min(i, p.tiles - 1 - first) * row_bytes + b * kTileBlock + s * 1024, 0));
     };
     // scales and biases, for the end
     for (int r = threadIdx.x; r < kRows; r += 64 * kWaves) scales.row[r] = rows.scale(rows.source(r));
@@ -502,46 +506,48 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void i8_wide_kernel(const I8Params
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][t][e] = 0;
 #pragma unroll
-    for (int j = 0; j < 3 * kLoads; ++j) stage(j / kLoads, j % kLoads);
+    for (int j = 0; j < (kBuffers - 1) * kLoads; ++j) stage(j / kLoads, j % kLoads);
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+    for (int s = 0; s < 4 * D; ++s)
 #pragma unroll
-        for (int i = 0; i < TN; ++i) request(0, s, i);
+        for (int i = 0; i < TN; ++i) request(w[s / 4], s / 4, s % 4, i);
     auto arrive = [&] {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads + 4 * TN) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(most_on_their_way((kBuffers - 2) * kLoads + 4 * TN * D)) : "memory");
     arrive();
     const int at = (wm * TM * 32 + lane % 32) * kBlk + ((lane / 32) ^ (lane % 8)) * 16;
     auto rows_from = [&](int b, int s, int t) { return *reinterpret_cast<const v4i*>(staged + b % kBuffers * kBuffer + (at ^ (s * 32)) + t * 32 * kBlk); };
-    v4i x[2][TM];
+    v4i x[2 * kAhead];
 #pragma unroll
-    for (int t = 0; t < TM; ++t) x[0][t] = rows_from(0, 0, t);
-    for (int b = 0; b < blocks; ++b) {
-        // all but the loads of the block before
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLoads + 4 * TN) : "memory");
+    for (int f = 0; f < kAhead; ++f) x[f] = rows_from(0, f / TM, f % TM);
+    auto block = [&](v4i (&w)[4][TN], int b, int ring) {  // `ring`: where in x its rows begin
+        // all but the loads of the block before (and the first ones' weights)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(most_on_their_way((kBuffers - 3) * (kLoads + 4 * TN))) : "memory");
         arrive();
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
 #pragma unroll
             for (int u = 0; u < kProducts; ++u) {
-                const int t = u / TN, i = u % TN;
-                if (i == 0) x[(s + 1) % 2][t] = s < 3 ? rows_from(b, s + 1, t) : rows_from(b + 1, 0, t);
+                const int t = u / TN, i = u % TN, f = s * TM + t, ahead = f + kAhead;
+                if (i == 0) x[(ring + ahead) % (2 * kAhead)] = ahead < 4 * TM ? rows_from(b, ahead / TM, ahead % TM) : rows_from(b + 1, ahead / TM - 4, ahead % TM);
                 if (u == kProducts / 4)
 #pragma unroll
-                    for (int j = s * kLoads / 4; j < (s + 1) * kLoads / 4; ++j) stage(b + 3, j);
-                acc[i][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[s][i], x[s % 2][t], acc[i][t], 0, 0, 0);
-                if (u >= kProducts - TN) request(b + 1, s, u - (kProducts - TN));
+                    for (int j = s * kLoads / 4; j < (s + 1) * kLoads / 4; ++j) stage(b + kBuffers - 1, j);
+                acc[i][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[s][i], x[(ring + f) % (2 * kAhead)], acc[i][t], 0, 0, 0);
+                if (u >= kProducts - TN) request(w, b + D, s, u - (kProducts - TN));
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-    }
+    };
+    for (int first_block = 0; first_block < blocks; first_block += D)
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+            if (first_block + d < blocks) block(w[d], first_block + d, d * 4 * TM % (2 * kAhead));
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was staged behind the end, in front of the results' barrier
     write_group<WN, WM, TN, TM, GATED, kRoom>(p, part, acc, wn, wm, lane, staged, scales);
 }
-
-constexpr int kCus = 256;
 
 int blocks_of(int v) { return v / kBlk + (v % kBlk != 0); }
 int tiles_of(int n, bool gated_product) { return gated_product ? (n + 15) / 16 : (n + 31) / 32; }
@@ -583,12 +589,31 @@ int launch(exhip_ctx* ctx, K kernel, I8Params p, int tiles, int rows, int thread
     return 0;
 }
 
+// One way to run a product: the tiles of 32 outputs (of both projections) and the rows that a group takes.
+struct Form {
+    int (*run)(exhip_ctx*, const I8Params&);
+    int tiles, rows, least_blocks;
+};
+template <int TN, int TM, int WK, int D, bool GATED, bool GROUPED>
+int run_rows(exhip_ctx* ctx, const I8Params& p) {
+    return launch(ctx, i8_rows_kernel<TN, TM, WK, D, GATED, GROUPED>, p, TN / 2, 16 * TM, 64 * WK);
+}
+template <int TN, int TM, int WN, int WM, int BUFFERS, int D, bool GATED, bool GROUPED>
+int run_wide(exhip_ctx* ctx, const I8Params& p) {
+    return launch(ctx, i8_wide_kernel<TN, TM, WN, WM, BUFFERS, D, GATED, GROUPED>, p, TN * WN, 32 * TM * WM, 64 * WN * WM);
+}
+template <bool GATED, bool GROUPED>
+constexpr Form kForms[] = {
+    {run_rows<2, 1, 8, 2, GATED, GROUPED>, 1, 16},         {run_rows<2, 2, 8, 2, GATED, GROUPED>, 1, 32},         {run_rows<4, 2, 8, 1, GATED, GROUPED>, 2, 32},
+    {run_wide<1, 1, 2, 1, 8, 8, GATED, GROUPED>, 2, 32},   {run_wide<1, 1, 4, 1, 4, 4, GATED, GROUPED>, 4, 32},
+    {run_wide<1, 2, 4, 1, 4, 4, GATED, GROUPED>, 4, 64},   {run_wide<2, 2, 4, 1, 5, 2, GATED, GROUPED>, 8, 64},   {run_wide<2, 4, 4, 1, 4, 1, GATED, GROUPED>, 8, 128},
+};
+
 template <bool GATED, bool GROUPED>
 int run_best(exhip_ctx* ctx, const I8Params& p) {
-    const int form = p.blocks < 4 ? 1 : g_exhip_options.i8_form > 0 ? g_exhip_options.i8_form : p.m <= 64 ? 1 : (long long)p.m * p.tiles <= 1 << 17 ? 2 : 3;
-    if (form >= 3) return launch(ctx, i8_wide_kernel<2, 4, 4, 1, GATED, GROUPED>, p, 8, 128, 256);
-    if (form == 2) return launch(ctx, i8_wide_kernel<2, 2, 4, 1, GATED, GROUPED>, p, 8, 64, 256);
-    return launch(ctx, i8_rows_kernel<2, 1, 8, 2, GATED, GROUPED>, p, 1, 16, 512);
+    const int n = sizeof(kForms<GATED, GROUPED>) / sizeof(Form);
+    int f = g_exhip_options.i8_form > 0 ? (g_exhip_options.i8_form < n ? g_exhip_options.i8_form : n) - 1 : p.m <= 64 ? 0 : (long long)p.m * p.tiles <= 1 << 17 ? 5 : 7;
+    return kForms<GATED, GROUPED>[f].run(ctx, p);
 }
 
 struct Experts {  // of a product by experts
