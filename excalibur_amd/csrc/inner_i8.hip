@@ -4,6 +4,8 @@
 // v_mfma_i32_16x16x64_i8 in 32 bits and exact for as many as 131071 values a row. A result is sum * row's scale * output's scale + bias, rounded in that order; which kernel
 // takes a call, and how it cuts the sums, changes no bit of it. Weights are the first operand, rows of the input the second: a lane's results are then
 // runs of four neighbouring outputs of one row.
+#include <math.h>
+
 #include "inner.h"
 
 namespace {
@@ -589,10 +591,11 @@ int launch(exhip_ctx* ctx, K kernel, I8Params p, int tiles, int rows, int thread
     return 0;
 }
 
-// One way to run a product: the tiles of 32 outputs (of both projections) and the rows that a group takes.
+// One way to run a product: the tiles of 32 outputs (of both projections) and the rows that a group takes, how many groups a CU runs at once and how many waves share
+// a group's blocks.
 struct Form {
     int (*run)(exhip_ctx*, const I8Params&);
-    int tiles, rows, least_blocks;
+    int tiles, rows, at_once, split;
 };
 template <int TN, int TM, int WK, int D, bool GATED, bool GROUPED>
 int run_rows(exhip_ctx* ctx, const I8Params& p) {
@@ -602,18 +605,65 @@ template <int TN, int TM, int WN, int WM, int BUFFERS, int D, bool GATED, bool G
 int run_wide(exhip_ctx* ctx, const I8Params& p) {
     return launch(ctx, i8_wide_kernel<TN, TM, WN, WM, BUFFERS, D, GATED, GROUPED>, p, TN * WN, 32 * TM * WM, 64 * WN * WM);
 }
+constexpr int kCount = 8;
 template <bool GATED, bool GROUPED>
-constexpr Form kForms[] = {
-    {run_rows<2, 1, 8, 2, GATED, GROUPED>, 1, 16},         {run_rows<2, 2, 8, 2, GATED, GROUPED>, 1, 32},         {run_rows<4, 2, 8, 1, GATED, GROUPED>, 2, 32},
-    {run_wide<1, 1, 2, 1, 8, 8, GATED, GROUPED>, 2, 32},   {run_wide<1, 1, 4, 1, 4, 4, GATED, GROUPED>, 4, 32},
-    {run_wide<1, 2, 4, 1, 4, 4, GATED, GROUPED>, 4, 64},   {run_wide<2, 2, 4, 1, 5, 2, GATED, GROUPED>, 8, 64},   {run_wide<2, 4, 4, 1, 4, 1, GATED, GROUPED>, 8, 128},
+constexpr Form kForms[kCount] = {
+    {run_rows<2, 1, 8, 2, GATED, GROUPED>, 1, 16, 2, 8},       {run_rows<2, 2, 8, 2, GATED, GROUPED>, 1, 32, 2, 8},
+    {run_rows<4, 2, 8, 1, GATED, GROUPED>, 2, 32, 2, 8},       {run_wide<1, 1, 2, 1, 8, 8, GATED, GROUPED>, 2, 32, 4, 1},
+    {run_wide<1, 1, 4, 1, 4, 4, GATED, GROUPED>, 4, 32, 4, 1}, {run_wide<1, 2, 4, 1, 4, 4, GATED, GROUPED>, 4, 64, 2, 1},
+    {run_wide<2, 2, 4, 1, 5, 2, GATED, GROUPED>, 8, 64, 3, 1}, {run_wide<2, 4, 4, 1, 4, 1, GATED, GROUPED>, 8, 128, 2, 1},
 };
+// What a launch takes, in us: `start`; each time that all CUs are given groups, `round`, and for each block of one wave `alone`, or `share` for each group on a CU where that is more,
+// and `gate` for an activation; but no less than reading the weights from memory and what groups read again from L2, at so many bytes a us. Chosen so that the form with the least of
+// these times is as near to the fastest as it can be over 372 products and 350 products by experts, from 1 to 4096 rows and 512 x 512 to 11264 x 4096, 2 to 256 experts: it takes 0.6 % and
+// 1.2 % longer on average, 20 % and 32 % at most (profiles/inner_i8_forms.txt). Without any one form the products would take up to 1.28 times as long.
+struct Cost {
+    float start, round, alone, share, memory, gate, l2;
+};
+constexpr Cost kPlainCosts[kCount] = {
+    {1.84f, 0.06f, 1.00f, 1.43f, 5.99e6f, 0.20f, 485e6f},  {2.26f, 0.f, 1.58f, 0.23f, 13.3e6f, 0.22f, 12.2e6f},   {3.14f, 0.f, 0.76f, 1.56f, 8.14e6f, 0.04f, 17.8e6f},
+    {2.16f, 1.51f, 0.26f, 0.14f, 5.57e6f, 0.76f, 36.1e6f}, {2.81f, 0.f, 0.01f, 0.31f, 5.40e6f, 0.50f, 26.3e6f},   {3.01f, 0.f, 0.f, 0.31f, 5.01e6f, 0.70f, 20.8e6f},
+    {2.13f, 1.69f, 0.60f, 0.03f, 4.56e6f, 1.73f, 19.0e6f}, {4.02f, 0.15f, 0.78f, 0.52f, 3.44e6f, 3.90f, 22.6e6f},
+};
+constexpr Cost kGroupedCosts[kCount] = {
+    {0.54f, 3.70f, 0.f, 0.20f, 6.47e6f, 0.03f, 4.37e6f},   {3.19f, 2.71f, 0.06f, 0.93f, 10.8e6f, 0.11f, 87.8e6f}, {6.57f, 0.53f, 1.87f, 0.01f, 6.87e6f, 0.13f, 14.3e6f},
+    {3.17f, 0.11f, 0.f, 0.37f, 6.58e6f, 0.53f, 21.7e6f},   {3.52f, 1.61f, 0.30f, 0.27f, 6.56e6f, 0.45f, 29.8e6f}, {2.92f, 3.22f, 0.04f, 0.32f, 6.60e6f, 0.42f, 12.2e6f},
+    {4.34f, 2.31f, 0.51f, 0.38f, 6.79e6f, 1.94f, 19.7e6f}, {5.42f, 1.37f, 0.23f, 0.63f, 6.65e6f, 5.17f, 13.9e6f},
+};
+
+constexpr int kCus = 256;
+
+float time_of(const Form& f, const Cost& c, const I8Params& p, bool gated_product) {
+    // By experts the rows of each are not known here: as many have rows as would have by chance, and the last tile of each is half full.
+    const float m = (float)p.m, experts = p.offsets ? (float)p.experts * (1.f - expf(-m / (float)p.experts)) : 1.f;
+    const float tiles_m = !p.offsets ? (float)((p.m - 1) / f.rows + 1) : fmaxf(experts, m / experts > 0.25f * (float)f.rows ? m / (float)f.rows + 0.5f * experts : 0.f);
+    const float groups = (float)((p.tiles + f.tiles - 1) / f.tiles) * tiles_m, times = ceilf(groups / kCus), full = floorf(times / (float)f.at_once), rest = times - full * (float)f.at_once;
+    const float blocks = (float)((p.blocks - 1) / f.split + 1), gate = gated_product ? c.gate : 0.f;
+    float us = c.start + full * (c.round + blocks * fmaxf(c.alone, (float)f.at_once * c.share)) + gate * times;
+    if (rest > 0.f) us += c.round + blocks * fmaxf(c.alone, rest * c.share);
+    const float weights = experts * (float)p.tiles * (float)p.blocks * (float)kTileBlock;
+    const float again = fmaxf(0.f, groups * blocks * (float)(f.tiles * kTileBlock + f.rows * kBlk) - weights);
+    return fmaxf(us, c.start + 1.f + gate + weights / c.memory + again / c.l2);
+}
 
 template <bool GATED, bool GROUPED>
 int run_best(exhip_ctx* ctx, const I8Params& p) {
-    const int n = sizeof(kForms<GATED, GROUPED>) / sizeof(Form);
-    int f = g_exhip_options.i8_form > 0 ? (g_exhip_options.i8_form < n ? g_exhip_options.i8_form : n) - 1 : p.m <= 64 ? 0 : (long long)p.m * p.tiles <= 1 << 17 ? 5 : 7;
-    return kForms<GATED, GROUPED>[f].run(ctx, p);
+    const Form(&forms)[kCount] = kForms<GATED, GROUPED>;
+    const int pinned = g_exhip_options.i8_form;
+    int best = 0;
+    if (pinned > 0) {
+        best = (pinned < kCount ? pinned : kCount) - 1;
+    } else {
+        float least = 0.f;
+        for (int i = 0; i < kCount; ++i) {
+            const float us = time_of(forms[i], (GROUPED ? kGroupedCosts : kPlainCosts)[i], p, GATED);
+            if (i == 0 || us < least) {
+                least = us;
+                best = i;
+            }
+        }
+    }
+    return forms[best].run(ctx, p);
 }
 
 struct Experts {  // of a product by experts
