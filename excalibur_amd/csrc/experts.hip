@@ -9,42 +9,48 @@ constexpr int kMostChoices = 1 << 28;
 
 // An expert a group: its waves count, each in its own stretch of the choices, those of earlier experts and those of this one, and go over the stretch again to
 // write where they stand. No count depends on another group, so one launch does it and the order is that of the choices. Four choices a lane and 256 a wave at a
-// time, of which HELD stay in registers between the counting and the writing; where a stretch has more they are read again.
-typedef int v4i_of_four __attribute__((ext_vector_type(4), aligned(4)));
-
+// time, of which HELD stay in registers between the counting and the writing; where a stretch has more they are read again. Lanes count for themselves, two instructions a
+// choice and count, and are added up once. (65528 choices of 256 experts: every CU reads all of them from L2.)
 template <int HELD>
-__global__ __launch_bounds__(1024) void group_rows_kernel(const int* __restrict__ ids, int choices, int each, int experts, int* __restrict__ offsets, int* __restrict__ rows,
-                                                          int* __restrict__ places) {
+__global__ __launch_bounds__(1024) void group_rows_kernel(const int* __restrict__ ids, int choices, exhip_divisor row_of, int experts, int* __restrict__ offsets,
+                                                          int* __restrict__ rows, int* __restrict__ places) {
     constexpr int kWaves = 16;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, expert = blockIdx.x;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), expert = blockIdx.x;
     const int stretch = ((choices + kWaves - 1) / kWaves + 255) / 256 * 256;
     const long long from = (long long)wave * stretch;
     const int begin = from < choices ? (int)from : choices, end = min(choices - begin, stretch) + begin, pieces = (end - begin + 255) / 256;
+    const __amdgpu_buffer_rsrc_t view = uniform_view(ids + begin, (unsigned)(end - begin) * 4u);
     __shared__ int before[kWaves], own[kWaves];
-    auto four = [&](int piece) {  // -1 behind the end
-        const int at = begin + piece * 256 + lane * 4;
-        v4i v = {-1, -1, -1, -1};
-        if (at + 4 <= end) v = *reinterpret_cast<const v4i_of_four*>(ids + at);
-        else
+    auto four = [&](int piece) { return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(view, piece * 1024 + lane * 16, 0, 0)); };
+    auto ended = [&](v4i v, int piece) {  // -1 behind the end
+        if (begin + (piece + 1) * 256 > end)
 #pragma unroll
-            for (int e = 0; e < 3; ++e)
-                if (at + e < end) v[e] = ids[at + e];
+            for (int e = 0; e < 4; ++e) v[e] = begin + piece * 256 + lane * 4 + e < end ? v[e] : -1;
         return v;
     };
     int less = 0, equal = 0;
     auto count = [&](const v4i& v) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            less += __popcll(__ballot((unsigned)v[e] < (unsigned)expert));
-            equal += __popcll(__ballot(v[e] == expert));
+            less += (unsigned)v[e] < (unsigned)expert ? 1 : 0;
+            equal += v[e] == expert ? 1 : 0;
         }
     };
     v4i held[HELD];
 #pragma unroll
     for (int i = 0; i < HELD; ++i) held[i] = four(i);
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) count(held[i]);
-    for (int i = HELD; i < pieces; ++i) count(four(i));
+    for (int i = 0; i < HELD; ++i) {
+        held[i] = ended(held[i], i);
+        count(held[i]);
+    }
+#pragma unroll 4
+    for (int i = HELD; i < pieces; ++i) count(ended(four(i), i));
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        less += __shfl_xor(less, d);
+        equal += __shfl_xor(equal, d);
+    }
     if (lane == 0) {
         before[wave] = less;
         own[wave] = equal;
@@ -62,20 +68,22 @@ __global__ __launch_bounds__(1024) void group_rows_kernel(const int* __restrict_
         offsets[expert] = first;
         if (expert == experts - 1) offsets[experts] = first + all;
     }
+    int its = expert;
+    asm volatile("" : "+s"(its));  // or the counting's comparisons are kept, two scalar registers each, and there are not so many
     auto write = [&](int piece, const v4i& v) {
         const int at = begin + piece * 256 + lane * 4;
-        unsigned long long mask[4], any = 0;
+        unsigned long long mask[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) any |= mask[e] = __ballot(v[e] == expert);
-        if (any) {
-            const unsigned long long earlier = (1ull << lane) - 1;
-            int to = place;
+        for (int e = 0; e < 4; ++e) mask[e] = __ballot(v[e] == its);
+        if (mask[0] | mask[1] | mask[2] | mask[3]) {
+            int to = place;  // behind those of earlier lanes
 #pragma unroll
-            for (int e = 0; e < 4; ++e) to += __popcll(mask[e] & earlier);
+            for (int e = 0; e < 4; ++e) to = __builtin_amdgcn_mbcnt_hi((unsigned)(mask[e] >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask[e], to));
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (v[e] == expert) {
-                    rows[to] = (at + e) / each;
+                if (mask[e] == 0) continue;
+                if (v[e] == its) {
+                    rows[to] = (int)row_of(at + e);
                     places[at + e] = to++;
                 }
                 place += __popcll(mask[e]);
@@ -86,10 +94,11 @@ __global__ __launch_bounds__(1024) void group_rows_kernel(const int* __restrict_
             for (int e = 0; e < 4; ++e)
                 if ((unsigned)v[e] >= (unsigned)experts && at + e < end) places[at + e] = -1;
         }
+        __builtin_amdgcn_sched_barrier(0);
     };
 #pragma unroll
     for (int i = 0; i < HELD; ++i) write(i, held[i]);
-    for (int i = HELD; i < pieces; ++i) write(i, four(i));
+    for (int i = HELD; i < pieces; ++i) write(i, ended(four(i), i));
     if (expert == experts - 1)
         for (int i = first + all + threadIdx.x; i < choices; i += 1024) rows[i] = -1;
 }
@@ -179,7 +188,7 @@ int combine_rows(exhip_ctx* ctx, const char* name, const uint16_t* z, int z_stri
     EXHIP_REQUIRE(groups <= 0x7fffffff / 256, "%s: %d rows of %d outputs are more than one launch takes", name, m, n);
     const exhip_on_device on(ctx->device);
     EXHIP_CHECK(on.error);
-    hipLaunchKernelGGL((combine_rows_kernel<O, 4>), dim3((unsigned)groups), dim3(256), 0, ctx->stream, z, z_stride, z_rows, places, weights, kind, each, n, y, y_stride, waves_a_row, waves);
+    hipLaunchKernelGGL((combine_rows_kernel<O, 2>), dim3((unsigned)groups), dim3(256), 0, ctx->stream, z, z_stride, z_rows, places, weights, kind, each, n, y, y_stride, waves_a_row, waves);
     EXHIP_LAUNCH_CHECK();
     return 0;
 }
@@ -195,8 +204,10 @@ extern "C" int exhip_group_rows(exhip_ctx* ctx, const int32_t* ids, int m, int e
     const exhip_on_device on(ctx->device);
     EXHIP_CHECK(on.error);
     const int choices = m * each;
+    exhip_divisor row_of;
+    row_of.set(each);
     const auto kernel = choices <= 16 * 256 ? group_rows_kernel<1> : choices <= 16 * 1024 ? group_rows_kernel<4> : group_rows_kernel<16>;
-    hipLaunchKernelGGL(kernel, dim3(experts), dim3(1024), 0, ctx->stream, ids, choices, each, experts, offsets, rows, places);
+    hipLaunchKernelGGL(kernel, dim3(experts), dim3(1024), 0, ctx->stream, ids, choices, row_of, experts, offsets, rows, places);
     EXHIP_LAUNCH_CHECK();
     return 0;
 }

@@ -568,9 +568,13 @@ int quantize_rows(exhip_ctx* ctx, const char* name, const T* x, int x_stride, in
     constexpr int kWave = 64 * Piece<T>::kValues;
     auto run = [&](auto kernel, int rows) { hipLaunchKernelGGL(kernel, dim3((m - 1) / rows + 1), dim3(256), 0, ctx->stream, x, x_stride, m, k, y, y_stride, scale); };
     if (k <= kWave) run(quantize_rows_i8_kernel<T, 1, 1>, 4);
+    else if (k <= 2 * kWave && m > 512) run(quantize_rows_i8_kernel<T, 1, 2>, 4);
+    else if (k <= 3 * kWave && m > 512) run(quantize_rows_i8_kernel<T, 1, 3>, 4);
     else if (k <= 4 * kWave) run(quantize_rows_i8_kernel<T, 4, 1>, 1);
     else if (k <= 8 * kWave) run(quantize_rows_i8_kernel<T, 4, 2>, 1);
+    else if (k <= 12 * kWave) run(quantize_rows_i8_kernel<T, 4, 3>, 1);
     else if (k <= 16 * kWave) run(quantize_rows_i8_kernel<T, 4, 4>, 1);
+    else if (k <= 24 * kWave) run(quantize_rows_i8_kernel<T, 4, 6>, 1);
     else run(quantize_rows_i8_kernel<T, 4, 8>, 1);
     EXHIP_LAUNCH_CHECK();
     return 0;
