@@ -150,6 +150,19 @@ class F8Desc(ctypes.Structure):
 
 class I8Desc(ctypes.Structure):
     _fields_ = [(k, ctypes.c_int) for k in ("m", "n_out", "k_in", "x_stride", "y_stride")]
+    _counts = None
+
+    def __setattr__(self, name, value):
+        super().__setattr__(name, value)
+        if name != "_counts":
+            self._counts = None
+
+    def counts(self, experts=1, gated=False):
+        """Of how many experts and which product this is, and how many values its operands have: rows of the input where there are as many as of the result, packed
+        bytes, scales of the outputs, a result. Counted once for the calls that follow."""
+        packed = Ctx.i8_packed_bytes(self.n_out, self.k_in, gated, experts)
+        self._counts = (experts, gated), (self.m - 1) * self.x_stride + self.k_in, packed, experts * self.n_out, (self.m - 1) * self.y_stride + self.n_out
+        return self._counts
 
 
 F8_BLOCK = 128  # values that share a scale
@@ -771,7 +784,7 @@ class Ctx:
         if scale is None:
             scale = self.empty((m,), np.float32)
         y_stride = y.shape[1]
-        if not (_holds(x, (m - 1) * stride + k, _ROWS) and _holds(y, (m - 1) * y_stride + k, _CODES) and _holds(scale, m, _FLOATS)):
+        if not (x.size >= (m - 1) * stride + k and x.char in _ROWS and y.size >= (m - 1) * y_stride + k and y.char in _CODES and scale.size >= m and scale.char in _FLOATS):
             _refused(("x", x, (m - 1) * stride + k, _ROWS), ("y", y, (m - 1) * y_stride + k, _CODES), ("scale", scale, m, _FLOATS))
         entry = (_lib or lib()).exhip_quantize_rows_f32_to_i8 if x.char == "f" else (_lib or lib()).exhip_quantize_rows_f16_to_i8
         rc = entry(self.h, x.ptr, stride, m, k, y.ptr, y_stride, scale.ptr)
@@ -805,29 +818,39 @@ class Ctx:
             _size_refused(m, n_out, k_in, x_stride, y_stride)
         return I8Desc(m, n_out, k_in, x_stride, y_stride)
 
-    def _check_i8(self, d, experts, gated, x_rows, offsets, rows, x, x_scale, w, w_scale, w_scale_up, bias, bias_up, y_f32, y_f16):
-        """Operands of the products in 8-bit integers: their types, and that they hold what the call reads and writes."""
-        m, n, k = d.m, d.n_out, d.k_in
-        source = m if rows is None else x_rows
-        codes, packed, result, outputs = (source - 1) * d.x_stride + k, self.i8_packed_bytes(n, k, gated, experts), (m - 1) * d.y_stride + n, experts * n
-        if not (_holds(x, codes, _CODES) and _holds(x_scale, source, _FLOATS) and _holds(w, packed, _CODES) and _holds(w_scale, outputs, _FLOATS)
-                and _holds(w_scale_up, outputs, _FLOATS) and _holds(bias, outputs, _FLOATS) and _holds(bias_up, outputs, _FLOATS) and _holds(y_f32, result, _FLOATS)
-                and _holds(y_f16, result, _HALVES) and _holds(offsets, experts + 1, _IDS) and _holds(rows, m, _IDS)):
-            scale, b = ("w_scale_gate", "bias_gate") if gated else ("w_scale", "bias")
-            _refused(("x", x, codes, _CODES), ("x_scale", x_scale, source, _FLOATS), ("w", w, packed, _CODES), (scale, w_scale, outputs, _FLOATS),
-                     ("w_scale_up", w_scale_up, outputs, _FLOATS), (b, bias, outputs, _FLOATS), ("bias_up", bias_up, outputs, _FLOATS), ("y_f32", y_f32, result, _FLOATS),
-                     ("y_f16", y_f16, result, _HALVES), ("offsets", offsets, experts + 1, _IDS), ("rows", rows, m, _IDS))
+    @staticmethod
+    def _refused_i8(d, experts, gated, source, offsets, rows, x, x_scale, w, w_scale, w_scale_up, bias, bias_up, y_f32, y_f16):
+        """Says which operand of a product is of another type or too small; `source` rows of the input."""
+        _, _, packed, outputs, result = d.counts(experts, gated)
+        scale, b = ("w_scale_gate", "bias_gate") if gated else ("w_scale", "bias")
+        _refused(("x", x, (source - 1) * d.x_stride + d.k_in, _CODES), ("x_scale", x_scale, source, _FLOATS), ("w", w, packed, _CODES), (scale, w_scale, outputs, _FLOATS),
+                 ("w_scale_up", w_scale_up, outputs, _FLOATS), (b, bias, outputs, _FLOATS), ("bias_up", bias_up, outputs, _FLOATS), ("y_f32", y_f32, result, _FLOATS),
+                 ("y_f16", y_f16, result, _HALVES), ("offsets", offsets, experts + 1, _IDS), ("rows", rows, d.m, _IDS))
 
     def innerproduct_i8(self, d, x, x_scale, w, w_scale, bias=None, y_f32=None, y_f16=None):
-        self._check_i8(d, 1, False, 0, None, None, x, x_scale, w, w_scale, None, bias, None, y_f32, y_f16)
-        rc = (_lib or lib()).exhip_innerproduct_i8(self.h, ctypes.byref(d), x.ptr, x_scale.ptr, w.ptr, w_scale.ptr, _ptr(bias), _ptr(y_f32), _ptr(y_f16))
+        counts = d._counts
+        if counts is None or counts[0] != (1, False):
+            counts = d.counts()
+        _, codes, packed, n, result = counts
+        if not (x.size >= codes and x.char in _CODES and x_scale.size >= d.m and x_scale.char in _FLOATS and w.size >= packed and w.char in _CODES and w_scale.size >= n
+                and w_scale.char in _FLOATS and (bias is None or bias.size >= n and bias.char in _FLOATS) and (y_f32 is None or y_f32.size >= result and y_f32.char in _FLOATS)
+                and (y_f16 is None or y_f16.size >= result and y_f16.char in _HALVES)):
+            self._refused_i8(d, 1, False, d.m, None, None, x, x_scale, w, w_scale, None, bias, None, y_f32, y_f16)
+        rc = (_lib or lib()).exhip_innerproduct_i8(self.h, ctypes.byref(d), x.ptr, x_scale.ptr, w.ptr, w_scale.ptr, bias and bias.ptr, y_f32 and y_f32.ptr, y_f16 and y_f16.ptr)
         if rc:
             _check(rc)
 
     def innerproduct_gated_i8(self, d, x, x_scale, w, w_scale_gate, w_scale_up, gate="silu", bias_gate=None, bias_up=None, y_f32=None, y_f16=None):
-        self._check_i8(d, 1, True, 0, None, None, x, x_scale, w, w_scale_gate, w_scale_up, bias_gate, bias_up, y_f32, y_f16)
+        counts = d._counts
+        if counts is None or counts[0] != (1, True):
+            counts = d.counts(1, True)
+        _, codes, packed, n, result = counts
+        if not (x.size >= codes and x.char in _CODES and x_scale.size >= d.m and x_scale.char in _FLOATS and w.size >= packed and w.char in _CODES and w_scale_gate.size >= n
+                and w_scale_gate.char in _FLOATS and w_scale_up.size >= n and w_scale_up.char in _FLOATS and _holds(bias_gate, n, _FLOATS) and _holds(bias_up, n, _FLOATS)
+                and _holds(y_f32, result, _FLOATS) and _holds(y_f16, result, _HALVES)):
+            self._refused_i8(d, 1, True, d.m, None, None, x, x_scale, w, w_scale_gate, w_scale_up, bias_gate, bias_up, y_f32, y_f16)
         rc = (_lib or lib()).exhip_innerproduct_gated_i8(self.h, ctypes.byref(d), self.GATES[gate], x.ptr, x_scale.ptr, w.ptr, w_scale_gate.ptr, w_scale_up.ptr,
-                                                         _ptr(bias_gate), _ptr(bias_up), _ptr(y_f32), _ptr(y_f16))
+                                                         bias_gate and bias_gate.ptr, bias_up and bias_up.ptr, y_f32 and y_f32.ptr, y_f16 and y_f16.ptr)
         if rc:
             _check(rc)
 
@@ -842,7 +865,9 @@ class Ctx:
         offsets = self.empty((experts + 1,), np.int32) if offsets is None else offsets
         rows = self.empty((m * each,), np.int32) if rows is None else rows
         places = self.empty((m, each), np.int32) if places is None else places
-        if not (_holds(ids, m * each, _IDS) and _holds(offsets, experts + 1, _IDS) and _holds(rows, m * each, _IDS) and _holds(places, m * each, _IDS)):
+        count = m * each
+        if not (ids.size >= count and ids.char in _IDS and offsets.size > experts and offsets.char in _IDS and rows.size >= count and rows.char in _IDS and places.size >= count
+                and places.char in _IDS):
             _refused(("ids", ids, m * each, _IDS), ("offsets", offsets, experts + 1, _IDS), ("rows", rows, m * each, _IDS), ("places", places, m * each, _IDS))
         rc = (_lib or lib()).exhip_group_rows(self.h, ids.ptr, m, each, experts, offsets.ptr, rows.ptr, places.ptr)
         if rc:
@@ -851,18 +876,43 @@ class Ctx:
 
     def innerproduct_grouped_i8(self, d, experts, offsets, x, x_scale, w, w_scale, bias=None, rows=None, x_rows=0, y_f32=None, y_f16=None):
         """d.m rows in order by expert; with `rows` they are those of the x_rows rows of x."""
-        self._check_i8(d, experts, False, x_rows, offsets, rows, x, x_scale, w, w_scale, None, bias, None, y_f32, y_f16)
-        rc = (_lib or lib()).exhip_innerproduct_grouped_i8(self.h, ctypes.byref(d), experts, offsets.ptr, _ptr(rows), x_rows, x.ptr, x_scale.ptr, w.ptr, w_scale.ptr,
-                                                           _ptr(bias), _ptr(y_f32), _ptr(y_f16))
+        counts = d._counts
+        if counts is None or counts[0] != (experts, False):
+            counts = d.counts(experts, False)
+        _, codes, packed, n, result = counts
+        source = d.m
+        if rows is not None:
+            if x_rows > _MOST:
+                _size_refused(x_rows)
+            source, codes = x_rows, (x_rows - 1) * d.x_stride + d.k_in
+        if not (x.size >= codes and x.char in _CODES and x_scale.size >= source and x_scale.char in _FLOATS and w.size >= packed and w.char in _CODES and w_scale.size >= n
+                and w_scale.char in _FLOATS and _holds(bias, n, _FLOATS) and _holds(y_f32, result, _FLOATS) and _holds(y_f16, result, _HALVES)
+                and offsets.size > experts and offsets.char in _IDS and _holds(rows, d.m, _IDS)):
+            self._refused_i8(d, experts, False, source, offsets, rows, x, x_scale, w, w_scale, None, bias, None, y_f32, y_f16)
+        rc = (_lib or lib()).exhip_innerproduct_grouped_i8(self.h, ctypes.byref(d), experts, offsets.ptr, rows and rows.ptr, x_rows, x.ptr, x_scale.ptr, w.ptr, w_scale.ptr,
+                                                           bias and bias.ptr, y_f32 and y_f32.ptr, y_f16 and y_f16.ptr)
         if rc:
             _check(rc)
 
     def innerproduct_grouped_gated_i8(self, d, experts, offsets, x, x_scale, w, w_scale_gate, w_scale_up, gate="silu", bias_gate=None, bias_up=None, rows=None, x_rows=0,
                                       y_f32=None, y_f16=None):
         """d.m rows in order by expert; with `rows` they are those of the x_rows rows of x."""
-        self._check_i8(d, experts, True, x_rows, offsets, rows, x, x_scale, w, w_scale_gate, w_scale_up, bias_gate, bias_up, y_f32, y_f16)
-        rc = (_lib or lib()).exhip_innerproduct_grouped_gated_i8(self.h, ctypes.byref(d), self.GATES[gate], experts, offsets.ptr, _ptr(rows), x_rows, x.ptr, x_scale.ptr, w.ptr,
-                                                                 w_scale_gate.ptr, w_scale_up.ptr, _ptr(bias_gate), _ptr(bias_up), _ptr(y_f32), _ptr(y_f16))
+        counts = d._counts
+        if counts is None or counts[0] != (experts, True):
+            counts = d.counts(experts, True)
+        _, codes, packed, n, result = counts
+        source = d.m
+        if rows is not None:
+            if x_rows > _MOST:
+                _size_refused(x_rows)
+            source, codes = x_rows, (x_rows - 1) * d.x_stride + d.k_in
+        if not (x.size >= codes and x.char in _CODES and x_scale.size >= source and x_scale.char in _FLOATS and w.size >= packed and w.char in _CODES and w_scale_gate.size >= n
+                and w_scale_gate.char in _FLOATS and w_scale_up.size >= n and w_scale_up.char in _FLOATS and _holds(bias_gate, n, _FLOATS) and _holds(bias_up, n, _FLOATS)
+                and _holds(y_f32, result, _FLOATS) and _holds(y_f16, result, _HALVES) and offsets.size > experts and offsets.char in _IDS and _holds(rows, d.m, _IDS)):
+            self._refused_i8(d, experts, True, source, offsets, rows, x, x_scale, w, w_scale_gate, w_scale_up, bias_gate, bias_up, y_f32, y_f16)
+        rc = (_lib or lib()).exhip_innerproduct_grouped_gated_i8(self.h, ctypes.byref(d), self.GATES[gate], experts, offsets.ptr, rows and rows.ptr, x_rows, x.ptr, x_scale.ptr,
+                                                                 w.ptr, w_scale_gate.ptr, w_scale_up.ptr, bias_gate and bias_gate.ptr, bias_up and bias_up.ptr,
+                                                                 y_f32 and y_f32.ptr, y_f16 and y_f16.ptr)
         if rc:
             _check(rc)
 
@@ -877,7 +927,8 @@ class Ctx:
         if max(m, each, z_rows, z_stride, n, y_stride) > _MOST:
             _size_refused(m, each, z_rows, z_stride, n, y_stride)
         source, result, types = (z_rows - 1) * z_stride + n, (m - 1) * y_stride + n, _FLOATS if y_f16 is None else _HALVES
-        if not (_holds(z, source, _HALVES) and _holds(places, m * each, _IDS) and _holds(weights, m * each, _FLOATS) and _holds(y, result, types)):
+        if not (z.size >= source and z.char in _HALVES and places.size >= m * each and places.char in _IDS and weights.size >= m * each and weights.char in _FLOATS
+                and y.size >= result and y.char in types):
             _refused(("z", z, source, _HALVES), ("places", places, m * each, _IDS), ("weights", weights, m * each, _FLOATS), ("y_f32" if y_f16 is None else "y_f16", y, result, types))
         entry = (_lib or lib()).exhip_combine_rows_f32 if y_f16 is None else (_lib or lib()).exhip_combine_rows_f16
         rc = entry(self.h, z.ptr, z_stride, z_rows, places.ptr, weights.ptr, self.WEIGHTS[kind], m, each, n, y.ptr, y_stride)
