@@ -353,42 +353,43 @@ __global__ __launch_bounds__(64 * WK, 2) void i8_rows_kernel(const I8Params p) {
         }
     }
     constexpr int kWidth = TN * 16, kPitch = kWidth + 4, kThreads = 64 * WK, kQuads = kWidth / 4 / kSide;
-    static_assert(kRows * kQuads <= kThreads, "a thread has four outputs of one row");
     __shared__ __attribute__((aligned(16))) int joined[WK][kRows][kPitch];
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
         for (int t = 0; t < TM; ++t) *reinterpret_cast<v4i*>(&joined[wk][16 * t + col][i * 16 + q * 4]) = acc[i][t];
     __syncthreads();
-    const int quad = threadIdx.x % kQuads, row = threadIdx.x / kQuads, j = part.group_n * (kWidth / kSide) + quad * 4;
-    if (row >= part.rows || j >= p.n) return;
-    const float x_scale = rows.scale(rows.source(row));
     const size_t own = (size_t)part.expert * p.n;
-    const v4f w_scale = four_of(p.w_scale + own, j, p.n), bias = four_of(p.bias ? p.bias + own : nullptr, j, p.n);
-    const int from = GATED ? quad / 4 * 32 + quad % 4 * 4 : quad * 4;
-    v4i sum = {0, 0, 0, 0}, sum_up = {0, 0, 0, 0};
+    for (int i = threadIdx.x; i < kRows * kQuads; i += kThreads) {
+        const int quad = i % kQuads, row = i / kQuads, j = part.group_n * (kWidth / kSide) + quad * 4;
+        if (row >= part.rows || j >= p.n) continue;
+        const float x_scale = rows.scale(rows.source(row));
+        const v4f w_scale = four_of(p.w_scale + own, j, p.n), bias = four_of(p.bias ? p.bias + own : nullptr, j, p.n);
+        const int from = GATED ? quad / 4 * 32 + quad % 4 * 4 : quad * 4;
+        v4i sum = {0, 0, 0, 0}, sum_up = {0, 0, 0, 0};
 #pragma unroll
-    for (int k = 0; k < WK; ++k) {
-        sum += *reinterpret_cast<const v4i*>(&joined[k][row][from]);
-        if constexpr (GATED) sum_up += *reinterpret_cast<const v4i*>(&joined[k][row][from + 16]);
-    }
-    v4f v;
+        for (int k = 0; k < WK; ++k) {
+            sum += *reinterpret_cast<const v4i*>(&joined[k][row][from]);
+            if constexpr (GATED) sum_up += *reinterpret_cast<const v4i*>(&joined[k][row][from + 16]);
+        }
+        v4f v;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = result_of(sum[e], x_scale, w_scale[e], bias[e]);
-    if constexpr (GATED) {
-        const v4f w_scale_up = four_of(p.w_scale_up + own, j, p.n), bias_up = four_of(p.bias_up ? p.bias_up + own : nullptr, j, p.n);
+        for (int e = 0; e < 4; ++e) v[e] = result_of(sum[e], x_scale, w_scale[e], bias[e]);
+        if constexpr (GATED) {
+            const v4f w_scale_up = four_of(p.w_scale_up + own, j, p.n), bias_up = four_of(p.bias_up ? p.bias_up + own : nullptr, j, p.n);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = gated_value(p.gate, v[e], result_of(sum_up[e], x_scale, w_scale_up[e], bias_up[e]));
-    }
-    const size_t to = (size_t)(part.row0 + row) * p.y_stride + j;
-    const bool whole = j + 4 <= p.n;
-    if (p.y_f32) {
-        if (whole) *reinterpret_cast<v4f_any*>(p.y_f32 + to) = v;
-        else store_cut(p.y_f32 + to, v, p.n - j);
-    }
-    if (p.y_f16) {
-        if (whole) *reinterpret_cast<v4h_any*>(p.y_f16 + to) = __builtin_convertvector(v, v4h);
-        else store_cut(p.y_f16 + to, v, p.n - j);
+            for (int e = 0; e < 4; ++e) v[e] = gated_value(p.gate, v[e], result_of(sum_up[e], x_scale, w_scale_up[e], bias_up[e]));
+        }
+        const size_t to = (size_t)(part.row0 + row) * p.y_stride + j;
+        const bool whole = j + 4 <= p.n;
+        if (p.y_f32) {
+            if (whole) *reinterpret_cast<v4f_any*>(p.y_f32 + to) = v;
+            else store_cut(p.y_f32 + to, v, p.n - j);
+        }
+        if (p.y_f16) {
+            if (whole) *reinterpret_cast<v4h_any*>(p.y_f16 + to) = __builtin_convertvector(v, v4h);
+            else store_cut(p.y_f16 + to, v, p.n - j);
+        }
     }
 }
 
@@ -622,12 +623,12 @@ template <int TN, int TM, int WN, int WM, int BUFFERS, int D, bool GATED, bool G
 int run_wide(exhip_ctx* ctx, const I8Params& p) {
     return launch(ctx, i8_wide_kernel<TN, TM, WN, WM, BUFFERS, D, GATED, GROUPED>, p, TN * WN, 32 * TM * WM, 64 * WN * WM);
 }
-constexpr int kCount = 8;
+constexpr int kCount = 11;
 template <bool GATED, bool GROUPED>
 constexpr Form kForms[kCount] = {
-    {run_rows<2, 1, 8, 2, GATED, GROUPED>, 1, 16, 2, 8},       {run_rows<2, 2, 8, 2, GATED, GROUPED>, 1, 32, 2, 8},
-    {run_rows<4, 2, 8, 1, GATED, GROUPED>, 2, 32, 2, 8},       {run_wide<1, 1, 2, 1, 8, 8, GATED, GROUPED>, 2, 32, 4, 1},
-    {run_wide<1, 1, 4, 1, 4, 4, GATED, GROUPED>, 4, 32, 4, 1}, {run_wide<1, 2, 4, 1, 4, 4, GATED, GROUPED>, 4, 64, 2, 1},
+    {run_rows<2, 1, 8, 2, GATED, GROUPED>, 1, 16, 2, 8},       {run_rows<2, 1, 4, 2, GATED, GROUPED>, 1, 16, 5, 4},       {run_rows<2, 2, 4, 2, GATED, GROUPED>, 1, 32, 4, 4},
+    {run_rows<4, 1, 4, 2, GATED, GROUPED>, 2, 16, 3, 4},       {run_rows<4, 2, 4, 1, GATED, GROUPED>, 2, 32, 3, 4},       {run_rows<4, 4, 4, 1, GATED, GROUPED>, 2, 64, 2, 4},
+    {run_wide<1, 1, 2, 1, 8, 8, GATED, GROUPED>, 2, 32, 4, 1}, {run_wide<1, 1, 4, 1, 4, 4, GATED, GROUPED>, 4, 32, 4, 1}, {run_wide<1, 2, 4, 1, 4, 4, GATED, GROUPED>, 4, 64, 2, 1},
     {run_wide<2, 2, 4, 1, 5, 2, GATED, GROUPED>, 8, 64, 3, 1}, {run_wide<2, 4, 4, 1, 4, 1, GATED, GROUPED>, 8, 128, 2, 1},
 };
 // What a launch takes, in us: `start`; each time that all CUs are given groups, `round`, and for each block of one wave `alone`, or `share` for each group on a CU where that is more,
