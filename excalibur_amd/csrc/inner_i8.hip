@@ -603,11 +603,13 @@ int launch(exhip_ctx* ctx, K kernel, I8Params p, int tiles, int rows, int thread
     return 0;
 }
 
-// One way to run a product: the tiles of 32 outputs (of both projections) and the rows that a group takes, how many groups a CU runs at once and how many waves share
-// a group's blocks.
+// One way to run a product: the tiles of 32 outputs (of both projections) and the rows that a group takes, how many groups a CU runs at once, how many waves share a
+// group's blocks, and what a launch takes, in us: `start`; each time that all CUs are given groups, `round`, and for each block of one wave `alone`, or `share` for each
+// group on a CU where that is more; `gate` for an activation, each time; but no less than reading the weights from memory and what groups read again from L2, at so many bytes a us.
 struct Form {
     int (*run)(exhip_ctx*, const I8Params&);
     int tiles, rows, at_once, split;
+    float start, round, alone, share, memory, gate, l2;
 };
 constexpr long long kManyWeights = 40 << 20;
 template <int TN, int TM, int WK, int D, bool GATED, bool GROUPED>
@@ -623,58 +625,58 @@ template <int TN, int TM, int WN, int WM, int BUFFERS, int D, bool GATED, bool G
 int run_wide(exhip_ctx* ctx, const I8Params& p) {
     return launch(ctx, i8_wide_kernel<TN, TM, WN, WM, BUFFERS, D, GATED, GROUPED>, p, TN * WN, 32 * TM * WM, 64 * WN * WM);
 }
-constexpr int kCount = 11;
-template <bool GATED, bool GROUPED>
-constexpr Form kForms[kCount] = {
-    {run_rows<2, 1, 8, 2, GATED, GROUPED>, 1, 16, 2, 8},       {run_rows<2, 1, 4, 2, GATED, GROUPED>, 1, 16, 5, 4},       {run_rows<2, 2, 4, 2, GATED, GROUPED>, 1, 32, 4, 4},
-    {run_rows<4, 1, 4, 2, GATED, GROUPED>, 2, 16, 3, 4},       {run_rows<4, 2, 4, 1, GATED, GROUPED>, 2, 32, 3, 4},       {run_rows<4, 4, 4, 1, GATED, GROUPED>, 2, 64, 2, 4},
-    {run_wide<1, 1, 2, 1, 8, 8, GATED, GROUPED>, 2, 32, 4, 1}, {run_wide<1, 1, 4, 1, 4, 4, GATED, GROUPED>, 4, 32, 4, 1}, {run_wide<1, 2, 4, 1, 4, 4, GATED, GROUPED>, 4, 64, 2, 1},
-    {run_wide<2, 2, 4, 1, 5, 2, GATED, GROUPED>, 8, 64, 3, 1}, {run_wide<2, 4, 4, 1, 4, 1, GATED, GROUPED>, 8, 128, 2, 1},
+// Chosen so that the form with the least of these times is as near to the fastest as it can be over 522 products and 440 products by experts of 1 to 8192 rows, 200 to 11264
+// outputs and inputs and 2 to 256 experts: it takes 0.8 % and 2.3 % longer on average, 28 % and 23 % at most. Without any one form of the first list some product would take
+// 8 to 36 % longer, without one of the second 6 to 27 % (profiles/inner_i8_forms.txt).
+template <bool GATED>
+constexpr Form kPlain[] = {
+    {run_rows<2, 1, 8, 2, GATED, false>, 1, 16, 2, 8, 2.11f, 0.33f, 0.24f, 0.93f, 14.5e6f, 0.5f, 19.02e6f},
+    {run_rows<2, 1, 4, 2, GATED, false>, 1, 16, 5, 4, 2.09f, 0.07f, 1.09f, 0.03f, 10.4e6f, 0.45f, 19.65e6f},
+    {run_rows<2, 2, 4, 2, GATED, false>, 1, 32, 4, 4, 2.2f, 0.97f, 0.47f, 0.1f, 16e6f, 0.26f, 12.14e6f},
+    {run_rows<4, 1, 4, 2, GATED, false>, 2, 16, 3, 4, 2.35f, 0.57f, 0.08f, 0.67f, 8.8e6f, 0.33f, 25.06e6f},
+    {run_rows<4, 2, 4, 1, GATED, false>, 2, 32, 3, 4, 2.93f, 0.27f, 0.73f, 0.67f, 7.56e6f, 0.f, 18.71e6f},
+    {run_rows<4, 4, 4, 1, GATED, false>, 2, 64, 2, 4, 1.05f, 4.37f, 0.15f, 0.96f, 11.32e6f, 0.75f, 135.9e6f},
+    {run_wide<1, 1, 2, 1, 8, 8, GATED, false>, 2, 32, 4, 1, 2.01f, 2.31f, 0.2f, 0.12f, 4.77e6f, 0.18f, 30.28e6f},
+    {run_wide<1, 1, 4, 1, 4, 4, GATED, false>, 4, 32, 4, 1, 2.69f, 0.02f, 0.21f, 0.27f, 6.19e6f, 0.51f, 19.89e6f},
+    {run_wide<1, 2, 4, 1, 4, 4, GATED, false>, 4, 64, 2, 1, 1.44f, 2.16f, 0.32f, 0.26f, 4.29e6f, 0.67f, 18.4e6f},
+    {run_wide<2, 2, 4, 1, 5, 2, GATED, false>, 8, 64, 3, 1, 1.09f, 3.1f, 0.47f, 0.43f, 3.01e6f, 1.55f, 19.61e6f},
+    {run_wide<2, 4, 4, 1, 4, 1, GATED, false>, 8, 128, 2, 1, 4.54f, 0.02f, 0.69f, 0.63f, 2.96e6f, 5.88f, 132.6e6f},
 };
-// What a launch takes, in us: `start`; each time that all CUs are given groups, `round`, and for each block of one wave `alone`, or `share` for each group on a CU where that is more,
-// and `gate` for an activation; but no less than reading the weights from memory and what groups read again from L2, at so many bytes a us. Chosen so that the form with the least of
-// these times is as near to the fastest as it can be over 372 products and 350 products by experts, from 1 to 4096 rows and 512 x 512 to 11264 x 4096, 2 to 256 experts: it takes 0.6 % and
-// 1.2 % longer on average, 20 % and 32 % at most (profiles/inner_i8_forms.txt). Without any one form the products would take up to 1.28 times as long.
-struct Cost {
-    float start, round, alone, share, memory, gate, l2;
-};
-constexpr Cost kPlainCosts[kCount] = {
-    {1.84f, 0.06f, 1.00f, 1.43f, 5.99e6f, 0.20f, 485e6f},  {2.26f, 0.f, 1.58f, 0.23f, 13.3e6f, 0.22f, 12.2e6f},   {3.14f, 0.f, 0.76f, 1.56f, 8.14e6f, 0.04f, 17.8e6f},
-    {2.16f, 1.51f, 0.26f, 0.14f, 5.57e6f, 0.76f, 36.1e6f}, {2.81f, 0.f, 0.01f, 0.31f, 5.40e6f, 0.50f, 26.3e6f},   {3.01f, 0.f, 0.f, 0.31f, 5.01e6f, 0.70f, 20.8e6f},
-    {2.13f, 1.69f, 0.60f, 0.03f, 4.56e6f, 1.73f, 19.0e6f}, {4.02f, 0.15f, 0.78f, 0.52f, 3.44e6f, 3.90f, 22.6e6f},
-};
-constexpr Cost kGroupedCosts[kCount] = {
-    {0.54f, 3.70f, 0.f, 0.20f, 6.47e6f, 0.03f, 4.37e6f},   {3.19f, 2.71f, 0.06f, 0.93f, 10.8e6f, 0.11f, 87.8e6f}, {6.57f, 0.53f, 1.87f, 0.01f, 6.87e6f, 0.13f, 14.3e6f},
-    {3.17f, 0.11f, 0.f, 0.37f, 6.58e6f, 0.53f, 21.7e6f},   {3.52f, 1.61f, 0.30f, 0.27f, 6.56e6f, 0.45f, 29.8e6f}, {2.92f, 3.22f, 0.04f, 0.32f, 6.60e6f, 0.42f, 12.2e6f},
-    {4.34f, 2.31f, 0.51f, 0.38f, 6.79e6f, 1.94f, 19.7e6f}, {5.42f, 1.37f, 0.23f, 0.63f, 6.65e6f, 5.17f, 13.9e6f},
+template <bool GATED>
+constexpr Form kGrouped[] = {
+    {run_rows<2, 1, 4, 2, GATED, true>, 1, 16, 5, 4, 2.76f, 1.31f, 0.08f, 0.07f, 6.89e6f, 0.32f, 17.43e6f},
+    {run_rows<4, 1, 4, 2, GATED, true>, 2, 16, 3, 4, 2.89f, 1.04f, 0.11f, 0.57f, 6.69e6f, 0.16f, 17.23e6f},
+    {run_rows<4, 2, 4, 1, GATED, true>, 2, 32, 3, 4, 3.43f, 0.11f, 0.06f, 0.88f, 6.8e6f, 0.f, 15.1e6f},
+    {run_wide<1, 1, 4, 1, 4, 4, GATED, true>, 4, 32, 4, 1, 3.14f, 1.75f, 0.31f, 0.27f, 6.26e6f, 0.55f, 32.34e6f},
+    {run_wide<1, 2, 4, 1, 4, 4, GATED, true>, 4, 64, 2, 1, 3.11f, 2.12f, 0.06f, 0.29f, 6.48e6f, 0.9f, 19.75e6f},
+    {run_wide<2, 2, 4, 1, 5, 2, GATED, true>, 8, 64, 3, 1, 4.63f, 0.7f, 0.56f, 0.42f, 6.73e6f, 2.05f, 22.82e6f},
+    {run_wide<2, 4, 4, 1, 4, 1, GATED, true>, 8, 128, 2, 1, 5.32f, 1.94f, 0.27f, 0.58f, 6.92e6f, 5.23f, 14.45e6f},
 };
 
 constexpr int kCus = 256;
 
-float time_of(const Form& f, const Cost& c, const I8Params& p, bool gated_product) {
+// What a launch of a form takes, in us.
+float time_of(const Form& f, const I8Params& p, bool gated_product) {
     // By experts the rows of each are not known here: as many have rows as would have by chance, and the last tile of each is half full.
     const float m = (float)p.m, experts = p.offsets ? (float)p.experts * (1.f - expf(-m / (float)p.experts)) : 1.f;
     const float tiles_m = !p.offsets ? (float)((p.m - 1) / f.rows + 1) : fmaxf(experts, m / experts > 0.25f * (float)f.rows ? m / (float)f.rows + 0.5f * experts : 0.f);
     const float groups = (float)((p.tiles + f.tiles - 1) / f.tiles) * tiles_m, times = ceilf(groups / kCus), full = floorf(times / (float)f.at_once), rest = times - full * (float)f.at_once;
-    const float blocks = (float)((p.blocks - 1) / f.split + 1), gate = gated_product ? c.gate : 0.f;
-    float us = c.start + full * (c.round + blocks * fmaxf(c.alone, (float)f.at_once * c.share)) + gate * times;
-    if (rest > 0.f) us += c.round + blocks * fmaxf(c.alone, rest * c.share);
+    const float blocks = (float)((p.blocks - 1) / f.split + 1), gate = gated_product ? f.gate : 0.f;
+    float us = f.start + full * (f.round + blocks * fmaxf(f.alone, (float)f.at_once * f.share)) + gate * times;
+    if (rest > 0.f) us += f.round + blocks * fmaxf(f.alone, rest * f.share);
     const float weights = experts * (float)p.tiles * (float)p.blocks * (float)kTileBlock;
     const float again = fmaxf(0.f, groups * blocks * (float)(f.tiles * kTileBlock + f.rows * kBlk) - weights);
-    return fmaxf(us, c.start + 1.f + gate + weights / c.memory + again / c.l2);
+    return fmaxf(us, f.start + 1.f + gate + weights / f.memory + again / f.l2);
 }
 
-template <bool GATED, bool GROUPED>
-int run_best(exhip_ctx* ctx, const I8Params& p) {
-    const Form(&forms)[kCount] = kForms<GATED, GROUPED>;
+template <int N>
+int run_best(exhip_ctx* ctx, const I8Params& p, const Form (&forms)[N], bool gated_product) {
     const int pinned = g_exhip_options.i8_form;
-    int best = 0;
-    if (pinned > 0) {
-        best = (pinned < kCount ? pinned : kCount) - 1;
-    } else {
+    int best = pinned < N ? pinned - 1 : N - 1;
+    if (pinned <= 0) {
         float least = 0.f;
-        for (int i = 0; i < kCount; ++i) {
-            const float us = time_of(forms[i], (GROUPED ? kGroupedCosts : kPlainCosts)[i], p, GATED);
+        for (int i = 0; i < N; ++i) {
+            const float us = time_of(forms[i], p, gated_product);
             if (i == 0 || us < least) {
                 least = us;
                 best = i;
@@ -722,7 +724,7 @@ int product(exhip_ctx* ctx, const char* name, const exhip_i8_desc* d, const Expe
     p.blocks = blocks_of(d->k_in);
     p.tiles = tiles_of(d->n_out, gated_product);
     p.gate = gate;
-    if (!by) return gated_product ? run_best<true, false>(ctx, p) : run_best<false, false>(ctx, p);
+    if (!by) return gated_product ? run_best(ctx, p, kPlain<true>, true) : run_best(ctx, p, kPlain<false>, false);
     EXHIP_REQUIRE(by->count > 0 && by->count <= kMostExperts, "%s: %d experts: 1 to %d", name, by->count, kMostExperts);
     EXHIP_REQUIRE(aligned(by->offsets, 4) && aligned(by->rows, 4), "%s: an operand's address is not that of its type", name);
     p.experts = by->count;
@@ -733,7 +735,7 @@ int product(exhip_ctx* ctx, const char* name, const exhip_i8_desc* d, const Expe
                       by->x_rows, d->x_stride);
         p.x_rows = by->x_rows;
     }
-    return gated_product ? run_best<true, true>(ctx, p) : run_best<false, true>(ctx, p);
+    return gated_product ? run_best(ctx, p, kGrouped<true>, true) : run_best(ctx, p, kGrouped<false>, false);
 }
 
 }  // namespace
