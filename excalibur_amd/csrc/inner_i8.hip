@@ -625,32 +625,32 @@ template <int TN, int TM, int WN, int WM, int BUFFERS, int D, bool GATED, bool G
 int run_wide(exhip_ctx* ctx, const I8Params& p) {
     return launch(ctx, i8_wide_kernel<TN, TM, WN, WM, BUFFERS, D, GATED, GROUPED>, p, TN * WN, 32 * TM * WM, 64 * WN * WM);
 }
-// Chosen so that the form with the least of these times is as near to the fastest as it can be over 522 products and 440 products by experts of 1 to 8192 rows, 200 to 11264
-// outputs and inputs and 2 to 256 experts: it takes 0.8 % and 2.3 % longer on average, 28 % and 23 % at most. Without any one form of the first list some product would take
+// Chosen so that the form with the least of these times is as near to the fastest as it can be over 782 products and 700 products by experts of 1 to 8192 rows, 64 to 16384
+// outputs and inputs and 2 to 256 experts: it takes 1.4 % and 2.2 % longer on average, 34 % and 25 % at most. Without any one form of the first list some product would take
 // 8 to 36 % longer, without one of the second 6 to 27 % (profiles/inner_i8_forms.txt).
 template <bool GATED>
 constexpr Form kPlain[] = {
-    {run_rows<2, 1, 8, 2, GATED, false>, 1, 16, 2, 8, 2.11f, 0.33f, 0.24f, 0.93f, 14.5e6f, 0.5f, 19.02e6f},
-    {run_rows<2, 1, 4, 2, GATED, false>, 1, 16, 5, 4, 2.09f, 0.07f, 1.09f, 0.03f, 10.4e6f, 0.45f, 19.65e6f},
-    {run_rows<2, 2, 4, 2, GATED, false>, 1, 32, 4, 4, 2.2f, 0.97f, 0.47f, 0.1f, 16e6f, 0.26f, 12.14e6f},
-    {run_rows<4, 1, 4, 2, GATED, false>, 2, 16, 3, 4, 2.35f, 0.57f, 0.08f, 0.67f, 8.8e6f, 0.33f, 25.06e6f},
-    {run_rows<4, 2, 4, 1, GATED, false>, 2, 32, 3, 4, 2.93f, 0.27f, 0.73f, 0.67f, 7.56e6f, 0.f, 18.71e6f},
-    {run_rows<4, 4, 4, 1, GATED, false>, 2, 64, 2, 4, 1.05f, 4.37f, 0.15f, 0.96f, 11.32e6f, 0.75f, 135.9e6f},
-    {run_wide<1, 1, 2, 1, 8, 8, GATED, false>, 2, 32, 4, 1, 2.01f, 2.31f, 0.2f, 0.12f, 4.77e6f, 0.18f, 30.28e6f},
-    {run_wide<1, 1, 4, 1, 4, 4, GATED, false>, 4, 32, 4, 1, 2.69f, 0.02f, 0.21f, 0.27f, 6.19e6f, 0.51f, 19.89e6f},
-    {run_wide<1, 2, 4, 1, 4, 4, GATED, false>, 4, 64, 2, 1, 1.44f, 2.16f, 0.32f, 0.26f, 4.29e6f, 0.67f, 18.4e6f},
-    {run_wide<2, 2, 4, 1, 5, 2, GATED, false>, 8, 64, 3, 1, 1.09f, 3.1f, 0.47f, 0.43f, 3.01e6f, 1.55f, 19.61e6f},
-    {run_wide<2, 4, 4, 1, 4, 1, GATED, false>, 8, 128, 2, 1, 4.54f, 0.02f, 0.69f, 0.63f, 2.96e6f, 5.88f, 132.6e6f},
+    {run_rows<2, 1, 8, 2, GATED, false>, 1, 16, 2, 8, 2.01f, 0.84f, 0.27f, 0.58f, 12.86e6f, 0.22f, 13.23e6f},
+    {run_rows<2, 1, 4, 2, GATED, false>, 1, 16, 5, 4, 2.03f, 0.58f, 0.49f, 0.25f, 12.1e6f, 0.25f, 15.44e6f},
+    {run_rows<2, 2, 4, 2, GATED, false>, 1, 32, 4, 4, 2.24f, 0.65f, 0.49f, 0.04f, 9.57e6f, 0.17f, 15.64e6f},
+    {run_rows<4, 1, 4, 2, GATED, false>, 2, 16, 3, 4, 4.2f, 0.52f, 0.18f, 0.25f, 11.52e6f, 5.74f, 8.18e6f},
+    {run_rows<4, 2, 4, 1, GATED, false>, 2, 32, 3, 4, 2.83f, 0.1f, 0.68f, 0.87f, 8.26e6f, 0.f, 31.34e6f},
+    {run_rows<4, 4, 4, 1, GATED, false>, 2, 64, 2, 4, 1.68f, 2.92f, 0.09f, 1.1f, 13.96e6f, 0.f, 10.62e6f},
+    {run_wide<1, 1, 2, 1, 8, 8, GATED, false>, 2, 32, 4, 1, 2.05f, 1.46f, 0.14f, 0.13f, 3.76e6f, 0.72f, 24.88e6f},
+    {run_wide<1, 1, 4, 1, 4, 4, GATED, false>, 4, 32, 4, 1, 2.12f, 0.02f, 0.41f, 0.34f, 9.74e6f, 0.54f, 18.38e6f},
+    {run_wide<1, 2, 4, 1, 4, 4, GATED, false>, 4, 64, 2, 1, 1.62f, 1.4f, 0.38f, 0.25f, 6.75e6f, 0.91f, 18.39e6f},
+    {run_wide<2, 2, 4, 1, 5, 2, GATED, false>, 8, 64, 3, 1, 3.07f, 0.03f, 0.18f, 0.48f, 3.3e6f, 1.46f, 26.03e6f},
+    {run_wide<2, 4, 4, 1, 4, 1, GATED, false>, 8, 128, 2, 1, 4.34f, 0.36f, 0.13f, 0.65f, 3.92e6f, 4.82f, 27.51e6f},
 };
 template <bool GATED>
 constexpr Form kGrouped[] = {
-    {run_rows<2, 1, 4, 2, GATED, true>, 1, 16, 5, 4, 2.76f, 1.31f, 0.08f, 0.07f, 6.89e6f, 0.32f, 17.43e6f},
-    {run_rows<4, 1, 4, 2, GATED, true>, 2, 16, 3, 4, 2.89f, 1.04f, 0.11f, 0.57f, 6.69e6f, 0.16f, 17.23e6f},
-    {run_rows<4, 2, 4, 1, GATED, true>, 2, 32, 3, 4, 3.43f, 0.11f, 0.06f, 0.88f, 6.8e6f, 0.f, 15.1e6f},
-    {run_wide<1, 1, 4, 1, 4, 4, GATED, true>, 4, 32, 4, 1, 3.14f, 1.75f, 0.31f, 0.27f, 6.26e6f, 0.55f, 32.34e6f},
-    {run_wide<1, 2, 4, 1, 4, 4, GATED, true>, 4, 64, 2, 1, 3.11f, 2.12f, 0.06f, 0.29f, 6.48e6f, 0.9f, 19.75e6f},
-    {run_wide<2, 2, 4, 1, 5, 2, GATED, true>, 8, 64, 3, 1, 4.63f, 0.7f, 0.56f, 0.42f, 6.73e6f, 2.05f, 22.82e6f},
-    {run_wide<2, 4, 4, 1, 4, 1, GATED, true>, 8, 128, 2, 1, 5.32f, 1.94f, 0.27f, 0.58f, 6.92e6f, 5.23f, 14.45e6f},
+    {run_rows<2, 1, 4, 2, GATED, true>, 1, 16, 5, 4, 2.74f, 1.03f, 0.07f, 0.22f, 6.85e6f, 0.2f, 16.25e6f},
+    {run_rows<4, 1, 4, 2, GATED, true>, 2, 16, 3, 4, 2.62f, 0.61f, 0.05f, 0.93f, 6.46e6f, 0.15f, 17.93e6f},
+    {run_rows<4, 2, 4, 1, GATED, true>, 2, 32, 3, 4, 3.34f, 0.45f, 0.02f, 0.79f, 6.8e6f, 0.1f, 14.06e6f},
+    {run_wide<1, 1, 4, 1, 4, 4, GATED, true>, 4, 32, 4, 1, 3.39f, 0.19f, 0.36f, 0.26f, 6.38e6f, 0.59f, 21.9e6f},
+    {run_wide<1, 2, 4, 1, 4, 4, GATED, true>, 4, 64, 2, 1, 2.76f, 2.02f, 0.1f, 0.35f, 5.85e6f, 0.81f, 14.74e6f},
+    {run_wide<2, 2, 4, 1, 5, 2, GATED, true>, 8, 64, 3, 1, 3.37f, 0.08f, 0.66f, 0.42f, 5.92e6f, 1.55f, 21.59e6f},
+    {run_wide<2, 4, 4, 1, 4, 1, GATED, true>, 8, 128, 2, 1, 4.28f, 0.03f, 0.43f, 0.66f, 6e6f, 4.28f, 14.95e6f},
 };
 
 constexpr int kCus = 256;
