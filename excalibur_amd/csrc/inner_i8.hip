@@ -625,22 +625,22 @@ template <int TN, int TM, int WN, int WM, int BUFFERS, int D, bool GATED, bool G
 int run_wide(exhip_ctx* ctx, const I8Params& p) {
     return launch(ctx, i8_wide_kernel<TN, TM, WN, WM, BUFFERS, D, GATED, GROUPED>, p, TN * WN, 32 * TM * WM, 64 * WN * WM);
 }
-// Chosen so that the form with the least of these times is as near to the fastest as it can be over 782 products and 700 products by experts of 1 to 8192 rows, 64 to 16384
-// outputs and inputs and 2 to 256 experts: it takes 1.4 % and 2.2 % longer on average, 34 % and 25 % at most. Without any one form of the first list some product would take
+// Chosen so that the form with the least of these times is as near to the fastest as it can be over 952 products and 700 products by experts of 1 to 8192 rows, 64 to 16384
+// outputs and inputs and 2 to 256 experts: it takes 1.5 % and 2.2 % longer on average, 29 % and 25 % at most. Without any one form of the first list some product would take
 // 8 to 36 % longer, without one of the second 6 to 27 % (profiles/inner_i8_forms.txt).
 template <bool GATED>
 constexpr Form kPlain[] = {
-    {run_rows<2, 1, 8, 2, GATED, false>, 1, 16, 2, 8, 2.01f, 0.84f, 0.27f, 0.58f, 12.86e6f, 0.22f, 13.23e6f},
-    {run_rows<2, 1, 4, 2, GATED, false>, 1, 16, 5, 4, 2.03f, 0.58f, 0.49f, 0.25f, 12.1e6f, 0.25f, 15.44e6f},
-    {run_rows<2, 2, 4, 2, GATED, false>, 1, 32, 4, 4, 2.24f, 0.65f, 0.49f, 0.04f, 9.57e6f, 0.17f, 15.64e6f},
-    {run_rows<4, 1, 4, 2, GATED, false>, 2, 16, 3, 4, 4.2f, 0.52f, 0.18f, 0.25f, 11.52e6f, 5.74f, 8.18e6f},
-    {run_rows<4, 2, 4, 1, GATED, false>, 2, 32, 3, 4, 2.83f, 0.1f, 0.68f, 0.87f, 8.26e6f, 0.f, 31.34e6f},
-    {run_rows<4, 4, 4, 1, GATED, false>, 2, 64, 2, 4, 1.68f, 2.92f, 0.09f, 1.1f, 13.96e6f, 0.f, 10.62e6f},
-    {run_wide<1, 1, 2, 1, 8, 8, GATED, false>, 2, 32, 4, 1, 2.05f, 1.46f, 0.14f, 0.13f, 3.76e6f, 0.72f, 24.88e6f},
-    {run_wide<1, 1, 4, 1, 4, 4, GATED, false>, 4, 32, 4, 1, 2.12f, 0.02f, 0.41f, 0.34f, 9.74e6f, 0.54f, 18.38e6f},
-    {run_wide<1, 2, 4, 1, 4, 4, GATED, false>, 4, 64, 2, 1, 1.62f, 1.4f, 0.38f, 0.25f, 6.75e6f, 0.91f, 18.39e6f},
-    {run_wide<2, 2, 4, 1, 5, 2, GATED, false>, 8, 64, 3, 1, 3.07f, 0.03f, 0.18f, 0.48f, 3.3e6f, 1.46f, 26.03e6f},
-    {run_wide<2, 4, 4, 1, 4, 1, GATED, false>, 8, 128, 2, 1, 4.34f, 0.36f, 0.13f, 0.65f, 3.92e6f, 4.82f, 27.51e6f},
+    {run_rows<2, 1, 8, 2, GATED, false>, 1, 16, 2, 8, 1.77f, 0.97f, 0.23f, 0.5f, 10.3e6f, 0.27f, 16.62e6f},
+    {run_rows<2, 1, 4, 2, GATED, false>, 1, 16, 5, 4, 1.99f, 0.27f, 0.84f, 0.34f, 13.65e6f, 0.12f, 9.77e6f},
+    {run_rows<2, 2, 4, 2, GATED, false>, 1, 32, 4, 4, 2.3f, 0.15f, 0.5f, 0.42f, 9.5e6f, 0.07f, 18.12e6f},
+    {run_rows<4, 1, 4, 2, GATED, false>, 2, 16, 3, 4, 2.37f, 0.33f, 0.18f, 0.48f, 6.31e6f, 0.24f, 25.39e6f},
+    {run_rows<4, 2, 4, 1, GATED, false>, 2, 32, 3, 4, 2.67f, 0.3f, 0.75f, 0.66f, 7.86e6f, 0.f, 20.93e6f},
+    {run_rows<4, 4, 4, 1, GATED, false>, 2, 64, 2, 4, 2.75f, 1.91f, 0.44f, 1.02f, 6.61e6f, 0.01f, 39.62e6f},
+    {run_wide<1, 1, 2, 1, 8, 8, GATED, false>, 2, 32, 4, 1, 1.6f, 1.41f, 0.14f, 0.17f, 2.5e6f, 0.49f, 17.03e6f},
+    {run_wide<1, 1, 4, 1, 4, 4, GATED, false>, 4, 32, 4, 1, 2.35f, 0.02f, 0.32f, 0.25f, 5.93e6f, 0.63f, 23.21e6f},
+    {run_wide<1, 2, 4, 1, 4, 4, GATED, false>, 4, 64, 2, 1, 1.35f, 1.62f, 0.32f, 0.3f, 4.04e6f, 0.9f, 18.56e6f},
+    {run_wide<2, 2, 4, 1, 5, 2, GATED, false>, 8, 64, 3, 1, 3.33f, 0.11f, 0.53f, 0.49f, 3.78e6f, 1.39f, 19.96e6f},
+    {run_wide<2, 4, 4, 1, 4, 1, GATED, false>, 8, 128, 2, 1, 3.75f, 0.12f, 0.79f, 0.69f, 3.8e6f, 5.02f, 17.45e6f},
 };
 template <bool GATED>
 constexpr Form kGrouped[] = {
