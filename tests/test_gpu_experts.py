@@ -104,7 +104,8 @@ def test_combined_rows_within_their_roundings(ctx, m, each, n, pad, kind):
     bad = np.isnan(want)
     assert np.array_equal(np.isnan(got), bad)
     assert np.all(np.abs(got.astype(np.float64) - want)[~bad] <= bound[~bad])
-    assert np.array_equal(y16[:m, :n].copy().view(np.float16), got.astype(np.float16), equal_nan=True)
+    with np.errstate(over="ignore"):
+        assert np.array_equal(y16[:m, :n].copy().view(np.float16), got.astype(np.float16), equal_nan=True)
     for y, fill in ((y32, 7.25), (y16, 0x4567)):
         assert np.all(y[m] == fill) and np.all(y[:, n:] == fill)
     if m > 2:

@@ -320,6 +320,58 @@ def test_rows_that_the_input_does_not_have_are_not_numbers(ctx, m):
         assert np.array_equal(y[at[~bad]], o.want(rows=source[at[~bad]], expert=e)[0])
 
 
+# ---- every kernel at the sizes of the others ----
+FORMS, GROUPED_FORMS = 11, 7
+
+
+@pytest.fixture
+def pinned():
+    from excalibur_amd import hip
+    yield lambda form: hip.set_option("i8_form", form)
+    hip.set_option("i8_form", 0)
+
+
+FORM_SIZES = [(1, 1, 1), (2, 17, 127), (33, 300, 129), (65, 513, 500), (130, 257, 520), (300, 520, 1531), (1, 96, 4200)]
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("form", range(1, FORMS + 1))
+def test_every_form_at_the_sizes_of_the_others(ctx, pinned, form, gated):
+    pinned(form)
+    for m, n, k in FORM_SIZES:
+        _product(ctx, m, n, k, m % 2 == 0, ("silu", "gelu", "sigmoid", "relu")[(form + m) % 4] if gated else None)
+
+
+FORM_GROUPED = [(1, 1, 33, 64, "one"), (50, 3, 100, 300, "chance"), (130, 7, 129, 140, "holes"), (300, 4, 530, 520, "inside"), (64, 100, 20, 128, "chance"), (20, 6, 40, 100, "none"), (257, 130, 35, 40, "holes")]
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("form", range(1, GROUPED_FORMS + 1))
+def test_every_form_by_experts_at_the_sizes_of_the_others(ctx, pinned, form, gated):
+    pinned(form)
+    for m, experts, n, k, how in FORM_GROUPED:
+        _grouped(ctx, m, experts, n, k, how, gate=("silu", "gelu", "sigmoid", "relu")[(form + m) % 4] if gated else None, gather=(form + m) % 2 == 0, bias=m % 3 == 0)
+
+
+@pytest.mark.parametrize("form", range(1, FORMS + 1))
+def test_every_form_has_the_same_bits(ctx, pinned, form):
+    """Sums are exact and results are rounded in one order: which kernel takes a call changes nothing, an activation's value neither."""
+    o = Operands(ctx, np.random.default_rng(21), 150, 290, 600, sides=2, bias=True, pad=16)
+    want, got = ctx.empty((150, 290), np.float32), ctx.empty((150, 290), np.float32)
+    for gate in (None, "gelu", "silu"):
+        pinned(1)
+        o.run(ctx, o.desc(ctx), gate, y_f32=want) if gate else ctx.innerproduct_i8(o.desc(ctx), o.dx, o.dx_scale, ctx.pack_i8_weights(290, 600, ctx.array(o.w[0])), o.dw_scale[0], o.dbias[0], y_f32=want)
+        pinned(form)
+        o.run(ctx, o.desc(ctx), gate, y_f32=got) if gate else ctx.innerproduct_i8(o.desc(ctx), o.dx, o.dx_scale, ctx.pack_i8_weights(290, 600, ctx.array(o.w[0])), o.dw_scale[0], o.dbias[0], y_f32=got)
+        assert np.array_equal(want.download(), got.download()), gate
+
+
+def test_weights_that_go_past_l2(ctx):
+    """One tile of rows and more than 40 MB of weights: the form that reads them past L2, alone and by experts."""
+    _product(ctx, 2, 11000, 4100, True)
+    _grouped(ctx, 40, 30, 1000, 1500, "chance", gate="silu", gather=True)
+
+
 # ---- recorded, and beside others ----
 def test_products_recorded_and_replayed(ctx):
     """A quantizer and the products behind it in one graph, with other rows and other experts at every replay."""
