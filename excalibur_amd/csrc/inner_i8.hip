@@ -6,6 +6,7 @@
 // runs of four neighbouring outputs of one row.
 #include <math.h>
 
+#include "i8_rows.h"
 #include "inner.h"
 
 namespace {
@@ -282,7 +283,7 @@ __device__ __forceinline__ float result_of(int sum, float row, float output, flo
 
 // The activation of one side times the other, from the hardware's 2^x and 1 / x (one unit of the last place each). What 2^x makes of the rounding of its argument, 2^-24 of
 // that, counts where the activation is near 0 alone: less than 2^-23 of max(|g|, 1) in all. erf is Abramowitz and Stegun's 7.1.26, off by 1.5e-7 at most; on the side where
-// 1 + erf is small it is what is computed. (The library's expf, erff and divisions took 10 us of 4096 x 8 of 64 x 1536 x 2048's 260.)
+// 1 + erf is small it is what is computed. (With expf, erff and divisions 4096 rows x 8 of 64 experts of 1536 x 2048 took 262 us instead of 243.)
 __device__ __forceinline__ float gated_value(int gate, float g, float u) {
     if (gate == EXHIP_GATE_RELU) return (g > 0.f ? g : g != g ? g : 0.f) * u;
     if (gate == EXHIP_GATE_GELU) {
@@ -299,7 +300,9 @@ __device__ __forceinline__ float gated_value(int gate, float g, float u) {
 
 // ---- few rows, or few products ----
 // A group takes TN x 16 outputs (of both projections) and 16 TM rows; its WK waves every WK-th block, with nothing between memory and their registers: the codes of
-// D of a wave's blocks are on their way at a time. The sums meet in LDS, and every thread finishes four neighbouring outputs of a row.
+// D of a wave's blocks are on their way at a time. The sums meet in LDS, and every thread finishes four neighbouring outputs of a row. What bounds it is the memory: one
+// row of the gated 11264 x 4096 takes 16.6 us, 5.6 TB/s of weights. Four waves a group, so that a CU has several groups, where there are many outputs (one row's 8 of 64 experts of
+// 1536 x 2048, gated, 9.1 us, with eight waves 12.1); eight where one group a CU has all of them (4096 x 4096 5.2 us, with four 5.7).
 template <int TN, int TM, int WK, int D, bool PAST, bool GATED, bool GROUPED>
 __global__ __launch_bounds__(64 * WK, 2) void i8_rows_kernel(const I8Params p) {
     exhip_touch_args(p);
@@ -308,6 +311,7 @@ __global__ __launch_bounds__(64 * WK, 2) void i8_rows_kernel(const I8Params p) {
     const Tiles<GROUPED, kRows> tiles(p);
     if ((int)blockIdx.x >= p.groups_n * tiles.total) return;
     const Part part = tiles.part(p);
+    if (part.rows <= 0) return;  // offsets that do not rise
     const int lane = threadIdx.x % 64, wk = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), q = lane / 16, col = lane % 16;
     const int blocks = p.blocks, row_bytes = blocks * kTileBlock, tile0 = part.group_n * (TN / 2), last = p.tiles - 1;
     const __amdgpu_buffer_rsrc_t weights = uniform_view(p.w + ((size_t)part.expert * p.tiles + tile0) * row_bytes, (unsigned)(min(TN / 2, p.tiles - tile0) * row_bytes));
@@ -399,10 +403,9 @@ __global__ __launch_bounds__(64 * WK, 2) void i8_rows_kernel(const I8Params p) {
 // the waves after the other's where float32 results of all of them do not fit.
 typedef int v16i __attribute__((ext_vector_type(16)));
 
-template <int WIDTH>
-struct Scales {  // of a group's rows and outputs, in LDS
-    float output[WIDTH], output_up[WIDTH], bias[WIDTH], bias_up[WIDTH];
-    float row[1];  // as many as the group has
+template <int WIDTH, int ROWS>
+struct __attribute__((aligned(16))) Scales {  // of a group's outputs and rows, in LDS
+    float output[WIDTH], output_up[WIDTH], bias[WIDTH], bias_up[WIDTH], row[ROWS];
 };
 
 template <typename O, int WN, int WM, int TM, int FOURS, int ROOM>
@@ -428,8 +431,8 @@ __device__ __forceinline__ void store_group(O* y, size_t stride, const v4f (&v)[
     }
 }
 
-template <int WN, int WM, int TN, int TM, bool GATED, int ROOM, int WIDTH>
-__device__ __forceinline__ void write_group(const I8Params& p, const Part& part, const v16i (&acc)[TN][TM], int wn, int wm, int lane, char* lds, const Scales<WIDTH>& scales) {
+template <int WN, int WM, int TN, int TM, bool GATED, int ROOM, int WIDTH, int ROWS>
+__device__ __forceinline__ void write_group(const I8Params& p, const Part& part, const v16i (&acc)[TN][TM], int wn, int wm, int lane, char* lds, const Scales<WIDTH, ROWS>& scales) {
     constexpr int kFours = TN * (GATED ? 2 : 4), kOwn = kFours * 8;
     static_assert(kOwn * WN == WIDTH);
     const int at = wn * kOwn + lane / 32 * 4, row = wm * TM * 32 + lane % 32;
@@ -461,10 +464,14 @@ __device__ __forceinline__ void write_group(const I8Params& p, const Part& part,
     if (p.y_f16) store_group<uint16_t, WN, WM, TM, kFours, ROOM>(p.y_f16, p.y_stride, v, part, j0, p.n, wn, wm, lane, lds);
 }
 
-// A group of WN x WM waves takes 32 TN WN outputs and 32 TM WM rows. Rows' codes come straight into LDS, three blocks ahead in four buffers; a wave's weights from
-// L2 straight into registers, those of a step of 32 values as soon as the same step of the block before is done with them. Every step's rows are read from LDS while the
-// products of the step before run, and loads stand between the products one by one. A block's one barrier, at its start, says that the next block's rows are there and that
+// A group of WN x WM waves takes 32 TN WN outputs and 32 TM WM rows. Rows' codes come straight into LDS, BUFFERS - 1 blocks ahead; a wave's weights from L2 straight into
+// registers, D blocks ahead, those of a step of 32 values as soon as that step is done with the ones in their place. Rows are read from LDS a step before their products, or a
+// block where a step's products are few, and loads stand between the products one by one. A block's one barrier, at its start, says that the next block's rows are there and that
 // the last block's buffer may be filled.
+// Two groups of 128 rows x 256 outputs a CU are what measured fastest for many rows: 8192 x 8192 x 4096 in 213 to 227 us, by the box, 2.4 to 2.6 POP/s, where the library's int8 product takes
+// 296. The card's power bounds it: the clock stands at 1.65 GHz, and with codes of 0 the same launch takes 151 us. Eight waves a group with 256 rows took 8 % longer (nothing runs beside
+// a group's results), four with 64 x 256 outputs each 5 %, and groups that go on to their next tile, its first blocks on their way while results are stored, 2 to 5 %. Few rows are
+// bound by what a CU draws, 85 bytes a ns: 64 rows x 256 outputs, 64 x 128, and 32 rows with weights eight blocks ahead.
 constexpr int most_on_their_way(int loads) { return loads < 63 ? loads : 63; }  // as many as a wait can name
 
 template <int TN, int TM, int WN, int WM, int BUFFERS, int D, bool GATED, bool GROUPED>
@@ -475,22 +482,24 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void i8_wide_kernel(const I8Params
     static_assert(D * 4 * TM % (2 * kAhead) == 0 && D >= kBuffers - 3);
     constexpr int kResults = kRows * kWidth * 2, kRoom = kBuffers * kBuffer > kResults ? kBuffers * kBuffer : kResults;
     __shared__ __attribute__((aligned(16))) char staged[kRoom];
-    __shared__ __attribute__((aligned(16))) char scale_room[sizeof(Scales<kWidth>) + kRows * 4];
-    Scales<kWidth>& scales = *reinterpret_cast<Scales<kWidth>*>(scale_room);
+    __shared__ Scales<kWidth, kRows> scales;
     const Tiles<GROUPED, kRows> tiles(p);
     if ((int)blockIdx.x >= p.groups_n * tiles.total) return;
     const Part part = tiles.part(p);
+    if (part.rows <= 0) return;  // offsets that do not rise
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)staged;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wn = wave % WN, wm = wave / WN;
     const int blocks = p.blocks, row_bytes = blocks * kTileBlock, tile0 = (part.group_n * WN + wn) * TN, first = min(tile0, p.tiles - 1);
     const __amdgpu_buffer_rsrc_t weights = uniform_view(p.w + ((size_t)part.expert * p.tiles + first) * row_bytes, (unsigned)(min(TN, p.tiles - first) * row_bytes));
     const Rows<GROUPED> rows(p, part);
     // A wave stages 8 kLoads rows, eight with a load: lane l holds piece (l % 8) ^ (l / 8) of row l / 8, so that a piece of eight neighbouring rows lies in all banks.
+    // Pieces behind a row's end, in its last block, are not loaded (the view's bounds do not see the block's offset).
+    const int staged_piece = ((lane % 8) ^ (lane / 8)) * 16, staged_blocks = i8_blocks_of_piece(p.k, staged_piece);
     unsigned off[kLoads];
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) off[j] = rows.begin(rows.source((wave * kLoads + j) * 8 + lane / 8)) + ((lane % 8) ^ (lane / 8)) * 16;
+    for (int j = 0; j < kLoads; ++j) off[j] = rows.begin(rows.source((wave * kLoads + j) * 8 + lane / 8)) + staged_piece;
     auto stage = [&](int buffer, int j) {  // behind the last block zeros, which nothing reads
-        load16_to_lds(rows.view, buffer < blocks ? off[j] : kNoRow, buffer * kBlk, lds0 + buffer % kBuffers * kBuffer + (wave * kLoads + j) * 1024);
+        load16_to_lds(rows.view, buffer < staged_blocks ? off[j] : kNoRow, buffer * kBlk, lds0 + buffer % kBuffers * kBuffer + (wave * kLoads + j) * 1024);
     };
     v4i w[D][4][TN];
     auto request = [&](v4i (&w)[4][TN], int b, int s, int i) {
