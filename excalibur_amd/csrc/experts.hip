@@ -7,18 +7,17 @@ constexpr int kMostExperts = 1024;
 constexpr int kMostEach = 64;
 constexpr int kMostChoices = 1 << 28;
 
-// An expert a group: its waves count, each in its own stretch of the choices, those of earlier experts and those of this one, and go over the stretch again to
-// write where they stand. No count depends on another group, so one launch does it and the order is that of the choices. Four choices a lane and 256 a wave at a
-// time, of which HELD stay in registers between the counting and the writing; where a stretch has more they are read again. Lanes count for themselves, two instructions a
-// choice and count, and are added up once. (65528 choices of 256 experts: every CU reads all of them from L2.)
+// Few choices: an expert a group, whose waves count, each in its own stretch of the choices, those of earlier experts and those of this one, four choices a lane and 256 a wave at
+// a time, and write where theirs stand from the registers that they were counted in. Lanes count for themselves, two instructions a choice and count.
+constexpr int kWaves = 16, kByExpert = 16384;  // of a group; the most choices
+
 template <int HELD>
-__global__ __launch_bounds__(1024) void group_rows_kernel(const int* __restrict__ ids, int choices, exhip_divisor row_of, int experts, int* __restrict__ offsets,
+__global__ __launch_bounds__(1024) void group_rows_by_expert(const int* __restrict__ ids, int choices, exhip_divisor row_of, int experts, int* __restrict__ offsets,
                                                           int* __restrict__ rows, int* __restrict__ places) {
-    constexpr int kWaves = 16;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), expert = blockIdx.x;
     const int stretch = ((choices + kWaves - 1) / kWaves + 255) / 256 * 256;
     const long long from = (long long)wave * stretch;
-    const int begin = from < choices ? (int)from : choices, end = min(choices - begin, stretch) + begin, pieces = (end - begin + 255) / 256;
+    const int begin = from < choices ? (int)from : choices, end = min(choices - begin, stretch) + begin;
     const __amdgpu_buffer_rsrc_t view = uniform_view(ids + begin, (unsigned)(end - begin) * 4u);
     __shared__ int before[kWaves], own[kWaves];
     auto four = [&](int piece) { return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(view, piece * 1024 + lane * 16, 0, 0)); };
@@ -44,8 +43,6 @@ __global__ __launch_bounds__(1024) void group_rows_kernel(const int* __restrict_
         held[i] = ended(held[i], i);
         count(held[i]);
     }
-#pragma unroll 4
-    for (int i = HELD; i < pieces; ++i) count(ended(four(i), i));
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         less += __shfl_xor(less, d);
@@ -89,7 +86,7 @@ __global__ __launch_bounds__(1024) void group_rows_kernel(const int* __restrict_
                 place += __popcll(mask[e]);
             }
         }
-        if (expert == 0) {  // those that chose nothing
+        if ((wave * HELD + piece) % experts == expert) {  // those that chose nothing: every group has its share of the pieces
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if ((unsigned)v[e] >= (unsigned)experts && at + e < end) places[at + e] = -1;
@@ -98,9 +95,108 @@ __global__ __launch_bounds__(1024) void group_rows_kernel(const int* __restrict_
     };
 #pragma unroll
     for (int i = 0; i < HELD; ++i) write(i, held[i]);
-    for (int i = HELD; i < pieces; ++i) write(i, ended(four(i), i));
     if (expert == experts - 1)
         for (int i = first + all + threadIdx.x; i < choices; i += 1024) rows[i] = -1;
+}
+
+// Many choices: a group has a run of them, 1024 or more, and counts all of them by expert: those ahead of its run and the others, in LDS, where the counts of an expert stand in as
+// many copies as there is room for, so that the lanes of an addition meet seldom. From the counts every group has where each expert's rows begin and how many of them stand
+// ahead of its run, and it places its own choices, 1024 at a time: behind those of earlier waves, and within a wave behind the earlier lanes with the same expert. Nothing waits for
+// another group, so one launch does it; whole numbers are added, so no order of additions shows. What bounds it is a CU's reading of all choices and their additions: 65528 choices of
+// 256 experts take 8.5 us and of 1024 10.0, where a group an expert takes 12 and 28; 16384 of 64 take 7, where that takes 5.5.
+constexpr int kRun = 64 * kWaves, kCounts = 4096;  // choices at a time; counts of either kind in LDS, all copies
+
+__global__ __launch_bounds__(kRun) void group_rows_by_run(const int* __restrict__ ids, int choices, exhip_divisor row_of, int experts, int copies, int bits, int run,
+                                                          int* __restrict__ offsets, int* __restrict__ rows, int* __restrict__ places) {
+    constexpr int kTogether = 8;  // loads on their way
+    __shared__ int counts[2][kCounts + 64];  // [ahead of the run, from there on][expert][copy], and behind them 64 that nothing reads
+    __shared__ int base[kMostExperts];       // where the next choice of each expert goes
+    __shared__ unsigned short in_wave[kWaves][kMostExperts];
+    __shared__ int sums[kWaves];
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), begin = blockIdx.x * run, end = min(choices - begin, run) + begin;
+    const __amdgpu_buffer_rsrc_t view = uniform_view(ids, (unsigned)choices * 4u);
+    int id = begin + (int)threadIdx.x < end ? ids[begin + threadIdx.x] : -1;  // this thread's choice of the first 1024
+    for (int i = threadIdx.x; i < experts * copies; i += kRun) counts[0][i] = counts[1][i] = 0;
+    __syncthreads();
+    const int copy = lane & (copies - 1);
+    for (int first = wave * 256; first < choices; first += kWaves * 256 * kTogether) {
+        v4i got[kTogether];
+#pragma unroll
+        for (int i = 0; i < kTogether; ++i) got[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(view, (first + i * (kWaves * 256)) * 4 + lane * 16, 0, 0));
+#pragma unroll
+        for (int i = 0; i < kTogether; ++i) {
+            const int at = first + i * (kWaves * 256);
+            if (at >= choices) continue;
+            if (at + 256 > choices)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) got[i][e] = at + lane * 4 + e < choices ? got[i][e] : -1;
+            int* const of = counts[at >= begin] + copy;  // (runs begin on multiples of 1024)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) atomicAdd(of + (int)min((unsigned)got[i][e], (unsigned)experts) * copies, 1);
+        }
+    }
+    __syncthreads();
+    // every expert's, a thread each: where its rows begin
+    int ahead = 0, all = 0;
+    if ((int)threadIdx.x < experts)
+        for (int c = 0; c < copies; ++c) {  // each thread from a copy of its own, for the banks
+            const int at = threadIdx.x * copies + ((threadIdx.x + c) & (copies - 1));
+            ahead += counts[0][at];
+            all += counts[1][at];
+        }
+    all += ahead;
+    int upto = all;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int before = __shfl_up(upto, d);
+        if (lane >= d) upto += before;
+    }
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        if (w < wave) upto += sums[w];
+        total += sums[w];
+    }
+    if ((int)threadIdx.x < experts) {
+        base[threadIdx.x] = upto - all + ahead;
+        if (blockIdx.x == 0) {
+            offsets[threadIdx.x] = upto - all;
+            if ((int)threadIdx.x == experts - 1) offsets[experts] = total;
+        }
+    }
+    for (int first = begin; first < end; first += kRun) {
+        for (int i = lane; i < experts; i += 64) in_wave[wave][i] = 0;
+        const int i = first + threadIdx.x;
+        const bool chooses = (unsigned)id < (unsigned)experts;
+        unsigned long long same = __ballot(chooses);
+        for (int bit = 0; bit < bits; ++bit) {
+            const unsigned long long set = __ballot(id >> bit & 1);
+            same &= id >> bit & 1 ? set : ~set;
+        }
+        const int earlier = __builtin_amdgcn_mbcnt_hi((unsigned)(same >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)same, 0));
+        if (chooses && earlier == 0) in_wave[wave][id] = (unsigned short)__popcll(same);
+        __syncthreads();
+        int place = -1;
+        if (chooses) {
+            place = base[id] + earlier;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) place += w < wave ? in_wave[w][id] : 0;
+            rows[place] = (int)row_of(i);
+        }
+        if (i < end) {
+            places[i] = place;
+            if (i >= total) rows[i] = -1;
+        }
+        if (first + kRun < end) {
+            id = i + kRun < end ? ids[i + kRun] : -1;
+            __syncthreads();
+            if ((int)threadIdx.x < experts)
+                for (int w = 0; w < kWaves; ++w) base[threadIdx.x] += in_wave[w][threadIdx.x];
+            __syncthreads();
+        }
+    }
 }
 
 // ---- the sum of the answers ----
@@ -215,8 +311,16 @@ extern "C" int exhip_group_rows(exhip_ctx* ctx, const int32_t* ids, int m, int e
     const int choices = m * each;
     exhip_divisor row_of;
     row_of.set(each);
-    const auto kernel = choices <= 16 * 256 ? group_rows_kernel<1> : choices <= 16 * 1024 ? group_rows_kernel<4> : group_rows_kernel<16>;
-    hipLaunchKernelGGL(kernel, dim3(experts), dim3(1024), 0, ctx->stream, ids, choices, row_of, experts, offsets, rows, places);
+    if (choices <= kByExpert && experts <= 256) {
+        const auto kernel = choices <= kByExpert / 4 ? group_rows_by_expert<1> : group_rows_by_expert<4>;
+        hipLaunchKernelGGL(kernel, dim3(experts), dim3(64 * kWaves), 0, ctx->stream, ids, choices, row_of, experts, offsets, rows, places);
+    } else {
+        int copies = 64, bits = 0;
+        while (copies * experts > kCounts) copies /= 2;
+        while ((1 << bits) < experts) ++bits;
+        const int run = (choices / 256 + kRun) / kRun * kRun, groups = (choices - 1) / run + 1;  // no more groups than CUs: each reads all choices
+        hipLaunchKernelGGL(group_rows_by_run, dim3(groups), dim3(kRun), 0, ctx->stream, ids, choices, row_of, experts, copies, bits, run, offsets, rows, places);
+    }
     EXHIP_LAUNCH_CHECK();
     return 0;
 }

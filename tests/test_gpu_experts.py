@@ -45,7 +45,8 @@ def recorded(ctx, step, fill, results, turns=4):
 
 # ---- in order by expert ----
 GROUPS = [(1, 1, 1, "all"), (1, 8, 64, "all"), (3, 2, 5, "all"), (16, 8, 64, "all"), (63, 1, 2, "all"), (65, 1, 3, "some"), (100, 3, 20, "some"), (1024, 1, 7, "all"), (1025, 4, 256, "some"),
-          (700, 64, 100, "all"), (5, 4, 1024, "some"), (3000, 6, 1, "some"), (4097, 8, 128, "one"), (200, 5, 33, "none"), (20000, 8, 300, "some"), (8191, 8, 64, "all")]
+          (700, 64, 100, "all"), (5, 4, 1024, "some"), (3000, 6, 1, "some"), (4097, 8, 128, "one"), (200, 5, 33, "none"), (20000, 8, 300, "some"), (8191, 8, 64, "all"),
+          (2048, 8, 256, "some"), (2049, 8, 7, "all"), (8191, 8, 256, "none"), (8191, 8, 1024, "all"), (3, 5, 600, "some"), (40000, 8, 2, "some"), (70000, 5, 1000, "some"), (300000, 1, 5, "all")]
 
 
 @pytest.mark.parametrize("m,each,experts,which", GROUPS)
