@@ -664,18 +664,22 @@ constexpr Form kGrouped[] = {
 
 constexpr int kCus = 256;
 
-// What a launch of a form takes, in us.
-float time_of(const Form& f, const I8Params& p, bool gated_product) {
+// How many `of` (a power of two) hold v > 0: the choice is made for every row of a serving program, and divisions are most of it.
+int in_all(int v, int of) { return ((v - 1) >> __builtin_ctz(of)) + 1; }
+float larger(float a, float b) { return a > b ? a : b; }  // (fmaxf is a call)
+
+// What a launch of a form takes, in us; `experts` that have rows, 1 for a product without.
+float time_of(const Form& f, const I8Params& p, float experts, bool gated_product) {
+    const float m = (float)p.m;
     // By experts the rows of each are not known here: as many have rows as would have by chance, and the last tile of each is half full.
-    const float m = (float)p.m, experts = p.offsets ? (float)p.experts * (1.f - expf(-m / (float)p.experts)) : 1.f;
-    const float tiles_m = !p.offsets ? (float)((p.m - 1) / f.rows + 1) : fmaxf(experts, m / experts > 0.25f * (float)f.rows ? m / (float)f.rows + 0.5f * experts : 0.f);
-    const float groups = (float)((p.tiles + f.tiles - 1) / f.tiles) * tiles_m, times = ceilf(groups / kCus), full = floorf(times / (float)f.at_once), rest = times - full * (float)f.at_once;
-    const float blocks = (float)((p.blocks - 1) / f.split + 1), gate = gated_product ? f.gate : 0.f;
-    float us = f.start + full * (f.round + blocks * fmaxf(f.alone, (float)f.at_once * f.share)) + gate * times;
-    if (rest > 0.f) us += f.round + blocks * fmaxf(f.alone, rest * f.share);
+    const float tiles_m = !p.offsets ? (float)in_all(p.m, f.rows) : larger(experts, m > 0.25f * (float)f.rows * experts ? m / (float)f.rows + 0.5f * experts : 0.f);
+    const float groups = (float)in_all(p.tiles, f.tiles) * tiles_m, blocks = (float)in_all(p.blocks, f.split), gate = gated_product ? f.gate : 0.f;
+    const int down = (int)((groups < 1e9f ? groups : 1e9f) * (1.f / kCus)), times = down + ((float)down * kCus < groups ? 1 : 0), full = times / f.at_once, rest = times - full * f.at_once;
+    float us = f.start + (float)full * (f.round + blocks * larger(f.alone, (float)f.at_once * f.share)) + gate * (float)times;
+    if (rest > 0) us += f.round + blocks * larger(f.alone, (float)rest * f.share);
     const float weights = experts * (float)p.tiles * (float)p.blocks * (float)kTileBlock;
-    const float again = fmaxf(0.f, groups * blocks * (float)(f.tiles * kTileBlock + f.rows * kBlk) - weights);
-    return fmaxf(us, f.start + 1.f + gate + weights / f.memory + again / f.l2);
+    const float again = larger(0.f, groups * blocks * (float)(f.tiles * kTileBlock + f.rows * kBlk) - weights);
+    return larger(us, f.start + 1.f + gate + weights / f.memory + again / f.l2);
 }
 
 template <int N>
@@ -683,9 +687,10 @@ int run_best(exhip_ctx* ctx, const I8Params& p, const Form (&forms)[N], bool gat
     const int pinned = g_exhip_options.i8_form;
     int best = pinned < N ? pinned - 1 : N - 1;
     if (pinned <= 0) {
+        const float experts = p.offsets ? (float)p.experts * (1.f - expf(-(float)p.m / (float)p.experts)) : 1.f;
         float least = 0.f;
         for (int i = 0; i < N; ++i) {
-            const float us = time_of(forms[i], p, gated_product);
+            const float us = time_of(forms[i], p, experts, gated_product);
             if (i == 0 || us < least) {
                 least = us;
                 best = i;

@@ -89,6 +89,19 @@ def test_quantized_rows_at_any_alignment_of_their_type(ctx, k):
             assert np.array_equal(got.download()[:, :k], want) and np.array_equal(scale.download(), want_scale)
 
 
+def test_quantized_rows_that_lie_behind_four_gigabytes(ctx):
+    from excalibur_amd import hip
+    stride = 1_100_000_000  # of halves: the third row's bytes begin behind 2^32
+    x = ctx.empty((2 * stride + 128,), np.uint16)
+    rows = np.random.default_rng(6).standard_normal((3, 100)).astype(np.float16)
+    for r in range(3):
+        hip._check(hip.lib().exhip_memcpy_h2d(ctx.h, x.at(2 * r * stride).ptr, rows[r].ctypes.data_as(hip.ctypes.c_void_p), hip.ctypes.c_size_t(200)))
+    got, scale = ctx.quantize_rows_i8(ctx.view(x.ptr.value, (3, stride), np.uint16), 100, y=ctx.empty((3, 112), np.int8))
+    want, want_scale = i8ref.quantize_rows(rows.astype(np.float32))
+    assert np.array_equal(got.download()[:, :100], want) and np.array_equal(scale.download(), want_scale)
+    x.free()
+
+
 # ---- the products ----
 class Operands:
     """Rows and weights as codes of every value, on the host and on the device; codes that are not zero stand behind every row's end."""
