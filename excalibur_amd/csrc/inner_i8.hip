@@ -635,8 +635,8 @@ int run_wide(exhip_ctx* ctx, const I8Params& p) {
     return launch(ctx, i8_wide_kernel<TN, TM, WN, WM, BUFFERS, D, GATED, GROUPED>, p, TN * WN, 32 * TM * WM, 64 * WN * WM);
 }
 // Chosen so that the form with the least of these times is as near to the fastest as it can be over 952 products and 700 products by experts of 1 to 8192 rows, 64 to 16384
-// outputs and inputs and 2 to 256 experts: it takes 1.5 % and 2.2 % longer on average, 29 % and 25 % at most. Without any one form of the first list some product would take
-// 8 to 36 % longer, without one of the second 6 to 27 % (profiles/inner_i8_forms.txt).
+// outputs and inputs and 2 to 256 experts: it takes 1.5 % and 2.2 % longer on average, 32 % and 25 % at most, and over 53 and 60 others 2.6 % and 2.0 %, 21 % and 18 % at most.
+// Without any one form of the first list some product would take 10 to 36 % longer, without one of the second 9 to 31 %.
 template <bool GATED>
 constexpr Form kPlain[] = {
     {run_rows<2, 1, 8, 2, GATED, false>, 1, 16, 2, 8, 1.77f, 0.97f, 0.23f, 0.5f, 10.3e6f, 0.27f, 16.62e6f},
@@ -673,12 +673,12 @@ float time_of(const Form& f, const I8Params& p, float experts, bool gated_produc
     const float m = (float)p.m;
     // By experts the rows of each are not known here: as many have rows as would have by chance, and the last tile of each is half full.
     const float tiles_m = !p.offsets ? (float)in_all(p.m, f.rows) : larger(experts, m > 0.25f * (float)f.rows * experts ? m / (float)f.rows + 0.5f * experts : 0.f);
-    const float groups = (float)in_all(p.tiles, f.tiles) * tiles_m, blocks = (float)in_all(p.blocks, f.split), gate = gated_product ? f.gate : 0.f;
+    const float groups = (float)in_all(p.tiles, f.tiles) * tiles_m, all = (float)p.blocks, blocks = (float)in_all(p.blocks, f.split), gate = gated_product ? f.gate : 0.f;
     const int down = (int)((groups < 1e9f ? groups : 1e9f) * (1.f / kCus)), times = down + ((float)down * kCus < groups ? 1 : 0), full = times / f.at_once, rest = times - full * f.at_once;
     float us = f.start + (float)full * (f.round + blocks * larger(f.alone, (float)f.at_once * f.share)) + gate * (float)times;
     if (rest > 0) us += f.round + blocks * larger(f.alone, (float)rest * f.share);
-    const float weights = experts * (float)p.tiles * (float)p.blocks * (float)kTileBlock;
-    const float again = larger(0.f, groups * blocks * (float)(f.tiles * kTileBlock + f.rows * kBlk) - weights);
+    const float weights = experts * (float)p.tiles * all * (float)kTileBlock;
+    const float again = larger(0.f, groups * all * (float)(f.tiles * kTileBlock + f.rows * kBlk) - weights);
     return larger(us, f.start + 1.f + gate + weights / f.memory + again / f.l2);
 }
 
