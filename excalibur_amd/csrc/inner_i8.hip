@@ -614,7 +614,7 @@ int launch(exhip_ctx* ctx, K kernel, I8Params p, int tiles, int rows, int thread
 
 // One way to run a product: the tiles of 32 outputs (of both projections) and the rows that a group takes, how many groups a CU runs at once, how many waves share a
 // group's blocks, and what a launch takes, in us: `start`; each time that all CUs are given groups, `round`, and for each block of one wave `alone`, or `share` for each
-// group on a CU where that is more; `gate` for an activation, each time; but no less than reading the weights from memory and what groups read again from L2, at so many bytes a us.
+// group on a CU where that is more; `gate` for an activation, each time; but no less than reading the weights from memory and what groups read from L2, weights again and the rows there are, at so many bytes a us.
 struct Form {
     int (*run)(exhip_ctx*, const I8Params&);
     int tiles, rows, at_once, split;
@@ -635,31 +635,31 @@ int run_wide(exhip_ctx* ctx, const I8Params& p) {
     return launch(ctx, i8_wide_kernel<TN, TM, WN, WM, BUFFERS, D, GATED, GROUPED>, p, TN * WN, 32 * TM * WM, 64 * WN * WM);
 }
 // Chosen so that the form with the least of these times is as near to the fastest as it can be over 952 products and 700 products by experts of 1 to 8192 rows, 64 to 16384
-// outputs and inputs and 2 to 256 experts: it takes 1.5 % and 2.2 % longer on average, 32 % and 25 % at most, and over 53 and 60 others 2.6 % and 2.0 %, 21 % and 18 % at most.
-// Without any one form of the first list some product would take 10 to 36 % longer, without one of the second 9 to 31 %.
+// outputs and inputs and 2 to 256 experts, those of at most 64 rows counted twice: it takes 1.1 % and 1.6 % longer on average, 25 % at most, and over 102 and 125 others 1.2 %
+// and 1.8 %, 24 % at most. Without any one form of the first list some product would take 10 to 36 % longer, without one of the second 9 to 31 %.
 template <bool GATED>
 constexpr Form kPlain[] = {
-    {run_rows<2, 1, 8, 2, GATED, false>, 1, 16, 2, 8, 1.77f, 0.97f, 0.23f, 0.5f, 10.3e6f, 0.27f, 16.62e6f},
-    {run_rows<2, 1, 4, 2, GATED, false>, 1, 16, 5, 4, 1.99f, 0.27f, 0.84f, 0.34f, 13.65e6f, 0.12f, 9.77e6f},
-    {run_rows<2, 2, 4, 2, GATED, false>, 1, 32, 4, 4, 2.3f, 0.15f, 0.5f, 0.42f, 9.5e6f, 0.07f, 18.12e6f},
-    {run_rows<4, 1, 4, 2, GATED, false>, 2, 16, 3, 4, 2.37f, 0.33f, 0.18f, 0.48f, 6.31e6f, 0.24f, 25.39e6f},
-    {run_rows<4, 2, 4, 1, GATED, false>, 2, 32, 3, 4, 2.67f, 0.3f, 0.75f, 0.66f, 7.86e6f, 0.f, 20.93e6f},
-    {run_rows<4, 4, 4, 1, GATED, false>, 2, 64, 2, 4, 2.75f, 1.91f, 0.44f, 1.02f, 6.61e6f, 0.01f, 39.62e6f},
-    {run_wide<1, 1, 2, 1, 8, 8, GATED, false>, 2, 32, 4, 1, 1.6f, 1.41f, 0.14f, 0.17f, 2.5e6f, 0.49f, 17.03e6f},
-    {run_wide<1, 1, 4, 1, 4, 4, GATED, false>, 4, 32, 4, 1, 2.35f, 0.02f, 0.32f, 0.25f, 5.93e6f, 0.63f, 23.21e6f},
-    {run_wide<1, 2, 4, 1, 4, 4, GATED, false>, 4, 64, 2, 1, 1.35f, 1.62f, 0.32f, 0.3f, 4.04e6f, 0.9f, 18.56e6f},
-    {run_wide<2, 2, 4, 1, 5, 2, GATED, false>, 8, 64, 3, 1, 3.33f, 0.11f, 0.53f, 0.49f, 3.78e6f, 1.39f, 19.96e6f},
-    {run_wide<2, 4, 4, 1, 4, 1, GATED, false>, 8, 128, 2, 1, 3.75f, 0.12f, 0.79f, 0.69f, 3.8e6f, 5.02f, 17.45e6f},
+    {run_rows<2, 1, 8, 2, GATED, false>, 1, 16, 2, 8, 2.05f, 0.76f, 0.04f, 0.63f, 12.01e6f, 0.05f, 17.94e6f},
+    {run_rows<2, 1, 4, 2, GATED, false>, 1, 16, 5, 4, 2.09f, 0.54f, 0.57f, 0.33f, 13.59e6f, 0.07f, 13.61e6f},
+    {run_rows<2, 2, 4, 2, GATED, false>, 1, 32, 4, 4, 2.28f, 0.19f, 0.07f, 0.55f, 9.19e6f, 0.03f, 18.79e6f},
+    {run_rows<4, 1, 4, 2, GATED, false>, 2, 16, 3, 4, 2.82f, 0.67f, 0.02f, 0.48f, 5.38e6f, 1.33f, 164.9e6f},
+    {run_rows<4, 2, 4, 1, GATED, false>, 2, 32, 3, 4, 2.7f, 0.41f, 0.32f, 0.76f, 8.02e6f, 0.f, 29.22e6f},
+    {run_rows<4, 4, 4, 1, GATED, false>, 2, 64, 2, 4, 3.14f, 1.08f, 0.11f, 1.04f, 8.19e6f, 0.f, 15.35e6f},
+    {run_wide<1, 1, 2, 1, 8, 8, GATED, false>, 2, 32, 4, 1, 1.68f, 1.84f, 0.03f, 0.14f, 2.5e6f, 0.46f, 16.48e6f},
+    {run_wide<1, 1, 4, 1, 4, 4, GATED, false>, 4, 32, 4, 1, 2.53f, 0.03f, 0.31f, 0.22f, 7.43e6f, 0.74f, 20.29e6f},
+    {run_wide<1, 2, 4, 1, 4, 4, GATED, false>, 4, 64, 2, 1, 0.98f, 1.92f, 0.4f, 0.29f, 6.37e6f, 1.36f, 13.82e6f},
+    {run_wide<2, 2, 4, 1, 5, 2, GATED, false>, 8, 64, 3, 1, 3.68f, 0.11f, 0.07f, 0.48f, 3.95e6f, 1.19f, 20.52e6f},
+    {run_wide<2, 4, 4, 1, 4, 1, GATED, false>, 8, 128, 2, 1, 3.5f, 0.06f, 0.8f, 0.67f, 4.03e6f, 4.73f, 15.65e6f},
 };
 template <bool GATED>
 constexpr Form kGrouped[] = {
-    {run_rows<2, 1, 4, 2, GATED, true>, 1, 16, 5, 4, 2.74f, 1.03f, 0.07f, 0.22f, 6.85e6f, 0.2f, 16.25e6f},
-    {run_rows<4, 1, 4, 2, GATED, true>, 2, 16, 3, 4, 2.62f, 0.61f, 0.05f, 0.93f, 6.46e6f, 0.15f, 17.93e6f},
-    {run_rows<4, 2, 4, 1, GATED, true>, 2, 32, 3, 4, 3.34f, 0.45f, 0.02f, 0.79f, 6.8e6f, 0.1f, 14.06e6f},
-    {run_wide<1, 1, 4, 1, 4, 4, GATED, true>, 4, 32, 4, 1, 3.39f, 0.19f, 0.36f, 0.26f, 6.38e6f, 0.59f, 21.9e6f},
-    {run_wide<1, 2, 4, 1, 4, 4, GATED, true>, 4, 64, 2, 1, 2.76f, 2.02f, 0.1f, 0.35f, 5.85e6f, 0.81f, 14.74e6f},
-    {run_wide<2, 2, 4, 1, 5, 2, GATED, true>, 8, 64, 3, 1, 3.37f, 0.08f, 0.66f, 0.42f, 5.92e6f, 1.55f, 21.59e6f},
-    {run_wide<2, 4, 4, 1, 4, 1, GATED, true>, 8, 128, 2, 1, 4.28f, 0.03f, 0.43f, 0.66f, 6e6f, 4.28f, 14.95e6f},
+    {run_rows<2, 1, 4, 2, GATED, true>, 1, 16, 5, 4, 2.72f, 1.31f, 0.02f, 0.34f, 6.03e6f, 0.21f, 18.15e6f},
+    {run_rows<4, 1, 4, 2, GATED, true>, 2, 16, 3, 4, 2.83f, 0.82f, 0.73f, 0.47f, 6.08e6f, 0.26f, 12.29e6f},
+    {run_rows<4, 2, 4, 1, GATED, true>, 2, 32, 3, 4, 3.61f, 0.51f, 0.1f, 1.05f, 6.16e6f, 0.2f, 24.34e6f},
+    {run_wide<1, 1, 4, 1, 4, 4, GATED, true>, 4, 32, 4, 1, 3.37f, 0.79f, 0.43f, 0.29f, 6.05e6f, 0.54f, 21.2e6f},
+    {run_wide<1, 2, 4, 1, 4, 4, GATED, true>, 4, 64, 2, 1, 1.97f, 2.31f, 0.53f, 0.44f, 4.62e6f, 0.83f, 41.98e6f},
+    {run_wide<2, 2, 4, 1, 5, 2, GATED, true>, 8, 64, 3, 1, 3.32f, 0.51f, 0.79f, 0.47f, 5.53e6f, 1.87f, 20.65e6f},
+    {run_wide<2, 4, 4, 1, 4, 1, GATED, true>, 8, 128, 2, 1, 3.92f, 1.12f, 0.79f, 0.69f, 5.31e6f, 5.46f, 13.18e6f},
 };
 
 constexpr int kCus = 256;
@@ -673,12 +673,12 @@ float time_of(const Form& f, const I8Params& p, float experts, bool gated_produc
     const float m = (float)p.m;
     // By experts the rows of each are not known here: as many have rows as would have by chance, and the last tile of each is half full.
     const float tiles_m = !p.offsets ? (float)in_all(p.m, f.rows) : larger(experts, m > 0.25f * (float)f.rows * experts ? m / (float)f.rows + 0.5f * experts : 0.f);
-    const float groups = (float)in_all(p.tiles, f.tiles) * tiles_m, all = (float)p.blocks, blocks = (float)in_all(p.blocks, f.split), gate = gated_product ? f.gate : 0.f;
+    const float groups_n = (float)in_all(p.tiles, f.tiles), groups = groups_n * tiles_m, all = (float)p.blocks, blocks = (float)in_all(p.blocks, f.split), gate = gated_product ? f.gate : 0.f;
     const int down = (int)((groups < 1e9f ? groups : 1e9f) * (1.f / kCus)), times = down + ((float)down * kCus < groups ? 1 : 0), full = times / f.at_once, rest = times - full * f.at_once;
     float us = f.start + (float)full * (f.round + blocks * larger(f.alone, (float)f.at_once * f.share)) + gate * (float)times;
     if (rest > 0) us += f.round + blocks * larger(f.alone, (float)rest * f.share);
     const float weights = experts * (float)p.tiles * all * (float)kTileBlock;
-    const float again = larger(0.f, groups * all * (float)(f.tiles * kTileBlock + f.rows * kBlk) - weights);
+    const float again = larger(0.f, all * (groups * (float)(f.tiles * kTileBlock) + groups_n * m * (float)kBlk) - weights);
     return larger(us, f.start + 1.f + gate + weights / f.memory + again / f.l2);
 }
 

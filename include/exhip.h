@@ -79,7 +79,8 @@ const char* exhip_last_error(void);
  * order). "f32_tile" pins the float32 convolution's wave tile and split (0 = its rule, n = the n-th of its list;
  * sums then run in another order).
  * "f8_form" pins the kernel of the products in 8-bit floating point (0 = its rule, n = the n-th of the entry point's list for the result's type; sums
- * then run in another order), "f8_front" has such a product's first rows, that many, in a launch of their own (0 = its rule).
+ * then run in another order), "f8_front" has such a product's first rows, that many, in a launch of their own (0 = its rule). "i8_form" pins the kernel of the products in
+ * 8-bit integers (0 = its rule, n = the n-th of the list of those alone or by experts; the same values).
  * Process-wide; packed weights depend on the first three, so set them before packing. */
 int exhip_set_option(const char* name, int value);
 unsigned exhip_options_version(void); /* counts the calls above: plans made under other options are made again */
