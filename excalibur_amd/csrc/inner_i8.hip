@@ -653,31 +653,31 @@ int run_wide(exhip_ctx* ctx, const I8Params& p) {
     return launch(ctx, i8_wide_kernel<TN, TM, WN, WM, BUFFERS, D, GATED, GROUPED>, p, TN * WN, 32 * TM * WM, 64 * WN * WM);
 }
 // Chosen so that the form with the least of these times is as near to the fastest as it can be over 952 products and 700 products by experts of 1 to 8192 rows, 64 to 16384
-// outputs and inputs and 2 to 256 experts, those of at most 64 rows counted twice: it takes 1.1 % and 1.6 % longer on average, 25 % at most, and over 102 and 125 others 1.2 %
-// and 1.8 %, 24 % at most. Without any one form of the first list some product would take 10 to 36 % longer, without one of the second 9 to 31 %.
+// outputs and inputs and 2 to 256 experts, those of at most 64 rows counted twice: it takes 0.9 % and 1.3 % longer on average, 25 % at most, and over 102 and 125 others 0.7 %
+// and 1.8 %, 20 % at most. Without any one form of the first list some product would take 8 to 36 % longer, without one of the second 8 to 30 %.
 template <bool GATED>
 constexpr Form kPlain[] = {
-    {run_rows<2, 1, 8, 2, GATED, false>, 1, 16, 2, 8, 2.05f, 0.76f, 0.04f, 0.63f, 12.01e6f, 0.05f, 17.94e6f},
-    {run_rows<2, 1, 4, 2, GATED, false>, 1, 16, 5, 4, 2.09f, 0.54f, 0.57f, 0.33f, 13.59e6f, 0.07f, 13.61e6f},
-    {run_rows<2, 2, 4, 2, GATED, false>, 1, 32, 4, 4, 2.28f, 0.19f, 0.07f, 0.55f, 9.19e6f, 0.03f, 18.79e6f},
-    {run_rows<4, 1, 4, 2, GATED, false>, 2, 16, 3, 4, 2.82f, 0.67f, 0.02f, 0.48f, 5.38e6f, 1.33f, 164.9e6f},
-    {run_rows<4, 2, 4, 1, GATED, false>, 2, 32, 3, 4, 2.7f, 0.41f, 0.32f, 0.76f, 8.02e6f, 0.f, 29.22e6f},
-    {run_rows<4, 4, 4, 1, GATED, false>, 2, 64, 2, 4, 3.14f, 1.08f, 0.11f, 1.04f, 8.19e6f, 0.f, 15.35e6f},
-    {run_wide<1, 1, 2, 1, 8, 8, GATED, false>, 2, 32, 4, 1, 1.68f, 1.84f, 0.03f, 0.14f, 2.5e6f, 0.46f, 16.48e6f},
-    {run_wide<1, 1, 4, 1, 4, 4, GATED, false>, 4, 32, 4, 1, 2.53f, 0.03f, 0.31f, 0.22f, 7.43e6f, 0.74f, 20.29e6f},
-    {run_wide<1, 2, 4, 1, 4, 4, GATED, false>, 4, 64, 2, 1, 0.98f, 1.92f, 0.4f, 0.29f, 6.37e6f, 1.36f, 13.82e6f},
-    {run_wide<2, 2, 4, 1, 5, 2, GATED, false>, 8, 64, 3, 1, 3.68f, 0.11f, 0.07f, 0.48f, 3.95e6f, 1.19f, 20.52e6f},
-    {run_wide<2, 4, 4, 1, 4, 1, GATED, false>, 8, 128, 2, 1, 3.5f, 0.06f, 0.8f, 0.67f, 4.03e6f, 4.73f, 15.65e6f},
+    {run_rows<2, 1, 8, 2, GATED, false>, 1, 16, 2, 8, 2.05f, 0.67f, 0.44f, 0.65f, 6.86e6f, 0.07f, 20.24e6f},
+    {run_rows<2, 1, 4, 2, GATED, false>, 1, 16, 5, 4, 1.95f, 0.14f, 0.95f, 0.17f, 7.28e6f, 0.14f, 6.75e6f},
+    {run_rows<2, 2, 4, 2, GATED, false>, 1, 32, 4, 4, 2.29f, 0.04f, 0.09f, 0.62f, 7.59e6f, 0.f, 16.16e6f},
+    {run_rows<4, 1, 4, 2, GATED, false>, 2, 16, 3, 4, 2.38f, 0.44f, 0.6f, 0.46f, 6.6e6f, 0.11f, 23.17e6f},
+    {run_rows<4, 2, 4, 1, GATED, false>, 2, 32, 3, 4, 2.81f, 0.23f, 0.58f, 0.85f, 6.79e6f, 0.f, 20.37e6f},
+    {run_rows<4, 4, 4, 1, GATED, false>, 2, 64, 2, 4, 5.77f, 0.02f, 0.17f, 0.99f, 14.54e6f, 0.f, 172.2e6f},
+    {run_wide<1, 1, 2, 1, 8, 8, GATED, false>, 2, 32, 4, 1, 1.3f, 1.86f, 0.21f, 0.18f, 2.5e6f, 3.f, 14.53e6f},
+    {run_wide<1, 1, 4, 1, 4, 4, GATED, false>, 4, 32, 4, 1, 1.24f, 1.93f, 0.02f, 0.29f, 3.13e6f, 0.39f, 74.39e6f},
+    {run_wide<1, 2, 4, 1, 4, 4, GATED, false>, 4, 64, 2, 1, 1.22f, 1.98f, 0.48f, 0.34f, 5.6e6f, 0.42f, 29.71e6f},
+    {run_wide<2, 2, 4, 1, 5, 2, GATED, false>, 8, 64, 3, 1, 1.66f, 3.12f, 0.24f, 0.47f, 2.5e6f, 0.1f, 30.8e6f},
+    {run_wide<2, 4, 4, 1, 4, 1, GATED, false>, 8, 128, 2, 1, 2.39f, 3.15f, 0.03f, 0.67f, 8.48e6f, 0.55f, 30.59e6f},
 };
 template <bool GATED>
 constexpr Form kGrouped[] = {
-    {run_rows<2, 1, 4, 2, GATED, true>, 1, 16, 5, 4, 2.72f, 1.31f, 0.02f, 0.34f, 6.03e6f, 0.21f, 18.15e6f},
-    {run_rows<4, 1, 4, 2, GATED, true>, 2, 16, 3, 4, 2.83f, 0.82f, 0.73f, 0.47f, 6.08e6f, 0.26f, 12.29e6f},
-    {run_rows<4, 2, 4, 1, GATED, true>, 2, 32, 3, 4, 3.61f, 0.51f, 0.1f, 1.05f, 6.16e6f, 0.2f, 24.34e6f},
-    {run_wide<1, 1, 4, 1, 4, 4, GATED, true>, 4, 32, 4, 1, 3.37f, 0.79f, 0.43f, 0.29f, 6.05e6f, 0.54f, 21.2e6f},
-    {run_wide<1, 2, 4, 1, 4, 4, GATED, true>, 4, 64, 2, 1, 1.97f, 2.31f, 0.53f, 0.44f, 4.62e6f, 0.83f, 41.98e6f},
-    {run_wide<2, 2, 4, 1, 5, 2, GATED, true>, 8, 64, 3, 1, 3.32f, 0.51f, 0.79f, 0.47f, 5.53e6f, 1.87f, 20.65e6f},
-    {run_wide<2, 4, 4, 1, 4, 1, GATED, true>, 8, 128, 2, 1, 3.92f, 1.12f, 0.79f, 0.69f, 5.31e6f, 5.46f, 13.18e6f},
+    {run_rows<2, 1, 4, 2, GATED, true>, 1, 16, 5, 4, 2.88f, 1.05f, 0.16f, 0.44f, 6.27e6f, 0.43f, 18.35e6f},
+    {run_rows<4, 1, 4, 2, GATED, true>, 2, 16, 3, 4, 2.83f, 0.68f, 0.42f, 0.93f, 5.38e6f, 0.04f, 29.14e6f},
+    {run_rows<4, 2, 4, 1, GATED, true>, 2, 32, 3, 4, 3.4f, 0.87f, 0.02f, 1.12f, 6.34e6f, 0.08f, 19.34e6f},
+    {run_wide<1, 1, 4, 1, 4, 4, GATED, true>, 4, 32, 4, 1, 3.36f, 1.96f, 0.41f, 0.25f, 6.04e6f, 0.38f, 33.05e6f},
+    {run_wide<1, 2, 4, 1, 4, 4, GATED, true>, 4, 64, 2, 1, 2.33f, 2.75f, 0.1f, 0.49f, 5.5e6f, 0.77f, 17.46e6f},
+    {run_wide<2, 2, 4, 1, 5, 2, GATED, true>, 8, 64, 3, 1, 2.8f, 1.93f, 0.47f, 0.78f, 5.97e6f, 1.34f, 27.32e6f},
+    {run_wide<2, 4, 4, 1, 4, 1, GATED, true>, 8, 128, 2, 1, 3.1f, 4.97f, 1.14f, 0.89f, 5.96e6f, 2.17f, 39.69e6f},
 };
 
 constexpr int kCus = 256;
