@@ -311,27 +311,29 @@ __device__ __forceinline__ void by_gate(int gate, F values) {
 }
 
 // ---- few rows, or few products ----
-// A group takes TN x 16 outputs (of both projections) and 16 TM rows; its WK waves every WK-th block, with nothing between memory and their registers: the codes of
-// D of a wave's blocks are on their way at a time. The sums meet in LDS, and every thread finishes four neighbouring outputs of a row. What bounds it is the memory: one
-// row of the gated 11264 x 4096 takes 16.6 us, 5.6 TB/s of weights. Four waves a group, so that a CU has several groups, where there are many outputs (one row's 8 of 64 experts of
-// 1536 x 2048, gated, 9.1 us, with eight waves 12.1); eight where one group a CU has all of them (4096 x 4096 5.2 us, with four 5.7).
+// A group takes TN x 16 outputs (of both projections), whole tiles or half of one, and 16 TM rows; its WK waves every WK-th block, with nothing between memory and their registers:
+// the codes of D of a wave's blocks are on their way at a time. The sums meet in LDS, and every thread finishes four neighbouring outputs of a row. What bounds it is the memory:
+// one row of the gated 11264 x 4096 takes 16.6 us, 5.6 TB/s of weights. Four waves a group, so that a CU has several groups, where there are many outputs (one row's 8 of 64
+// experts of 1536 x 2048, gated, 9.0 us, with eight waves 12.1); eight where one group a CU has all of them (4096 x 4096 5.2 us, with four 5.7), and then half a tile a group without
+// an activation, so that more CUs have one (16 rows of 4096 x 11264 11.5 us, with whole tiles 14.3). More blocks on their way, or sixteen waves, measured no faster.
 template <int TN, int TM, int WK, int D, bool PAST, bool GATED, bool GROUPED>
 __global__ __launch_bounds__(64 * WK, 2) void i8_rows_kernel(const I8Params p) {
     exhip_touch_args(p);
     constexpr int kRows = 16 * TM, kSide = GATED ? 2 : 1;
-    static_assert(TN % 2 == 0, "whole tiles");
+    static_assert(TN % 2 == 0 || (TN == 1 && !GATED), "whole tiles, or half of one");
+    constexpr int kTiles = (TN + 1) / 2;
     const Tiles<GROUPED, kRows> tiles(p);
     if ((int)blockIdx.x >= p.groups_n * tiles.total) return;
     const Part part = tiles.part(p);
     if (part.rows <= 0) return;  // offsets that do not rise
     const int lane = threadIdx.x % 64, wk = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), q = lane / 16, col = lane % 16;
-    const int blocks = p.blocks, row_bytes = blocks * kTileBlock, tile0 = part.group_n * (TN / 2), last = p.tiles - 1;
-    const __amdgpu_buffer_rsrc_t weights = uniform_view(p.w + ((size_t)part.expert * p.tiles + tile0) * row_bytes, (unsigned)(min(TN / 2, p.tiles - tile0) * row_bytes));
+    const int blocks = p.blocks, row_bytes = blocks * kTileBlock, tile0 = TN == 1 ? part.group_n / 2 : part.group_n * kTiles, last = p.tiles - 1;
+    const __amdgpu_buffer_rsrc_t weights = uniform_view(p.w + ((size_t)part.expert * p.tiles + tile0) * row_bytes, (unsigned)(min(kTiles, p.tiles - tile0) * row_bytes));
     const Rows<GROUPED> rows(p, part);
     unsigned off[TM];
 #pragma unroll
     for (int t = 0; t < TM; ++t) off[t] = rows.begin(rows.source(16 * t + col)) + q * 16;
-    const int at = q * 512 + col * 16;
+    const int at = q * 512 + col * 16 + (TN == 1 ? part.group_n % 2 * 256 : 0);
     struct Codes {
         v4i w[TN][2], x[TM][2];
     } codes[D];
@@ -616,8 +618,8 @@ int quantize_rows(exhip_ctx* ctx, const char* name, const T* x, int x_stride, in
 }
 
 template <typename K>
-int launch(exhip_ctx* ctx, K kernel, I8Params p, int tiles, int rows, int threads) {
-    p.groups_n = (p.tiles + tiles - 1) / tiles;
+int launch(exhip_ctx* ctx, K kernel, I8Params p, int halves, int rows, int threads) {
+    p.groups_n = (2 * p.tiles + halves - 1) / halves;
     // By experts each one's rows are cut by themselves: at most rows - 1 missing in each, and no more tiles than rows.
     const long long most = p.offsets ? ((long long)p.m + (long long)p.experts * (rows - 1)) / rows : (p.m - 1) / rows + 1;
     const long long groups_m = most < p.m ? most : p.m, groups = p.groups_n * groups_m;
@@ -630,12 +632,12 @@ int launch(exhip_ctx* ctx, K kernel, I8Params p, int tiles, int rows, int thread
     return 0;
 }
 
-// One way to run a product: the tiles of 32 outputs (of both projections) and the rows that a group takes, how many groups a CU runs at once, how many waves share a
-// group's blocks, and what a launch takes, in us: `start`; each time that all CUs are given groups, `round`, and for each block of one wave `alone`, or `share` for each
-// group on a CU where that is more; `gate` for an activation, each time; but no less than reading the weights from memory and what groups read from L2, weights again and the rows there are, at so many bytes a us.
+// One way to run a product: how many 16 outputs (of both projections) and rows a group takes, how many groups a CU runs at once, how many waves share a group's blocks, and what
+// a launch takes, in us: `start`; each time that all CUs are given groups, `round`, and for each block of one wave `alone`, or `share` for each group on a CU where that is more;
+// `gate` for an activation, each time; but no less than reading the weights from memory and what groups read from L2, weights again and the rows there are, at so many bytes a us.
 struct Form {
     int (*run)(exhip_ctx*, const I8Params&);
-    int tiles, rows, at_once, split;
+    int halves, rows, at_once, split;
     float start, round, alone, share, memory, gate, l2;
 };
 constexpr long long kManyWeights = 40 << 20;
@@ -645,39 +647,39 @@ int run_rows(exhip_ctx* ctx, const I8Params& p) {
     // 4096 x 4096 would take 5.8 instead of 5.3).
     const bool once = GROUPED ? p.m <= p.experts * 4 * TM : p.m <= 16 * TM;
     if (once && (long long)(p.m < p.experts ? p.m : GROUPED ? p.experts : 1) * p.tiles * p.blocks * kTileBlock >= kManyWeights)
-        return launch(ctx, i8_rows_kernel<TN, TM, WK, D, true, GATED, GROUPED>, p, TN / 2, 16 * TM, 64 * WK);
-    return launch(ctx, i8_rows_kernel<TN, TM, WK, D, false, GATED, GROUPED>, p, TN / 2, 16 * TM, 64 * WK);
+        return launch(ctx, i8_rows_kernel<TN, TM, WK, D, true, GATED, GROUPED>, p, TN, 16 * TM, 64 * WK);
+    return launch(ctx, i8_rows_kernel<TN, TM, WK, D, false, GATED, GROUPED>, p, TN, 16 * TM, 64 * WK);
 }
 template <int TN, int TM, int WN, int WM, int BUFFERS, int D, bool GATED, bool GROUPED>
 int run_wide(exhip_ctx* ctx, const I8Params& p) {
-    return launch(ctx, i8_wide_kernel<TN, TM, WN, WM, BUFFERS, D, GATED, GROUPED>, p, TN * WN, 32 * TM * WM, 64 * WN * WM);
+    return launch(ctx, i8_wide_kernel<TN, TM, WN, WM, BUFFERS, D, GATED, GROUPED>, p, 2 * TN * WN, 32 * TM * WM, 64 * WN * WM);
 }
 // Chosen so that the form with the least of these times is as near to the fastest as it can be over 952 products and 700 products by experts of 1 to 8192 rows, 64 to 16384
-// outputs and inputs and 2 to 256 experts, those of at most 64 rows counted twice: it takes 0.9 % and 1.3 % longer on average, 25 % at most, and over 102 and 125 others 0.7 %
-// and 1.8 %, 20 % at most. Without any one form of the first list some product would take 8 to 36 % longer, without one of the second 8 to 30 %.
+// outputs and inputs and 2 to 256 experts, those of at most 64 rows counted twice: it takes 1.0 % and 1.3 % longer on average, 25 % at most, and over 109 and 125 others 0.7 %
+// and 1.6 %, 21 % at most. Without any one form of the first list some product would take 8 to 45 % longer, without one of the second 8 to 30 %.
 template <bool GATED>
 constexpr Form kPlain[] = {
-    {run_rows<2, 1, 8, 2, GATED, false>, 1, 16, 2, 8, 2.05f, 0.67f, 0.44f, 0.65f, 6.86e6f, 0.07f, 20.24e6f},
-    {run_rows<2, 1, 4, 2, GATED, false>, 1, 16, 5, 4, 1.95f, 0.14f, 0.95f, 0.17f, 7.28e6f, 0.14f, 6.75e6f},
-    {run_rows<2, 2, 4, 2, GATED, false>, 1, 32, 4, 4, 2.29f, 0.04f, 0.09f, 0.62f, 7.59e6f, 0.f, 16.16e6f},
-    {run_rows<4, 1, 4, 2, GATED, false>, 2, 16, 3, 4, 2.38f, 0.44f, 0.6f, 0.46f, 6.6e6f, 0.11f, 23.17e6f},
-    {run_rows<4, 2, 4, 1, GATED, false>, 2, 32, 3, 4, 2.81f, 0.23f, 0.58f, 0.85f, 6.79e6f, 0.f, 20.37e6f},
-    {run_rows<4, 4, 4, 1, GATED, false>, 2, 64, 2, 4, 5.77f, 0.02f, 0.17f, 0.99f, 14.54e6f, 0.f, 172.2e6f},
-    {run_wide<1, 1, 2, 1, 8, 8, GATED, false>, 2, 32, 4, 1, 1.3f, 1.86f, 0.21f, 0.18f, 2.5e6f, 3.f, 14.53e6f},
-    {run_wide<1, 1, 4, 1, 4, 4, GATED, false>, 4, 32, 4, 1, 1.24f, 1.93f, 0.02f, 0.29f, 3.13e6f, 0.39f, 74.39e6f},
-    {run_wide<1, 2, 4, 1, 4, 4, GATED, false>, 4, 64, 2, 1, 1.22f, 1.98f, 0.48f, 0.34f, 5.6e6f, 0.42f, 29.71e6f},
-    {run_wide<2, 2, 4, 1, 5, 2, GATED, false>, 8, 64, 3, 1, 1.66f, 3.12f, 0.24f, 0.47f, 2.5e6f, 0.1f, 30.8e6f},
-    {run_wide<2, 4, 4, 1, 4, 1, GATED, false>, 8, 128, 2, 1, 2.39f, 3.15f, 0.03f, 0.67f, 8.48e6f, 0.55f, 30.59e6f},
+    {run_rows<GATED ? 2 : 1, 1, 8, 2, GATED, false>, GATED ? 2 : 1, 16, 2, 8, 1.91f, 0.98f, 0.44f, 0.55f, 6.81e6f, 0.2f, 16.53e6f},
+    {run_rows<2, 1, 4, 2, GATED, false>, 2, 16, 5, 4, 2.14f, 0.58f, 0.49f, 0.31f, 12.75e6f, 0.17f, 13.59e6f},
+    {run_rows<2, 2, 4, 2, GATED, false>, 2, 32, 4, 4, 2.44f, 0.36f, 0.02f, 0.53f, 6.92e6f, 0.06f, 24.24e6f},
+    {run_rows<4, 1, 4, 2, GATED, false>, 4, 16, 3, 4, 2.33f, 1.07f, 0.5f, 0.45f, 5.3e6f, 0.f, 24.76e6f},
+    {run_rows<4, 2, 4, 1, GATED, false>, 4, 32, 3, 4, 2.63f, 0.17f, 0.65f, 0.87f, 6.47e6f, 0.f, 23.95e6f},
+    {run_rows<4, 4, 4, 1, GATED, false>, 4, 64, 2, 4, 4.8f, 0.1f, 0.85f, 0.98f, 7.08e6f, 0.16f, 42.56e6f},
+    {run_wide<1, 1, 2, 1, 8, 8, GATED, false>, 4, 32, 4, 1, 1.45f, 2.09f, 0.05f, 0.16f, 2.64e6f, 5.33f, 19.75e6f},
+    {run_wide<1, 1, 4, 1, 4, 4, GATED, false>, 8, 32, 4, 1, 1.09f, 1.98f, 0.03f, 0.28f, 4.3e6f, 0.12f, 28e6f},
+    {run_wide<1, 2, 4, 1, 4, 4, GATED, false>, 8, 64, 2, 1, 1.26f, 1.82f, 0.41f, 0.33f, 5.45e6f, 0.f, 30.7e6f},
+    {run_wide<2, 2, 4, 1, 5, 2, GATED, false>, 16, 64, 3, 1, 0.57f, 4.26f, 0.07f, 0.43f, 2.65e6f, 0.14f, 21.42e6f},
+    {run_wide<2, 4, 4, 1, 4, 1, GATED, false>, 16, 128, 2, 1, 0.87f, 4.51f, 0.67f, 0.62f, 4.83e6f, 0.85f, 200e6f},
 };
 template <bool GATED>
 constexpr Form kGrouped[] = {
-    {run_rows<2, 1, 4, 2, GATED, true>, 1, 16, 5, 4, 2.88f, 1.05f, 0.16f, 0.44f, 6.27e6f, 0.43f, 18.35e6f},
-    {run_rows<4, 1, 4, 2, GATED, true>, 2, 16, 3, 4, 2.83f, 0.68f, 0.42f, 0.93f, 5.38e6f, 0.04f, 29.14e6f},
-    {run_rows<4, 2, 4, 1, GATED, true>, 2, 32, 3, 4, 3.4f, 0.87f, 0.02f, 1.12f, 6.34e6f, 0.08f, 19.34e6f},
-    {run_wide<1, 1, 4, 1, 4, 4, GATED, true>, 4, 32, 4, 1, 3.36f, 1.96f, 0.41f, 0.25f, 6.04e6f, 0.38f, 33.05e6f},
-    {run_wide<1, 2, 4, 1, 4, 4, GATED, true>, 4, 64, 2, 1, 2.33f, 2.75f, 0.1f, 0.49f, 5.5e6f, 0.77f, 17.46e6f},
-    {run_wide<2, 2, 4, 1, 5, 2, GATED, true>, 8, 64, 3, 1, 2.8f, 1.93f, 0.47f, 0.78f, 5.97e6f, 1.34f, 27.32e6f},
-    {run_wide<2, 4, 4, 1, 4, 1, GATED, true>, 8, 128, 2, 1, 3.1f, 4.97f, 1.14f, 0.89f, 5.96e6f, 2.17f, 39.69e6f},
+    {run_rows<2, 1, 4, 2, GATED, true>, 2, 16, 5, 4, 2.88f, 1.05f, 0.16f, 0.44f, 6.27e6f, 0.43f, 18.35e6f},
+    {run_rows<4, 1, 4, 2, GATED, true>, 4, 16, 3, 4, 2.83f, 0.68f, 0.42f, 0.93f, 5.38e6f, 0.04f, 29.14e6f},
+    {run_rows<4, 2, 4, 1, GATED, true>, 4, 32, 3, 4, 3.4f, 0.87f, 0.02f, 1.12f, 6.34e6f, 0.08f, 19.34e6f},
+    {run_wide<1, 1, 4, 1, 4, 4, GATED, true>, 8, 32, 4, 1, 3.36f, 1.96f, 0.41f, 0.25f, 6.04e6f, 0.38f, 33.05e6f},
+    {run_wide<1, 2, 4, 1, 4, 4, GATED, true>, 8, 64, 2, 1, 2.33f, 2.75f, 0.1f, 0.49f, 5.5e6f, 0.77f, 17.46e6f},
+    {run_wide<2, 2, 4, 1, 5, 2, GATED, true>, 16, 64, 3, 1, 2.8f, 1.93f, 0.47f, 0.78f, 5.97e6f, 1.34f, 27.32e6f},
+    {run_wide<2, 4, 4, 1, 4, 1, GATED, true>, 16, 128, 2, 1, 3.1f, 4.97f, 1.14f, 0.89f, 5.96e6f, 2.17f, 39.69e6f},
 };
 
 constexpr int kCus = 256;
@@ -691,12 +693,12 @@ float time_of(const Form& f, const I8Params& p, float experts, bool gated_produc
     const float m = (float)p.m;
     // By experts the rows of each are not known here: as many have rows as would have by chance, and the last tile of each is half full.
     const float tiles_m = !p.offsets ? (float)in_all(p.m, f.rows) : larger(experts, m > 0.25f * (float)f.rows * experts ? m / (float)f.rows + 0.5f * experts : 0.f);
-    const float groups_n = (float)in_all(p.tiles, f.tiles), groups = groups_n * tiles_m, all = (float)p.blocks, blocks = (float)in_all(p.blocks, f.split), gate = gated_product ? f.gate : 0.f;
+    const float groups_n = (float)in_all(2 * p.tiles, f.halves), groups = groups_n * tiles_m, all = (float)p.blocks, blocks = (float)in_all(p.blocks, f.split), gate = gated_product ? f.gate : 0.f;
     const int down = (int)((groups < 1e9f ? groups : 1e9f) * (1.f / kCus)), times = down + ((float)down * kCus < groups ? 1 : 0), full = times / f.at_once, rest = times - full * f.at_once;
     float us = f.start + (float)full * (f.round + blocks * larger(f.alone, (float)f.at_once * f.share)) + gate * (float)times;
     if (rest > 0) us += f.round + blocks * larger(f.alone, (float)rest * f.share);
     const float weights = experts * (float)p.tiles * all * (float)kTileBlock;
-    const float again = larger(0.f, all * (groups * (float)(f.tiles * kTileBlock) + groups_n * m * (float)kBlk) - weights);
+    const float again = larger(0.f, all * (groups * (float)(f.halves * (kTileBlock / 2)) + groups_n * m * (float)kBlk) - weights);
     return larger(us, f.start + 1.f + gate + weights / f.memory + again / f.l2);
 }
 
