@@ -355,6 +355,13 @@ def test_every_form_at_the_sizes_of_the_others(ctx, pinned, form, gated):
         _product(ctx, m, n, k, m % 2 == 0, ("silu", "gelu", "sigmoid", "relu")[(form + m) % 4] if gated else None)
 
 
+@pytest.mark.parametrize("gate", ["silu", "gelu", "sigmoid", "relu"])
+def test_every_form_with_every_activation(ctx, pinned, gate):
+    for form in range(1, FORMS + 1):
+        pinned(form)
+        _product(ctx, 70, 150, 200, form % 2 == 0, gate)
+
+
 FORM_GROUPED = [(1, 1, 33, 64, "one"), (50, 3, 100, 300, "chance"), (130, 7, 129, 140, "holes"), (300, 4, 530, 520, "inside"), (64, 100, 20, 128, "chance"), (20, 6, 40, 100, "none"), (257, 130, 35, 40, "holes")]
 
 
