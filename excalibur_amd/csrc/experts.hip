@@ -200,8 +200,10 @@ __global__ __launch_bounds__(kRun) void group_rows_by_run(const int* __restrict_
 }
 
 // ---- the sum of the answers ----
-// A row's weights: a choice's own, in a lane each.
-__device__ __forceinline__ float weight_of(const float* weights, int kind, int each, int j) {
+// A row's weights: a choice's own, in a lane each. `none`: all of them are logarithms of 0 and nothing divides them; the row is 0 then, whatever its answers are (0 times
+// an infinity, or times what a row that nothing computed holds, would be no number).
+__device__ __forceinline__ float weight_of(const float* weights, int kind, int each, int j, bool* none) {
+    *none = false;
     const float given = j < each ? weights[j] : -__builtin_inff();
     if (kind == EXHIP_WEIGHTS_PLAIN) return given;
     if (kind == EXHIP_WEIGHTS_LOG) return expf(given);
@@ -212,7 +214,8 @@ __device__ __forceinline__ float weight_of(const float* weights, int kind, int e
     float total = own;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
-    return total == 0.f ? 0.f : own / total;
+    *none = total == 0.f;
+    return own / total;
 }
 
 // A wave takes a row and eight outputs a lane; its lanes hold the row's places and weights, which the sum takes from them one choice at a time, always in the
@@ -227,8 +230,10 @@ __global__ __launch_bounds__(256) void combine_rows_kernel(const uint16_t* __res
     const int lane = threadIdx.x % 64;
     const size_t row = wave / waves_a_row;
     const int at = (int)(wave % waves_a_row) * 512 + lane * 8;
-    const int place = lane < each ? places[row * each + lane] : -1;
-    const float weight = weight_of(weights + row * each, kind, each, lane);
+    const int chosen = lane < each ? places[row * each + lane] : -1;
+    bool none;
+    const float weight = weight_of(weights + row * each, kind, each, lane, &none);
+    const int place = none ? -1 : chosen;
     const bool whole = at + 8 <= n;
     float sum[8];
 #pragma unroll

@@ -621,7 +621,7 @@ int exhip_innerproduct_grouped_gated_i8(exhip_ctx* ctx, const exhip_i8_desc* d, 
                                         const float* bias_gate, const float* bias_up, float* y_f32, uint16_t* y_f16);
 /* What the experts of each row answered, added up: y[r] = sum over its choices, in their order, of weight * z[places[r][choice]] (halves z[z_rows][n], row stride z_stride;
  * y's row stride y_stride, both in elements and at least n), sums in float32. A place below 0 adds nothing, one from z_rows on gives NaN. weights[m][each] are taken as they are,
- * as logarithms, or as logarithms of weights that are divided by their sum over all of the row's choices; where all of these are -infinity the row is 0. */
+ * as logarithms, or as logarithms of weights that are divided by their sum over all of the row's choices; where all of these are -infinity the row is 0 and none of its answers is read. */
 #define EXHIP_WEIGHTS_PLAIN 0
 #define EXHIP_WEIGHTS_LOG 1
 #define EXHIP_WEIGHTS_LOG_NORMALIZED 2
