@@ -618,9 +618,14 @@ int quantize_rows(exhip_ctx* ctx, const char* name, const T* x, int x_stride, in
     constexpr int kWave = 64 * Piece<T>::kValues;
     const bool past_l2 = (size_t)m * k * sizeof(T) > kPastL2 && k > kWave;
     auto run = [&](auto kernel, int rows) { hipLaunchKernelGGL(kernel, dim3((m - 1) / rows + 1), dim3(256), 0, ctx->stream, x, x_stride, m, k, y, y_stride, scale, past_l2); };
+    // A kernel holds the whole row where there is one that does: with a piece to read again 4096 rows of 5120 floats take 18.7 to 22.9 us, held in six 17.6, one row of 6144 halves 4.0 and 3.6;
+    // every piece that a row does not fill costs 0.1 us for a float row alone and 0.3 for a half one, 8 % for each of 16384 rows of one. Up to three waves' values the row has one wave where
+    // there are so many rows that a group's barrier costs more than its four times as many waves give: 768 floats 3.2 us with four waves and 3.3 with one at 520 rows, 4.1 and 3.6 at 2048;
+    // 1024 halves 3.5 and 4.1 at 768 rows, 5.1 and 4.6 at 2560; 1536 halves 6.6 and 7.2 at 3500, 6.8 and 6.4 at 4096 that stay in cache, 18.0 and 16.4 at 16384.
+    constexpr bool kFloats = sizeof(T) == 4;
     if (k <= kWave) run(quantize_rows_i8_kernel<T, 1, 1>, 4);
-    else if (k <= 2 * kWave && m > 512) run(quantize_rows_i8_kernel<T, 1, 2>, 4);
-    else if (k <= 3 * kWave && m > 512) run(quantize_rows_i8_kernel<T, 1, 3>, 4);
+    else if (k <= 2 * kWave && m > (kFloats ? 512 : 2048)) run(quantize_rows_i8_kernel<T, 1, 2>, 4);
+    else if (k <= 3 * kWave && m > (kFloats ? 512 : 3500)) run(quantize_rows_i8_kernel<T, 1, 3>, 4);
     else if (k <= 4 * kWave) run(quantize_rows_i8_kernel<T, 4, 1>, 1);
     else if (k <= 8 * kWave) run(quantize_rows_i8_kernel<T, 4, 2>, 1);
     else if (k <= 12 * kWave) run(quantize_rows_i8_kernel<T, 4, 3>, 1);

@@ -25,8 +25,9 @@ def pinned():
 
 
 # ---- the quantizer ----
-# A wave's pieces are 256 floats or 512 halves: rows of up to three waves' from 512 rows on, 515 being no multiple of a group's four; the longer forms of one row a group; more than 64 MB.
-QUANTIZED = [(515, 300, 0), (515, 513, 3), (515, 700, 0), (515, 768, 1), (515, 1000, 0), (515, 1500, 5), (515, 1536, 0), (5, 1500, 0), (5, 2048, 2), (5, 3500, 1), (5, 6000, 0), (5, 11264, 0), (6, 12289, 1),
+# A wave's pieces are 256 floats or 512 halves: rows of up to three waves' with one wave each (from 512 rows of floats, 2048 and 3500 of halves on, none of these a multiple of a group's four) and with
+# four; the longer forms of one row a group; more than 64 MB.
+QUANTIZED = [(515, 300, 0), (515, 513, 3), (515, 700, 0), (515, 768, 1), (515, 1000, 0), (515, 1500, 5), (515, 1536, 0), (2051, 700, 1), (2051, 1024, 0), (3503, 1300, 3), (3503, 1536, 0), (5, 1500, 0), (5, 2048, 2), (5, 3500, 1), (5, 6000, 0), (5, 11264, 0), (6, 12289, 1),
              (4, 20000, 0)]
 PAST_L2 = {"f32": [(4100, 4101, 0), (60001, 300, 1), (24003, 760, 0)], "f16": [(8195, 4101, 0), (50001, 700, 1), (24003, 1500, 0)]}
 
