@@ -18,7 +18,7 @@ constexpr int kTileBlock = 32 * kBlk;    // bytes of a tile's weights for them
 constexpr int kMostInputs = 131071;      // 2^14 each, 2^31 - 1 at most together
 constexpr int kMostStride = 1 << 22;     // of a row of codes
 constexpr int kMostExperts = 1024;
-constexpr size_t kPastL2 = 64 << 20;     // what is read once and more than this is not kept in L2, 32 MB of it
+constexpr size_t kRowsPastL2 = 128 << 20;  // half of the cache behind L2
 constexpr float kLargest = 127.f;
 constexpr float kLeastScale = 0x1p-100f;  // keeps 1 / scale finite and rows of zeros at zero
 constexpr int kNonTemporal = 2;           // of a buffer load: past L2
@@ -48,10 +48,11 @@ struct Piece {
         T v[kValues];
     };
     T v[kValues];
-    __device__ __forceinline__ void load(const T* row, int at, int k, bool past_l2) {  // zeros behind the row's end
+    template <bool PAST>
+    __device__ __forceinline__ void load(const T* row, int at, int k) {  // zeros behind the row's end
         if (at + kValues <= k) {
             Packed p;
-            if (past_l2) p = __builtin_bit_cast(Packed, __builtin_nontemporal_load(reinterpret_cast<const v4i_any*>(row + at)));
+            if constexpr (PAST) p = __builtin_bit_cast(Packed, __builtin_nontemporal_load(reinterpret_cast<const v4i_any*>(row + at)));
             else p = *reinterpret_cast<const Packed*>(row + at);
 #pragma unroll
             for (int e = 0; e < kValues; ++e) v[e] = p.v[e];
@@ -93,11 +94,9 @@ struct Piece {
 };
 
 // WAVES waves a row (a wave takes its own row where that is one), HELD pieces a lane that stay in registers between the largest value and the codes; what a longer
-// row has behind them is read again. Rows go past L2 where they are more than it holds: 8000 x 5001 float32 39.5 -> 35.1 us, 8192 x 11264 halves 58.8 -> 53.6; 8192 x 2048 would take 14.4
-// instead of 12.5.
-template <typename T, int WAVES, int HELD>
-__global__ __launch_bounds__(256) void quantize_rows_i8_kernel(const T* __restrict__ x, int x_stride, int m, int k, int8_t* __restrict__ y, int y_stride, float* __restrict__ scale,
-                                                               bool past_l2) {
+// row has behind them is read again. PAST: rows go past L2 (a kernel of its own: where both loads stand in one, the compiler makes one of them, without it).
+template <typename T, int WAVES, int HELD, bool PAST>
+__global__ __launch_bounds__(256) void quantize_rows_i8_kernel(const T* __restrict__ x, int x_stride, int m, int k, int8_t* __restrict__ y, int y_stride, float* __restrict__ scale) {
     constexpr int kStep = 64 * WAVES * Piece<T>::kValues;
     const int wave = threadIdx.x / 64, row = blockIdx.x * (4 / WAVES) + wave / WAVES;
     if (row >= m) return;  // a whole wave, and a whole group where several have a row
@@ -105,13 +104,13 @@ __global__ __launch_bounds__(256) void quantize_rows_i8_kernel(const T* __restri
     const int first = threadIdx.x % (64 * WAVES) * Piece<T>::kValues;
     Piece<T> held[HELD];
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) held[i].load(from, first + i * kStep, k, past_l2);
+    for (int i = 0; i < HELD; ++i) held[i].template load<PAST>(from, first + i * kStep, k);
     float most = 0.f;
 #pragma unroll
     for (int i = 0; i < HELD; ++i) most = held[i].most(most);
     for (int at = first + HELD * kStep; at < k; at += kStep) {
         Piece<T> p;
-        p.load(from, at, k, past_l2);
+        p.template load<PAST>(from, at, k);
         most = p.most(most);
     }
     // as whole numbers the bits of values that are not negative are in their order, and those of NaN above all
@@ -138,7 +137,7 @@ __global__ __launch_bounds__(256) void quantize_rows_i8_kernel(const T* __restri
         if (first + i * kStep < k) held[i].store(to, first + i * kStep, k, s, inverse);
     for (int at = first + HELD * kStep; at < k; at += kStep) {
         Piece<T> p;
-        p.load(from, at, k, past_l2);
+        p.template load<PAST>(from, at, k);
         p.store(to, at, k, s, inverse);
     }
 }
@@ -616,22 +615,25 @@ int quantize_rows(exhip_ctx* ctx, const char* name, const T* x, int x_stride, in
     const exhip_on_device on(ctx->device);
     EXHIP_CHECK(on.error);
     constexpr int kWave = 64 * Piece<T>::kValues;
-    const bool past_l2 = (size_t)m * k * sizeof(T) > kPastL2 && k > kWave;
-    auto run = [&](auto kernel, int rows) { hipLaunchKernelGGL(kernel, dim3((m - 1) / rows + 1), dim3(256), 0, ctx->stream, x, x_stride, m, k, y, y_stride, scale, past_l2); };
+    auto run = [&](auto kernel, int rows) { hipLaunchKernelGGL(kernel, dim3((m - 1) / rows + 1), dim3(256), 0, ctx->stream, x, x_stride, m, k, y, y_stride, scale); };
+    // Rows that are read once, and that neither L2 nor the cache behind it, 256 MB, holds together with what else a program has under way, go past L2: 8000 x 5001 floats 38.4 -> 33.8 us,
+    // 60000 x 700 40.7 -> 34.5, 65536 x 8192 halves 286 -> 271. Where they are still in that cache it is the longer way: the 8000 x 5001 once more 30.2 -> 33.6, 8192 x 2048 13.9 -> 16.5; and for
+    // half rows with a wave each (60000 x 1500 56 -> 54 to 63) and rows that are read again (3000 x 16000 floats 59 -> 61).
+    constexpr bool kFloats = sizeof(T) == 4;
+    const bool past = (size_t)m * k * sizeof(T) > kRowsPastL2 && (kFloats || k > 3 * kWave) && k <= 32 * kWave;
     // A kernel holds the whole row where there is one that does: with a piece to read again 4096 rows of 5120 floats take 18.7 to 22.9 us, held in six 17.6, one row of 6144 halves 4.0 and 3.6;
     // every piece that a row does not fill costs 0.1 us for a float row alone and 0.3 for a half one, 8 % for each of 16384 rows of one. Up to three waves' values the row has one wave where
     // there are so many rows that a group's barrier costs more than its four times as many waves give: 768 floats 3.2 us with four waves and 3.3 with one at 520 rows, 4.1 and 3.6 at 2048;
     // 1024 halves 3.5 and 4.1 at 768 rows, 5.1 and 4.6 at 2560; 1536 halves 6.6 and 7.2 at 3500, 6.8 and 6.4 at 4096 that stay in cache, 18.0 and 16.4 at 16384.
-    constexpr bool kFloats = sizeof(T) == 4;
-    if (k <= kWave) run(quantize_rows_i8_kernel<T, 1, 1>, 4);
-    else if (k <= 2 * kWave && m > (kFloats ? 512 : 2048)) run(quantize_rows_i8_kernel<T, 1, 2>, 4);
-    else if (k <= 3 * kWave && m > (kFloats ? 512 : 3500)) run(quantize_rows_i8_kernel<T, 1, 3>, 4);
-    else if (k <= 4 * kWave) run(quantize_rows_i8_kernel<T, 4, 1>, 1);
-    else if (k <= 8 * kWave) run(quantize_rows_i8_kernel<T, 4, 2>, 1);
-    else if (k <= 12 * kWave) run(quantize_rows_i8_kernel<T, 4, 3>, 1);
-    else if (k <= 16 * kWave) run(quantize_rows_i8_kernel<T, 4, 4>, 1);
-    else if (k <= 24 * kWave) run(quantize_rows_i8_kernel<T, 4, 6>, 1);
-    else run(quantize_rows_i8_kernel<T, 4, 8>, 1);
+    if (k <= kWave) run(quantize_rows_i8_kernel<T, 1, 1, false>, 4);
+    else if (k <= 2 * kWave && m > (kFloats ? 512 : 2048)) run(past ? quantize_rows_i8_kernel<T, 1, 2, kFloats> : quantize_rows_i8_kernel<T, 1, 2, false>, 4);
+    else if (k <= 3 * kWave && m > (kFloats ? 512 : 3500)) run(past ? quantize_rows_i8_kernel<T, 1, 3, kFloats> : quantize_rows_i8_kernel<T, 1, 3, false>, 4);
+    else if (k <= 4 * kWave) run(past ? quantize_rows_i8_kernel<T, 4, 1, true> : quantize_rows_i8_kernel<T, 4, 1, false>, 1);
+    else if (k <= 8 * kWave) run(past ? quantize_rows_i8_kernel<T, 4, 2, true> : quantize_rows_i8_kernel<T, 4, 2, false>, 1);
+    else if (k <= 12 * kWave) run(past ? quantize_rows_i8_kernel<T, 4, 3, true> : quantize_rows_i8_kernel<T, 4, 3, false>, 1);
+    else if (k <= 16 * kWave) run(past ? quantize_rows_i8_kernel<T, 4, 4, true> : quantize_rows_i8_kernel<T, 4, 4, false>, 1);
+    else if (k <= 24 * kWave) run(past ? quantize_rows_i8_kernel<T, 4, 6, true> : quantize_rows_i8_kernel<T, 4, 6, false>, 1);
+    else run(past ? quantize_rows_i8_kernel<T, 4, 8, true> : quantize_rows_i8_kernel<T, 4, 8, false>, 1);
     EXHIP_LAUNCH_CHECK();
     return 0;
 }

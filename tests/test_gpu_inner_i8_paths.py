@@ -26,30 +26,34 @@ def pinned():
 
 # ---- the quantizer ----
 # A wave's pieces are 256 floats or 512 halves: rows of up to three waves' with one wave each (from 512 rows of floats, 2048 and 3500 of halves on, none of these a multiple of a group's four) and with
-# four; the longer forms of one row a group; more than 64 MB.
+# four; the longer forms of one row a group; more than 128 MB, the same rows again and again.
 QUANTIZED = [(515, 300, 0), (515, 513, 3), (515, 700, 0), (515, 768, 1), (515, 1000, 0), (515, 1500, 5), (515, 1536, 0), (2051, 700, 1), (2051, 1024, 0), (3503, 1300, 3), (3503, 1536, 0), (5, 1500, 0), (5, 2048, 2), (5, 3500, 1), (5, 6000, 0), (5, 11264, 0), (6, 12289, 1),
              (4, 20000, 0)]
-PAST_L2 = {"f32": [(4100, 4101, 0), (60001, 300, 1), (24003, 760, 0)], "f16": [(8195, 4101, 0), (50001, 700, 1), (24003, 1500, 0)]}
+PAST_L2 = {"f32": [(8203, 4101, 0), (112003, 300, 1), (46001, 760, 0), (16387, 2050, 1), (3801, 9000, 0)], "f16": [(16391, 4101, 0), (96003, 700, 1), (46001, 1500, 0), (6001, 11264, 0), (4001, 17000, 0)]}
 
 
-def _quantized(ctx, dtype, m, k, pad):
+def _quantized(ctx, dtype, m, k, pad, distinct=None):
     rng = np.random.default_rng(m + k)
-    x = rng.standard_normal((m, k), np.float32)
-    x *= np.exp(rng.standard_normal((m, 1))).astype(np.float32)
+    distinct = m if distinct is None else distinct
+    x = rng.standard_normal((distinct, k), np.float32)
+    x *= np.exp(rng.standard_normal((distinct, 1))).astype(np.float32)
     x = x.astype(np.float16 if dtype == "f16" else np.float32)
     x[0] = 0
     x[1, -1] = np.nan
-    x[m - 1, 0] = np.inf
+    x[distinct - 1, 0] = np.inf
     x[2] = np.where(rng.random(k) < 0.5, 1, -1)
     want, scale = i8ref.quantize_rows(x.astype(np.float32))
-    dx = ctx.array(_wide(x, k + pad, np.nan).view(np.uint16 if dtype == "f16" else np.float32))
+    dx = ctx.array(_wide(x, k + pad, np.nan)[np.arange(m) % distinct].view(np.uint16 if dtype == "f16" else np.float32))
     y = ctx.array(np.full((m + 1, (k + 15) // 16 * 16 + 16), 0x25, np.int8))
     scales = ctx.array(np.full(m + 1, 7.25, np.float32))
     ctx.quantize_rows_i8(dx, k, y=y, scale=scales)
     got, got_scale = y.download(), scales.download()
-    assert np.array_equal(got_scale[:m], scale, equal_nan=True) and got_scale[m] == 7.25
-    assert np.array_equal(got[:m, :k], want)
-    assert np.all(got[:m, k:] == 0x25) and np.all(got[m] == 0x25)
+    for first in range(0, m, distinct):
+        rows = slice(first, min(m, first + distinct))
+        count = rows.stop - first
+        assert np.array_equal(got_scale[rows], scale[:count], equal_nan=True)
+        assert np.array_equal(got[rows, :k], want[:count])
+    assert got_scale[m] == 7.25 and np.all(got[:m, k:] == 0x25) and np.all(got[m] == 0x25)
     for a in (dx, y, scales):
         a.free()
 
@@ -62,7 +66,8 @@ def test_quantized_rows_of_every_kernel(ctx, dtype, m, k, pad):
 
 @pytest.mark.parametrize("dtype,m,k,pad", [(t, *s) for t, sizes in PAST_L2.items() for s in sizes])
 def test_quantized_rows_that_go_past_l2(ctx, dtype, m, k, pad):
-    _quantized(ctx, dtype, m, k, pad)
+    assert m * k * (4 if dtype == "f32" else 2) > 128 << 20
+    _quantized(ctx, dtype, m, k, pad, distinct=1031)
 
 
 # ---- results that begin on lines ----
