@@ -103,7 +103,8 @@ __global__ __launch_bounds__(1024) void group_rows_by_expert(const int* __restri
 // many copies as there is room for, so that the lanes of an addition meet seldom. From the counts every group has where each expert's rows begin and how many of them stand
 // ahead of its run, and it places its own choices, 1024 at a time: behind those of earlier waves, and within a wave behind the earlier lanes with the same expert. Nothing waits for
 // another group, so one launch does it; whole numbers are added, so no order of additions shows. What bounds it is a CU's reading of all choices and their additions: 65528 choices of
-// 256 experts take 8.5 us and of 1024 10.0, where a group an expert takes 12 and 28; 16384 of 64 take 7, where that takes 5.5.
+// 256 experts take 8.3 us and of 1024 9.7, where a group an expert takes 12 and 28; 16384 of 64 take 7, where that takes 5.4. From 262144 choices on, 256 groups, the time grows with the choices:
+// 524288 of 64 take 30 us, 8388608 387.
 constexpr int kRun = 64 * kWaves, kCounts = 4096;  // choices at a time; counts of either kind in LDS, all copies
 
 __global__ __launch_bounds__(kRun) void group_rows_by_run(const int* __restrict__ ids, int choices, exhip_divisor row_of, int experts, int copies, int bits, int run,
@@ -220,7 +221,7 @@ __device__ __forceinline__ float weight_of(const float* weights, int kind, int e
 
 // A wave takes a row and eight outputs a lane; its lanes hold the row's places and weights, which the sum takes from them one choice at a time, always in the
 // choices' order. AHEAD answers are on their way at a time. Every answer is read once, and past L2, as the
-// result is written: what bounds it is the memory (8191 x 6 answers of 4099 to float32 134 us through L2, 115 with answers past it, 102 with both, 5.3 TB/s; with four or eight on their
+// result is written: what bounds it is the memory (8191 x 6 answers of 4099 to float32 134 us through L2, 115 with answers past it, 100 with both, 5.3 TB/s; with four or eight on their
 // way no less).
 template <typename O, int AHEAD>
 __global__ __launch_bounds__(256) void combine_rows_kernel(const uint16_t* __restrict__ z, int z_stride, int z_rows, const int* __restrict__ places, const float* __restrict__ weights,

@@ -314,7 +314,7 @@ __device__ __forceinline__ float gated_value(float g, float u) {
     return GATE == EXHIP_GATE_SILU ? divided(from, d) * u : divided(u, d);
 }
 // `values` for an activation that is known when they are compiled: one choice in front of them all, which are then computed side by side (with a choice in each of them
-// 4096 rows x 8 of 64 experts of 1536 x 2048 took 241 us instead of 227, one group's 512 x 512 12.0 instead of 7.7).
+// 4096 rows x 8 of 64 experts of 1536 x 2048 took 6 % longer, one group's 512 x 512 half as long again).
 template <typename F>
 __device__ __forceinline__ void by_gate(int gate, F values) {
     if (gate == EXHIP_GATE_SILU) values(std::integral_constant<int, EXHIP_GATE_SILU>{});
@@ -326,9 +326,9 @@ __device__ __forceinline__ void by_gate(int gate, F values) {
 // ---- few rows, or few products ----
 // A group takes TN x 16 outputs (of both projections), whole tiles or half of one, and 16 TM rows; its WK waves every WK-th block, with nothing between memory and their registers:
 // the codes of D of a wave's blocks are on their way at a time. The sums meet in LDS, and every thread finishes four neighbouring outputs of a row. What bounds it is the memory:
-// one row of the gated 11264 x 4096 takes 16.6 us, 5.6 TB/s of weights. Four waves a group, so that a CU has several groups, where there are many outputs (one row's 8 of 64
-// experts of 1536 x 2048, gated, 9.0 us, with eight waves 12.1); eight where one group a CU has all of them (4096 x 4096 5.2 us, with four 5.7), and then half a tile a group without
-// an activation, so that more CUs have one (16 rows of 4096 x 11264 11.5 us, with whole tiles 14.3). More blocks on their way, or sixteen waves, measured no faster.
+// one row of the gated 11264 x 4096 takes 16.6 us, 5.6 TB/s of weights. Four waves a group, so that a CU has several groups, where there are many outputs (that row with eight waves 18.4 us);
+// eight where one group a CU has all of them (4096 x 4096 5.2 us, with four 5.7), and then half a tile a group without an activation, so that more CUs have one (16 rows of 4096 x 11264
+// 11.5 us, with whole tiles 14.3). More blocks on their way, or sixteen waves, measured no faster.
 template <int TN, int TM, int WK, int D, bool PAST, bool GATED, bool GROUPED>
 __global__ __launch_bounds__(64 * WK, 2) void i8_rows_kernel(const I8Params p) {
     exhip_touch_args(p);
@@ -502,7 +502,7 @@ __device__ __forceinline__ void write_group(const I8Params& p, const Part& part,
 // block where a step's products are few, and loads stand between the products one by one. A block's one barrier, at its start, says that the next block's rows are there and that
 // the last block's buffer may be filled.
 // Two groups of 128 rows x 256 outputs a CU are what measured fastest for many rows: 8192 x 8192 x 4096 in 213 to 227 us, by the box, 2.4 to 2.6 POP/s, where the library's int8 product takes
-// 296. The card's power bounds it: the clock stands at 1.65 GHz, and with codes of 0 the same launch takes 151 us. Eight waves a group with 256 rows took 8 % longer (nothing runs beside
+// 290 to 296. The card's power bounds it: with codes of 0 the same launch takes 149 us beside 221, and the matrix cores are as many cycles busy in both. Eight waves a group with 256 rows took 8 % longer (nothing runs beside
 // a group's results), four with 64 x 256 outputs each 5 %, and groups that go on to their next tile, its first blocks on their way while results are stored, 2 to 5 %. Few rows are
 // bound by what a CU draws, 85 bytes a ns: 64 rows x 256 outputs, 64 x 128, and 32 rows with weights eight blocks ahead.
 constexpr int most_on_their_way(int loads) { return loads < 63 ? loads : 63; }  // as many as a wait can name
@@ -653,9 +653,11 @@ int launch(exhip_ctx* ctx, K kernel, I8Params p, int halves, int rows, int threa
     return 0;
 }
 
-// One way to run a product: how many 16 outputs (of both projections) and rows a group takes, how many groups a CU runs at once, how many waves share a group's blocks, and what
-// a launch takes, in us: `start`; each time that all CUs are given groups, `round`, and for each block of one wave `alone`, or `share` for each group on a CU where that is more;
+// One way to run a product: how many 16 outputs (of both projections) and rows a group takes, how many groups a CU runs at once, how many waves share a group's blocks, and seven figures of
+// what a launch takes, in us: `start`; each time that all CUs are given groups, `round`, and for each block of one wave `alone`, or `share` for each group on a CU where that is more;
 // `gate` for an activation, each time; but no less than reading the weights from memory and what groups read from L2, weights again and the rows there are, at so many bytes a us.
+// The figures are fitted, all of a list's together, to which form is the fastest: what never bounds a form among the shapes (memory at 12.75 TB/s, L2 at 200) has a figure that says so and no more,
+// and the times that they give are not those of launches.
 struct Form {
     int (*run)(exhip_ctx*, const I8Params&);
     int halves, rows, at_once, split;
@@ -664,8 +666,10 @@ struct Form {
 constexpr long long kManyWeights = 40 << 20;
 template <int TN, int TM, int WK, int D, bool GATED, bool GROUPED>
 int run_rows(exhip_ctx* ctx, const I8Params& p) {
-    // Weights that are read once, by the one tile of rows that there is, and are many: past L2 (11264 x 4096 of a gated product 19.8 -> 18.3 us, 8 of 64 experts of 1536 x 2048 13.2 -> 12.1;
-    // 4096 x 4096 would take 5.8 instead of 5.3).
+    // Weights that are read once, by the one tile of rows that there is, and are many: past L2 (one row of the gated 11264 x 4096 18.3 -> 16.5 us, its 8 of 64 experts of 1536 x 2048 11.5 -> 8.8;
+    // 4096 x 4096 would take 5.35 instead of 5.25). How many rows an expert has, and which have any, is not known here: a tile each on average, and as many experts as there are rows, is what is
+    // expected. Where rows are spread so (1024 rows over 256 experts of 1024 x 2048, gated) it saves 5 to 10 %; where one or two experts have all of them and the same weights are read for many
+    // tiles it costs 0 to 6 % for those 1024 and 512 rows, 1 to 2 us for 16 rows x 2 of 16 experts of 4096 x 4096 (10.2 -> 11.7).
     const bool once = GROUPED ? p.m <= p.experts * 4 * TM : p.m <= 16 * TM;
     if (once && (long long)(p.m < p.experts ? p.m : GROUPED ? p.experts : 1) * p.tiles * p.blocks * kTileBlock >= kManyWeights)
         return launch(ctx, i8_rows_kernel<TN, TM, WK, D, true, GATED, GROUPED>, p, TN, 16 * TM, 64 * WK);
@@ -676,8 +680,10 @@ int run_wide(exhip_ctx* ctx, const I8Params& p) {
     return launch(ctx, i8_wide_kernel<TN, TM, WN, WM, BUFFERS, D, GATED, GROUPED>, p, 2 * TN * WN, 32 * TM * WM, 64 * WN * WM);
 }
 // Chosen so that the form with the least of these times is as near to the fastest as it can be over 952 products and 700 products by experts of 1 to 8192 rows, 64 to 16384
-// outputs and inputs and 2 to 256 experts, those of at most 64 rows counted twice: it takes 1.0 % and 1.3 % longer on average, 25 % at most, and over 109 and 125 others 0.7 %
-// and 1.6 %, 21 % at most. Without any one form of the first list some product would take 8 to 45 % longer, without one of the second 8 to 30 %.
+// outputs and inputs and 2 to 256 experts, those of at most 64 rows counted twice (perf/inner_i8_forms.py times the forms and fits the figures): it takes 1.1 % and 1.4 % longer on average, 26 % at
+// most, and over 109 and 125 others of these sizes 1.2 % and 1.8 %, 22 % at most. Beyond them, up to the most inputs, 250000 outputs and 1024 experts, 4.5 % over 25 products, 38 % at most (64 rows
+// of 130000 gated outputs), and 6.7 % over 16 by experts, 76 % at most (16 rows x 8 of 1024 experts: small tiles, whose groups each search the offsets). Without any one form of the first list
+// some product would take 6 to 47 % longer, without one of the second 12 to 32 %.
 template <bool GATED>
 constexpr Form kPlain[] = {
     {run_rows<GATED ? 2 : 1, 1, 8, 2, GATED, false>, GATED ? 2 : 1, 16, 2, 8, 1.91f, 0.98f, 0.44f, 0.55f, 6.81e6f, 0.2f, 16.53e6f},

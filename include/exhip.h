@@ -581,7 +581,8 @@ int exhip_innerproduct_gated_cut_f8(exhip_ctx* ctx, const exhip_f8_desc* d, int 
 
 /* ---- inner products in 8-bit integers, alone and by experts (no counterpart in the reference) ---- */
 /* Operands are codes from -128 to 127 with float32 scales, one for each row of the input and one for each output of the weights: a code stands for its value times
- * its row's (its output's) scale. Codes' rows begin on 16 bytes (base and stride); what lies between a row's end and its stride is neither used nor written.
+ * its row's (its output's) scale. Codes' rows begin on 16 bytes (base and stride); what lies between a row's end and its stride is neither used nor written, but the products
+ * read the 16 bytes that hold a row's last values whole, the last row's too.
  * Results may not overlap operands.
  * Rows x[m][k] (row stride x_stride elements, at least k; any alignment of the element type) to codes y (row stride y_stride bytes) and scales [m]:
  * scale = max(max |x| / 127, 2^-100), code = the whole number nearest to x / scale, ties to the even one. A row with a NaN or an infinity has codes 0 and
