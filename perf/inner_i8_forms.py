@@ -3,7 +3,7 @@
     python3 perf/inner_i8_forms.py time PART/PARTS > FILE        on the GPU: the shapes of the table anew, every PARTS-th of them, for instance 1/3
     python3 perf/inner_i8_forms.py table FILE ...                the table from what `time` wrote for all its parts
     python3 perf/inner_i8_forms.py check                         how much longer the form that the figures choose takes than the fastest, section by section
-    python3 perf/inner_i8_forms.py fit products|experts [SEED]   other figures for a list, from its section (minutes; seeds differ, the best of some is taken)
+    python3 perf/inner_i8_forms.py fit products|experts [SEED]   other figures for a list, from its section (some seconds; seeds differ, the best of some is taken)
 
 The table is profiles/inner_i8_forms.txt, and its lines are the shapes: for others, add lines with no times to it.
 """
